@@ -9,11 +9,14 @@ from __future__ import annotations
 
 import ctypes
 import os
+from collections.abc import Callable
+
+import torch
 
 LIBRARY_NAME = "libcfmoe_reader.so"
 LIBRARY_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIBRARY_NAME)
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 POINT = 1
 GELU = 2
@@ -25,6 +28,9 @@ WEIGHTS_BF16 = 64
 INPUT_PREPARED = 128
 CHARGE_KEPT = 256
 ENCODER_TILES = 512
+RENORMALISE = 1024
+FP32 = 2048
+FP4 = 4096
 
 EINVAL = 1
 EHIP = 2
@@ -170,6 +176,19 @@ def library() -> ctypes.CDLL:
         ctypes.c_int32,
         ctypes.c_void_p,
     ]
+    pointer, count, flags = ctypes.c_void_p, ctypes.c_int32, ctypes.c_uint32
+    lib.cfmoe_route_scratch_bytes.restype = ctypes.c_int64
+    lib.cfmoe_route_scratch_bytes.argtypes = [count, count]
+    lib.cfmoe_route.restype = ctypes.c_int
+    lib.cfmoe_route.argtypes = [count, count, count, flags] + [pointer] * 6 + [count, pointer]
+    lib.cfmoe_quantise_fp4.restype = ctypes.c_int
+    lib.cfmoe_quantise_fp4.argtypes = [ctypes.c_int64, flags] + [pointer] * 4
+    lib.cfmoe_dequantise_fp4.restype = ctypes.c_int
+    lib.cfmoe_dequantise_fp4.argtypes = [ctypes.c_int64] + [pointer] * 4
+    lib.cfmoe_routed_experts_scratch_bytes.restype = ctypes.c_int64
+    lib.cfmoe_routed_experts_scratch_bytes.argtypes = [count] * 4 + [flags, count]
+    lib.cfmoe_routed_experts.restype = ctypes.c_int
+    lib.cfmoe_routed_experts.argtypes = [count] * 4 + [flags] + [pointer] * 10 + [count, pointer]
     if lib.cfmoe_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{LIBRARY_NAME} ABI mismatch; rebuild the library")
     _library = lib
@@ -201,3 +220,12 @@ def trit_plane_bytes(dims: Dims) -> int:
     if size < 0:
         check(-size)
     return size
+
+
+def launch_on(device: torch.device, call: Callable[[int], int]) -> None:
+    """Run `call(stream)` on the tensors' device and its current stream; check its status."""
+    if torch.cuda.current_device() == device.index:
+        check(call(torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            check(call(torch.cuda.current_stream(device).cuda_stream))

@@ -1,0 +1,110 @@
+"""Router of one MoE layer: hidden rows to the expert ids and weights a reader takes.
+
+The reference leaves routing to its host runtime, whose outputs its operator
+takes (calibration_free_moe/reader/progressive.py:3876-3885). Here `route` makes
+them on the caller's stream in two HIP launches (cfmoe_route in the reader's
+library), so that a layer is `route` followed by a `ProgressiveReader` call or by
+`routed_experts`. Forward only, as the reader.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from calibration_free_moe.reader import _ext
+
+MAX_EXPERTS = 1024
+MAX_TOP_K = 64
+
+
+@torch.no_grad()
+def route(
+    hidden: Tensor,
+    router: Tensor,
+    top_k: int,
+    *,
+    renormalise: bool = True,
+    expert_scale: Tensor | None = None,
+    ids_dtype: torch.dtype = torch.int32,
+    weights_dtype: torch.dtype = torch.float32,
+    out: tuple[Tensor, Tensor] | None = None,
+) -> tuple[Tensor, Tensor]:
+    """Return (ids, weights), both [tokens, top_k], of a softmax top-k router.
+
+    hidden BF16 [tokens, H] and router BF16 [E, H], contiguous; the logits are
+    hidden @ router.T. Each token's `top_k` largest logits are kept, largest
+    first: equal logits go to the lowest expert, NaN counts as the largest, and
+    the order is that of the exact logits, not of their FP32 sums. Weights are
+    the softmax over the kept experts (`renormalise`) or the kept part of the
+    softmax over all, times `expert_scale` (FP32 [E]) at each kept expert if it
+    is given. Ids are always distinct and inside [0, E), whatever the rows hold.
+
+    `out` takes (ids, weights) to write instead of new tensors; their types then
+    stand for `ids_dtype` (int32 or int64) and `weights_dtype` (FP32 or BF16).
+    H is a multiple of 128, E at most 1024, top_k at most 64 and E. Zero tokens
+    give empty outputs. The work is enqueued on the current stream of the
+    tensors' device and can be captured in a graph.
+    """
+    if out is not None:
+        ids, weights = out
+        ids_dtype, weights_dtype = ids.dtype, weights.dtype
+    if (
+        hidden.dim() != 2
+        or router.dim() != 2
+        or hidden.shape[1] != router.shape[1]
+        or hidden.shape[1] % 128
+        or not hidden.shape[1]
+        or not 1 <= router.shape[0] <= MAX_EXPERTS
+        or not 1 <= top_k <= min(MAX_TOP_K, router.shape[0])
+        or hidden.dtype != torch.bfloat16
+        or router.dtype != torch.bfloat16
+        or not hidden.is_cuda
+        or router.device != hidden.device
+        or not hidden.is_contiguous()
+        or not router.is_contiguous()
+        or ids_dtype not in (torch.int32, torch.int64)
+        or weights_dtype not in (torch.float32, torch.bfloat16)
+    ):
+        raise ValueError(
+            "Expected contiguous BF16 CUDA rows [tokens, H] and router [E, H] with H a multiple "
+            "of 128, at most 1024 experts and 64 kept, int32/int64 ids and FP32/BF16 weights"
+        )
+    tokens, experts, device = hidden.shape[0], router.shape[0], hidden.device
+    if expert_scale is not None and (
+        expert_scale.shape != (experts,)
+        or expert_scale.dtype != torch.float32
+        or expert_scale.device != device
+        or not expert_scale.is_contiguous()
+    ):
+        raise ValueError("expert_scale must be contiguous FP32 [E] on the router's device")
+    if out is None:
+        ids = torch.empty((tokens, top_k), dtype=ids_dtype, device=device)
+        weights = torch.empty((tokens, top_k), dtype=weights_dtype, device=device)
+    elif any(
+        t.shape != (tokens, top_k) or t.device != device or not t.is_contiguous() for t in out
+    ):
+        raise ValueError("out must be contiguous (ids, weights) [tokens, top_k] on the rows' device")
+    if not tokens:
+        return ids, weights
+    flags = (
+        (_ext.IDS_INT64 if ids_dtype == torch.int64 else 0)
+        | (_ext.WEIGHTS_BF16 if weights_dtype == torch.bfloat16 else 0)
+        | (_ext.RENORMALISE if renormalise else 0)
+    )
+    lib = _ext.library()
+    scratch = torch.empty(
+        lib.cfmoe_route_scratch_bytes(tokens, experts), dtype=torch.uint8, device=device
+    )
+    _ext.launch_on(
+        device,
+        lambda stream: lib.cfmoe_route(
+            hidden.shape[1], experts, top_k, flags, hidden.data_ptr(), router.data_ptr(),
+            None if expert_scale is None else expert_scale.data_ptr(), ids.data_ptr(),
+            weights.data_ptr(), scratch.data_ptr(), tokens, stream,
+        ),
+    )
+    return ids, weights
+
+
+__all__ = ["route"]

@@ -36,7 +36,7 @@ extern "C" {
 
 typedef struct ihipStream_t *cfmoe_stream;
 
-#define CFMOE_ABI_VERSION 10
+#define CFMOE_ABI_VERSION 11
 
 /* cfmoe_dims.flags */
 #define CFMOE_POINT 1u          /* point score (else five-node Gauss-Hermite) */
@@ -53,6 +53,11 @@ typedef struct ihipStream_t *cfmoe_stream;
                                    follow each token's kept count (slots 0, 3, 6, 7, 12,
                                    13, 19); for thresholded calls, whose `charges` then
                                    hold the terms every active token adds */
+
+#define CFMOE_RENORMALISE 1024u /* cfmoe_route: weights sum to 1 over the kept experts (else
+                                   they are the kept part of the softmax over all) */
+#define CFMOE_FP32 2048u        /* cfmoe_quantise_fp4: FP32 weights (else BF16) */
+#define CFMOE_FP4 4096u         /* cfmoe_routed_experts: microscaled 4-bit weights (else BF16) */
 
 /* Stages of one call, in launch order (cfmoe_launch_stage). */
 #define CFMOE_STAGE_PREPARE 0 /* route, rotate, mask, grid quantisation */
@@ -244,6 +249,58 @@ CFMOE_API int cfmoe_forward_noalloc(const cfmoe_dims *dims, const cfmoe_weights 
 
 /* Bytes of the static device array behind cfmoe_forward_noalloc. */
 CFMOE_API int64_t cfmoe_noalloc_scratch_bytes(void);
+
+/* Router of one layer: logits x router^T of hidden bf16 [T, H] and router
+ * bf16 [E, H], the top_k largest per token (largest first, ties to the lowest
+ * expert, NaN above all; the order is that of the exact logits), their softmax
+ * weights, times expert_scale [E] fp32 unless NULL. flags: CFMOE_IDS_INT64,
+ * CFMOE_WEIGHTS_BF16, CFMOE_RENORMALISE. ids and weights are [T, top_k], as
+ * cfmoe_forward and cfmoe_routed_experts take them. H a multiple of 128, E at
+ * most 1024, top_k at most 64. scratch: cfmoe_route_scratch_bytes(T, E) bytes,
+ * 16-byte aligned like hidden and router; calls that overlap need their own.
+ * T = 0 does nothing. The reference leaves routing to its host runtime. */
+CFMOE_API int64_t cfmoe_route_scratch_bytes(int32_t tokens, int32_t experts);
+CFMOE_API int cfmoe_route(int32_t hidden_size, int32_t experts, int32_t top_k, uint32_t flags,
+                          const void *hidden, const void *router, const float *expert_scale,
+                          void *ids, void *weights, void *scratch, int32_t tokens,
+                          cfmoe_stream stream);
+
+/* Weights to microscaled 4-bit floating point and back. `blocks` blocks of 32
+ * consecutive values share one E8M0 scale byte each (`scales` [blocks]) and hold
+ * two E2M1 codes a byte (`codes` [16 blocks], the even element low). The scale is
+ * 2^(floor(log2 max|v|) - 2), at least 2^-125; codes round to nearest even and
+ * saturate at 6; a block with a NaN or an infinity gets scale byte 255 (NaN).
+ * Values read back are BF16, exact. flags: CFMOE_FP32 (weights fp32, else bf16).
+ * weights and values 16-byte aligned, codes 4-byte aligned. No reference
+ * counterpart. */
+CFMOE_API int cfmoe_quantise_fp4(int64_t blocks, uint32_t flags, const void *weights, void *codes,
+                                 uint8_t *scales, cfmoe_stream stream);
+CFMOE_API int cfmoe_dequantise_fp4(int64_t blocks, const void *codes, const uint8_t *scales,
+                                   void *values, cfmoe_stream stream);
+
+/* The whole routed part of one layer for a batch of few tokens:
+ *   out[t] = sum_k weights[t, k] D_e (phi(G_e x_t) * (U_e x_t)), e = ids[t, k]
+ * with FP32 sums; the weighted activations are rounded to BF16 once, and so is
+ * out [T, H]. gate_up [E, 2I, H] and down are bf16, down channel-major (physical
+ * [E, I, H]) as for cfmoe_forward, and the scale pointers are unused; or with
+ * CFMOE_FP4 both hold the codes of cfmoe_quantise_fp4 over the rows [E, 2I, H] and
+ * [E, H, I], and gate_up_scales [E, 2I, H/32], down_scales [E, H, I/32] their
+ * scales. ids outside [0, E) contribute nothing; rows marked in padding uint8 [T]
+ * (or NULL) read no weights and come out zero. flags: CFMOE_GELU,
+ * CFMOE_IDS_INT64, CFMOE_WEIGHTS_BF16, CFMOE_FP4. H a multiple of 128, I of 16 (of
+ * 32 with CFMOE_FP4), both at most 16384; E at most 4096, top_k 64, T top_k 8192.
+ * Weights, hidden, out and scratch are 16-byte aligned (down_scales and
+ * gate_up_scales 1). scratch: cfmoe_routed_experts_scratch_bytes of the same
+ * arguments; calls that overlap need their own. T = 0 does nothing. */
+CFMOE_API int64_t cfmoe_routed_experts_scratch_bytes(int32_t hidden_size, int32_t width,
+                                                     int32_t experts, int32_t top_k,
+                                                     uint32_t flags, int32_t tokens);
+CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t experts,
+                                   int32_t top_k, uint32_t flags, const void *gate_up,
+                                   const uint8_t *gate_up_scales, const void *down,
+                                   const uint8_t *down_scales, const void *hidden, const void *ids,
+                                   const void *weights, const uint8_t *padding, void *out,
+                                   void *scratch, int32_t tokens, cfmoe_stream stream);
 
 /* Thread-local message of the last failing call. */
 CFMOE_API const char *cfmoe_last_error(void);
