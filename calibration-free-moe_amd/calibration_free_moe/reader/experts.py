@@ -45,7 +45,7 @@ def routed_experts(
     activations are rounded to BF16 once, and so is the output. Results do not
     depend on the other tokens of the batch in more than the order of FP32 sums.
 
-    H is a multiple of 128 and I of 16 (of 32 in 4 bits), both at most 16384; at
+    H is a multiple of 128 and I of 16 (of 32 in 4 bits), both at most 4096; at
     most 4096 experts, 64 ids per token and 8192 pairs per call. Zero tokens give
     an empty output. The scratch is allocated per call: calls may overlap on
     different streams, and captured graphs share nothing.

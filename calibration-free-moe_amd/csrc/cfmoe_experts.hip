@@ -8,9 +8,10 @@
 // it gathers them from the ids itself (pairs of one expert, ascending), 16 to a
 // matrix instruction's columns. Three launches:
 //
-//   experts_up_kernel    act[p, c] = bf16(w phi(g) u), g and u in FP32
-//   experts_down_kernel  partial[s, p, h] = FP32 sum over split s of the channels
-//   experts_join_kernel  out[t, h] = bf16(sum over t's slots and splits, in order)
+//   up    act[p, c] = bf16(w phi(g) u), g and u in FP32 (experts_rows_kernel)
+//   down  partial[p, h] = FP32 sum over the channels (experts_down_kernel over
+//         channel-major BF16 rows, experts_rows_kernel over 4-bit rows)
+//   join  out[t, h] = bf16(sum over t's slots, in order) (experts_join_kernel)
 //
 // A pair whose id lies outside [0, E) or whose token is padded belongs to no
 // expert: nothing computes it, and the join leaves it out.
@@ -25,23 +26,27 @@
 namespace cfmoe {
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kMaxPairs = 8192;
+constexpr int kMaxLength = 4096;  // of a row: 16 operand loads of eight waves
 constexpr int kColumns = 16;      // pairs of a matrix instruction
-constexpr int kUpChannels = 8;    // channels of 16 rows: gate and up row in turn
-constexpr int kDownRows = 128;    // outputs of a BF16 down workgroup
-constexpr int kFp4DownRows = 64;  // of an FP4 one, 16 a wave
-
+constexpr int kRows = 16;         // weight rows of one
+constexpr int kDownOutputs = 64;  // outputs of a BF16 down workgroup
+constexpr int kJoinThreads = 256;
 struct ExpertArgs {
   const uint16_t *x;
   const void *ids, *weights;
   const uint8_t *padding;
   const uint8_t *gate_up, *gate_up_scales, *down, *down_scales;
-  uint16_t *act;   // [pairs, act_stride]
-  float *partial;  // [splits, pairs, hidden]
+  uint16_t *act;   // [pairs, width]
+  float *partial;  // [pairs, hidden]
   uint16_t *out;
-  int tokens, top_k, pairs, experts, hidden, width, act_stride, tiles, splits;
+  int tokens, top_k, pairs, experts, hidden, width;
+  int groups;   // workgroups of an item
+  int tiles;    // row tiles of an item
+  int share;    // row tiles of a workgroup
+  int splits;   // waves that share a row's products (experts_rows_kernel)
   bool ids64, weights16, gelu, by_pair;
 };
 
@@ -58,172 +63,278 @@ __device__ __forceinline__ float pair_weight(const ExpertArgs &a, int pair) {
                      : static_cast<const float *>(a.weights)[pair];
 }
 
-// The pairs of item z's expert into `list`, ascending; returns their number (the
-// same in every thread). With by_pair the items are the pairs, and an expert's
-// first pair takes all of them: the others' items get none.
-__device__ __forceinline__ int gather_pairs(const ExpertArgs &a, int z, int &expert, uint16_t *list,
-                                            int *counts) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  expert = a.by_pair ? pair_expert(a, z) : z;
-  if (expert < 0) return 0;
-  const int share = (a.pairs + kThreads - 1) / kThreads * 64;  // pairs a wave looks at
-  const int begin = min(wave * share, a.pairs), end = min(begin + share, a.pairs);
-  int mine = 0;
-  for (int p = begin + lane; p - lane < end; p += 64)
-    mine += __builtin_popcountll(__ballot(p < end && pair_expert(a, p) == expert));
-  if (lane == 0) counts[wave] = mine;
-  __syncthreads();
-  int at = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    at += w < wave ? counts[w] : 0;
-    total += counts[w];
-  }
-  for (int p = begin + lane; p - lane < end; p += 64) {
-    const uint64_t found = __ballot(p < end && pair_expert(a, p) == expert);
-    if (found >> lane & 1) list[at + __builtin_popcountll(found & ((1ull << lane) - 1))] = p;
-    at += __builtin_popcountll(found);
-  }
-  __syncthreads();
-  return a.by_pair && list[0] != z ? 0 : total;
+// A uniform base and a lane's 32-bit offset: one register an address.
+template <class T>
+__device__ __forceinline__ T load_at(const void *base, uint32_t offset) {
+  return *reinterpret_cast<const T *>(static_cast<const uint8_t *>(base) + offset);
 }
+
+// The pairs of one item's expert. With by_pair the items are the pairs, and an
+// expert's first pair takes all of them: the others' items get none. (A single
+// token's pairs are left apart: its experts differ, or one named twice is read
+// twice.) Each wave looks at a share of the pairs, its first kHeld 64s at once:
+// their loads leave together, and the list is made of what they found; only the
+// further ones of a large batch are looked at twice. `count` is known a barrier
+// before the list is.
+template <int kTeam>
+struct Pairs {
+  static constexpr int kHeld = 4;
+  int expert, count;
+  int begin, end, at;
+  uint64_t found[kHeld];
+
+  __device__ __forceinline__ bool alone(const ExpertArgs &a) const { return a.tokens == 1 && a.by_pair; }
+
+  __device__ __forceinline__ void find(const ExpertArgs &a, int z, int *counts) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    expert = __builtin_amdgcn_readfirstlane(a.by_pair ? pair_expert(a, z) : z);
+    count = 0;
+    begin = z;
+    if (expert < 0) return;
+    if (alone(a)) {
+      count = 1;
+      return;
+    }
+    const int share = (a.pairs + 64 * kTeam - 1) / (64 * kTeam) * 64;
+    begin = min(wave * share, a.pairs);
+    end = min(begin + share, a.pairs);
+    int mine = 0;
+    bool earlier = false;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const int p = begin + 64 * j + lane;
+      found[j] = 0;
+      if (64 * j < share) found[j] = __ballot(p < end && pair_expert(a, p) == expert);
+    }
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      mine += __builtin_popcountll(found[j]);
+      earlier |= (found[j] & __ballot(begin + 64 * j + lane < z)) != 0;
+    }
+    for (int p = begin + 64 * kHeld + lane; p - lane < end; p += 64) {
+      const uint64_t more = __ballot(p < end && pair_expert(a, p) == expert);
+      mine += __builtin_popcountll(more);
+      earlier |= (more & __ballot(p < z)) != 0;
+    }
+    if (lane == 0) counts[wave] = mine | (a.by_pair && earlier ? kNotFirst : 0);
+    __syncthreads();
+    at = 0;
+    bool first = true;
+#pragma unroll
+    for (int w = 0; w < kTeam; ++w) {
+      const int theirs = counts[w];
+      first &= theirs < kNotFirst;
+      at += w < wave ? theirs : 0;
+      count += theirs;
+    }
+    if (!first) count = 0;
+  }
+
+  // The list, ascending, into LDS.
+  __device__ __forceinline__ void list(const ExpertArgs &a, uint16_t *out) const {
+    const int lane = threadIdx.x & 63;
+    if (alone(a)) {
+      if (threadIdx.x == 0) out[0] = begin;
+    } else {
+      const uint64_t below = (1ull << lane) - 1;
+      int to = at;
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j) {
+        if (found[j] >> lane & 1) out[to + __builtin_popcountll(found[j] & below)] = begin + 64 * j + lane;
+        to += __builtin_popcountll(found[j]);
+      }
+      for (int p = begin + 64 * kHeld + lane; p - lane < end; p += 64) {
+        const uint64_t more = __ballot(p < end && pair_expert(a, p) == expert);
+        if (more >> lane & 1) out[to + __builtin_popcountll(more & below)] = p;
+        to += __builtin_popcountll(more);
+      }
+    }
+    __syncthreads();
+  }
+
+ private:
+  static constexpr int kNotFirst = 1 << 20;
+};
 
 __device__ __forceinline__ float activated(float gate, float up, bool gelu) {
   const float inner = gelu ? 1.5957691216057308f * (gate + 0.044715f * gate * gate * gate) : gate;
   return gate / (1.0f + __expf(-inner)) * up;
 }
 
-// The wave sums of a tile, added in order, become activations: lane l of tile
-// (m, n) holds rows 4 (l / 16) .. + 3 of pair l % 16, that is gate and up of two
-// channels.
-template <int kTiles, int kCols>
-__device__ __forceinline__ void store_activations(const ExpertArgs &a, const f32x4 *sums, const uint16_t *list,
-                                                  int count, int base, int channel0) {
-  __syncthreads();
-  for (int i = threadIdx.x; i < kTiles * kCols * 64; i += kThreads) {
-    f32x4 v = sums[i];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) v += sums[w * kTiles * kCols * 64 + i];
-    const int lane = i % 64, n = i / 64 % kCols, m = i / (64 * kCols);
-    const int column = base + n * kColumns + lane % 16;
-    const int channel = channel0 + m * kUpChannels + lane / 16 * 2;
-    if (column < count && channel < a.width) {
-      const int pair = list[column];
-      const float w = pair_weight(a, pair);
-      *reinterpret_cast<uint32_t *>(a.act + static_cast<int64_t>(pair) * a.act_stride + channel) =
-          bf16_pair(w * activated(v[0], v[1], a.gelu), w * activated(v[2], v[3], a.gelu));
-    }
-  }
-  __syncthreads();
-}
+// What a row product is of.
+enum Product { kUpBf16, kUpFp4, kDownFp4 };
 
-// Rows of x for a pass of kCols column tiles; a column past the last pair is not
-// live (its products are not stored).
-template <int kCols>
-struct Columns {
-  const u32x4 *row[kCols];
-  bool live[kCols];
-  __device__ __forceinline__ Columns(const ExpertArgs &a, const uint16_t *list, int count, int base) {
-    const int lane = threadIdx.x & 63;
+// Weight rows times the pairs' vectors. `splits` waves share a row's products, the
+// others take further row tiles, and a round's sums meet in LDS. A wave keeps its
+// piece of the pairs' vectors in registers as matrix operands, kSteps products of 32
+// for kCols x 16 pairs, and multiplies its rows by them (a column past the last pair
+// repeats it; nothing of it is stored).
+//
+// BF16: a lane's 16 bytes are eight values, step j the wave's j-th 32. FP4: they
+// are a whole block of 32, lane group g taking block g of 128 values, so that
+// steps 4 i .. 4 i + 3 are the four words of the wave's i-th block. The scales of
+// all the workgroup's rows go to LDS first: they are rows of length / 32 bytes, of
+// which a wave wants a few bytes each (byte loads from memory took a third of the
+// up product's time, 87 us of it 27 at 1024 pairs, 128 experts of 2048 x 768).
+//
+// Unless kFull a wave may hold fewer loads than the kernel has: it repeats its last
+// one with every bit cleared, weights and vectors both, so that what a row holds
+// cannot reach the sum a second time.
+template <Product kProduct, int kSteps, bool kFull, int kCols>
+struct RowPass {
+  static constexpr bool kFp4 = kProduct != kUpBf16, kDown = kProduct == kDownFp4;
+  static constexpr int kLoads = kFp4 ? kSteps / 4 : kSteps;
+
+  template <class Ready>
+  static __device__ __forceinline__ void run(const ExpertArgs &a, int expert, int first, int last,
+                                             const uint16_t *list, int count, int base, f32x4 *sums,
+                                             const uint8_t *scales, Ready ready) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int split = wave % a.splits, sub = wave / a.splits, subs = kWaves / a.splits;
+    const int length = kDown ? a.width : a.hidden;
+    const int units = kFp4 ? (length + 127) / 128 : length / 32;
+    const int begin = units * split / a.splits, steps = units * (split + 1) / a.splits - begin;
+    const int rounds = (last - first + subs - 1) / subs;
+    const uint32_t row_bytes = kFp4 ? length / 2 : length * 2, scale_bytes = length / 32;
+    // the lane's row of a tile: in the up product gate and up row of a channel in turn
+    const uint32_t row = kDown ? lane % 16 : (lane & 1) * a.width + lane % 16 / 2;
+    const uint32_t lane_row = row * row_bytes + lane / 16 * 16;
+    const uint32_t kept_row = kDown ? lane % 16 : (lane & 1) * (a.share * (kRows / 2)) + lane % 16 / 2;
+    const uint8_t *lane_scales = scales + kept_row * scale_bytes + 4 * begin;
+
+    // load i is one of the wave's own (in 4 bits a row's last 128 values may end at a
+    // block), and where it starts, in units of 64 bytes from the wave's first
+    auto own = [&](int i) {
+      const bool inside = i < steps && (!kFp4 || 4 * (begin + i) + lane / 16 < length / 32);
+      return kFull || inside ? ~0u : 0u;
+    };
+    auto unit = [&](int i) { return kFull ? i : min(i, steps - 1); };
+
+    u32x4 words[kLoads];
+    auto load = [&](int tile) {
+      tile = min(tile, last - 1);
+      const int64_t row0 = kDown ? static_cast<int64_t>(expert) * a.hidden + tile * kRows
+                                 : static_cast<int64_t>(expert) * 2 * a.width + tile * (kRows / 2);
+      const uint8_t *w = (kDown ? a.down : a.gate_up) + row0 * row_bytes + begin * 64;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const bool whole = kFull || !kFp4 || own(unit(i));
+        words[i] = load_at<u32x4>(w + unit(i) * 64, whole ? lane_row : lane_row - lane / 16 * 16);
+      }
+    };
+    load(first + sub);
+    ready();
+    const void *rows = kDown ? a.act : a.x;
+    u32x4 b[kCols][kSteps];
 #pragma unroll
     for (int n = 0; n < kCols; ++n) {
-      const int column = base + n * kColumns + lane % 16;
-      live[n] = column < count;
-      const int token = live[n] ? list[column] / a.top_k : 0;
-      row[n] = reinterpret_cast<const u32x4 *>(a.x + static_cast<int64_t>(token) * a.hidden);
+      const uint32_t pair = list[min(base + n * kColumns + lane % 16, count - 1)];
+      const uint32_t vector = (kDown ? pair * a.width : pair / a.top_k * a.hidden) * 2;
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        // (element 32 block + 8 (j % 4) in 4 bits, block 4 i + lane / 16)
+        const int i = unit(kFp4 ? j / 4 : j);
+        const uint32_t place = kFp4 ? (4 * (begin + i) + (own(i) ? lane / 16 : 0)) * 64 + j % 4 * 16
+                                    : (begin + i) * 64 + lane / 16 * 16;
+        b[n][j] = load_at<u32x4>(rows, vector + place) & own(kFp4 ? j / 4 : j);
+      }
     }
-  }
-  __device__ __forceinline__ u32x4 load(int n, int at) const {
-    u32x4 v = {0, 0, 0, 0};
-    if (live[n]) v = row[n][at];
-    return v;
+    // what a wave adds up and stores: of a round's subs x kCols sums every eighth; its
+    // column tile is the same in each
+    const int column = base + wave % kCols * kColumns + lane % 16;
+    const bool stores = column < count;
+    const uint32_t pair = list[min(column, count - 1)];
+    const uint32_t to = kDown ? pair * a.hidden + lane / 16 * 4 : pair * a.width + lane / 16 * 2;
+    const float weight = kDown ? 0.0f : pair_weight(a, pair);
+
+    for (int r = 0; r < rounds; ++r) {
+      f32x4 d[kCols];
+#pragma unroll
+      for (int n = 0; n < kCols; ++n) d[n] = f32x4{0, 0, 0, 0};
+      const int kept = min(r * subs + sub, last - 1 - first) * (kDown ? kRows : kRows / 2) * scale_bytes;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const u32x4 w = words[i] & own(i);
+        if constexpr (kFp4) {
+          const uint32_t byte = lane_scales[kept + 4 * unit(i) + (own(unit(i)) ? lane / 16 : 0)];
+          const float by = __uint_as_float((byte & own(i)) << 23);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const u32x4 values = fp4_values(w[q], by);
+#pragma unroll
+            for (int n = 0; n < kCols; ++n) d[n] = mma(values, b[n][4 * i + q], d[n]);
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) d[n] = mma(w, b[n][i], d[n]);
+        }
+      }
+      // (the sums alternate between two buffers: what a round overwrites was read
+      // before the last barrier)
+      f32x4 *in = sums + (r & 1) * (kWaves * kCols * 64) + lane;
+#pragma unroll
+      for (int n = 0; n < kCols; ++n) in[(wave * kCols + n) * 64] = d[n];
+      if (r + 1 < rounds) load(first + (r + 1) * subs + sub);
+      __syncthreads();
+      for (int i = wave; i < subs * kCols; i += kWaves) {
+        const int tile = first + r * subs + i / kCols;
+        if (!stores || tile >= last) break;
+        f32x4 v = in[(i / kCols * a.splits * kCols + i % kCols) * 64];
+        for (int w = 1; w < a.splits; ++w) v += in[((i / kCols * a.splits + w) * kCols + i % kCols) * 64];
+        if (kDown)
+          *reinterpret_cast<f32x4 *>(a.partial + (to + tile * kRows)) = v;
+        else
+          *reinterpret_cast<uint32_t *>(a.act + (to + tile * (kRows / 2))) =
+              bf16_pair(weight * activated(v[0], v[1], a.gelu), weight * activated(v[2], v[3], a.gelu));
+      }
+    }
+    __syncthreads();
   }
 };
 
-template <bool kFp4, int kTiles, int kCols>
-__device__ __forceinline__ void up_pass(const ExpertArgs &a, int expert, int channel0, const uint16_t *list,
-                                        int count, int base, f32x4 *sums) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Columns<kCols> columns(a, list, count, base);
-  f32x4 d[kTiles][kCols];
-#pragma unroll
-  for (int m = 0; m < kTiles; ++m)
-#pragma unroll
-    for (int n = 0; n < kCols; ++n) d[m][n] = f32x4{0, 0, 0, 0};
-  int64_t row[kTiles];
-#pragma unroll
-  for (int m = 0; m < kTiles; ++m) {
-    const int channel = min(channel0 + m * kUpChannels + lane % 16 / 2, a.width - 1);
-    row[m] = static_cast<int64_t>(expert) * 2 * a.width + (lane & 1) * a.width + channel;
-  }
-  if (kFp4) {
-    // a lane's 16 bytes are one block of 32: four products of eight, lane group g
-    // taking block g of the 128 hidden values of a step
-    for (int s = wave; s < a.hidden / 128; s += kWaves) {
-      u32x4 codes[kTiles];
-      float scale[kTiles];
-#pragma unroll
-      for (int m = 0; m < kTiles; ++m) {
-        codes[m] = reinterpret_cast<const u32x4 *>(a.gate_up + row[m] * (a.hidden / 2))[4 * s + lane / 16];
-        scale[m] = __int_as_float(
-            static_cast<int>(a.gate_up_scales[row[m] * (a.hidden / 32) + 4 * s + lane / 16]) << 23);
-      }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        u32x4 b[kCols];
-#pragma unroll
-        for (int n = 0; n < kCols; ++n) b[n] = columns.load(n, 16 * s + lane / 16 * 4 + q);
-#pragma unroll
-        for (int m = 0; m < kTiles; ++m) {
-          const u32x4 w = fp4_values(codes[m][q], scale[m]);
-#pragma unroll
-          for (int n = 0; n < kCols; ++n) d[m][n] = mma(w, b[n], d[m][n]);
-        }
-      }
-    }
-  } else {
-#pragma unroll 4
-    for (int s = wave; s < a.hidden / 32; s += kWaves) {
-      u32x4 w[kTiles], b[kCols];
-#pragma unroll
-      for (int m = 0; m < kTiles; ++m)
-        w[m] = reinterpret_cast<const u32x4 *>(a.gate_up + row[m] * (2 * a.hidden))[4 * s + lane / 16];
-#pragma unroll
-      for (int n = 0; n < kCols; ++n) b[n] = columns.load(n, 4 * s + lane / 16);
-#pragma unroll
-      for (int m = 0; m < kTiles; ++m)
-#pragma unroll
-        for (int n = 0; n < kCols; ++n) d[m][n] = mma(w[m], b[n], d[m][n]);
-    }
-  }
-#pragma unroll
-  for (int m = 0; m < kTiles; ++m)
-#pragma unroll
-    for (int n = 0; n < kCols; ++n) sums[((wave * kTiles + m) * kCols + n) * 64 + lane] = d[m][n];
-  store_activations<kTiles, kCols>(a, sums, list, count, base, channel0);
-}
-
-constexpr int kUpTiles = 2;
-constexpr int kUpCols = 4;
-
-template <bool kFp4>
-__global__ __launch_bounds__(kThreads) void experts_up_kernel(ExpertArgs a) {
-  __shared__ f32x4 sums[kWaves * kUpTiles * kUpCols * 64];
+// Workgroup = `share` row tiles of one item, for all of its pairs, up to kMaxCols x 16
+// at a time. Dynamic LDS: the scales of its rows, then the list of pairs.
+template <Product kProduct, int kSteps, bool kFull, int kMaxCols>
+__global__ __launch_bounds__(kThreads, kMaxCols <= 2 && kSteps <= 8 ? 4 : 2) void experts_rows_kernel(ExpertArgs a) {
+  constexpr bool kFp4 = kProduct != kUpBf16, kDown = kProduct == kDownFp4;
+  __shared__ f32x4 sums[2 * kWaves * kMaxCols * 64];
   __shared__ int counts[kWaves];
-  extern __shared__ uint16_t list[];
-  const int tile = blockIdx.x % a.tiles;
-  int expert;
-  const int count = gather_pairs(a, blockIdx.x / a.tiles, expert, list, counts);
-  const int channel0 = tile * kUpTiles * kUpChannels;
+  extern __shared__ __align__(16) uint8_t lds[];
+  Pairs<kWaves> pairs;
+  pairs.find(a, blockIdx.x / a.groups, counts);
+  const int count = pairs.count, expert = pairs.expert;
+  if (count == 0) return;
+  const int first = blockIdx.x % a.groups * a.share, last = min(first + a.share, a.tiles);
+  const uint32_t scale_bytes = kFp4 ? (kDown ? a.width : a.hidden) / 32 : 0;
+  uint16_t *list = reinterpret_cast<uint16_t *>(lds + a.share * kRows * scale_bytes);
+
+  // 16 bytes a thread of the scales of rows first .. last - 1 (gate rows, then up)
+  const int tile_rows = kDown ? kRows : kRows / 2, parts = kDown ? 1 : 2;
+  const int chunks = (last - first) * tile_rows * scale_bytes / 16, kept = a.share * tile_rows * scale_bytes / 16;
+  const uint8_t *scales = (kDown ? a.down_scales + static_cast<int64_t>(expert) * a.hidden * scale_bytes
+                                 : a.gate_up_scales + static_cast<int64_t>(expert) * 2 * a.width * scale_bytes) +
+                          first * tile_rows * scale_bytes;
+  for (int i = threadIdx.x; kFp4 && i < parts * kept; i += kThreads) {
+    const int part = i / kept, chunk = i - part * kept;
+    if (chunk < chunks)
+      reinterpret_cast<u32x4 *>(lds)[i] = load_at<u32x4>(scales, part * a.width * scale_bytes + chunk * 16);
+  }
+
   for (int base = 0; base < count;) {
-    if (count - base > 2 * kColumns) {
-      up_pass<kFp4, kUpTiles, 4>(a, expert, channel0, list, count, base, sums);
+    const int left = count - base;
+    auto ready = [&] {
+      if (base == 0) pairs.list(a, list);
+    };
+    if (kMaxCols >= 4 && left > 2 * kColumns) {
+      if constexpr (kMaxCols >= 4)
+        RowPass<kProduct, kSteps, kFull, 4>::run(a, expert, first, last, list, count, base, sums, lds, ready);
       base += 4 * kColumns;
-    } else if (count - base > kColumns) {
-      up_pass<kFp4, kUpTiles, 2>(a, expert, channel0, list, count, base, sums);
+    } else if (kMaxCols >= 2 && left > kColumns) {
+      if constexpr (kMaxCols >= 2)
+        RowPass<kProduct, kSteps, kFull, 2>::run(a, expert, first, last, list, count, base, sums, lds, ready);
       base += 2 * kColumns;
     } else {
-      up_pass<kFp4, kUpTiles, 1>(a, expert, channel0, list, count, base, sums);
+      RowPass<kProduct, kSteps, kFull, 1>::run(a, expert, first, last, list, count, base, sums, lds, ready);
       base += kColumns;
     }
   }
@@ -231,11 +342,11 @@ __global__ __launch_bounds__(kThreads) void experts_up_kernel(ExpertArgs a) {
 
 // Channel-major down rows hold an output per element, where the matrix operand
 // wants eight channels of one output: a lane loads eight channels' rows at its
-// eight outputs and turns the 8 x 8 square in registers. Output 8 (l % 16) + j of
+// four outputs and turns the 8 x 4 piece in registers. Output 4 (l % 16) + j of
 // the tile is row l % 16 of product j.
-__device__ __forceinline__ void turn(const u32x4 (&rows)[8], u32x4 (&turned)[8]) {
+__device__ __forceinline__ void turn(const u32x2 (&rows)[8], u32x4 (&turned)[4]) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 4; ++j) {
     const uint32_t select = j & 1 ? 0x07060302u : 0x05040100u;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
@@ -243,178 +354,116 @@ __device__ __forceinline__ void turn(const u32x4 (&rows)[8], u32x4 (&turned)[8])
   }
 }
 
-// Workgroup = 128 outputs of one expert over one split of its channels, the waves
-// every fourth 32 channels of it.
-template <int kCols>
-__device__ __forceinline__ void down_pass(const ExpertArgs &a, int expert, int row0, int split, const uint16_t *list,
-                                          int count, int base, f32x4 *sums) {
+// Workgroup = 64 outputs of one expert, the waves an eighth of its channels each
+// (kSteps products of 32 at most; wider layers take several chunks). The weights
+// stay in registers for all of the expert's pairs, 16 at a time.
+template <int kSteps>
+__global__ __launch_bounds__(kThreads, kSteps <= 4 ? 4 : 2) void experts_down_kernel(ExpertArgs a) {
+  __shared__ f32x4 sums[kWaves * 4 * 64];
+  __shared__ int counts[kWaves];
+  extern __shared__ uint16_t list[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int steps = (a.width + 31) / 32;
-  const int begin = steps * split / a.splits, end = steps * (split + 1) / a.splits;
-  const uint16_t *act[kCols];
-  bool live[kCols];
+  Pairs<kWaves> pairs;
+  pairs.find(a, blockIdx.x / a.groups, counts);
+  const int count = pairs.count, expert = pairs.expert;
+  if (count == 0) return;
+  const int row0 = blockIdx.x % a.groups * kDownOutputs;
+  const int row_bytes = 2 * a.hidden, steps = (a.width + 31) / 32;
+  const uint8_t *down = a.down + (static_cast<int64_t>(expert) * a.width * a.hidden + row0) * 2;
+  const uint32_t lane_channel = lane / 16 * 8, lane_row = lane_channel * row_bytes + lane % 16 * 8;
+  // the last 32 channels may be 16: their second half repeats the first, cleared
+  const bool half = a.width % 32 != 0 && lane >= 32;
+  const uint32_t last_channel = half ? lane_channel - 16 : lane_channel;
+  const uint32_t last_row = last_channel * row_bytes + lane % 16 * 8;
+  for (int chunk = 0; chunk < steps; chunk += kWaves * kSteps) {
+    // the wave's products are every eighth 32 channels; one past the last repeats it
+    // with every bit cleared
+    u32x4 w[kSteps][4];
 #pragma unroll
-  for (int n = 0; n < kCols; ++n) {
-    const int column = base + n * kColumns + lane % 16;
-    live[n] = column < count;
-    act[n] = a.act + static_cast<int64_t>(live[n] ? list[column] : 0) * a.act_stride;
-  }
-  f32x4 d[8][kCols];
+    for (int s = 0; s < kSteps; ++s) {
+      const int step = min(chunk + s * kWaves + wave, steps - 1);
+      const bool own = chunk + s * kWaves + wave < steps && !(step == steps - 1 && half);
+      const uint8_t *channel = down + static_cast<int64_t>(32 * step) * row_bytes;
+      const uint32_t offset = step == steps - 1 ? last_row : lane_row;
+      u32x2 rows[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-#pragma unroll
-    for (int n = 0; n < kCols; ++n) d[j][n] = f32x4{0, 0, 0, 0};
-  const uint16_t *down = reinterpret_cast<const uint16_t *>(a.down) +
-                         static_cast<int64_t>(expert) * a.width * a.hidden + row0 + lane % 16 * 8;
-  for (int s = begin + wave; s < end; s += kWaves) {
-    const int channel = 32 * s + lane / 16 * 8;
-    const bool inside = channel < a.width;  // (the width is a multiple of 16)
-    u32x4 rows[8], turned[8], b[kCols];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      rows[i] = u32x4{0, 0, 0, 0};
-      if (inside) rows[i] = *reinterpret_cast<const u32x4 *>(down + static_cast<int64_t>(channel + i) * a.hidden);
+      for (int i = 0; i < 8; ++i)
+        rows[i] = *reinterpret_cast<const u32x2 *>(channel + i * row_bytes + offset) & (own ? ~0u : 0u);
+      turn(rows, w[s]);
     }
+    if (chunk == 0) pairs.list(a, list);
+    for (int base = 0; base < count; base += kColumns) {
+      const uint32_t pair = list[min(base + lane % 16, count - 1)];
+      const uint8_t *act = reinterpret_cast<const uint8_t *>(a.act);
+      u32x4 b[kSteps];
 #pragma unroll
-    for (int n = 0; n < kCols; ++n) {
-      b[n] = u32x4{0, 0, 0, 0};
-      if (inside && live[n]) b[n] = *reinterpret_cast<const u32x4 *>(act[n] + channel);
-    }
-    turn(rows, turned);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int n = 0; n < kCols; ++n) d[j][n] = mma(turned[j], b[n], d[j][n]);
-  }
-  // sums[wave][column tile][product j][lane]
-#pragma unroll
-  for (int n = 0; n < kCols; ++n)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sums[((wave * kCols + n) * 8 + j) * 64 + lane] = d[j][n];
-  __syncthreads();
-  for (int i = threadIdx.x; i < kCols * 8 * 64; i += kThreads) {
-    f32x4 v = sums[i];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) v += sums[w * kCols * 8 * 64 + i];
-    const int at = i % 64, j = i / 64 % 8, n = i / 512;
-    const int column = base + n * kColumns + at % 16;
-    if (column < count) {
-      float *out = a.partial + (static_cast<int64_t>(split) * a.pairs + list[column]) * a.hidden + row0 + j;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) out[8 * (at / 16 * 4 + r)] = v[r];
-    }
-  }
-  __syncthreads();
-}
-
-__global__ __launch_bounds__(kThreads) void experts_down_kernel(ExpertArgs a) {
-  __shared__ f32x4 sums[kWaves * 8 * 64];
-  __shared__ int counts[kWaves];
-  extern __shared__ uint16_t list[];
-  const int tile = blockIdx.x % a.tiles, rest = blockIdx.x / a.tiles;
-  int expert;
-  const int count = gather_pairs(a, rest / a.splits, expert, list, counts);
-  for (int base = 0; base < count;) {
-    down_pass<1>(a, expert, tile * kDownRows, rest % a.splits, list, count, base, sums);
-    base += kColumns;
-  }
-}
-
-// Wave = 16 outputs of one expert, all its channels: a lane's 16 bytes are one
-// block of its row, as in up_pass. A last step's groups past the width are zero.
-template <int kCols>
-__device__ __forceinline__ void fp4_down_pass(const ExpertArgs &a, int expert, int row0, const uint16_t *list,
-                                              int count, int base) {
-  const int lane = threadIdx.x & 63;
-  const int blocks = a.width / 32;
-  const int64_t row = static_cast<int64_t>(expert) * a.hidden + row0 + lane % 16;
-  const u32x4 *codes = reinterpret_cast<const u32x4 *>(a.down + row * (a.width / 2));
-  const uint8_t *scales = a.down_scales + row * blocks;
-  const u32x4 *act[kCols];
-  bool live[kCols];
-  int pair[kCols];
-  f32x4 d[kCols];
-#pragma unroll
-  for (int n = 0; n < kCols; ++n) {
-    const int column = base + n * kColumns + lane % 16;
-    live[n] = column < count;
-    pair[n] = live[n] ? list[column] : 0;
-    act[n] = reinterpret_cast<const u32x4 *>(a.act + static_cast<int64_t>(pair[n]) * a.act_stride);
-    d[n] = f32x4{0, 0, 0, 0};
-  }
-  for (int block = lane / 16; block - lane / 16 < blocks; block += 4) {
-    const bool inside = block < blocks;
-    u32x4 word = {0, 0, 0, 0};
-    float scale = 0.0f;
-    if (inside) {
-      word = codes[block];
-      scale = __int_as_float(static_cast<int>(scales[block]) << 23);
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const u32x4 w = fp4_values(word[q], scale);
-#pragma unroll
-      for (int n = 0; n < kCols; ++n) {
-        u32x4 b = {0, 0, 0, 0};
-        if (inside && live[n]) b = act[n][4 * block + q];
-        d[n] = mma(w, b, d[n]);
+      for (int s = 0; s < kSteps; ++s) {
+        const int step = min(chunk + s * kWaves + wave, steps - 1);
+        const bool own = chunk + s * kWaves + wave < steps && !(step == steps - 1 && half);
+        const uint32_t offset = (pair * a.width + (step == steps - 1 ? last_channel : lane_channel)) * 2;
+        b[s] = *reinterpret_cast<const u32x4 *>(act + 64 * step + offset) & (own ? ~0u : 0u);
       }
-    }
-  }
+      f32x4 d[4];
 #pragma unroll
-  for (int n = 0; n < kCols; ++n)
-    if (live[n])
-      *reinterpret_cast<f32x4 *>(a.partial + static_cast<int64_t>(pair[n]) * a.hidden + row0 + lane / 16 * 4) = d[n];
-}
-
-__global__ __launch_bounds__(kThreads) void experts_fp4_down_kernel(ExpertArgs a) {
-  __shared__ int counts[kWaves];
-  extern __shared__ uint16_t list[];
-  const int tile = blockIdx.x % a.tiles;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int expert;
-  const int count = gather_pairs(a, blockIdx.x / a.tiles, expert, list, counts);
-  const int row0 = tile * kFp4DownRows + wave * 16;
-  for (int base = 0; base < count;) {
-    if (count - base > 2 * kColumns) {
-      fp4_down_pass<4>(a, expert, row0, list, count, base);
-      base += 4 * kColumns;
-    } else {
-      fp4_down_pass<2>(a, expert, row0, list, count, base);
-      base += 2 * kColumns;
+      for (int j = 0; j < 4; ++j) d[j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[j] = mma(w[s][j], b[s], d[j]);
+      // a lane holds outputs 16 g + 4 r + j of its pair, g = l / 16
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        sums[(wave * 4 + r) * 64 + lane] = f32x4{d[0][r], d[1][r], d[2][r], d[3][r]};
+      __syncthreads();
+      if (threadIdx.x < 256) {
+        f32x4 v = sums[threadIdx.x];
+#pragma unroll
+        for (int k = 1; k < kWaves; ++k) v += sums[k * 256 + threadIdx.x];
+        const int column = base + lane % 16;
+        if (column < count) {
+          f32x4 *out = reinterpret_cast<f32x4 *>(a.partial + (static_cast<uint32_t>(list[column]) * a.hidden + row0 +
+                                                 lane / 16 * 16 + wave * 4));
+          *out = chunk ? *out + v : v;
+        }
+      }
+      __syncthreads();
     }
   }
 }
 
-// Thread = eight outputs of one token: its slots' partials in order, each split's
-// in order within a slot.
-__global__ __launch_bounds__(kThreads) void experts_join_kernel(ExpertArgs a) {
-  const int groups = a.hidden / 8;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int t = static_cast<int>(i / groups), h = static_cast<int>(i % groups) * 8;
+// Thread = four outputs of one token: its slots' partials in order.
+__global__ __launch_bounds__(kJoinThreads) void experts_join_kernel(ExpertArgs a) {
+  constexpr int kAhead = 8;
+  const int groups = a.hidden / 4;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kJoinThreads + threadIdx.x;
+  const int t = static_cast<int>(i / groups), h = static_cast<int>(i % groups) * 4;
   if (t >= a.tokens) return;
-  f32x4 low = {0, 0, 0, 0}, high = {0, 0, 0, 0};
-  for (int k = 0; k < a.top_k; ++k) {
-    const int pair = t * a.top_k + k;
-    if (pair_expert(a, pair) < 0) continue;
-    for (int s = 0; s < a.splits; ++s) {
-      const f32x4 *p = reinterpret_cast<const f32x4 *>(
-          a.partial + (static_cast<int64_t>(s) * a.pairs + pair) * a.hidden + h);
-      low += p[0];
-      high += p[1];
+  f32x4 sum = {0, 0, 0, 0};
+  const float *row = a.partial + static_cast<int64_t>(t) * a.top_k * a.hidden + h;
+  for (int k = 0; k < a.top_k; k += kAhead) {
+    f32x4 v[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      // (a slot that no expert computed holds whatever the scratch held)
+      const int slot = min(k + j, a.top_k - 1);
+      v[j] = *reinterpret_cast<const f32x4 *>(row + static_cast<int64_t>(slot) * a.hidden);
+      const bool routed = k + j < a.top_k && pair_expert(a, t * a.top_k + slot) >= 0;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[j][r] = routed ? v[j][r] : 0.0f;
     }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) sum += v[j];
   }
-  const u32x4 out = {bf16_pair(low[0], low[1]), bf16_pair(low[2], low[3]), bf16_pair(high[0], high[1]),
-                     bf16_pair(high[2], high[3])};
-  *reinterpret_cast<u32x4 *>(a.out + static_cast<int64_t>(t) * a.hidden + h) = out;
+  const u32x2 out = {bf16_pair(sum[0], sum[1]), bf16_pair(sum[2], sum[3])};
+  *reinterpret_cast<u32x2 *>(a.out + static_cast<int64_t>(t) * a.hidden + h) = out;
 }
 
 int validate(int hidden, int width, int experts, int top_k, uint32_t flags, int tokens) {
-  if (hidden <= 0 || hidden % 128 || hidden > 16384)
-    return fail(CFMOE_EINVAL, "routed_experts needs a hidden size that is a multiple of 128, at most 16384");
+  if (hidden <= 0 || hidden % 128 || hidden > kMaxLength)
+    return fail(CFMOE_EINVAL, "routed_experts needs a hidden size that is a multiple of 128, at most 4096");
   const int grain = flags & CFMOE_FP4 ? 32 : 16;
-  if (width <= 0 || width % grain || width > 16384)
-    return fail(CFMOE_EINVAL, "routed_experts needs a width that is a multiple of 16 (of 32 with 4-bit weights), at most 16384");
+  if (width <= 0 || width % grain || width > kMaxLength)
+    return fail(CFMOE_EINVAL, "routed_experts needs a width that is a multiple of 16 (of 32 with 4-bit weights), at most 4096");
   if (experts < 1 || experts > 4096) return fail(CFMOE_EINVAL, "routed_experts needs 1 to 4096 experts");
   if (top_k < 1 || top_k > 64) return fail(CFMOE_EINVAL, "routed_experts needs 1 to 64 experts per token");
   if (tokens < 0 || static_cast<int64_t>(tokens) * top_k > kMaxPairs)
@@ -422,19 +471,57 @@ int validate(int hidden, int width, int experts, int top_k, uint32_t flags, int 
   return 0;
 }
 
-// Down splits: workgroups that share an expert's channels, so that a batch of few
-// pairs still covers the compute units.
-int down_splits(int hidden, int width, int experts, int top_k, uint32_t flags, int tokens) {
-  if (flags & CFMOE_FP4) return 1;
-  const int items = std::min(tokens * top_k, experts) * (hidden / kDownRows);
-  const int steps = (width + 31) / 32;
-  int splits = 1;
-  while (items * splits < 256 && splits * 2 * kWaves <= steps) splits *= 2;
-  return splits;
+// How a row of `units` operand loads (32 BF16 values, or 128 in 4 bits) is cut: the
+// waves that share it, and each one's loads, one of the counts that kernels exist
+// for. Fewest idle loads first, then the most waves.
+struct Cut {
+  int splits, loads;
+};
+
+Cut cut_of(int units, bool fp4) {
+  Cut best = {0, 0};
+  for (int splits = kWaves; splits >= 1; splits /= 2)
+    for (int loads : {fp4 ? 2 : 8, fp4 ? 3 : 12, fp4 ? 4 : 16})
+      if (loads * splits >= units && (!best.splits || loads * splits < best.loads * best.splits))
+        best = {splits, loads};
+  return best;
 }
 
 int64_t act_bytes(int width, int pairs) {
   return static_cast<int64_t>(pairs) * width * 2;  // (a row is a multiple of 32 bytes)
+}
+
+template <Product kProduct, int kSteps>
+auto rows_kernel(bool full, bool wide) {
+  // (registers: 4 x 16 pairs beside eight steps, 2 x 16 beside 12, or 16 in 4 bits)
+  constexpr int kNarrow = kProduct == kUpFp4 && kSteps == 8 ? 2 : 1;
+  constexpr int kWide = kSteps == 8 ? 4 : kSteps == 12 || kProduct != kUpBf16 ? 2 : 1;
+  return wide ? full ? experts_rows_kernel<kProduct, kSteps, true, kWide> : experts_rows_kernel<kProduct, kSteps, false, kWide>
+              : full ? experts_rows_kernel<kProduct, kSteps, true, kNarrow> : experts_rows_kernel<kProduct, kSteps, false, kNarrow>;
+}
+
+template <Product kProduct>
+int launch_rows(ExpertArgs a, int items, unsigned list, cfmoe_stream stream) {
+  constexpr bool kFp4 = kProduct != kUpBf16, kDown = kProduct == kDownFp4;
+  const int length = kDown ? a.width : a.hidden;
+  const int units = kFp4 ? (length + 127) / 128 : length / 32;
+  const Cut cut = cut_of(units, kFp4);
+  const int steps = cut.loads * (kFp4 ? 4 : 1);
+  const bool full = units == cut.splits * cut.loads && length % 128 == 0;
+  const bool wide = a.pairs >= 12 * a.experts;
+  a.splits = cut.splits;
+  a.tiles = kDown ? a.hidden / kRows : a.width / (kRows / 2);
+  // enough workgroups to fill the chip, then fewer loads of the pairs' vectors
+  const int subs = kWaves / cut.splits;
+  a.share = subs;
+  while (static_cast<int64_t>(items) * a.tiles / (2 * a.share) >= 1024 && a.share < 8 * subs) a.share *= 2;
+  a.groups = (a.tiles + a.share - 1) / a.share;
+  const auto kernel = steps <= 8    ? rows_kernel<kProduct, 8>(full, wide)
+                      : steps <= 12 ? rows_kernel<kProduct, 12>(full, wide)
+                                    : rows_kernel<kProduct, 16>(full, wide);
+  const unsigned scales = kFp4 ? a.share * kRows * (length / 32) : 0;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.groups) * items), dim3(kThreads), scales + list, stream, a);
+  return check_launch(kDown ? "experts_down" : "experts_up");
 }
 
 }  // namespace
@@ -448,8 +535,7 @@ CFMOE_API int64_t cfmoe_routed_experts_scratch_bytes(int32_t hidden_size, int32_
                                                      int32_t top_k, uint32_t flags, int32_t tokens) {
   if (int rc = validate(hidden_size, width, experts, top_k, flags, tokens)) return -rc;
   const int pairs = tokens * top_k;
-  const int splits = down_splits(hidden_size, width, experts, top_k, flags, tokens);
-  return act_bytes(width, pairs) + static_cast<int64_t>(splits) * pairs * hidden_size * 4;
+  return act_bytes(width, pairs) + static_cast<int64_t>(pairs) * hidden_size * 4;
 }
 
 CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t experts, int32_t top_k,
@@ -464,7 +550,8 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
       (fp4 && (!gate_up_scales || !down_scales)))
     return fail(CFMOE_EINVAL, "NULL argument");
   uintptr_t addresses = 0;
-  for (const void *p : {gate_up, down, hidden, static_cast<const void *>(out), static_cast<const void *>(scratch)})
+  for (const void *p : {gate_up, down, hidden, static_cast<const void *>(out), static_cast<const void *>(scratch),
+                        static_cast<const void *>(gate_up_scales), static_cast<const void *>(down_scales)})
     addresses |= reinterpret_cast<uintptr_t>(p);
   if (addresses % 16)
     return fail(CFMOE_EINVAL, "routed_experts needs 16-byte aligned weights, hidden rows, output and scratch");
@@ -484,8 +571,6 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   a.experts = experts;
   a.hidden = hidden_size;
   a.width = width;
-  a.act_stride = width;
-  a.splits = down_splits(hidden_size, width, experts, top_k, flags, tokens);
   a.act = static_cast<uint16_t *>(scratch);
   a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + act_bytes(width, a.pairs));
   a.ids64 = flags & CFMOE_IDS_INT64;
@@ -495,21 +580,24 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   const int items = a.by_pair ? a.pairs : experts;
   const unsigned list = static_cast<unsigned>((a.pairs * 2 + 15) / 16 * 16);
 
-  a.tiles = (width + kUpTiles * kUpChannels - 1) / (kUpTiles * kUpChannels);
-  const dim3 up(static_cast<unsigned>(a.tiles) * items);
-  if (fp4) hipLaunchKernelGGL(experts_up_kernel<true>, up, dim3(kThreads), list, stream, a);
-  else hipLaunchKernelGGL(experts_up_kernel<false>, up, dim3(kThreads), list, stream, a);
-  if (int rc = check_launch("experts_up")) return rc;
+  if (int rc = fp4 ? launch_rows<kUpFp4>(a, items, list, stream) : launch_rows<kUpBf16>(a, items, list, stream)) return rc;
+  if (fp4) {
+    if (int rc = launch_rows<kDownFp4>(a, items, list, stream)) return rc;
+  } else {
+    a.groups = hidden_size / kDownOutputs;
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.groups) * items), dim3(kThreads), list, stream, a);
+    };
+    if (width <= 32 * kWaves * 2) launch(experts_down_kernel<2>);
+    else if (width <= 32 * kWaves * 3) launch(experts_down_kernel<3>);
+    else if (width <= 32 * kWaves * 4) launch(experts_down_kernel<4>);
+    else launch(experts_down_kernel<8>);
+    if (int rc = check_launch("experts_down")) return rc;
+  }
 
-  a.tiles = hidden_size / (fp4 ? kFp4DownRows : kDownRows);
-  const dim3 grid(static_cast<unsigned>(a.tiles) * items * a.splits);
-  if (fp4) hipLaunchKernelGGL(experts_fp4_down_kernel, grid, dim3(kThreads), list, stream, a);
-  else hipLaunchKernelGGL(experts_down_kernel, grid, dim3(kThreads), list, stream, a);
-  if (int rc = check_launch("experts_down")) return rc;
-
-  const int64_t threads = static_cast<int64_t>(tokens) * (hidden_size / 8);
-  hipLaunchKernelGGL(experts_join_kernel, dim3(static_cast<unsigned>((threads + kThreads - 1) / kThreads)),
-                     dim3(kThreads), 0, stream, a);
+  const int64_t threads = static_cast<int64_t>(tokens) * (hidden_size / 4);
+  hipLaunchKernelGGL(experts_join_kernel, dim3(static_cast<unsigned>((threads + kJoinThreads - 1) / kJoinThreads)),
+                     dim3(kJoinThreads), 0, stream, a);
   return check_launch("experts_join");
 }
 

@@ -288,9 +288,8 @@ CFMOE_API int cfmoe_dequantise_fp4(int64_t blocks, const void *codes, const uint
  * scales. ids outside [0, E) contribute nothing; rows marked in padding uint8 [T]
  * (or NULL) read no weights and come out zero. flags: CFMOE_GELU,
  * CFMOE_IDS_INT64, CFMOE_WEIGHTS_BF16, CFMOE_FP4. H a multiple of 128, I of 16 (of
- * 32 with CFMOE_FP4), both at most 16384; E at most 4096, top_k 64, T top_k 8192.
- * Weights, hidden, out and scratch are 16-byte aligned (down_scales and
- * gate_up_scales 1). scratch: cfmoe_routed_experts_scratch_bytes of the same
+ * 32 with CFMOE_FP4), both at most 4096; E at most 4096, top_k 64, T top_k 8192.
+ * Weights, scales, hidden, out and scratch are 16-byte aligned. scratch: cfmoe_routed_experts_scratch_bytes of the same
  * arguments; calls that overlap need their own. T = 0 does nothing. */
 CFMOE_API int64_t cfmoe_routed_experts_scratch_bytes(int32_t hidden_size, int32_t width,
                                                      int32_t experts, int32_t top_k,

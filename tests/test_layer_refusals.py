@@ -89,15 +89,16 @@ def call_experts(hidden=256, width=64, experts=8, top_k=2, flags=0, gate_up=AT, 
 
 
 @pytest.mark.parametrize("arguments,words", [
-    (dict(hidden=192), "multiple of 128"), (dict(hidden=16512), "at most 16384"),
+    (dict(hidden=192), "multiple of 128"), (dict(hidden=4224), "at most 4096"),
     (dict(width=8), "multiple of 16"), (dict(width=0), "multiple of 16"),
-    (dict(width=48, flags=_ext.FP4), "of 32"), (dict(width=16400), "at most 16384"),
+    (dict(width=48, flags=_ext.FP4), "of 32"), (dict(width=4112), "at most 4096"),
     (dict(experts=0), "4096"), (dict(experts=4097), "4096"), (dict(top_k=65), "1 to 64"),
     (dict(tokens=4097), "8192"), (dict(tokens=-1), "8192"), (dict(tokens=2_000_000_000), "8192"),
     (dict(gate_up=None), "NULL"), (dict(down=None), "NULL"), (dict(x=None), "NULL"),
     (dict(out=None), "NULL"), (dict(scratch=None), "NULL"),
     (dict(flags=_ext.FP4), "NULL"), (dict(flags=_ext.FP4, gate_up_scales=AT), "NULL"),
     (dict(x=AT + 8), "16-byte"), (dict(down=AT + 2), "16-byte"), (dict(out=AT + 4), "16-byte"),
+    (dict(flags=_ext.FP4, gate_up_scales=AT + 4, down_scales=AT), "16-byte"),
 ])
 def test_routed_experts_refuses(arguments, words):
     refused(call_experts(**arguments), words)
