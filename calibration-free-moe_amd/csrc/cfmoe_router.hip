@@ -7,10 +7,13 @@
 //                   exp(l_k - l_0) / sum_e exp(l_e - l_0)         (otherwise)
 //                   times expert_scale[ids[t, k]] where it is given
 //
-// The ids are those of the exact logits. router_logits_kernel forms FP32 logits by
-// matrix instructions, and with the same operands' magnitudes a bound on how far
-// an FP32 sum can be off; router_select_kernel recomputes in FP64 those logits
-// whose order the bound leaves open.
+// The ids are those of the exact logits. A first launch forms FP32 logits by matrix
+// instructions (router_logits_kernel, router_bulk_kernel for many tokens), and with
+// the same operands' magnitudes a bound on how far an FP32 sum can be off;
+// router_select_kernel recomputes in FP64 those logits whose order the bound leaves
+// open.
+
+#include <algorithm>
 
 #include "cfmoe_device.h"
 
@@ -19,9 +22,12 @@ namespace {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTop = 64;
-constexpr int kTile = 16;             // experts, and tokens, of a tile
-constexpr int kLogitWaves = 4;        // waves that share a tile's hidden dimension
-constexpr int kSelectWaves = 4;       // tokens of a selecting workgroup
+constexpr int kTile = 16;          // experts, and tokens, of a matrix instruction
+constexpr int kSplitWaves = 16;    // waves that share a tile's hidden dimension
+constexpr int kBulkWaves = 8;      // expert tiles of a bulk workgroup
+constexpr int kBulkTokens = 32;
+constexpr int kBulkHidden = 2048;  // hidden values in LDS at a time
+constexpr int kSelectWaves = 4;    // tokens of a selecting workgroup
 constexpr int kPerLane = kMaxExperts / 64;
 
 struct RouteArgs {
@@ -30,89 +36,224 @@ struct RouteArgs {
   void *ids, *weights;
   float *logits;     // [T, E]
   float *magnitude;  // [T, expert tiles]: largest sum_h |x r| of the tile's experts
-  int hidden, experts, top_k, tokens, tiles;
+  int hidden, experts, top_k, tokens, tiles, chain;
   bool ids64, weights16, renormalise;
 };
 
 __device__ __forceinline__ u32x4 magnitudes(u32x4 v) { return v & 0x7fff7fffu; }
 
-// Workgroup = 16 experts x 16 tokens, its waves a quarter of the hidden dimension
-// each (every fourth 32-block of it).
-__global__ __launch_bounds__(64 * kLogitWaves) void router_logits_kernel(RouteArgs a) {
-  __shared__ f32x4 sums[2][kLogitWaves][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = blockIdx.x % a.tiles, token0 = blockIdx.x / a.tiles * kTile;
-  const int row = min(tile * kTile + lane % 16, a.experts - 1);
-  const int token = min(token0 + lane % 16, a.tokens - 1);
-  const u32x4 *r = reinterpret_cast<const u32x4 *>(a.router + static_cast<int64_t>(row) * a.hidden) + lane / 16;
-  const u32x4 *x = reinterpret_cast<const u32x4 *>(a.x + static_cast<int64_t>(token) * a.hidden) + lane / 16;
-  f32x4 dot = {0, 0, 0, 0}, size = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int s = wave; s < a.hidden / 32; s += kLogitWaves) {
-    const u32x4 rv = r[4 * s], xv = x[4 * s];
-    dot = mma(rv, xv, dot);
-    size = mma(magnitudes(rv), magnitudes(xv), size);
-  }
-  sums[0][wave][lane] = dot;
-  sums[1][wave][lane] = size;
-  __syncthreads();
-  if (wave) return;
-#pragma unroll
-  for (int w = 1; w < kLogitWaves; ++w) dot += sums[0][w][lane], size += sums[1][w][lane];
-  const int e0 = tile * kTile + lane / 16 * 4, t = token0 + lane % 16;
+// One tile's logits and the largest of its magnitude sums per token.
+__device__ __forceinline__ void store_logits(const RouteArgs &a, int tile, int t, f32x4 dot, f32x4 size) {
+  const int lane = threadIdx.x & 63, e0 = tile * kTile + lane / 16 * 4;
   // (fmaxf drops a NaN: a row whose magnitudes hold one has NaN logits, which the
   // selection ranks without a bound)
   float largest = fmaxf(fmaxf(size[0], size[1]), fmaxf(size[2], size[3]));
   largest = fmaxf(largest, __shfl_xor(largest, 16));
   largest = fmaxf(largest, __shfl_xor(largest, 32));
   if (t >= a.tokens) return;
-  float *out = a.logits + static_cast<int64_t>(t) * a.experts;
+  float *out = a.logits + static_cast<int64_t>(t) * a.experts + e0;
+  if (a.experts % 4 == 0) {
+    if (e0 < a.experts) *reinterpret_cast<f32x4 *>(out) = dot;
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (e0 + i < a.experts) out[e0 + i] = dot[i];
+    for (int i = 0; i < 4; ++i)
+      if (e0 + i < a.experts) out[i] = dot[i];
+  }
   if (lane < 16) a.magnitude[static_cast<int64_t>(t) * a.tiles + tile] = largest;
 }
 
-// Order of the logits as unsigned integers: -0 equals 0, NaN above all.
+// Few tiles: workgroup = 16 experts x 16 tokens, its waves every sixteenth 32 of the
+// hidden dimension.
+__global__ __launch_bounds__(64 * kSplitWaves) void router_logits_kernel(RouteArgs a) {
+  constexpr int kAhead = 4;
+  __shared__ f32x4 sums[2][kSplitWaves][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = blockIdx.x % a.tiles, token0 = blockIdx.x / a.tiles * kTile;
+  const int row = min(tile * kTile + lane % 16, a.experts - 1);
+  const int token = min(token0 + lane % 16, a.tokens - 1);
+  const u32x4 *r = reinterpret_cast<const u32x4 *>(a.router + static_cast<int64_t>(row) * a.hidden) + lane / 16;
+  const u32x4 *x = reinterpret_cast<const u32x4 *>(a.x + static_cast<int64_t>(token) * a.hidden) + lane / 16;
+  const int steps = a.hidden / 32;
+  f32x4 dot = {0, 0, 0, 0}, size = {0, 0, 0, 0};
+  for (int s = wave; s < steps; s += kAhead * kSplitWaves) {
+    u32x4 rv[kAhead], xv[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = min(s + i * kSplitWaves, steps - 1);
+      rv[i] = r[4 * at];
+      xv[i] = x[4 * at];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (s + i * kSplitWaves >= steps) break;
+      dot = mma(rv[i], xv[i], dot);
+      size = mma(magnitudes(rv[i]), magnitudes(xv[i]), size);
+    }
+  }
+  sums[0][wave][lane] = dot;
+  sums[1][wave][lane] = size;
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int w = 1; w < kSplitWaves; ++w) dot += sums[0][w][lane], size += sums[1][w][lane];
+  store_logits(a, tile, token0 + lane % 16, dot, size);
+}
+
+// Many tiles: workgroup = 32 tokens x 128 experts. The tokens' rows lie in LDS, 2048
+// values at a time, and each wave streams its 16 experts' rows past them.
+__global__ __launch_bounds__(64 * kBulkWaves) void router_bulk_kernel(RouteArgs a) {
+  constexpr int kCols = kBulkTokens / kTile, kRing = 8;
+  extern __shared__ __align__(16) uint8_t rows[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = (a.tiles + kBulkWaves - 1) / kBulkWaves;
+  const int tile = blockIdx.x % groups * kBulkWaves + wave, token0 = blockIdx.x / groups * kBulkTokens;
+  const int row = min(tile * kTile + lane % 16, a.experts - 1);
+  const u32x4 *r = reinterpret_cast<const u32x4 *>(a.router + static_cast<int64_t>(row) * a.hidden) + lane / 16;
+  f32x4 dot[kCols], size[kCols];
+#pragma unroll
+  for (int n = 0; n < kCols; ++n) dot[n] = size[n] = f32x4{0, 0, 0, 0};
+  for (int h0 = 0; h0 < a.hidden; h0 += kBulkHidden) {
+    const int length = min(kBulkHidden, a.hidden - h0), steps = length / 32;  // (a multiple of 4)
+    const int stride = length * 2 + 16;  // (equal places of 16 rows in different banks)
+    const u32x4 *rh = r + h0 / 8;
+    u32x4 ring[kRing];
+#pragma unroll
+    for (int i = 0; i < kRing; ++i) ring[i] = rh[4 * min(i, steps - 1)];
+    if (h0) __syncthreads();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kBulkTokens * length / 8; i += 64 * kBulkWaves) {
+      const int n = i / (length / 8), at = i - n * (length / 8);
+      const int token = min(token0 + n, a.tokens - 1);
+      *reinterpret_cast<u32x4 *>(rows + n * stride + at * 16) =
+          reinterpret_cast<const u32x4 *>(a.x + static_cast<int64_t>(token) * a.hidden + h0)[at];
+    }
+    __syncthreads();
+    const uint8_t *x = rows + lane % 16 * stride + lane / 16 * 16;
+    for (int s = 0; s < steps; s += kRing) {
+#pragma unroll
+      for (int i = 0; i < kRing; ++i) {
+        if (s + i < steps) {
+          const u32x4 rv = ring[i], rm = magnitudes(rv);
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) {
+            const u32x4 xv = *reinterpret_cast<const u32x4 *>(x + n * kTile * stride + (s + i) * 64);
+            dot[n] = mma(rv, xv, dot[n]);
+            size[n] = mma(rm, magnitudes(xv), size[n]);
+          }
+        }
+        ring[i] = rh[4 * min(s + i + kRing, steps - 1)];
+      }
+    }
+  }
+  if (tile < a.tiles)
+#pragma unroll
+    for (int n = 0; n < kCols; ++n) store_logits(a, tile, token0 + n * kTile + lane % 16, dot[n], size[n]);
+}
+
+// Order of the logits as unsigned integers: -0 equals 0, NaN above all; no logit's is 0.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (v != v) return ~0u;
+  const uint32_t bits = __float_as_uint(v + 0.0f);
+  return bits >> 31 ? ~bits : bits | 0x80000000u;
+}
+
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return key == ~0u ? NAN : __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
+}
+
 __device__ __forceinline__ uint64_t order_key(double v) {
   if (v != v) return ~0ull;
   const uint64_t bits = __builtin_bit_cast(uint64_t, v + 0.0);
   return bits >> 63 ? ~bits : bits | (1ull << 63);
 }
 
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) {
-    const uint64_t other = __shfl_xor(v, m);
-    v = v > other ? v : other;
-  }
-  return v;
+template <int kControl, class T>
+__device__ __forceinline__ T moved(T v) {
+  return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), kControl, 0xf, 0xf, true));
 }
 
-__device__ __forceinline__ int wave_min(int v) {
+// A wave's result in every lane: 16 lanes by lane moves (neighbours, pairs, half row
+// and row mirrored), the four rows by scalars.
+template <class T, class Op>
+__device__ __forceinline__ T wave_all(T v, Op op) {
+  v = op(v, moved<0xb1>(v));
+  v = op(v, moved<0x4e>(v));
+  v = op(v, moved<0x141>(v));
+  v = op(v, moved<0x140>(v));
+  T rows[4];
 #pragma unroll
-  for (int m = 1; m < 64; m *= 2) v = min(v, __shfl_xor(v, m));
-  return v;
+  for (int i = 0; i < 4; ++i)
+    rows[i] = __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 16 * i));
+  return op(op(rows[0], rows[1]), op(rows[2], rows[3]));
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) v = fmaxf(v, __shfl_xor(v, m));
-  return v;
+__device__ __forceinline__ float wave_sum(float v) {
+  return wave_all(v, [](float a, float b) { return a + b; });
 }
 
-template <class T>
-__device__ __forceinline__ T wave_sum(T v) {
+__device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m);
   return v;
 }
 
-// One selection: the `count` largest of the lanes' values (expert 64 j + lane),
-// largest first, ties to the lowest expert; value and expert i land in lane i.
+// Exact dot products of token t's row with two experts' (BF16 products fit FP64 with
+// bits to spare; a sum of some thousand is off by less than 2^-40 of its terms).
+__device__ __forceinline__ void exact_logits(const RouteArgs &a, int t, int first, int second, double &d0, double &d1) {
+  const int lane = threadIdx.x & 63;
+  const u32x4 *x = reinterpret_cast<const u32x4 *>(a.x + static_cast<int64_t>(t) * a.hidden);
+  const u32x4 *r0 = reinterpret_cast<const u32x4 *>(a.router + static_cast<int64_t>(first) * a.hidden);
+  const u32x4 *r1 = reinterpret_cast<const u32x4 *>(a.router + static_cast<int64_t>(second) * a.hidden);
+  d0 = d1 = 0.0;
+#pragma unroll 2
+  for (int i = lane; i < a.hidden / 8; i += 64) {
+    const u32x4 xv = x[i], v0 = r0[i], v1 = r1[i];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const double low = bf16_value(xv[w] & 0xffffu), high = __uint_as_float(xv[w] & 0xffff0000u);
+      d0 = fma(low, static_cast<double>(bf16_value(v0[w] & 0xffffu)), d0);
+      d0 = fma(high, static_cast<double>(__uint_as_float(v0[w] & 0xffff0000u)), d0);
+      d1 = fma(low, static_cast<double>(bf16_value(v1[w] & 0xffffu)), d1);
+      d1 = fma(high, static_cast<double>(__uint_as_float(v1[w] & 0xffff0000u)), d1);
+    }
+  }
+  d0 = wave_sum(d0);
+  d1 = wave_sum(d1);
+}
+
+// The `count` largest of the lanes' values (expert 64 j + lane), largest first, ties
+// to the lowest expert; the i-th lands in lane i.
 template <int kValues>
-__device__ __forceinline__ void select(const double (&v)[kValues], int experts, int count, int lane,
-                                       double &value, int &expert) {
+__device__ __forceinline__ void select(const float (&v)[kValues], int experts, int count, int lane, float &value,
+                                       int &expert) {
+  uint32_t key[kValues];
+#pragma unroll
+  for (int j = 0; j < kValues; ++j) key[j] = 64 * j + lane < experts ? order_key(v[j]) : 0;
+  uint32_t kept = 0;
+  expert = 0;
+  for (int i = 0; i < count; ++i) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int j = 1; j < kValues; ++j) best = max(best, key[j]);
+    best = wave_all(best, [](uint32_t a, uint32_t b) { return max(a, b); });
+    int at = 0;
+#pragma unroll
+    for (int j = kValues - 1; j >= 0; --j) {
+      const uint64_t equal = __ballot(key[j] == best);
+      if (equal) at = 64 * j + __builtin_ctzll(equal);
+    }
+#pragma unroll
+    for (int j = 0; j < kValues; ++j)
+      if (at == 64 * j + lane) key[j] = 0;
+    if (lane == i) kept = best, expert = at;
+  }
+  value = key_value(kept);
+}
+
+// The same by FP64 values, for rows whose order FP32 leaves open.
+template <int kValues>
+__device__ __forceinline__ void select(const double (&v)[kValues], int experts, int count, int lane, double &value,
+                                       int &expert) {
   uint64_t key[kValues];
 #pragma unroll
   for (int j = 0; j < kValues; ++j) key[j] = 64 * j + lane < experts ? order_key(v[j]) : 0;
@@ -121,12 +262,15 @@ __device__ __forceinline__ void select(const double (&v)[kValues], int experts, 
   for (int i = 0; i < count; ++i) {
     uint64_t best = 0;
 #pragma unroll
-    for (int j = 0; j < kValues; ++j) best = best > key[j] ? best : key[j];
-    best = wave_max(best);
-    int at = kMaxExperts;
+    for (int j = 0; j < kValues; ++j) best = max(best, key[j]);
 #pragma unroll
-    for (int j = kValues - 1; j >= 0; --j) at = key[j] == best ? 64 * j + lane : at;
-    at = wave_min(at);
+    for (int m = 1; m < 64; m *= 2) best = max(best, static_cast<uint64_t>(__shfl_xor(best, m)));
+    int at = 0;
+#pragma unroll
+    for (int j = kValues - 1; j >= 0; --j) {
+      const uint64_t equal = __ballot(key[j] == best);
+      if (equal) at = 64 * j + __builtin_ctzll(equal);
+    }
     double found = 0.0;
 #pragma unroll
     for (int j = 0; j < kValues; ++j)
@@ -143,64 +287,88 @@ __device__ __forceinline__ void select(const double (&v)[kValues], int experts, 
 template <int kValues>
 __global__ __launch_bounds__(64 * kSelectWaves) void router_select_kernel(RouteArgs a) {
   const int lane = threadIdx.x & 63;
-  const int t = blockIdx.x * kSelectWaves + (threadIdx.x >> 6);
+  const int t = blockIdx.x * kSelectWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (t >= a.tokens) return;
   const float *row = a.logits + static_cast<int64_t>(t) * a.experts;
-  double v[kValues];
+  float v[kValues];
 #pragma unroll
   for (int j = 0; j < kValues; ++j) v[j] = 64 * j + lane < a.experts ? row[64 * j + lane] : -INFINITY;
-  float largest = 0.0f;
-  for (int i = lane; i < a.tiles; i += 64)
-    largest = fmaxf(largest, a.magnitude[static_cast<int64_t>(t) * a.tiles + i]);
-  largest = wave_max(largest);
+  const float size = lane < a.tiles ? a.magnitude[static_cast<int64_t>(t) * a.tiles + lane] : 0.0f;
+  const float largest = wave_all(size, [](float a, float b) { return fmaxf(a, b); });
   // Each of the additions behind a logit rounds (or cuts off) by 2^-23 of a partial
-  // sum of at most `largest` at the most: 32 inside a matrix instruction, one for
-  // each instruction of a wave's chain, and the waves' own. Two logits may be off
-  // in opposite directions. (The last term covers products below the normal range.)
-  const int chain = (a.hidden / 32 + kLogitWaves - 1) / kLogitWaves;
-  const double open = 2.0 * (32 + chain + kLogitWaves) * 0x1p-23 * largest + 0x1p-110;
+  // sum of at most `largest` at the most; a term goes through at most `chain` of
+  // them. Two logits may be off in opposite directions. (The last term covers
+  // products below the normal range.)
+  const float open = 2.0f * a.chain * 0x1p-23f * largest + 0x1p-110f;
 
-  // the K + 1 largest by FP32, the smallest kept logit, and whose order is open
-  const int wanted = min(a.top_k + 1, a.experts);
-  const int most = min(wanted, 64);
-  double value;
+  // the K + 1 largest by FP32, and those whose order with a neighbour is open
+  const int wanted = min(a.top_k + 1, a.experts), most = min(wanted, 64);
+  float value32;
   int expert;
-  select<kValues>(v, a.experts, most, lane, value, expert);
-  const double cut = __shfl(value, a.top_k - 1);
-  const double next = __shfl_down(value, 1);
-  // (written so that a NaN or infinity in between counts as open)
-  bool unsure = lane + 1 < most && !(value - next > open);
-  if (most < wanted) unsure = true;  // (64 kept: what follows them was not looked at)
-  if (__ballot(unsure) != 0) {
-    // recompute every logit that lies within `open` of another that matters
-    bool contested[kValues];
+  select<kValues>(v, a.experts, most, lane, value32, expert);
+  const float next = __shfl_down(value32, 1);
+  // (written so that a NaN or infinity in between counts as open; 64 kept of more:
+  // what follows them was not looked at)
+  const bool unsure = (lane + 1 < most && !(value32 - next > open)) || most < wanted;
+  const uint64_t unsure_lanes = __ballot(unsure);
+  double value = value32;
+  if (unsure_lanes != 0) {
+    const float cut = __shfl(value32, a.top_k - 1);
+    int near = 0;  // experts that are kept or might be
 #pragma unroll
-    for (int j = 0; j < kValues; ++j) contested[j] = 64 * j + lane < a.experts && !(cut - v[j] > open);
-    const u32x4 *x = reinterpret_cast<const u32x4 *>(a.x + static_cast<int64_t>(t) * a.hidden);
-#pragma unroll
-    for (int j = 0; j < kValues; ++j) {
-      uint64_t todo = __ballot(contested[j]);
+    for (int j = 0; j < kValues; ++j)
+      near += __builtin_popcountll(__ballot(64 * j + lane < a.experts && !(cut - v[j] > open)));
+    if (near <= most && most == wanted) {
+      // All of them are at hand: the exact logits of the open ones, then each one's
+      // rank among the K + 1. (Others are further from their neighbours than either
+      // may be off, so their FP32 logits rank right among exact ones.)
+      uint64_t todo = unsure_lanes | unsure_lanes << 1;
       while (todo) {
-        const int owner = __builtin_ctzll(todo);
+        const int i = __builtin_ctzll(todo);
         todo &= todo - 1;
-        const u32x4 *r =
-            reinterpret_cast<const u32x4 *>(a.router + static_cast<int64_t>(64 * j + owner) * a.hidden);
-        double sum = 0.0;
-        for (int i = lane; i < a.hidden / 8; i += 64) {
-          const u32x4 rv = r[i], xv = x[i];
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            sum = fma(static_cast<double>(bf16_value(rv[w] & 0xffffu)),
-                      static_cast<double>(bf16_value(xv[w] & 0xffffu)), sum);
-            sum = fma(static_cast<double>(__uint_as_float(rv[w] & 0xffff0000u)),
-                      static_cast<double>(__uint_as_float(xv[w] & 0xffff0000u)), sum);
-          }
-        }
-        sum = wave_sum(sum);
-        if (lane == owner) v[j] = sum;
+        const int j = todo ? __builtin_ctzll(todo) : i;
+        todo &= todo - 1;
+        double di, dj;
+        exact_logits(a, t, __builtin_amdgcn_readlane(expert, i), __builtin_amdgcn_readlane(expert, j), di, dj);
+        if (lane == i) value = di;
+        if (lane == j) value = dj;
       }
+      const uint64_t mine = order_key(value);
+      int rank = 0;
+      for (int j = 0; j < most; ++j) {
+        const uint64_t theirs = __shfl(mine, j);
+        const int other = __builtin_amdgcn_readlane(expert, j);
+        rank += theirs > mine || (theirs == mine && other < expert);
+      }
+      double ranked = 0.0;
+      int ranked_expert = 0;
+      for (int j = 0; j < most; ++j) {
+        const int to = __builtin_amdgcn_readlane(rank, j), from = __builtin_amdgcn_readlane(expert, j);
+        const double moved_value = __shfl(value, j);
+        if (lane == to) ranked = moved_value, ranked_expert = from;
+      }
+      value = ranked;
+      expert = ranked_expert;
+    } else {
+      // more experts lie about the cut: the exact logits of all that might be kept
+      double exact[kValues];
+#pragma unroll
+      for (int j = 0; j < kValues; ++j) {
+        exact[j] = v[j];
+        uint64_t todo = __ballot(64 * j + lane < a.experts && !(cut - v[j] > open));
+        while (todo) {
+          const int i = __builtin_ctzll(todo);
+          todo &= todo - 1;
+          const int k = todo ? __builtin_ctzll(todo) : i;
+          todo &= todo - 1;
+          double di, dk;
+          exact_logits(a, t, 64 * j + i, 64 * j + k, di, dk);
+          if (lane == i) exact[j] = di;
+          if (lane == k) exact[j] = dk;
+        }
+      }
+      select<kValues>(exact, a.experts, a.top_k, lane, value, expert);
     }
-    select<kValues>(v, a.experts, a.top_k, lane, value, expert);
   }
 
   const double first = __shfl(value, 0);
@@ -267,9 +435,19 @@ CFMOE_API int cfmoe_route(int32_t hidden_size, int32_t experts, int32_t top_k, u
   a.ids64 = flags & CFMOE_IDS_INT64;
   a.weights16 = flags & CFMOE_WEIGHTS_BF16;
   a.renormalise = flags & CFMOE_RENORMALISE;
-  const int64_t groups = static_cast<int64_t>(a.tiles) * ((tokens + kTile - 1) / kTile);
-  if (groups > 0x7fffffffL / (64 * kLogitWaves)) return fail(CFMOE_EINVAL, "route has too many tokens for one launch");
-  hipLaunchKernelGGL(router_logits_kernel, dim3(static_cast<unsigned>(groups)), dim3(64 * kLogitWaves), 0, stream, a);
+  const int64_t tiles = static_cast<int64_t>(a.tiles) * ((tokens + kTile - 1) / kTile);
+  if (tiles > 0x1fffff) return fail(CFMOE_EINVAL, "route has too many tokens for one launch");
+  // 32 products inside a matrix instruction, one addition for each of a chain of
+  // them, and the waves' sums
+  if (tiles <= 1024) {
+    a.chain = 32 + (hidden_size / 32 + kSplitWaves - 1) / kSplitWaves + kSplitWaves;
+    hipLaunchKernelGGL(router_logits_kernel, dim3(static_cast<unsigned>(tiles)), dim3(64 * kSplitWaves), 0, stream, a);
+  } else {
+    a.chain = 32 + hidden_size / 32;
+    const int groups = (a.tiles + kBulkWaves - 1) / kBulkWaves * ((tokens + kBulkTokens - 1) / kBulkTokens);
+    const unsigned lds = kBulkTokens * (std::min(hidden_size, kBulkHidden) * 2 + 16);
+    hipLaunchKernelGGL(router_bulk_kernel, dim3(groups), dim3(64 * kBulkWaves), lds, stream, a);
+  }
   if (int rc = check_launch("router_logits")) return rc;
   auto select = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((tokens + kSelectWaves - 1) / kSelectWaves), dim3(64 * kSelectWaves), 0, stream, a);

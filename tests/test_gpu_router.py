@@ -118,10 +118,25 @@ def test_out_and_empty_batches():
     assert ids.shape == weights.shape == (0, 4)
 
 
-def test_large_batch_matches_its_parts():
-    x, router = rows(2500, 512, 19).to(DEVICE), rows(256, 512, 20, 0.02).to(DEVICE)
-    ids, weights = route(x, router, 8)
-    for begin in (0, 16, 1000, 2499):
-        part_ids, part = route(x[begin:begin + 37], router, 8)
-        assert torch.equal(part_ids, ids[begin:begin + 37])
-        assert torch.equal(part, weights[begin:begin + 37])
+@pytest.mark.parametrize("hidden,experts", [(512, 256), (128, 100), (2816, 130), (4096, 128)])
+def test_many_tokens(hidden, experts):
+    """The kernel of many tokens (over 1024 tiles of 16 experts and 16 tokens)."""
+    tokens = 16 * (1024 // ((experts + 15) // 16)) + 21
+    x, router = rows(tokens, hidden, 19), rows(experts, hidden, 20, 0.02)
+    x[:, :: 100] *= 20
+    router[7] = router[3]
+    check(x, router, 8)
+    check(x, router, 3, renormalise=False, ids_dtype=torch.int64)
+
+
+def test_open_order_about_the_cut():
+    """More experts than are kept lie within an FP32 sum's error of the cut."""
+    hidden, experts = 1024, 48
+    x, router = rows(40, hidden, 21), rows(experts, hidden, 22, 0.5)
+    x[:, 5] = 2.0 ** -26
+    for e in range(8, 40):
+        router[e] = router[8]
+        router[e, 5] = 1.0 + (e * 11 % 32) / 64
+    check(x, router, 12)
+    check(x, router, 1)
+    check(x, router, 48)
