@@ -8,6 +8,7 @@ fails to load, every reader call raises RuntimeError.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from collections.abc import Callable
 
@@ -222,10 +223,27 @@ def trit_plane_bytes(dims: Dims) -> int:
     return size
 
 
-def launch_on(device: torch.device, call: Callable[[int], int]) -> None:
-    """Run `call(stream)` on the tensors' device and its current stream; check its status."""
-    if torch.cuda.current_device() == device.index:
-        check(call(torch.cuda.current_stream(device).cuda_stream))
-    else:
-        with torch.cuda.device(device):
-            check(call(torch.cuda.current_stream(device).cuda_stream))
+def run(function: Callable[..., int], device: torch.device, *arguments: object) -> None:
+    """Call `function(*arguments, stream)` on `device` and its current stream; check its status."""
+    index = device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return run(function, device, *arguments)
+    # (the raw handle: a torch.cuda.Stream object costs 2 us more than the lookup)
+    status = function(*arguments, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status)
+
+
+@functools.lru_cache(maxsize=4096)
+def route_scratch_bytes(tokens: int, experts: int) -> int:
+    return library().cfmoe_route_scratch_bytes(tokens, experts)
+
+
+@functools.lru_cache(maxsize=4096)
+def routed_experts_scratch_bytes(*shape: int) -> int:
+    """Bytes for (hidden, width, experts, top_k, flags, tokens); ValueError if refused."""
+    size = library().cfmoe_routed_experts_scratch_bytes(*shape)
+    if size < 0:
+        check(-size)
+    return size

@@ -22,7 +22,6 @@ from calibration_free_moe.reader.microscale import Fp4Weights
 MAX_PAIRS = 8192  # routed (token, slot) pairs of a call, as the reader's
 
 
-@torch.no_grad()
 def routed_experts(
     hidden: Tensor,
     gate_up: Tensor | Fp4Weights,
@@ -124,10 +123,7 @@ def routed_experts(
         | (_ext.GELU if activation == "gelu_tanh" else 0)
         | (_ext.FP4 if fp4 else 0)
     )
-    lib = _ext.library()
-    size = lib.cfmoe_routed_experts_scratch_bytes(h, i, e, k, flags, tokens)
-    if size < 0:
-        _ext.check(-size)
+    size = _ext.routed_experts_scratch_bytes(h, i, e, k, flags, tokens)
     if not tokens:
         return out
     scratch = torch.empty(size, dtype=torch.uint8, device=device)
@@ -136,13 +132,11 @@ def routed_experts(
                     down.scales.data_ptr())
     else:
         pointers = (gate_up.data_ptr(), None, down.data_ptr(), None)
-    _ext.launch_on(
-        device,
-        lambda stream: lib.cfmoe_routed_experts(
-            h, i, e, k, flags, *pointers, hidden.data_ptr(), ids.data_ptr(), weights.data_ptr(),
-            None if padding is None else padding.data_ptr(), out.data_ptr(), scratch.data_ptr(),
-            tokens, stream,
-        ),
+    _ext.run(
+        _ext.library().cfmoe_routed_experts, device, h, i, e, k, flags, *pointers,
+        hidden.data_ptr(), ids.data_ptr(), weights.data_ptr(),
+        None if padding is None else padding.data_ptr(), out.data_ptr(), scratch.data_ptr(),
+        tokens,
     )
     return out
 

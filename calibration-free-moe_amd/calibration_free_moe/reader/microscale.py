@@ -56,7 +56,6 @@ class Fp4Weights:
         )
 
 
-@torch.no_grad()
 def quantise_fp4(weights: Tensor) -> Fp4Weights:
     """Quantise contiguous BF16 or FP32 weights [..., n] in one HIP launch.
 
@@ -81,30 +80,22 @@ def quantise_fp4(weights: Tensor) -> Fp4Weights:
     device = weights.device
     codes = torch.empty((*lead, n // 2), dtype=torch.uint8, device=device)
     scales = torch.empty((*lead, n // BLOCK), dtype=torch.uint8, device=device)
-    lib = _ext.library()
     flags = _ext.FP32 if weights.dtype == torch.float32 else 0
-    _ext.launch_on(
-        device,
-        lambda stream: lib.cfmoe_quantise_fp4(
-            scales.numel(), flags, weights.data_ptr(), codes.data_ptr(), scales.data_ptr(), stream
-        ),
+    _ext.run(
+        _ext.library().cfmoe_quantise_fp4, device, scales.numel(), flags, weights.data_ptr(),
+        codes.data_ptr(), scales.data_ptr(),
     )
     return Fp4Weights(codes, scales)
 
 
-@torch.no_grad()
 def dequantise_fp4(weights: Fp4Weights) -> Tensor:
     """The BF16 values [..., n] that codes and scales stand for, exactly."""
     if not weights.valid():
         raise ValueError("Expected contiguous CUDA codes [..., n / 2] and scales [..., n / 32]")
     values = torch.empty(weights.shape, dtype=torch.bfloat16, device=weights.device)
-    lib = _ext.library()
-    _ext.launch_on(
-        weights.device,
-        lambda stream: lib.cfmoe_dequantise_fp4(
-            weights.scales.numel(), weights.codes.data_ptr(), weights.scales.data_ptr(),
-            values.data_ptr(), stream,
-        ),
+    _ext.run(
+        _ext.library().cfmoe_dequantise_fp4, weights.device, weights.scales.numel(),
+        weights.codes.data_ptr(), weights.scales.data_ptr(), values.data_ptr(),
     )
     return values
 

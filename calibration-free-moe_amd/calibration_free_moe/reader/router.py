@@ -18,7 +18,6 @@ MAX_EXPERTS = 1024
 MAX_TOP_K = 64
 
 
-@torch.no_grad()
 def route(
     hidden: Tensor,
     router: Tensor,
@@ -92,17 +91,14 @@ def route(
         | (_ext.WEIGHTS_BF16 if weights_dtype == torch.bfloat16 else 0)
         | (_ext.RENORMALISE if renormalise else 0)
     )
-    lib = _ext.library()
     scratch = torch.empty(
-        lib.cfmoe_route_scratch_bytes(tokens, experts), dtype=torch.uint8, device=device
+        _ext.route_scratch_bytes(tokens, experts), dtype=torch.uint8, device=device
     )
-    _ext.launch_on(
-        device,
-        lambda stream: lib.cfmoe_route(
-            hidden.shape[1], experts, top_k, flags, hidden.data_ptr(), router.data_ptr(),
-            None if expert_scale is None else expert_scale.data_ptr(), ids.data_ptr(),
-            weights.data_ptr(), scratch.data_ptr(), tokens, stream,
-        ),
+    _ext.run(
+        _ext.library().cfmoe_route, device, hidden.shape[1], experts, top_k, flags,
+        hidden.data_ptr(), router.data_ptr(),
+        None if expert_scale is None else expert_scale.data_ptr(), ids.data_ptr(),
+        weights.data_ptr(), scratch.data_ptr(), tokens,
     )
     return ids, weights
 

@@ -34,6 +34,10 @@ constexpr int kColumns = 16;      // pairs of a matrix instruction
 constexpr int kRows = 16;         // weight rows of one
 constexpr int kDownOutputs = 64;  // outputs of a BF16 down workgroup
 constexpr int kJoinThreads = 256;
+#ifndef TOKENS_MOST
+#define TOKENS_MOST 4
+#endif
+
 struct ExpertArgs {
   const uint16_t *x;
   const void *ids, *weights;
@@ -431,6 +435,55 @@ __global__ __launch_bounds__(kThreads, kSteps <= 4 ? 4 : 2) void experts_down_ke
   }
 }
 
+// Few tokens over 4-bit rows: workgroup = 16 outputs of one token, its waves the
+// token's slots (every eighth), so that the slots' sum needs no launch of its own. An
+// expert that several tokens name is read for each of them.
+__global__ __launch_bounds__(kThreads) void experts_fp4_tokens_kernel(ExpertArgs a) {
+  constexpr int kAhead = 4;
+  __shared__ f32x4 sums[kWaves][4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = blockIdx.x / a.tiles, row = blockIdx.x % a.tiles * kRows;
+  const int blocks = a.width / 32, steps = (blocks + 3) / 4;
+  f32x4 d = {0, 0, 0, 0};
+  for (int k = wave; k < a.top_k; k += kWaves) {
+    const int pair = t * a.top_k + k;
+    const int expert = __builtin_amdgcn_readfirstlane(pair_expert(a, pair));
+    if (expert < 0) continue;
+    const int64_t row0 = static_cast<int64_t>(expert) * a.hidden + row;
+    const uint8_t *words = a.down + row0 * (a.width / 2), *scales = a.down_scales + row0 * blocks;
+    const uint8_t *act = reinterpret_cast<const uint8_t *>(a.act + static_cast<uint32_t>(pair) * a.width);
+    for (int s = 0; s < steps; s += kAhead) {
+      u32x4 word[kAhead], b[kAhead][4];
+      uint32_t scale[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        // (past the last block it comes again, cleared)
+        const uint32_t block = min(4 * (s + i) + lane / 16, blocks - 1);
+        const uint32_t own = 4 * (s + i) + lane / 16 < blocks ? ~0u : 0u;
+        word[i] = load_at<u32x4>(words, lane % 16 * (a.width / 2) + block * 16) & own;
+        scale[i] = load_at<uint8_t>(scales, lane % 16 * blocks + block) & own;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) b[i][q] = load_at<u32x4>(act, block * 64 + q * 16) & own;
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          d = mma(fp4_values(word[i][q], __uint_as_float(scale[i] << 23)), b[i][q], d);
+    }
+  }
+  // (all 16 columns are the one token's)
+  if (lane % 16 == 0) sums[wave][lane / 16] = d;
+  __syncthreads();
+  if (threadIdx.x < 4) {
+    f32x4 v = sums[0][threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v += sums[w][threadIdx.x];
+    *reinterpret_cast<u32x2 *>(a.out + (static_cast<uint32_t>(t) * a.hidden + row + threadIdx.x * 4)) =
+        u32x2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+  }
+}
+
 // Thread = four outputs of one token: its slots' partials in order.
 __global__ __launch_bounds__(kJoinThreads) void experts_join_kernel(ExpertArgs a) {
   constexpr int kAhead = 8;
@@ -581,6 +634,12 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   const unsigned list = static_cast<unsigned>((a.pairs * 2 + 15) / 16 * 16);
 
   if (int rc = fp4 ? launch_rows<kUpFp4>(a, items, list, stream) : launch_rows<kUpBf16>(a, items, list, stream)) return rc;
+  if (fp4 && a.by_pair && tokens <= TOKENS_MOST) {
+    a.tiles = hidden_size / kRows;
+    hipLaunchKernelGGL(experts_fp4_tokens_kernel, dim3(static_cast<unsigned>(a.tiles) * tokens), dim3(kThreads), 0,
+                       stream, a);
+    return check_launch("experts_down");
+  }
   if (fp4) {
     if (int rc = launch_rows<kDownFp4>(a, items, list, stream)) return rc;
   } else {
