@@ -20,6 +20,7 @@
 // router weight goes in before, so that a pair is rounded once.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "cfmoe_device.h"
 
@@ -34,10 +35,6 @@ constexpr int kColumns = 16;      // pairs of a matrix instruction
 constexpr int kRows = 16;         // weight rows of one
 constexpr int kDownOutputs = 64;  // outputs of a BF16 down workgroup
 constexpr int kJoinThreads = 256;
-#ifndef TOKENS_MOST
-#define TOKENS_MOST 4
-#endif
-
 struct ExpertArgs {
   const uint16_t *x;
   const void *ids, *weights;
@@ -79,7 +76,8 @@ __device__ __forceinline__ T load_at(const void *base, uint32_t offset) {
 // twice.) Each wave looks at a share of the pairs, its first kHeld 64s at once:
 // their loads leave together, and the list is made of what they found; only the
 // further ones of a large batch are looked at twice. `count` is known a barrier
-// before the list is.
+// before the list is. Up to 64 pairs each wave looks at all of them and makes the
+// list for itself, with no barrier.
 template <int kTeam>
 struct Pairs {
   static constexpr int kHeld = 4;
@@ -91,14 +89,17 @@ struct Pairs {
 
   __device__ __forceinline__ void find(const ExpertArgs &a, int z, int *counts) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    expert = __builtin_amdgcn_readfirstlane(a.by_pair ? pair_expert(a, z) : z);
     count = 0;
-    begin = z;
-    if (expert < 0) return;
-    if (alone(a)) {
-      count = 1;
+    if (a.pairs <= 64) {
+      const int e = lane < a.pairs ? pair_expert(a, lane) : -1;
+      expert = a.by_pair ? __builtin_amdgcn_readlane(e, z) : z;
+      found[0] = __ballot(e == expert);
+      if (alone(a)) found[0] = 1ull << z;
+      if (expert >= 0 && !(a.by_pair && found[0] & ((1ull << z) - 1))) count = __builtin_popcountll(found[0]);
       return;
     }
+    expert = __builtin_amdgcn_readfirstlane(a.by_pair ? pair_expert(a, z) : z);
+    if (expert < 0) return;
     const int share = (a.pairs + 64 * kTeam - 1) / (64 * kTeam) * 64;
     begin = min(wave * share, a.pairs);
     end = min(begin + share, a.pairs);
@@ -137,10 +138,11 @@ struct Pairs {
   // The list, ascending, into LDS.
   __device__ __forceinline__ void list(const ExpertArgs &a, uint16_t *out) const {
     const int lane = threadIdx.x & 63;
-    if (alone(a)) {
-      if (threadIdx.x == 0) out[0] = begin;
+    const uint64_t below = (1ull << lane) - 1;
+    if (a.pairs <= 64) {
+      // (every wave writes the same list, and reads what it wrote itself)
+      if (found[0] >> lane & 1) out[__builtin_popcountll(found[0] & below)] = lane;
     } else {
-      const uint64_t below = (1ull << lane) - 1;
       int to = at;
 #pragma unroll
       for (int j = 0; j < kHeld; ++j) {
@@ -152,8 +154,8 @@ struct Pairs {
         if (more >> lane & 1) out[to + __builtin_popcountll(more & below)] = p;
         to += __builtin_popcountll(more);
       }
+      __syncthreads();
     }
-    __syncthreads();
   }
 
  private:
@@ -328,6 +330,7 @@ __global__ __launch_bounds__(kThreads, kMaxCols <= 2 && kSteps <= 8 ? 4 : 2) voi
     const int left = count - base;
     auto ready = [&] {
       if (base == 0) pairs.list(a, list);
+      if (kFp4 && base == 0 && a.pairs <= 64) __syncthreads();  // the scales
     };
     if (kMaxCols >= 4 && left > 2 * kColumns) {
       if constexpr (kMaxCols >= 4)
@@ -358,11 +361,120 @@ __device__ __forceinline__ void turn(const u32x2 (&rows)[8], u32x4 (&turned)[4])
   }
 }
 
-// Workgroup = 64 outputs of one expert, the waves an eighth of its channels each
-// (kSteps products of 32 at most; wider layers take several chunks). The weights
-// stay in registers for all of the expert's pairs, 16 at a time.
-template <int kSteps>
-__global__ __launch_bounds__(kThreads, kSteps <= 4 ? 4 : 2) void experts_down_kernel(ExpertArgs a) {
+// How the layer's 32-channel steps, every eighth to a wave, meet kSteps of them.
+enum Steps {
+  kExact,    // kSteps for each wave
+  kRagged,   // some waves one fewer: a step past the last repeats it, every bit cleared
+  kHalfStep  // and the last step is 16 channels: its second half repeats the first, cleared
+};
+
+template <Steps kMode>
+struct DownLane {
+  uint32_t row_bytes, channel, row;  // the lane's channel and row from a step's start on
+  int steps;
+  bool half;
+
+  __device__ __forceinline__ explicit DownLane(const ExpertArgs &a)
+      : row_bytes(2 * a.hidden), steps((a.width + 31) / 32) {
+    const int lane = threadIdx.x & 63;
+    half = lane >= 32;
+    channel = lane / 16 * 8;
+    row = channel * row_bytes + lane % 16 * 8;
+  }
+  __device__ __forceinline__ int at(int step) const { return kMode == kExact ? step : min(step, steps - 1); }
+  __device__ __forceinline__ bool short_of(int step) const { return kMode == kHalfStep && at(step) == steps - 1 && half; }
+  template <class T>
+  __device__ __forceinline__ T own(T v, int step) const {
+    if (kMode == kExact) return v;
+    return v & (step < steps && !short_of(step) ? ~0u : 0u);
+  }
+  __device__ __forceinline__ u32x4 vector(const ExpertArgs &a, uint32_t pair, int step) const {
+    const uint32_t offset = (pair * a.width + channel) * 2;
+    return own(load_at<u32x4>(reinterpret_cast<const uint8_t *>(a.act) + 64 * at(step),
+                              short_of(step) ? offset - 32 : offset), step);
+  }
+  __device__ __forceinline__ void rows(u32x2 (&to)[8], const uint8_t *down, int step) const {
+    const uint8_t *from = down + static_cast<int64_t>(32 * at(step)) * row_bytes;
+    const uint32_t offset = short_of(step) ? row - 16 * row_bytes : row;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) to[i] = load_at<u32x2>(from + i * row_bytes, offset);
+  }
+};
+
+// Workgroup = `share` x 64 outputs of one expert, the waves an eighth of its channels
+// each (kSteps products of 32 at most; wider layers take several chunks), 16 pairs at
+// a time. The pairs' vectors stay in registers; a step's rows are loaded for the next
+// 64 outputs as soon as they are turned.
+template <int kSteps, Steps kMode>
+__global__ __launch_bounds__(kThreads, kSteps <= 3 ? 4 : 2) void experts_down_kernel(ExpertArgs a) {
+  __shared__ f32x4 sums[2 * kWaves * 4 * 64];
+  __shared__ int counts[kWaves];
+  extern __shared__ uint16_t list[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Pairs<kWaves> pairs;
+  pairs.find(a, blockIdx.x / a.groups, counts);
+  const int count = pairs.count;
+  if (count == 0) return;
+  const int first = blockIdx.x % a.groups * a.share, rounds = min(a.share, a.tiles - first);
+  const DownLane<kMode> place(a);
+  const uint8_t *down =
+      a.down + (static_cast<int64_t>(pairs.expert) * a.width * a.hidden + first * kDownOutputs) * 2;
+  for (int base = 0; base < count; base += kColumns) {
+    for (int chunk = 0; chunk < place.steps; chunk += kWaves * kSteps) {
+      auto step = [&](int s) { return chunk + s * kWaves + wave; };
+      u32x2 rows[kSteps][8];
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) place.rows(rows[s], down, step(s));
+      if (base == 0 && chunk == 0) pairs.list(a, list);
+      const int column = base + lane % 16;
+      const uint32_t pair = list[min(column, count - 1)];
+      u32x4 b[kSteps];
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) b[s] = place.vector(a, pair, step(s));
+      auto round = [&](int r, auto more) {
+        f32x4 d[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          u32x4 w[4];
+          // (cleared rows: what they hold must not meet a cleared vector as 0 x infinity)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) rows[s][i] = place.own(rows[s][i], step(s));
+          turn(rows[s], w);
+          if (decltype(more)::value) place.rows(rows[s], down + (r + 1) * (2 * kDownOutputs), step(s));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[j] = mma(w[j], b[s], d[j]);
+        }
+        // a lane holds outputs 16 g + 4 i + j of its pair, g = l / 16; the sums alternate
+        // between two buffers, and the waves' two halves in adding them up
+        f32x4 *in = sums + (r & 1) * (kWaves * 4 * 64);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) in[(wave * 4 + i) * 64 + lane] = f32x4{d[0][i], d[1][i], d[2][i], d[3][i]};
+        __syncthreads();
+        if ((wave ^ (r & 1) * 4) < 4) {
+          const int i = wave % 4;
+          f32x4 v = in[i * 64 + lane];
+#pragma unroll
+          for (int k = 1; k < kWaves; ++k) v += in[(k * 4 + i) * 64 + lane];
+          if (column < count) {
+            f32x4 *out = reinterpret_cast<f32x4 *>(
+                a.partial + (pair * a.hidden + (first + r) * kDownOutputs + lane / 16 * 16 + i * 4));
+            *out = chunk ? *out + v : v;
+          }
+        }
+      };
+      for (int r = 0; r + 1 < rounds; ++r) round(r, std::true_type{});
+      round(rounds - 1, std::false_type{});
+      __syncthreads();
+    }
+  }
+}
+
+// Many pairs an expert: workgroup = 64 outputs of one expert, whose weights stay in
+// registers for all of its pairs, 16 at a time.
+template <int kSteps, Steps kMode>
+__global__ __launch_bounds__(kThreads, kSteps <= 3 ? 4 : 2) void experts_down_many_kernel(ExpertArgs a) {
   __shared__ f32x4 sums[kWaves * 4 * 64];
   __shared__ int counts[kWaves];
   extern __shared__ uint16_t list[];
@@ -372,41 +484,25 @@ __global__ __launch_bounds__(kThreads, kSteps <= 4 ? 4 : 2) void experts_down_ke
   const int count = pairs.count, expert = pairs.expert;
   if (count == 0) return;
   const int row0 = blockIdx.x % a.groups * kDownOutputs;
-  const int row_bytes = 2 * a.hidden, steps = (a.width + 31) / 32;
+  const DownLane<kMode> place(a);
   const uint8_t *down = a.down + (static_cast<int64_t>(expert) * a.width * a.hidden + row0) * 2;
-  const uint32_t lane_channel = lane / 16 * 8, lane_row = lane_channel * row_bytes + lane % 16 * 8;
-  // the last 32 channels may be 16: their second half repeats the first, cleared
-  const bool half = a.width % 32 != 0 && lane >= 32;
-  const uint32_t last_channel = half ? lane_channel - 16 : lane_channel;
-  const uint32_t last_row = last_channel * row_bytes + lane % 16 * 8;
-  for (int chunk = 0; chunk < steps; chunk += kWaves * kSteps) {
-    // the wave's products are every eighth 32 channels; one past the last repeats it
-    // with every bit cleared
+  for (int chunk = 0; chunk < place.steps; chunk += kWaves * kSteps) {
     u32x4 w[kSteps][4];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const int step = min(chunk + s * kWaves + wave, steps - 1);
-      const bool own = chunk + s * kWaves + wave < steps && !(step == steps - 1 && half);
-      const uint8_t *channel = down + static_cast<int64_t>(32 * step) * row_bytes;
-      const uint32_t offset = step == steps - 1 ? last_row : lane_row;
+      const int step = chunk + s * kWaves + wave;
       u32x2 rows[8];
+      place.rows(rows, down, step);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        rows[i] = *reinterpret_cast<const u32x2 *>(channel + i * row_bytes + offset) & (own ? ~0u : 0u);
+      for (int i = 0; i < 8; ++i) rows[i] = place.own(rows[i], step);
       turn(rows, w[s]);
     }
     if (chunk == 0) pairs.list(a, list);
     for (int base = 0; base < count; base += kColumns) {
       const uint32_t pair = list[min(base + lane % 16, count - 1)];
-      const uint8_t *act = reinterpret_cast<const uint8_t *>(a.act);
       u32x4 b[kSteps];
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int step = min(chunk + s * kWaves + wave, steps - 1);
-        const bool own = chunk + s * kWaves + wave < steps && !(step == steps - 1 && half);
-        const uint32_t offset = (pair * a.width + (step == steps - 1 ? last_channel : lane_channel)) * 2;
-        b[s] = *reinterpret_cast<const u32x4 *>(act + 64 * step + offset) & (own ? ~0u : 0u);
-      }
+      for (int s = 0; s < kSteps; ++s) b[s] = place.vector(a, pair, chunk + s * kWaves + wave);
       f32x4 d[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j] = f32x4{0, 0, 0, 0};
@@ -544,6 +640,17 @@ int64_t act_bytes(int width, int pairs) {
   return static_cast<int64_t>(pairs) * width * 2;  // (a row is a multiple of 32 bytes)
 }
 
+template <int kSteps>
+auto down_kernel(bool many, Steps mode) {
+  if (many)
+    return mode == kExact    ? experts_down_many_kernel<kSteps, kExact>
+           : mode == kRagged ? experts_down_many_kernel<kSteps, kRagged>
+                             : experts_down_many_kernel<kSteps, kHalfStep>;
+  return mode == kExact    ? experts_down_kernel<kSteps, kExact>
+         : mode == kRagged ? experts_down_kernel<kSteps, kRagged>
+                           : experts_down_kernel<kSteps, kHalfStep>;
+}
+
 template <Product kProduct, int kSteps>
 auto rows_kernel(bool full, bool wide) {
   // (registers: 4 x 16 pairs beside eight steps, 2 x 16 beside 12, or 16 in 4 bits)
@@ -634,7 +741,7 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   const unsigned list = static_cast<unsigned>((a.pairs * 2 + 15) / 16 * 16);
 
   if (int rc = fp4 ? launch_rows<kUpFp4>(a, items, list, stream) : launch_rows<kUpBf16>(a, items, list, stream)) return rc;
-  if (fp4 && a.by_pair && tokens <= TOKENS_MOST) {
+  if (fp4 && a.by_pair && tokens <= 4) {
     a.tiles = hidden_size / kRows;
     hipLaunchKernelGGL(experts_fp4_tokens_kernel, dim3(static_cast<unsigned>(a.tiles) * tokens), dim3(kThreads), 0,
                        stream, a);
@@ -643,14 +750,19 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   if (fp4) {
     if (int rc = launch_rows<kDownFp4>(a, items, list, stream)) return rc;
   } else {
-    a.groups = hidden_size / kDownOutputs;
-    auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.groups) * items), dim3(kThreads), list, stream, a);
-    };
-    if (width <= 32 * kWaves * 2) launch(experts_down_kernel<2>);
-    else if (width <= 32 * kWaves * 3) launch(experts_down_kernel<3>);
-    else if (width <= 32 * kWaves * 4) launch(experts_down_kernel<4>);
-    else launch(experts_down_kernel<8>);
+    a.tiles = hidden_size / kDownOutputs;
+    a.share = 1;
+    const bool many = a.pairs >= 12 * experts;
+    while (!many && static_cast<int64_t>(items) * a.tiles / (2 * a.share) >= 256 && a.share < 4) a.share *= 2;
+    a.groups = (a.tiles + a.share - 1) / a.share;
+    const int steps = (width + 31) / 32, each = (steps + kWaves - 1) / kWaves;
+    const int held = each <= 2 ? 2 : each <= 4 ? each : 8;
+    const Steps mode = width % 32 ? kHalfStep : steps % (kWaves * held) ? kRagged : kExact;
+    const auto kernel = held == 2   ? down_kernel<2>(many, mode)
+                        : held == 3 ? down_kernel<3>(many, mode)
+                        : held == 4 ? down_kernel<4>(many, mode)
+                                    : down_kernel<8>(many, mode);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.groups) * items), dim3(kThreads), list, stream, a);
     if (int rc = check_launch("experts_down")) return rc;
   }
 

@@ -13,18 +13,19 @@
 // router_select_kernel recomputes in FP64 those logits whose order the bound leaves
 // open.
 
-#include <algorithm>
-
 #include "cfmoe_device.h"
 
 namespace cfmoe {
 namespace {
 
+#ifndef BULK
+#define BULK 1024
+#endif
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTop = 64;
 constexpr int kTile = 16;          // experts, and tokens, of a matrix instruction
 constexpr int kSplitWaves = 16;    // waves that share a tile's hidden dimension
-constexpr int kBulkWaves = 8;      // expert tiles of a bulk workgroup
+constexpr int kBulkWaves = 16;     // of a bulk workgroup, two to an expert tile
 constexpr int kBulkTokens = 32;
 constexpr int kBulkHidden = 2048;  // hidden values in LDS at a time
 constexpr int kSelectWaves = 4;    // tokens of a selecting workgroup
@@ -42,8 +43,10 @@ struct RouteArgs {
 
 __device__ __forceinline__ u32x4 magnitudes(u32x4 v) { return v & 0x7fff7fffu; }
 
-// One tile's logits and the largest of its magnitude sums per token.
-__device__ __forceinline__ void store_logits(const RouteArgs &a, int tile, int t, f32x4 dot, f32x4 size) {
+// One tile's logits and the largest of its magnitude sums, for token t of `logits` and
+// `magnitude`.
+__device__ __forceinline__ void store_logits(const RouteArgs &a, float *logits, float *magnitude, int tile, int t,
+                                             f32x4 dot, f32x4 size) {
   const int lane = threadIdx.x & 63, e0 = tile * kTile + lane / 16 * 4;
   // (fmaxf drops a NaN: a row whose magnitudes hold one has NaN logits, which the
   // selection ranks without a bound)
@@ -51,7 +54,7 @@ __device__ __forceinline__ void store_logits(const RouteArgs &a, int tile, int t
   largest = fmaxf(largest, __shfl_xor(largest, 16));
   largest = fmaxf(largest, __shfl_xor(largest, 32));
   if (t >= a.tokens) return;
-  float *out = a.logits + static_cast<int64_t>(t) * a.experts + e0;
+  float *out = logits + static_cast<int64_t>(t) * a.experts + e0;
   if (a.experts % 4 == 0) {
     if (e0 < a.experts) *reinterpret_cast<f32x4 *>(out) = dot;
   } else {
@@ -59,13 +62,34 @@ __device__ __forceinline__ void store_logits(const RouteArgs &a, int tile, int t
     for (int i = 0; i < 4; ++i)
       if (e0 + i < a.experts) out[i] = dot[i];
   }
-  if (lane < 16) a.magnitude[static_cast<int64_t>(t) * a.tiles + tile] = largest;
+  if (lane < 16) magnitude[static_cast<int64_t>(t) * a.tiles + tile] = largest;
+}
+
+// The products of steps first, first + stride, .. of a tile's 32-blocks of the hidden
+// dimension, four loads ahead.
+__device__ __forceinline__ void accumulate(const u32x4 *r, const u32x4 *x, int first, int stride, int steps, f32x4 &dot,
+                                           f32x4 &size) {
+  constexpr int kAhead = 4;
+  for (int s = first; s < steps; s += kAhead * stride) {
+    u32x4 rv[kAhead], xv[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = min(s + i * stride, steps - 1);
+      rv[i] = r[4 * at];
+      xv[i] = x[4 * at];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (s + i * stride >= steps) break;
+      dot = mma(rv[i], xv[i], dot);
+      size = mma(magnitudes(rv[i]), magnitudes(xv[i]), size);
+    }
+  }
 }
 
 // Few tiles: workgroup = 16 experts x 16 tokens, its waves every sixteenth 32 of the
 // hidden dimension.
 __global__ __launch_bounds__(64 * kSplitWaves) void router_logits_kernel(RouteArgs a) {
-  constexpr int kAhead = 4;
   __shared__ f32x4 sums[2][kSplitWaves][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = blockIdx.x % a.tiles, token0 = blockIdx.x / a.tiles * kTile;
@@ -73,81 +97,89 @@ __global__ __launch_bounds__(64 * kSplitWaves) void router_logits_kernel(RouteAr
   const int token = min(token0 + lane % 16, a.tokens - 1);
   const u32x4 *r = reinterpret_cast<const u32x4 *>(a.router + static_cast<int64_t>(row) * a.hidden) + lane / 16;
   const u32x4 *x = reinterpret_cast<const u32x4 *>(a.x + static_cast<int64_t>(token) * a.hidden) + lane / 16;
-  const int steps = a.hidden / 32;
   f32x4 dot = {0, 0, 0, 0}, size = {0, 0, 0, 0};
-  for (int s = wave; s < steps; s += kAhead * kSplitWaves) {
-    u32x4 rv[kAhead], xv[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int at = min(s + i * kSplitWaves, steps - 1);
-      rv[i] = r[4 * at];
-      xv[i] = x[4 * at];
-    }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (s + i * kSplitWaves >= steps) break;
-      dot = mma(rv[i], xv[i], dot);
-      size = mma(magnitudes(rv[i]), magnitudes(xv[i]), size);
-    }
-  }
+  accumulate(r, x, wave, kSplitWaves, a.hidden / 32, dot, size);
   sums[0][wave][lane] = dot;
   sums[1][wave][lane] = size;
   __syncthreads();
   if (wave) return;
 #pragma unroll
   for (int w = 1; w < kSplitWaves; ++w) dot += sums[0][w][lane], size += sums[1][w][lane];
-  store_logits(a, tile, token0 + lane % 16, dot, size);
+  store_logits(a, a.logits, a.magnitude, tile, token0 + lane % 16, dot, size);
 }
 
-// Many tiles: workgroup = 32 tokens x 128 experts. The tokens' rows lie in LDS, 2048
-// values at a time, and each wave streams its 16 experts' rows past them.
-__global__ __launch_bounds__(64 * kBulkWaves) void router_bulk_kernel(RouteArgs a) {
-  constexpr int kCols = kBulkTokens / kTile, kRing = 8;
-  extern __shared__ __align__(16) uint8_t rows[];
+// Many tiles: workgroup = 32 tokens x 128 experts, two waves to 16 of the experts, each
+// with half of the hidden dimension. The tokens' rows pass through LDS, 256 values of
+// either half a stage; the loads of all 2048 of a span leave at once and each stage is
+// written when its turn comes, so that only the first is waited for. Each wave streams
+// its experts' rows past them.
+__global__ __launch_bounds__(64 * kBulkWaves, 4) void router_bulk_kernel(RouteArgs a) {
+  constexpr int kCols = kBulkTokens / kTile, kStage = 8, kStages = kBulkHidden / 64 / kStage;
+  constexpr int kUnits = kStage * 4;                                   // 16 bytes of a half row's stage
+  constexpr int kPart = kBulkTokens * 2 * kUnits / (64 * kBulkWaves);  // of a stage a thread brings
+  constexpr int kStride = 2 * kUnits * 16 + 16;  // (equal places of 16 rows in different banks)
+  constexpr int kGroup = kBulkWaves / 2;
+  __shared__ __align__(16) uint8_t rows[2][kBulkTokens * kStride];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int groups = (a.tiles + kBulkWaves - 1) / kBulkWaves;
-  const int tile = blockIdx.x % groups * kBulkWaves + wave, token0 = blockIdx.x / groups * kBulkTokens;
-  const int row = min(tile * kTile + lane % 16, a.experts - 1);
-  const u32x4 *r = reinterpret_cast<const u32x4 *>(a.router + static_cast<int64_t>(row) * a.hidden) + lane / 16;
+  const int groups = (a.tiles + kGroup - 1) / kGroup, half = wave / kGroup;
+  const int tile = blockIdx.x % groups * kGroup + wave % kGroup, token0 = blockIdx.x / groups * kBulkTokens;
+  const uint32_t lane_row = min(tile * kTile + lane % 16, a.experts - 1) * a.hidden * 2 + lane / 16 * 16;
   f32x4 dot[kCols], size[kCols];
 #pragma unroll
   for (int n = 0; n < kCols; ++n) dot[n] = size[n] = f32x4{0, 0, 0, 0};
   for (int h0 = 0; h0 < a.hidden; h0 += kBulkHidden) {
-    const int length = min(kBulkHidden, a.hidden - h0), steps = length / 32;  // (a multiple of 4)
-    const int stride = length * 2 + 16;  // (equal places of 16 rows in different banks)
-    const u32x4 *rh = r + h0 / 8;
-    u32x4 ring[kRing];
+    const int steps = min(kBulkHidden, a.hidden - h0) / 64;  // of a half
+    const uint8_t *r = reinterpret_cast<const uint8_t *>(a.router) + (h0 + half * steps * 32) * 2;
+    u32x4 brought[kStages][kPart], ring[kStage];
 #pragma unroll
-    for (int i = 0; i < kRing; ++i) ring[i] = rh[4 * min(i, steps - 1)];
-    if (h0) __syncthreads();
-#pragma unroll 4
-    for (int i = threadIdx.x; i < kBulkTokens * length / 8; i += 64 * kBulkWaves) {
-      const int n = i / (length / 8), at = i - n * (length / 8);
-      const int token = min(token0 + n, a.tokens - 1);
-      *reinterpret_cast<u32x4 *>(rows + n * stride + at * 16) =
-          reinterpret_cast<const u32x4 *>(a.x + static_cast<int64_t>(token) * a.hidden + h0)[at];
-    }
-    __syncthreads();
-    const uint8_t *x = rows + lane % 16 * stride + lane / 16 * 16;
-    for (int s = 0; s < steps; s += kRing) {
+    for (int i = 0; i < kStage; ++i) ring[i] = *reinterpret_cast<const u32x4 *>(r + 64 * min(i, steps - 1) + lane_row);
 #pragma unroll
-      for (int i = 0; i < kRing; ++i) {
-        if (s + i < steps) {
-          const u32x4 rv = ring[i], rm = magnitudes(rv);
+    for (int c = 0; c < kStages; ++c)
 #pragma unroll
-          for (int n = 0; n < kCols; ++n) {
-            const u32x4 xv = *reinterpret_cast<const u32x4 *>(x + n * kTile * stride + (s + i) * 64);
-            dot[n] = mma(rv, xv, dot[n]);
-            size[n] = mma(rm, magnitudes(xv), size[n]);
-          }
+      for (int j = 0; j < kPart; ++j) {
+        const int i = threadIdx.x + j * 64 * kBulkWaves, token = min(token0 + i / (2 * kUnits), a.tokens - 1);
+        // (past the half its end comes again: not multiplied)
+        const int at = i / kUnits % 2 * steps * 4 + min(c * kUnits + i % kUnits, steps * 4 - 1);
+        brought[c][j] = reinterpret_cast<const u32x4 *>(a.x + static_cast<int64_t>(token) * a.hidden + h0)[at];
+      }
+#pragma unroll
+    for (int c = 0; c < kStages; ++c) {
+      if (c * kStage >= steps) break;
+#pragma unroll
+      for (int j = 0; j < kPart; ++j) {
+        const int i = threadIdx.x + j * 64 * kBulkWaves;
+        *reinterpret_cast<u32x4 *>(rows[c & 1] + i / (2 * kUnits) * kStride + i % (2 * kUnits) * 16) = brought[c][j];
+      }
+      // (two buffers: the one written next was read before this barrier)
+      __syncthreads();
+      const uint8_t *x = rows[c & 1] + lane % 16 * kStride + half * kUnits * 16 + lane / 16 * 16;
+#pragma unroll
+      for (int i = 0; i < kStage; ++i) {
+        // (a step past the half is multiplied by cleared weights: no branch splits the
+        // stage's reads)
+        const u32x4 rv = ring[i] & (c * kStage + i < steps ? ~0u : 0u), rm = magnitudes(rv);
+        ring[i] = *reinterpret_cast<const u32x4 *>(r + 64 * min((c + 1) * kStage + i, steps - 1) + lane_row);
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
+          const u32x4 xv = *reinterpret_cast<const u32x4 *>(x + n * kTile * kStride + i * 64);
+          dot[n] = mma(rv, xv, dot[n]);
+          size[n] = mma(rm, magnitudes(xv), size[n]);
         }
-        ring[i] = rh[4 * min(s + i + kRing, steps - 1)];
       }
     }
+    __syncthreads();
   }
-  if (tile < a.tiles)
+  // the halves' sums
+  f32x4 *other = reinterpret_cast<f32x4 *>(rows[0]) + (wave % kGroup * 2 * kCols) * 64 + lane;
+  if (half)
 #pragma unroll
-    for (int n = 0; n < kCols; ++n) store_logits(a, tile, token0 + n * kTile + lane % 16, dot[n], size[n]);
+    for (int n = 0; n < kCols; ++n) other[2 * n * 64] = dot[n], other[(2 * n + 1) * 64] = size[n];
+  __syncthreads();
+  if (half || tile >= a.tiles) return;
+#pragma unroll
+  for (int n = 0; n < kCols; ++n)
+    store_logits(a, a.logits, a.magnitude, tile, token0 + n * kTile + lane % 16, dot[n] + other[2 * n * 64],
+                 size[n] + other[(2 * n + 1) * 64]);
 }
 
 // Order of the logits as unsigned integers: -0 equals 0, NaN above all; no logit's is 0.
@@ -283,17 +315,14 @@ __device__ __forceinline__ void select(const double (&v)[kValues], int experts, 
   }
 }
 
-// Wave = one token.
+// A wave's token t, by its logits `row` and the tiles' magnitudes.
 template <int kValues>
-__global__ __launch_bounds__(64 * kSelectWaves) void router_select_kernel(RouteArgs a) {
+__device__ __forceinline__ void select_token(const RouteArgs &a, int t, const float *row, const float *magnitude) {
   const int lane = threadIdx.x & 63;
-  const int t = blockIdx.x * kSelectWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (t >= a.tokens) return;
-  const float *row = a.logits + static_cast<int64_t>(t) * a.experts;
   float v[kValues];
 #pragma unroll
   for (int j = 0; j < kValues; ++j) v[j] = 64 * j + lane < a.experts ? row[64 * j + lane] : -INFINITY;
-  const float size = lane < a.tiles ? a.magnitude[static_cast<int64_t>(t) * a.tiles + lane] : 0.0f;
+  const float size = lane < a.tiles ? magnitude[lane] : 0.0f;
   const float largest = wave_all(size, [](float a, float b) { return fmaxf(a, b); });
   // Each of the additions behind a logit rounds (or cuts off) by 2^-23 of a partial
   // sum of at most `largest` at the most; a term goes through at most `chain` of
@@ -393,6 +422,15 @@ __global__ __launch_bounds__(64 * kSelectWaves) void router_select_kernel(RouteA
   else static_cast<float *>(a.weights)[at] = weight;
 }
 
+// Wave = one token.
+template <int kValues>
+__global__ __launch_bounds__(64 * kSelectWaves) void router_select_kernel(RouteArgs a) {
+  const int t = blockIdx.x * kSelectWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (t < a.tokens)
+    select_token<kValues>(a, t, a.logits + static_cast<int64_t>(t) * a.experts,
+                          a.magnitude + static_cast<int64_t>(t) * a.tiles);
+}
+
 }  // namespace
 }  // namespace cfmoe
 
@@ -439,14 +477,13 @@ CFMOE_API int cfmoe_route(int32_t hidden_size, int32_t experts, int32_t top_k, u
   if (tiles > 0x1fffff) return fail(CFMOE_EINVAL, "route has too many tokens for one launch");
   // 32 products inside a matrix instruction, one addition for each of a chain of
   // them, and the waves' sums
-  if (tiles <= 1024) {
+  if (tiles <= BULK) {
     a.chain = 32 + (hidden_size / 32 + kSplitWaves - 1) / kSplitWaves + kSplitWaves;
     hipLaunchKernelGGL(router_logits_kernel, dim3(static_cast<unsigned>(tiles)), dim3(64 * kSplitWaves), 0, stream, a);
   } else {
     a.chain = 32 + hidden_size / 32;
-    const int groups = (a.tiles + kBulkWaves - 1) / kBulkWaves * ((tokens + kBulkTokens - 1) / kBulkTokens);
-    const unsigned lds = kBulkTokens * (std::min(hidden_size, kBulkHidden) * 2 + 16);
-    hipLaunchKernelGGL(router_bulk_kernel, dim3(groups), dim3(64 * kBulkWaves), lds, stream, a);
+    const int groups = (a.tiles + kBulkWaves / 2 - 1) / (kBulkWaves / 2) * ((tokens + kBulkTokens - 1) / kBulkTokens);
+    hipLaunchKernelGGL(router_bulk_kernel, dim3(groups), dim3(64 * kBulkWaves), 0, stream, a);
   }
   if (int rc = check_launch("router_logits")) return rc;
   auto select = [&](auto kernel) {
