@@ -35,6 +35,12 @@ constexpr int kColumns = 16;      // pairs of a matrix instruction
 constexpr int kRows = 16;         // weight rows of one
 constexpr int kDownOutputs = 64;  // outputs of a BF16 down workgroup
 constexpr int kJoinThreads = 256;
+#ifndef WIDE
+#define WIDE 12
+#endif
+#ifndef RUN
+#define RUN 32
+#endif
 struct ExpertArgs {
   const uint16_t *x;
   const void *ids, *weights;
@@ -49,6 +55,8 @@ struct ExpertArgs {
   int share;    // row tiles of a workgroup
   int splits;   // waves that share a row's products (experts_rows_kernel)
   bool ids64, weights16, gelu, by_pair;
+  const struct Run *runs;   // of the sorted pairs, or NULL
+  const uint16_t *sorted;
 };
 
 __device__ __forceinline__ int pair_expert(const ExpertArgs &a, int pair) {
@@ -70,97 +78,110 @@ __device__ __forceinline__ T load_at(const void *base, uint32_t offset) {
   return *reinterpret_cast<const T *>(static_cast<const uint8_t *>(base) + offset);
 }
 
-// The pairs of one item's expert. With by_pair the items are the pairs, and an
-// expert's first pair takes all of them: the others' items get none. (A single
-// token's pairs are left apart: its experts differ, or one named twice is read
-// twice.) Each wave looks at a share of the pairs, its first kHeld 64s at once:
-// their loads leave together, and the list is made of what they found; only the
-// further ones of a large batch are looked at twice. `count` is known a barrier
-// before the list is. Up to 64 pairs each wave looks at all of them and makes the
-// list for itself, with no barrier.
-template <int kTeam>
+// Some pairs of one expert: the item of a workgroup. Up to 64 pairs each wave looks at
+// all of the batch's itself: an item is a pair (by_pair) or an expert, has all of the
+// expert's pairs, and of the pairs' items only an expert's first has any. (A single
+// token's pairs are left apart: its experts differ, or one named twice is read twice.)
+// Larger batches are sorted by a launch of their own, whose items are runs of at most
+// kMaxRun pairs: an expert that many tokens share takes several workgroups, one behind
+// the other on its rows.
+constexpr int kMaxRun = 64;
+
+struct Run {
+  int32_t expert, begin, count, unused;
+};
+
 struct Pairs {
-  static constexpr int kHeld = 4;
   int expert, count;
-  int begin, end, at;
-  uint64_t found[kHeld];
+  uint64_t found;
+  int listed;  // the lane's pair of a sorted run
 
-  __device__ __forceinline__ bool alone(const ExpertArgs &a) const { return a.tokens == 1 && a.by_pair; }
-
-  __device__ __forceinline__ void find(const ExpertArgs &a, int z, int *counts) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    count = 0;
-    if (a.pairs <= 64) {
-      const int e = lane < a.pairs ? pair_expert(a, lane) : -1;
-      expert = a.by_pair ? __builtin_amdgcn_readlane(e, z) : z;
-      found[0] = __ballot(e == expert);
-      if (alone(a)) found[0] = 1ull << z;
-      if (expert >= 0 && !(a.by_pair && found[0] & ((1ull << z) - 1))) count = __builtin_popcountll(found[0]);
+  __device__ __forceinline__ explicit Pairs(const ExpertArgs &a, int z) {
+    const int lane = threadIdx.x & 63;
+    if (a.runs) {
+      const Run run = a.runs[z];
+      expert = __builtin_amdgcn_readfirstlane(run.expert);
+      count = __builtin_amdgcn_readfirstlane(run.count);
+      listed = lane < count ? a.sorted[run.begin + lane] : 0;
       return;
     }
-    expert = __builtin_amdgcn_readfirstlane(a.by_pair ? pair_expert(a, z) : z);
-    if (expert < 0) return;
-    const int share = (a.pairs + 64 * kTeam - 1) / (64 * kTeam) * 64;
-    begin = min(wave * share, a.pairs);
-    end = min(begin + share, a.pairs);
-    int mine = 0;
-    bool earlier = false;
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      const int p = begin + 64 * j + lane;
-      found[j] = 0;
-      if (64 * j < share) found[j] = __ballot(p < end && pair_expert(a, p) == expert);
-    }
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      mine += __builtin_popcountll(found[j]);
-      earlier |= (found[j] & __ballot(begin + 64 * j + lane < z)) != 0;
-    }
-    for (int p = begin + 64 * kHeld + lane; p - lane < end; p += 64) {
-      const uint64_t more = __ballot(p < end && pair_expert(a, p) == expert);
-      mine += __builtin_popcountll(more);
-      earlier |= (more & __ballot(p < z)) != 0;
-    }
-    if (lane == 0) counts[wave] = mine | (a.by_pair && earlier ? kNotFirst : 0);
-    __syncthreads();
-    at = 0;
-    bool first = true;
-#pragma unroll
-    for (int w = 0; w < kTeam; ++w) {
-      const int theirs = counts[w];
-      first &= theirs < kNotFirst;
-      at += w < wave ? theirs : 0;
-      count += theirs;
-    }
-    if (!first) count = 0;
+    const int e = lane < a.pairs ? pair_expert(a, lane) : -1;
+    expert = a.by_pair ? __builtin_amdgcn_readlane(e, z) : z;
+    found = __ballot(e == expert);
+    if (a.tokens == 1 && a.by_pair) found = 1ull << z;
+    const bool first = !a.by_pair || (found & ((1ull << z) - 1)) == 0;
+    count = expert >= 0 && first ? __builtin_popcountll(found) : 0;
   }
 
-  // The list, ascending, into LDS.
+  // The list into LDS. (Every wave writes the same list, and reads what it wrote.)
   __device__ __forceinline__ void list(const ExpertArgs &a, uint16_t *out) const {
     const int lane = threadIdx.x & 63;
-    const uint64_t below = (1ull << lane) - 1;
-    if (a.pairs <= 64) {
-      // (every wave writes the same list, and reads what it wrote itself)
-      if (found[0] >> lane & 1) out[__builtin_popcountll(found[0] & below)] = lane;
-    } else {
-      int to = at;
-#pragma unroll
-      for (int j = 0; j < kHeld; ++j) {
-        if (found[j] >> lane & 1) out[to + __builtin_popcountll(found[j] & below)] = begin + 64 * j + lane;
-        to += __builtin_popcountll(found[j]);
-      }
-      for (int p = begin + 64 * kHeld + lane; p - lane < end; p += 64) {
-        const uint64_t more = __ballot(p < end && pair_expert(a, p) == expert);
-        if (more >> lane & 1) out[to + __builtin_popcountll(more & below)] = p;
-        to += __builtin_popcountll(more);
-      }
-      __syncthreads();
+    if (a.runs) {
+      if (lane < count) out[lane] = listed;
+    } else if (found >> lane & 1) {
+      out[__builtin_popcountll(found & ((1ull << lane) - 1))] = lane;
     }
   }
-
- private:
-  static constexpr int kNotFirst = 1 << 20;
 };
+
+// The sort: one workgroup counts the experts' pairs in LDS, adds the counts and the
+// runs up, and writes the pairs expert by expert and the runs, the rest of them empty.
+// (The order of an expert's pairs is that of the atomics: a pair's results are those of
+// its own column of a product, whichever it is.)
+constexpr int kSortThreads = 1024;
+constexpr int kMaxExperts = 4096;
+
+__global__ __launch_bounds__(kSortThreads) void experts_sort_kernel(ExpertArgs a, Run *runs, uint16_t *sorted,
+                                                                    int items, int most) {
+  constexpr int kEach = kMaxExperts / kSortThreads;
+  __shared__ int counts[kMaxExperts];
+  __shared__ int wave_pairs[kSortThreads / 64], wave_runs[kSortThreads / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int e = threadIdx.x; e < a.experts; e += kSortThreads) counts[e] = 0;
+  __syncthreads();
+  for (int p = threadIdx.x; p < a.pairs; p += kSortThreads) {
+    const int e = pair_expert(a, p);
+    if (e >= 0) atomicAdd(&counts[e], 1);
+  }
+  __syncthreads();
+  // thread = kEach experts in a row
+  int mine[kEach], pairs = 0, parts = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int e = threadIdx.x * kEach + j;
+    mine[j] = e < a.experts ? counts[e] : 0;
+    pairs += mine[j];
+    parts += (mine[j] + most - 1) / most;
+  }
+  int pairs_to = pairs, parts_to = parts;  // inclusive sums
+  for (int m = 1; m < 64; m *= 2) {
+    const int p = __shfl_up(pairs_to, m), q = __shfl_up(parts_to, m);
+    pairs_to += lane >= m ? p : 0;
+    parts_to += lane >= m ? q : 0;
+  }
+  if (lane == 63) wave_pairs[wave] = pairs_to, wave_runs[wave] = parts_to;
+  __syncthreads();
+  int at = pairs_to - pairs, run = parts_to - parts, total = 0;
+  for (int w = 0; w < kSortThreads / 64; ++w) {
+    at += w < wave ? wave_pairs[w] : 0;
+    run += w < wave ? wave_runs[w] : 0;
+    total += wave_runs[w];
+  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int e = threadIdx.x * kEach + j;
+    if (e >= a.experts) break;
+    counts[e] = at;  // where the expert's next pair goes
+    for (int n = 0; n < mine[j]; n += most) runs[run++] = Run{e, at + n, min(most, mine[j] - n), 0};
+    at += mine[j];
+  }
+  for (int i = total + threadIdx.x; i < items; i += kSortThreads) runs[i] = Run{0, 0, 0, 0};
+  __syncthreads();
+  for (int p = threadIdx.x; p < a.pairs; p += kSortThreads) {
+    const int e = pair_expert(a, p);
+    if (e >= 0) sorted[atomicAdd(&counts[e], 1)] = p;
+  }
+}
 
 __device__ __forceinline__ float activated(float gate, float up, bool gelu) {
   const float inner = gelu ? 1.5957691216057308f * (gate + 0.044715f * gate * gate * gate) : gate;
@@ -299,20 +320,18 @@ struct RowPass {
 };
 
 // Workgroup = `share` row tiles of one item, for all of its pairs, up to kMaxCols x 16
-// at a time. Dynamic LDS: the scales of its rows, then the list of pairs.
+// at a time. Dynamic LDS: the scales of its rows.
 template <Product kProduct, int kSteps, bool kFull, int kMaxCols>
 __global__ __launch_bounds__(kThreads, kMaxCols <= 2 && kSteps <= 8 ? 4 : 2) void experts_rows_kernel(ExpertArgs a) {
   constexpr bool kFp4 = kProduct != kUpBf16, kDown = kProduct == kDownFp4;
   __shared__ f32x4 sums[2 * kWaves * kMaxCols * 64];
-  __shared__ int counts[kWaves];
+  __shared__ uint16_t list[kMaxRun];
   extern __shared__ __align__(16) uint8_t lds[];
-  Pairs<kWaves> pairs;
-  pairs.find(a, blockIdx.x / a.groups, counts);
+  const Pairs pairs(a, blockIdx.x / a.groups);
   const int count = pairs.count, expert = pairs.expert;
   if (count == 0) return;
   const int first = blockIdx.x % a.groups * a.share, last = min(first + a.share, a.tiles);
   const uint32_t scale_bytes = kFp4 ? (kDown ? a.width : a.hidden) / 32 : 0;
-  uint16_t *list = reinterpret_cast<uint16_t *>(lds + a.share * kRows * scale_bytes);
 
   // 16 bytes a thread of the scales of rows first .. last - 1 (gate rows, then up)
   const int tile_rows = kDown ? kRows : kRows / 2, parts = kDown ? 1 : 2;
@@ -330,7 +349,7 @@ __global__ __launch_bounds__(kThreads, kMaxCols <= 2 && kSteps <= 8 ? 4 : 2) voi
     const int left = count - base;
     auto ready = [&] {
       if (base == 0) pairs.list(a, list);
-      if (kFp4 && base == 0 && a.pairs <= 64) __syncthreads();  // the scales
+      if (kFp4 && base == 0) __syncthreads();  // the scales
     };
     if (kMaxCols >= 4 && left > 2 * kColumns) {
       if constexpr (kMaxCols >= 4)
@@ -408,11 +427,9 @@ struct DownLane {
 template <int kSteps, Steps kMode>
 __global__ __launch_bounds__(kThreads, kSteps <= 3 ? 4 : 2) void experts_down_kernel(ExpertArgs a) {
   __shared__ f32x4 sums[2 * kWaves * 4 * 64];
-  __shared__ int counts[kWaves];
-  extern __shared__ uint16_t list[];
+  __shared__ uint16_t list[kMaxRun];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Pairs<kWaves> pairs;
-  pairs.find(a, blockIdx.x / a.groups, counts);
+  const Pairs pairs(a, blockIdx.x / a.groups);
   const int count = pairs.count;
   if (count == 0) return;
   const int first = blockIdx.x % a.groups * a.share, rounds = min(a.share, a.tiles - first);
@@ -476,11 +493,9 @@ __global__ __launch_bounds__(kThreads, kSteps <= 3 ? 4 : 2) void experts_down_ke
 template <int kSteps, Steps kMode>
 __global__ __launch_bounds__(kThreads, kSteps <= 3 ? 4 : 2) void experts_down_many_kernel(ExpertArgs a) {
   __shared__ f32x4 sums[kWaves * 4 * 64];
-  __shared__ int counts[kWaves];
-  extern __shared__ uint16_t list[];
+  __shared__ uint16_t list[kMaxRun];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Pairs<kWaves> pairs;
-  pairs.find(a, blockIdx.x / a.groups, counts);
+  const Pairs pairs(a, blockIdx.x / a.groups);
   const int count = pairs.count, expert = pairs.expert;
   if (count == 0) return;
   const int row0 = blockIdx.x % a.groups * kDownOutputs;
@@ -613,7 +628,7 @@ int validate(int hidden, int width, int experts, int top_k, uint32_t flags, int 
   const int grain = flags & CFMOE_FP4 ? 32 : 16;
   if (width <= 0 || width % grain || width > kMaxLength)
     return fail(CFMOE_EINVAL, "routed_experts needs a width that is a multiple of 16 (of 32 with 4-bit weights), at most 4096");
-  if (experts < 1 || experts > 4096) return fail(CFMOE_EINVAL, "routed_experts needs 1 to 4096 experts");
+  if (experts < 1 || experts > kMaxExperts) return fail(CFMOE_EINVAL, "routed_experts needs 1 to 4096 experts");
   if (top_k < 1 || top_k > 64) return fail(CFMOE_EINVAL, "routed_experts needs 1 to 64 experts per token");
   if (tokens < 0 || static_cast<int64_t>(tokens) * top_k > kMaxPairs)
     return fail(CFMOE_EINVAL, "routed_experts takes at most 8192 routed pairs per call");
@@ -635,6 +650,9 @@ Cut cut_of(int units, bool fp4) {
         best = {splits, loads};
   return best;
 }
+
+// The most runs of at most `most` pairs that `pairs` pairs of `experts` can make.
+int run_items(int experts, int pairs, int most) { return std::min(experts, pairs) + pairs / most; }
 
 int64_t act_bytes(int width, int pairs) {
   return static_cast<int64_t>(pairs) * width * 2;  // (a row is a multiple of 32 bytes)
@@ -661,14 +679,13 @@ auto rows_kernel(bool full, bool wide) {
 }
 
 template <Product kProduct>
-int launch_rows(ExpertArgs a, int items, unsigned list, cfmoe_stream stream) {
+int launch_rows(ExpertArgs a, int items, bool wide, cfmoe_stream stream) {
   constexpr bool kFp4 = kProduct != kUpBf16, kDown = kProduct == kDownFp4;
   const int length = kDown ? a.width : a.hidden;
   const int units = kFp4 ? (length + 127) / 128 : length / 32;
   const Cut cut = cut_of(units, kFp4);
   const int steps = cut.loads * (kFp4 ? 4 : 1);
   const bool full = units == cut.splits * cut.loads && length % 128 == 0;
-  const bool wide = a.pairs >= 12 * a.experts;
   a.splits = cut.splits;
   a.tiles = kDown ? a.hidden / kRows : a.width / (kRows / 2);
   // enough workgroups to fill the chip, then fewer loads of the pairs' vectors
@@ -680,7 +697,7 @@ int launch_rows(ExpertArgs a, int items, unsigned list, cfmoe_stream stream) {
                       : steps <= 12 ? rows_kernel<kProduct, 12>(full, wide)
                                     : rows_kernel<kProduct, 16>(full, wide);
   const unsigned scales = kFp4 ? a.share * kRows * (length / 32) : 0;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.groups) * items), dim3(kThreads), scales + list, stream, a);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.groups) * items), dim3(kThreads), scales, stream, a);
   return check_launch(kDown ? "experts_down" : "experts_up");
 }
 
@@ -695,7 +712,9 @@ CFMOE_API int64_t cfmoe_routed_experts_scratch_bytes(int32_t hidden_size, int32_
                                                      int32_t top_k, uint32_t flags, int32_t tokens) {
   if (int rc = validate(hidden_size, width, experts, top_k, flags, tokens)) return -rc;
   const int pairs = tokens * top_k;
-  return act_bytes(width, pairs) + static_cast<int64_t>(pairs) * hidden_size * 4;
+  // activations, partials, and for more than 64 pairs the runs and the sorted pairs
+  const int64_t sorted = pairs > 64 ? run_items(experts, pairs, 16) * sizeof(Run) + pairs * 2 : 0;
+  return act_bytes(width, pairs) + static_cast<int64_t>(pairs) * hidden_size * 4 + sorted;
 }
 
 CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t experts, int32_t top_k,
@@ -737,10 +756,25 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   a.weights16 = flags & CFMOE_WEIGHTS_BF16;
   a.gelu = flags & CFMOE_GELU;
   a.by_pair = a.pairs <= experts;
-  const int items = a.by_pair ? a.pairs : experts;
-  const unsigned list = static_cast<unsigned>((a.pairs * 2 + 15) / 16 * 16);
+  // Sorted runs: of 64 pairs where an expert has many, so that few weights are read
+  // again; else of what a pass takes, twice.
+  const bool wide = a.pairs >= WIDE * experts;
+  int items = a.by_pair ? a.pairs : experts;
+  a.runs = nullptr;
+  a.sorted = nullptr;
+  if (a.pairs > 64) {
+    const int most = wide ? kMaxRun : RUN;
+    items = run_items(experts, a.pairs, most);
+    Run *runs = reinterpret_cast<Run *>(static_cast<uint8_t *>(scratch) + act_bytes(width, a.pairs) +
+                                        static_cast<int64_t>(a.pairs) * hidden_size * 4);
+    uint16_t *sorted = reinterpret_cast<uint16_t *>(runs + run_items(experts, a.pairs, 16));
+    hipLaunchKernelGGL(experts_sort_kernel, dim3(1), dim3(kSortThreads), 0, stream, a, runs, sorted, items, most);
+    if (int rc = check_launch("experts_sort")) return rc;
+    a.runs = runs;
+    a.sorted = sorted;
+  }
 
-  if (int rc = fp4 ? launch_rows<kUpFp4>(a, items, list, stream) : launch_rows<kUpBf16>(a, items, list, stream)) return rc;
+  if (int rc = fp4 ? launch_rows<kUpFp4>(a, items, wide, stream) : launch_rows<kUpBf16>(a, items, wide, stream)) return rc;
   if (fp4 && a.by_pair && tokens <= 4) {
     a.tiles = hidden_size / kRows;
     hipLaunchKernelGGL(experts_fp4_tokens_kernel, dim3(static_cast<unsigned>(a.tiles) * tokens), dim3(kThreads), 0,
@@ -748,11 +782,11 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
     return check_launch("experts_down");
   }
   if (fp4) {
-    if (int rc = launch_rows<kDownFp4>(a, items, list, stream)) return rc;
+    if (int rc = launch_rows<kDownFp4>(a, items, wide, stream)) return rc;
   } else {
     a.tiles = hidden_size / kDownOutputs;
     a.share = 1;
-    const bool many = a.pairs >= 12 * experts;
+    const bool many = wide;
     while (!many && static_cast<int64_t>(items) * a.tiles / (2 * a.share) >= 256 && a.share < 4) a.share *= 2;
     a.groups = (a.tiles + a.share - 1) / a.share;
     const int steps = (width + 31) / 32, each = (steps + kWaves - 1) / kWaves;
@@ -762,7 +796,7 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
                         : held == 3 ? down_kernel<3>(many, mode)
                         : held == 4 ? down_kernel<4>(many, mode)
                                     : down_kernel<8>(many, mode);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.groups) * items), dim3(kThreads), list, stream, a);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.groups) * items), dim3(kThreads), 0, stream, a);
     if (int rc = check_launch("experts_down")) return rc;
   }
 
