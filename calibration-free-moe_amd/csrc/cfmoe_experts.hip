@@ -35,12 +35,7 @@ constexpr int kColumns = 16;      // pairs of a matrix instruction
 constexpr int kRows = 16;         // weight rows of one
 constexpr int kDownOutputs = 64;  // outputs of a BF16 down workgroup
 constexpr int kJoinThreads = 256;
-#ifndef WIDE
-#define WIDE 12
-#endif
-#ifndef RUN
-#define RUN 32
-#endif
+
 struct ExpertArgs {
   const uint16_t *x;
   const void *ids, *weights;
@@ -238,8 +233,8 @@ struct RowPass {
     auto unit = [&](int i) { return kFull ? i : min(i, steps - 1); };
 
     u32x4 words[kLoads];
-    auto load = [&](int tile) {
-      tile = min(tile, last - 1);
+    auto load = [&](int r) {
+      const int tile = min(first + r * subs + sub, last - 1);
       const int64_t row0 = kDown ? static_cast<int64_t>(expert) * a.hidden + tile * kRows
                                  : static_cast<int64_t>(expert) * 2 * a.width + tile * (kRows / 2);
       const uint8_t *w = (kDown ? a.down : a.gate_up) + row0 * row_bytes + begin * 64;
@@ -249,7 +244,7 @@ struct RowPass {
         words[i] = load_at<u32x4>(w + unit(i) * 64, whole ? lane_row : lane_row - lane / 16 * 16);
       }
     };
-    load(first + sub);
+    load(0);
     ready();
     const void *rows = kDown ? a.act : a.x;
     u32x4 b[kCols][kSteps];
@@ -274,7 +269,7 @@ struct RowPass {
     const uint32_t to = kDown ? pair * a.hidden + lane / 16 * 4 : pair * a.width + lane / 16 * 2;
     const float weight = kDown ? 0.0f : pair_weight(a, pair);
 
-    for (int r = 0; r < rounds; ++r) {
+    auto product = [&](int r) {
       f32x4 d[kCols];
 #pragma unroll
       for (int n = 0; n < kCols; ++n) d[n] = f32x4{0, 0, 0, 0};
@@ -301,8 +296,10 @@ struct RowPass {
       f32x4 *in = sums + (r & 1) * (kWaves * kCols * 64) + lane;
 #pragma unroll
       for (int n = 0; n < kCols; ++n) in[(wave * kCols + n) * 64] = d[n];
-      if (r + 1 < rounds) load(first + (r + 1) * subs + sub);
+    };
+    auto add = [&](int r) {
       __syncthreads();
+      const f32x4 *in = sums + (r & 1) * (kWaves * kCols * 64) + lane;
       for (int i = wave; i < subs * kCols; i += kWaves) {
         const int tile = first + r * subs + i / kCols;
         if (!stores || tile >= last) break;
@@ -314,7 +311,17 @@ struct RowPass {
           *reinterpret_cast<uint32_t *>(a.act + (to + tile * (kRows / 2))) =
               bf16_pair(weight * activated(v[0], v[1], a.gelu), weight * activated(v[2], v[3], a.gelu));
       }
+    };
+    // The rows' registers are free once multiplied: the next round's loads leave before
+    // this one's sums are added up. (More rounds on their way than one, four of 4-bit
+    // rows, measured the same.)
+    for (int r = 0; r + 1 < rounds; ++r) {
+      product(r);
+      load(r + 1);
+      add(r);
     }
+    product(rounds - 1);
+    add(rounds - 1);
     __syncthreads();
   }
 };
@@ -671,11 +678,13 @@ auto down_kernel(bool many, Steps mode) {
 
 template <Product kProduct, int kSteps>
 auto rows_kernel(bool full, bool wide) {
-  // (registers: 4 x 16 pairs beside eight steps, 2 x 16 beside 12, or 16 in 4 bits)
-  constexpr int kNarrow = kProduct == kUpFp4 && kSteps == 8 ? 2 : 1;
-  constexpr int kWide = kSteps == 8 ? 4 : kSteps == 12 || kProduct != kUpBf16 ? 2 : 1;
+  // Column tiles of a wide kernel. BF16: as many as the registers hold with one
+  // workgroup to a compute unit. 4 bits: two, with which there are still two workgroups
+  // (four leave room for one: 256 Zipf tokens 103 us against 80).
+  constexpr int kWide = kProduct == kUpBf16 ? (kSteps == 8 ? 4 : kSteps == 12 ? 2 : 1)
+                                            : (kProduct == kUpFp4 && kSteps == 8 ? 2 : 1);
   return wide ? full ? experts_rows_kernel<kProduct, kSteps, true, kWide> : experts_rows_kernel<kProduct, kSteps, false, kWide>
-              : full ? experts_rows_kernel<kProduct, kSteps, true, kNarrow> : experts_rows_kernel<kProduct, kSteps, false, kNarrow>;
+              : full ? experts_rows_kernel<kProduct, kSteps, true, 1> : experts_rows_kernel<kProduct, kSteps, false, 1>;
 }
 
 template <Product kProduct>
@@ -691,7 +700,7 @@ int launch_rows(ExpertArgs a, int items, bool wide, cfmoe_stream stream) {
   // enough workgroups to fill the chip, then fewer loads of the pairs' vectors
   const int subs = kWaves / cut.splits;
   a.share = subs;
-  while (static_cast<int64_t>(items) * a.tiles / (2 * a.share) >= 1024 && a.share < 8 * subs) a.share *= 2;
+  while (static_cast<int64_t>(items) * a.tiles / (2 * a.share) >= (kFp4 || wide ? 1024 : 2048) && a.share < 8 * subs) a.share *= 2;
   a.groups = (a.tiles + a.share - 1) / a.share;
   const auto kernel = steps <= 8    ? rows_kernel<kProduct, 8>(full, wide)
                       : steps <= 12 ? rows_kernel<kProduct, 12>(full, wide)
@@ -756,14 +765,18 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   a.weights16 = flags & CFMOE_WEIGHTS_BF16;
   a.gelu = flags & CFMOE_GELU;
   a.by_pair = a.pairs <= experts;
-  // Sorted runs: of 64 pairs where an expert has many, so that few weights are read
-  // again; else of what a pass takes, twice.
-  const bool wide = a.pairs >= WIDE * experts;
+  // A wide kernel's sorted runs are of 64 pairs over BF16 rows and 32 over 4-bit rows,
+  // the others' of 16. Wide pays where experts have more than 16 pairs: BF16 from six an
+  // expert on average, since skewed routing gains more than uniform loses (128 tokens
+  // over 128 experts, top 8: uniform 175 us against 171, Zipf(1.2) 232 against 249; 64
+  // experts' 64 tokens of Zipf(1.2) 164 against 179), 4-bit rows from twelve (128 tokens
+  // 94 and 98 us, 256 tokens' up product 80 and 67).
+  const bool wide = a.pairs >= (fp4 ? 12 : 6) * experts;
   int items = a.by_pair ? a.pairs : experts;
   a.runs = nullptr;
   a.sorted = nullptr;
   if (a.pairs > 64) {
-    const int most = wide ? kMaxRun : RUN;
+    const int most = !wide ? 16 : fp4 ? 32 : kMaxRun;
     items = run_items(experts, a.pairs, most);
     Run *runs = reinterpret_cast<Run *>(static_cast<uint8_t *>(scratch) + act_bytes(width, a.pairs) +
                                         static_cast<int64_t>(a.pairs) * hidden_size * 4);
@@ -782,7 +795,7 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
     return check_launch("experts_down");
   }
   if (fp4) {
-    if (int rc = launch_rows<kDownFp4>(a, items, wide, stream)) return rc;
+    if (int rc = launch_rows<kDownFp4>(a, items, false, stream)) return rc;
   } else {
     a.tiles = hidden_size / kDownOutputs;
     a.share = 1;
