@@ -40,8 +40,8 @@ def routed_experts(
     gate_up BF16 [E, 2 I, H] and down the channel-major logical [E, H, I] (stride
     (H I, 1, H)), as the reader borrows them (`channel_major_down`), or both
     `Fp4Weights` of those logical shapes. Ids outside [0, E) contribute nothing; an
-    expert named twice by one token counts twice. Sums are FP32; the weighted
-    activations are rounded to BF16 once, and so is the output. Results do not
+    expert named twice by one token counts twice. Sums are FP32, the weighted
+    activations are held to 2^-16, and the output is rounded once. Results do not
     depend on the other tokens of the batch in more than the order of FP32 sums.
 
     H is a multiple of 128 and I of 16 (of 32 in 4 bits), both at most 4096; at

@@ -8,7 +8,7 @@
 // it gathers them from the ids itself (pairs of one expert, ascending), 16 to a
 // matrix instruction's columns. Three launches:
 //
-//   up    act[p, c] = bf16(w phi(g) u), g and u in FP32 (experts_rows_kernel)
+//   up    act[p, c] = w phi(g) u, g and u in FP32 (experts_rows_kernel)
 //   down  partial[p, h] = FP32 sum over the channels (experts_down_kernel over
 //         channel-major BF16 rows, experts_rows_kernel over 4-bit rows)
 //   join  out[t, h] = bf16(sum over t's slots, in order) (experts_join_kernel)
@@ -16,8 +16,11 @@
 // A pair whose id lies outside [0, E) or whose token is padded belongs to no
 // expert: nothing computes it, and the join leaves it out.
 //
-// Rounding act to BF16 makes it the matrix operand of the second product; the
-// router weight goes in before, so that a pair is rounded once.
+// The second product's matrix operand is BF16, so an activation (router weight and
+// all) is held as two BF16 numbers, high = bf16(v) and low = bf16(v - high), 2^-16 of
+// it off at most, and multiplied twice: the matrix cores have the time, and the
+// output's error stays that of its own rounding (one BF16 activation made it 1.45
+// times that).
 
 #include <algorithm>
 #include <type_traits>
@@ -41,7 +44,7 @@ struct ExpertArgs {
   const void *ids, *weights;
   const uint8_t *padding;
   const uint8_t *gate_up, *gate_up_scales, *down, *down_scales;
-  uint16_t *act;   // [pairs, width]
+  uint16_t *act;   // [pairs, act_row]
   float *partial;  // [pairs, hidden]
   uint16_t *out;
   int tokens, top_k, pairs, experts, hidden, width;
@@ -183,6 +186,36 @@ __device__ __forceinline__ float activated(float gate, float up, bool gelu) {
   return gate / (1.0f + __expf(-inner)) * up;
 }
 
+// A pair's activations are pieces of eight channels, their high parts and then their low
+// ones: a piece is a matrix operand's load of one lane. For 4-bit rows the pieces of each
+// 128 channels stand as the four lanes of a pair read them, 32 block + 8 q at piece
+// 4 q + block.
+template <bool kFp4>
+constexpr __host__ __device__ int act_row(int width) { return kFp4 ? (width + 127) / 128 * 256 : 2 * width; }
+template <bool kFp4>
+__device__ __forceinline__ uint32_t act_place(uint32_t piece) {
+  return 16 * (kFp4 ? (piece & ~15u) + piece % 4 * 4 + piece / 4 % 4 : piece);
+}
+
+// Both parts of a piece at element `to`, of which lane l, l + 16, l + 32 and l + 48 have
+// two channels each: after two swaps, of half waves and of odd with even quarters, two
+// words that stand side by side. (A store for each part took a sixth of the up product's
+// time.) An infinity or NaN has no low part: it would be NaN, and an infinite sum with it.
+__device__ __forceinline__ void store_activations(const ExpertArgs &a, uint32_t to, float first, float second) {
+  const uint32_t high = bf16_pair(first, second);
+  const float high0 = __uint_as_float(high << 16), high1 = __uint_as_float(high & 0xffff0000u);
+  const float low0 = isfinite(high0) ? first - high0 : 0.0f, low1 = isfinite(high1) ? second - high1 : 0.0f;
+  const auto halves = __builtin_amdgcn_permlane32_swap(high, bf16_pair(low0, low1), false, false);
+  const auto words = __builtin_amdgcn_permlane16_swap(halves[0], halves[1], false, false);
+  *reinterpret_cast<u32x2 *>(a.act + (to + (threadIdx.x & 63) / 16 * 4)) = u32x2{words[0], words[1]};
+}
+
+// v + the v of the lane eight columns on or back: a pair's high and low parts.
+__device__ __forceinline__ float parts_sum(float v) {
+  constexpr int kRotate8 = 0x128;  // of 16 lanes
+  return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), kRotate8, 0xf, 0xf, true));
+}
+
 // What a row product is of.
 enum Product { kUpBf16, kUpFp4, kDownFp4 };
 
@@ -206,6 +239,8 @@ template <Product kProduct, int kSteps, bool kFull, int kCols>
 struct RowPass {
   static constexpr bool kFp4 = kProduct != kUpBf16, kDown = kProduct == kDownFp4;
   static constexpr int kLoads = kFp4 ? kSteps / 4 : kSteps;
+  // pairs of a column tile: the down product's high parts are columns 0-7, their low parts 8-15
+  static constexpr int kPairs = kDown ? kColumns / 2 : kColumns;
 
   template <class Ready>
   static __device__ __forceinline__ void run(const ExpertArgs &a, int expert, int first, int last,
@@ -246,27 +281,29 @@ struct RowPass {
     };
     load(0);
     ready();
-    const void *rows = kDown ? a.act : a.x;
     u32x4 b[kCols][kSteps];
 #pragma unroll
     for (int n = 0; n < kCols; ++n) {
-      const uint32_t pair = list[min(base + n * kColumns + lane % 16, count - 1)];
-      const uint32_t vector = (kDown ? pair * a.width : pair / a.top_k * a.hidden) * 2;
+      const uint32_t pair = list[min(base + n * kPairs + lane % kPairs, count - 1)];
+      const uint32_t vector = kDown ? pair * (2 * act_row<kFp4>(a.width)) + lane % 16 / kPairs * 16 : pair / a.top_k * a.hidden * 2;
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
         // (element 32 block + 8 (j % 4) in 4 bits, block 4 i + lane / 16)
         const int i = unit(kFp4 ? j / 4 : j);
-        const uint32_t place = kFp4 ? (4 * (begin + i) + (own(i) ? lane / 16 : 0)) * 64 + j % 4 * 16
-                                    : (begin + i) * 64 + lane / 16 * 16;
-        b[n][j] = load_at<u32x4>(rows, vector + place) & own(kFp4 ? j / 4 : j);
+        const uint32_t place = kDown   ? (begin + i) * 512 + j % 4 * 128 + lane / 16 * 32
+                               : kFp4 ? (4 * (begin + i) + (own(i) ? lane / 16 : 0)) * 64 + j % 4 * 16
+                                      : (begin + i) * 64 + lane / 16 * 16;
+        b[n][j] = load_at<u32x4>(kDown ? a.act : a.x, vector + place) & own(kFp4 ? j / 4 : j);
       }
     }
-    // what a wave adds up and stores: of a round's subs x kCols sums every eighth; its
-    // column tile is the same in each
-    const int column = base + wave % kCols * kColumns + lane % 16;
-    const bool stores = column < count;
+    // What a wave adds up and stores: of a round's subs x kSums sums every eighth; its
+    // column tile is the same in each. Two column tiles of the down product make one sum,
+    // high and low parts' columns added first.
+    constexpr int kSums = kDown ? 1 : kCols, kStored = kDown ? kCols * kPairs : kColumns;
+    const int column = base + wave % kSums * kColumns + lane % kStored;
+    const bool stores = column < count && lane % 16 < kStored;
     const uint32_t pair = list[min(column, count - 1)];
-    const uint32_t to = kDown ? pair * a.hidden + lane / 16 * 4 : pair * a.width + lane / 16 * 2;
+    const uint32_t to = kDown ? pair * a.hidden + lane / 16 * 4 : pair * act_row<kFp4>(a.width);
     const float weight = kDown ? 0.0f : pair_weight(a, pair);
 
     auto product = [&](int r) {
@@ -293,23 +330,34 @@ struct RowPass {
       }
       // (the sums alternate between two buffers: what a round overwrites was read
       // before the last barrier)
-      f32x4 *in = sums + (r & 1) * (kWaves * kCols * 64) + lane;
+      f32x4 *in = sums + (r & 1) * (kWaves * kSums * 64) + lane;
+      if constexpr (kDown) {
+        f32x4 both;
 #pragma unroll
-      for (int n = 0; n < kCols; ++n) in[(wave * kCols + n) * 64] = d[n];
+        for (int e = 0; e < 4; ++e) {
+          // (both sums by all lanes: one reads a lane of the other half)
+          const float first = parts_sum(d[0][e]), second = parts_sum(d[kCols - 1][e]);
+          both[e] = kCols == 2 && (lane & 8) ? second : first;
+        }
+        in[wave * 64] = both;
+      } else {
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) in[(wave * kCols + n) * 64] = d[n];
+      }
     };
     auto add = [&](int r) {
       __syncthreads();
-      const f32x4 *in = sums + (r & 1) * (kWaves * kCols * 64) + lane;
-      for (int i = wave; i < subs * kCols; i += kWaves) {
-        const int tile = first + r * subs + i / kCols;
+      const f32x4 *in = sums + (r & 1) * (kWaves * kSums * 64) + lane;
+      for (int i = wave; i < subs * kSums; i += kWaves) {
+        const int tile = first + r * subs + i / kSums;
         if (!stores || tile >= last) break;
-        f32x4 v = in[(i / kCols * a.splits * kCols + i % kCols) * 64];
-        for (int w = 1; w < a.splits; ++w) v += in[((i / kCols * a.splits + w) * kCols + i % kCols) * 64];
+        f32x4 v = in[(i / kSums * a.splits * kSums + i % kSums) * 64];
+        for (int w = 1; w < a.splits; ++w) v += in[((i / kSums * a.splits + w) * kSums + i % kSums) * 64];
         if (kDown)
           *reinterpret_cast<f32x4 *>(a.partial + (to + tile * kRows)) = v;
         else
-          *reinterpret_cast<uint32_t *>(a.act + (to + tile * (kRows / 2))) =
-              bf16_pair(weight * activated(v[0], v[1], a.gelu), weight * activated(v[2], v[3], a.gelu));
+          store_activations(a, to + act_place<kFp4>(tile), weight * activated(v[0], v[1], a.gelu),
+                            weight * activated(v[2], v[3], a.gelu));
       }
     };
     // The rows' registers are free once multiplied: the next round's loads leave before
@@ -331,7 +379,7 @@ struct RowPass {
 template <Product kProduct, int kSteps, bool kFull, int kMaxCols>
 __global__ __launch_bounds__(kThreads, kMaxCols <= 2 && kSteps <= 8 ? 4 : 2) void experts_rows_kernel(ExpertArgs a) {
   constexpr bool kFp4 = kProduct != kUpBf16, kDown = kProduct == kDownFp4;
-  __shared__ f32x4 sums[2 * kWaves * kMaxCols * 64];
+  __shared__ f32x4 sums[2 * kWaves * (kDown ? 1 : kMaxCols) * 64];
   __shared__ uint16_t list[kMaxRun];
   extern __shared__ __align__(16) uint8_t lds[];
   const Pairs pairs(a, blockIdx.x / a.groups);
@@ -352,23 +400,24 @@ __global__ __launch_bounds__(kThreads, kMaxCols <= 2 && kSteps <= 8 ? 4 : 2) voi
       reinterpret_cast<u32x4 *>(lds)[i] = load_at<u32x4>(scales, part * a.width * scale_bytes + chunk * 16);
   }
 
+  constexpr int kPairs = RowPass<kProduct, kSteps, kFull, 1>::kPairs;
   for (int base = 0; base < count;) {
     const int left = count - base;
     auto ready = [&] {
       if (base == 0) pairs.list(a, list);
       if (kFp4 && base == 0) __syncthreads();  // the scales
     };
-    if (kMaxCols >= 4 && left > 2 * kColumns) {
+    if (kMaxCols >= 4 && left > 2 * kPairs) {
       if constexpr (kMaxCols >= 4)
         RowPass<kProduct, kSteps, kFull, 4>::run(a, expert, first, last, list, count, base, sums, lds, ready);
-      base += 4 * kColumns;
-    } else if (kMaxCols >= 2 && left > kColumns) {
+      base += 4 * kPairs;
+    } else if (kMaxCols >= 2 && left > kPairs) {
       if constexpr (kMaxCols >= 2)
         RowPass<kProduct, kSteps, kFull, 2>::run(a, expert, first, last, list, count, base, sums, lds, ready);
-      base += 2 * kColumns;
+      base += 2 * kPairs;
     } else {
       RowPass<kProduct, kSteps, kFull, 1>::run(a, expert, first, last, list, count, base, sums, lds, ready);
-      base += kColumns;
+      base += kPairs;
     }
   }
 }
@@ -414,10 +463,11 @@ struct DownLane {
     if (kMode == kExact) return v;
     return v & (step < steps && !short_of(step) ? ~0u : 0u);
   }
-  __device__ __forceinline__ u32x4 vector(const ExpertArgs &a, uint32_t pair, int step) const {
-    const uint32_t offset = (pair * a.width + channel) * 2;
-    return own(load_at<u32x4>(reinterpret_cast<const uint8_t *>(a.act) + 64 * at(step),
-                              short_of(step) ? offset - 32 : offset), step);
+  // a part of a pair's activations, high (0) or low (1)
+  __device__ __forceinline__ u32x4 vector(const ExpertArgs &a, uint32_t pair, int part, int step) const {
+    const uint32_t offset = (pair * a.width + channel) * 4 + part * 16;
+    return own(load_at<u32x4>(reinterpret_cast<const uint8_t *>(a.act) + 128 * at(step),
+                              short_of(step) ? offset - 64 : offset), step);
   }
   __device__ __forceinline__ void rows(u32x2 (&to)[8], const uint8_t *down, int step) const {
     const uint8_t *from = down + static_cast<int64_t>(32 * at(step)) * row_bytes;
@@ -452,9 +502,10 @@ __global__ __launch_bounds__(kThreads, kSteps <= 3 ? 4 : 2) void experts_down_ke
       if (base == 0 && chunk == 0) pairs.list(a, list);
       const int column = base + lane % 16;
       const uint32_t pair = list[min(column, count - 1)];
-      u32x4 b[kSteps];
+      u32x4 b[kSteps][2];
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) b[s] = place.vector(a, pair, step(s));
+      for (int s = 0; s < kSteps; ++s)
+        for (int part = 0; part < 2; ++part) b[s][part] = place.vector(a, pair, part, step(s));
       auto round = [&](int r, auto more) {
         f32x4 d[4];
 #pragma unroll
@@ -468,7 +519,9 @@ __global__ __launch_bounds__(kThreads, kSteps <= 3 ? 4 : 2) void experts_down_ke
           turn(rows[s], w);
           if (decltype(more)::value) place.rows(rows[s], down + (r + 1) * (2 * kDownOutputs), step(s));
 #pragma unroll
-          for (int j = 0; j < 4; ++j) d[j] = mma(w[j], b[s], d[j]);
+          for (int j = 0; j < 4; ++j) d[j] = mma(w[j], b[s][0], d[j]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[j] = mma(w[j], b[s][1], d[j]);
         }
         // a lane holds outputs 16 g + 4 i + j of its pair, g = l / 16; the sums alternate
         // between two buffers, and the waves' two halves in adding them up
@@ -522,16 +575,20 @@ __global__ __launch_bounds__(kThreads, kSteps <= 3 ? 4 : 2) void experts_down_ma
     if (chunk == 0) pairs.list(a, list);
     for (int base = 0; base < count; base += kColumns) {
       const uint32_t pair = list[min(base + lane % 16, count - 1)];
-      u32x4 b[kSteps];
+      u32x4 b[kSteps][2];
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) b[s] = place.vector(a, pair, chunk + s * kWaves + wave);
+      for (int s = 0; s < kSteps; ++s)
+        for (int part = 0; part < 2; ++part) b[s][part] = place.vector(a, pair, part, chunk + s * kWaves + wave);
       f32x4 d[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
+      for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) d[j] = mma(w[s][j], b[s], d[j]);
+        for (int j = 0; j < 4; ++j) d[j] = mma(w[s][j], b[s][0], d[j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[j] = mma(w[s][j], b[s][1], d[j]);
+      }
       // a lane holds outputs 16 g + 4 r + j of its pair, g = l / 16
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -558,7 +615,7 @@ __global__ __launch_bounds__(kThreads, kSteps <= 3 ? 4 : 2) void experts_down_ma
 // expert that several tokens name is read for each of them.
 __global__ __launch_bounds__(kThreads) void experts_fp4_tokens_kernel(ExpertArgs a) {
   constexpr int kAhead = 4;
-  __shared__ f32x4 sums[kWaves][4];
+  __shared__ f32x4 sums[kWaves][2][4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t = blockIdx.x / a.tiles, row = blockIdx.x % a.tiles * kRows;
   const int blocks = a.width / 32, steps = (blocks + 3) / 4;
@@ -569,9 +626,10 @@ __global__ __launch_bounds__(kThreads) void experts_fp4_tokens_kernel(ExpertArgs
     if (expert < 0) continue;
     const int64_t row0 = static_cast<int64_t>(expert) * a.hidden + row;
     const uint8_t *words = a.down + row0 * (a.width / 2), *scales = a.down_scales + row0 * blocks;
-    const uint8_t *act = reinterpret_cast<const uint8_t *>(a.act + static_cast<uint32_t>(pair) * a.width);
+    const uint8_t *act = reinterpret_cast<const uint8_t *>(a.act + static_cast<uint32_t>(pair) * act_row<true>(a.width));
     for (int s = 0; s < steps; s += kAhead) {
-      u32x4 word[kAhead], b[kAhead][4];
+      u32x4 word[kAhead];
+      u32x4 b[kAhead][4];
       uint32_t scale[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
@@ -581,22 +639,21 @@ __global__ __launch_bounds__(kThreads) void experts_fp4_tokens_kernel(ExpertArgs
         word[i] = load_at<u32x4>(words, lane % 16 * (a.width / 2) + block * 16) & own;
         scale[i] = load_at<uint8_t>(scales, lane % 16 * blocks + block) & own;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) b[i][q] = load_at<u32x4>(act, block * 64 + q * 16) & own;
+        for (int q = 0; q < 4; ++q) b[i][q] = load_at<u32x4>(act, min(s + i, steps - 1) * 512 + q * 128 + lane / 16 * 32 + lane % 2 * 16) & own;
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          d = mma(fp4_values(word[i][q], __uint_as_float(scale[i] << 23)), b[i][q], d);
+        for (int q = 0; q < 4; ++q) d = mma(fp4_values(word[i][q], __uint_as_float(scale[i] << 23)), b[i][q], d);
     }
   }
-  // (all 16 columns are the one token's)
-  if (lane % 16 == 0) sums[wave][lane / 16] = d;
+  // (all 16 columns are the one token's, high and low parts in turn)
+  if (lane % 16 < 2) sums[wave][lane % 2][lane / 16] = d;
   __syncthreads();
   if (threadIdx.x < 4) {
-    f32x4 v = sums[0][threadIdx.x];
+    f32x4 v = {0, 0, 0, 0};
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) v += sums[w][threadIdx.x];
+    for (int w = 0; w < kWaves; ++w) v += sums[w][0][threadIdx.x] + sums[w][1][threadIdx.x];
     *reinterpret_cast<u32x2 *>(a.out + (static_cast<uint32_t>(t) * a.hidden + row + threadIdx.x * 4)) =
         u32x2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
   }
@@ -644,16 +701,17 @@ int validate(int hidden, int width, int experts, int top_k, uint32_t flags, int 
 
 // How a row of `units` operand loads (32 BF16 values, or 128 in 4 bits) is cut: the
 // waves that share it, and each one's loads, one of the counts that kernels exist
-// for. Fewest idle loads first, then the most waves.
+// for. Fewest idle loads first, then the most waves. The 4-bit down product takes two
+// loads where eight waves can: three want more registers than two workgroups have.
 struct Cut {
   int splits, loads;
 };
 
-Cut cut_of(int units, bool fp4) {
+Cut cut_of(int units, bool fp4, bool down) {
   Cut best = {0, 0};
   for (int splits = kWaves; splits >= 1; splits /= 2)
     for (int loads : {fp4 ? 2 : 8, fp4 ? 3 : 12, fp4 ? 4 : 16})
-      if (loads * splits >= units && (!best.splits || loads * splits < best.loads * best.splits))
+      if (loads * splits >= units && !(down && loads > 2 && units <= 2 * kWaves) && (!best.splits || loads * splits < best.loads * best.splits))
         best = {splits, loads};
   return best;
 }
@@ -661,8 +719,8 @@ Cut cut_of(int units, bool fp4) {
 // The most runs of at most `most` pairs that `pairs` pairs of `experts` can make.
 int run_items(int experts, int pairs, int most) { return std::min(experts, pairs) + pairs / most; }
 
-int64_t act_bytes(int width, int pairs) {
-  return static_cast<int64_t>(pairs) * width * 2;  // (a row is a multiple of 32 bytes)
+int64_t act_bytes(int width, int pairs, bool fp4) {  // (a row is a multiple of 64 bytes)
+  return static_cast<int64_t>(pairs) * (fp4 ? act_row<true>(width) : act_row<false>(width)) * 2;
 }
 
 template <int kSteps>
@@ -682,9 +740,10 @@ auto rows_kernel(bool full, bool wide) {
   // workgroup to a compute unit. 4 bits: two, with which there are still two workgroups
   // (four leave room for one: 256 Zipf tokens 103 us against 80).
   constexpr int kWide = kProduct == kUpBf16 ? (kSteps == 8 ? 4 : kSteps == 12 ? 2 : 1)
-                                            : (kProduct == kUpFp4 && kSteps == 8 ? 2 : 1);
+                                            : (kProduct == kDownFp4 || kSteps == 8 ? 2 : 1);
+  constexpr int kNarrow = kProduct == kDownFp4 ? 2 : 1;
   return wide ? full ? experts_rows_kernel<kProduct, kSteps, true, kWide> : experts_rows_kernel<kProduct, kSteps, false, kWide>
-              : full ? experts_rows_kernel<kProduct, kSteps, true, 1> : experts_rows_kernel<kProduct, kSteps, false, 1>;
+              : full ? experts_rows_kernel<kProduct, kSteps, true, kNarrow> : experts_rows_kernel<kProduct, kSteps, false, kNarrow>;
 }
 
 template <Product kProduct>
@@ -692,7 +751,7 @@ int launch_rows(ExpertArgs a, int items, bool wide, cfmoe_stream stream) {
   constexpr bool kFp4 = kProduct != kUpBf16, kDown = kProduct == kDownFp4;
   const int length = kDown ? a.width : a.hidden;
   const int units = kFp4 ? (length + 127) / 128 : length / 32;
-  const Cut cut = cut_of(units, kFp4);
+  const Cut cut = cut_of(units, kFp4, kDown);
   const int steps = cut.loads * (kFp4 ? 4 : 1);
   const bool full = units == cut.splits * cut.loads && length % 128 == 0;
   a.splits = cut.splits;
@@ -723,7 +782,7 @@ CFMOE_API int64_t cfmoe_routed_experts_scratch_bytes(int32_t hidden_size, int32_
   const int pairs = tokens * top_k;
   // activations, partials, and for more than 64 pairs the runs and the sorted pairs
   const int64_t sorted = pairs > 64 ? run_items(experts, pairs, 16) * sizeof(Run) + pairs * 2 : 0;
-  return act_bytes(width, pairs) + static_cast<int64_t>(pairs) * hidden_size * 4 + sorted;
+  return act_bytes(width, pairs, flags & CFMOE_FP4) + static_cast<int64_t>(pairs) * hidden_size * 4 + sorted;
 }
 
 CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t experts, int32_t top_k,
@@ -760,7 +819,7 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   a.hidden = hidden_size;
   a.width = width;
   a.act = static_cast<uint16_t *>(scratch);
-  a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + act_bytes(width, a.pairs));
+  a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + act_bytes(width, a.pairs, fp4));
   a.ids64 = flags & CFMOE_IDS_INT64;
   a.weights16 = flags & CFMOE_WEIGHTS_BF16;
   a.gelu = flags & CFMOE_GELU;
@@ -778,7 +837,7 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   if (a.pairs > 64) {
     const int most = !wide ? 16 : fp4 ? 32 : kMaxRun;
     items = run_items(experts, a.pairs, most);
-    Run *runs = reinterpret_cast<Run *>(static_cast<uint8_t *>(scratch) + act_bytes(width, a.pairs) +
+    Run *runs = reinterpret_cast<Run *>(static_cast<uint8_t *>(scratch) + act_bytes(width, a.pairs, fp4) +
                                         static_cast<int64_t>(a.pairs) * hidden_size * 4);
     uint16_t *sorted = reinterpret_cast<uint16_t *>(runs + run_items(experts, a.pairs, 16));
     hipLaunchKernelGGL(experts_sort_kernel, dim3(1), dim3(kSortThreads), 0, stream, a, runs, sorted, items, most);

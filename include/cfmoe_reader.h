@@ -280,8 +280,8 @@ CFMOE_API int cfmoe_dequantise_fp4(int64_t blocks, const void *codes, const uint
 
 /* The whole routed part of one layer for a batch of few tokens:
  *   out[t] = sum_k weights[t, k] D_e (phi(G_e x_t) * (U_e x_t)), e = ids[t, k]
- * with FP32 sums; the weighted activations are rounded to BF16 once, and so is
- * out [T, H]. gate_up [E, 2I, H] and down are bf16, down channel-major (physical
+ * with FP32 sums; the weighted activations are held as two BF16 numbers each (2^-16
+ * off), and out [T, H] is rounded once. gate_up [E, 2I, H] and down are bf16, down channel-major (physical
  * [E, I, H]) as for cfmoe_forward, and the scale pointers are unused; or with
  * CFMOE_FP4 both hold the codes of cfmoe_quantise_fp4 over the rows [E, 2I, H] and
  * [E, H, I], and gate_up_scales [E, 2I, H/32], down_scales [E, H, I/32] their

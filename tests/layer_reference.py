@@ -64,8 +64,8 @@ def layer(x: Tensor, gate_up: Tensor, down: Tensor, ids: Tensor, weights: Tensor
             da = w.abs() * (dp * u.abs() + (p.abs() + dp) * du)
             out[t] += d @ a
             size[t] += d.abs() @ a.abs()
-            # the activation's one rounding to BF16
-            off[t] += d.abs() @ (da + HALF_BF16 * (a.abs() + da))
+            # the activation as a sum of two BF16 numbers: half a step of half a step
+            off[t] += d.abs() @ (da + HALF_BF16 ** 2 * (a.abs() + da))
     off = off + (chain(width) + ids.shape[1] * STEP) * (size + off)
     return out, off + HALF_BF16 * (out.abs() + off)
 

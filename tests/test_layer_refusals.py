@@ -106,11 +106,11 @@ def test_routed_experts_refuses(arguments, words):
 
 def test_scratch_sizes():
     lib = _ext.library()
-    # activations [pairs, I] BF16 and one FP32 partial row per pair and split at least
+    # activations [pairs, 2, I] BF16 and one FP32 partial row per pair at least
     for flags in (0, _ext.FP4):
         for tokens in (1, 7, 500):
             size = lib.cfmoe_routed_experts_scratch_bytes(2048, 768, 128, 8, flags, tokens)
-            assert size >= tokens * 8 * (2 * 768 + 4 * 2048)
+            assert size >= tokens * 8 * (4 * 768 + 4 * 2048)
     assert lib.cfmoe_routed_experts_scratch_bytes(100, 64, 8, 2, 0, 1) == -_ext.EINVAL
     assert lib.cfmoe_route_scratch_bytes(3, 2000) == -_ext.EINVAL
 
