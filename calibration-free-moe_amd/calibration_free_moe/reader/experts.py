@@ -5,7 +5,7 @@ weights: what a runtime runs for layers that its plan leaves dense, for rows it
 does not send to the reader (the reference's runtime sends it decode rows only,
 runtime/experts.py:334-378), for an always-on shared expert (one expert, one id),
 and as the exact output a sparse one is compared with. With `Fp4Weights` it reads
-the experts in 4.25 bits a weight instead of 16. Three HIP launches on the
+the experts in 4.25 bits a weight instead of 16. Two to four HIP launches on the
 caller's stream (cfmoe_routed_experts in the reader's library). Forward only, as
 the reader.
 """
@@ -18,8 +18,6 @@ from torch import Tensor
 from calibration_free_moe.activation import GatedActivation
 from calibration_free_moe.reader import _ext
 from calibration_free_moe.reader.microscale import Fp4Weights
-
-MAX_PAIRS = 8192  # routed (token, slot) pairs of a call, as the reader's
 
 
 def routed_experts(
@@ -46,7 +44,7 @@ def routed_experts(
 
     H is a multiple of 128 and I of 16 (of 32 in 4 bits), both at most 4096; at
     most 4096 experts, 64 ids per token and 8192 pairs per call. Zero tokens give
-    an empty output. The scratch is allocated per call: calls may overlap on
+    an empty output; `out` may be `hidden`. The scratch is allocated per call: calls may overlap on
     different streams, and captured graphs share nothing.
     """
     fp4 = isinstance(gate_up, Fp4Weights)

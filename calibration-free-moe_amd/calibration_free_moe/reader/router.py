@@ -14,6 +14,7 @@ from torch import Tensor
 
 from calibration_free_moe.reader import _ext
 
+MAX_HIDDEN = 65536
 MAX_EXPERTS = 1024
 MAX_TOP_K = 64
 
@@ -41,8 +42,8 @@ def route(
 
     `out` takes (ids, weights) to write instead of new tensors; their types then
     stand for `ids_dtype` (int32 or int64) and `weights_dtype` (FP32 or BF16).
-    H is a multiple of 128, E at most 1024, top_k at most 64 and E. Zero tokens
-    give empty outputs. The work is enqueued on the current stream of the
+    H is a multiple of 128, at most 65536, E at most 1024, top_k at most 64 and E.
+    Zero tokens give empty outputs. The work is enqueued on the current stream of the
     tensors' device and can be captured in a graph.
     """
     if out is not None:
@@ -53,7 +54,7 @@ def route(
         or router.dim() != 2
         or hidden.shape[1] != router.shape[1]
         or hidden.shape[1] % 128
-        or not hidden.shape[1]
+        or not 0 < hidden.shape[1] <= MAX_HIDDEN
         or not 1 <= router.shape[0] <= MAX_EXPERTS
         or not 1 <= top_k <= min(MAX_TOP_K, router.shape[0])
         or hidden.dtype != torch.bfloat16
@@ -67,7 +68,7 @@ def route(
     ):
         raise ValueError(
             "Expected contiguous BF16 CUDA rows [tokens, H] and router [E, H] with H a multiple "
-            "of 128, at most 1024 experts and 64 kept, int32/int64 ids and FP32/BF16 weights"
+            "of 128 up to 65536, at most 1024 experts and 64 kept, int32/int64 ids and FP32/BF16 weights"
         )
     tokens, experts, device = hidden.shape[0], router.shape[0], hidden.device
     if expert_scale is not None and (

@@ -4,23 +4,38 @@
 //
 // A (token, slot) pair is one row of its expert's products. The layer's time is
 // that of reading every touched expert's weights once, so each workgroup owns a
-// piece of one expert's weights and computes it for all of that expert's pairs:
-// it gathers them from the ids itself (pairs of one expert, ascending), 16 to a
-// matrix instruction's columns. Three launches:
+// piece of one expert's weights and computes it for all of that expert's pairs, 16 to
+// a matrix instruction's columns. Three launches, and one ahead of them for more than
+// 64 pairs:
 //
+//   sort  the pairs of each expert, in runs (experts_sort_kernel)
 //   up    act[p, c] = w phi(g) u, g and u in FP32 (experts_rows_kernel)
-//   down  partial[p, h] = FP32 sum over the channels (experts_down_kernel over
-//         channel-major BF16 rows, experts_rows_kernel over 4-bit rows)
+//   down  partial[p, h] = FP32 sum over the channels (experts_down_kernel and
+//         experts_down_many_kernel over channel-major BF16 rows, experts_rows_kernel
+//         over 4-bit rows)
 //   join  out[t, h] = bf16(sum over t's slots, in order) (experts_join_kernel)
+//
+// Few tokens over 4-bit rows have down and join in one (experts_fp4_tokens_kernel).
+//
+// Measured with 128 experts of 2048 x 768, top 8, in microseconds (floor = the touched
+// weights at 6.0 TB/s):                sort   up   down  join  floor
+//   1 token, BF16                        -    13     7     4    12.6
+//   1 token, 4 bits                      -     7     7     -     3.3
+//   32 tokens, BF16                      5   124    68     5   179
+//   256 tokens, Zipf(1.2), BF16          5   168   110     7   197
+//   128 tokens, 4 bits                   5    55    43     5    53.6
+// Large BF16 calls read at 5.4-6.0 TB/s; small ones are the launches and one pass of
+// memory latency each.
 //
 // A pair whose id lies outside [0, E) or whose token is padded belongs to no
 // expert: nothing computes it, and the join leaves it out.
 //
 // The second product's matrix operand is BF16, so an activation (router weight and
 // all) is held as two BF16 numbers, high = bf16(v) and low = bf16(v - high), 2^-16 of
-// it off at most, and multiplied twice: the matrix cores have the time, and the
-// output's error stays that of its own rounding (one BF16 activation made it 1.45
-// times that).
+// it off at most, and multiplied twice: the output's error stays that of its own
+// rounding (one BF16 activation made it 1.45 times that). It costs BF16 layers nothing
+// to 3 us in 100 and 4-bit ones of many tokens 9 (128 tokens 94 us and 103); one token
+// has columns to spare.
 
 #include <algorithm>
 #include <type_traits>
@@ -80,8 +95,8 @@ __device__ __forceinline__ T load_at(const void *base, uint32_t offset) {
 // all of the batch's itself: an item is a pair (by_pair) or an expert, has all of the
 // expert's pairs, and of the pairs' items only an expert's first has any. (A single
 // token's pairs are left apart: its experts differ, or one named twice is read twice.)
-// Larger batches are sorted by a launch of their own, whose items are runs of at most
-// kMaxRun pairs: an expert that many tokens share takes several workgroups, one behind
+// Larger batches are sorted by a launch of their own (5 us; at 64 pairs, which need none,
+// 106 us are 111 with it), whose items are runs of at most kMaxRun pairs: an expert that many tokens share takes several workgroups, one behind
 // the other on its rows.
 constexpr int kMaxRun = 64;
 
@@ -612,7 +627,9 @@ __global__ __launch_bounds__(kThreads, kSteps <= 3 ? 4 : 2) void experts_down_ma
 
 // Few tokens over 4-bit rows: workgroup = 16 outputs of one token, its waves the
 // token's slots (every eighth), so that the slots' sum needs no launch of its own. An
-// expert that several tokens name is read for each of them.
+// expert that several tokens name is read for each of them: 128 experts of 2048 x 768
+// and top 8, one token 7 us, two 7 against 14 with the join, four 12 against 17, eight
+// 23 against 25, sixteen 41 against 32. A pair's high and low parts are columns in turn.
 __global__ __launch_bounds__(kThreads) void experts_fp4_tokens_kernel(ExpertArgs a) {
   constexpr int kAhead = 4;
   __shared__ f32x4 sums[kWaves][2][4];
@@ -702,7 +719,8 @@ int validate(int hidden, int width, int experts, int top_k, uint32_t flags, int 
 // How a row of `units` operand loads (32 BF16 values, or 128 in 4 bits) is cut: the
 // waves that share it, and each one's loads, one of the counts that kernels exist
 // for. Fewest idle loads first, then the most waves. The 4-bit down product takes two
-// loads where eight waves can: three want more registers than two workgroups have.
+// loads where eight waves can: three want more registers than two workgroups have
+// (width 768, 1024 pairs 43 us against 46).
 struct Cut {
   int splits, loads;
 };
@@ -756,7 +774,9 @@ int launch_rows(ExpertArgs a, int items, bool wide, cfmoe_stream stream) {
   const bool full = units == cut.splits * cut.loads && length % 128 == 0;
   a.splits = cut.splits;
   a.tiles = kDown ? a.hidden / kRows : a.width / (kRows / 2);
-  // enough workgroups to fill the chip, then fewer loads of the pairs' vectors
+  // Enough workgroups to fill the chip, then fewer loads of the pairs' vectors. (Narrow
+  // BF16 kernels, three workgroups to a compute unit: 2048 for 1024 make 16 tokens over
+  // 128 experts 94 us of 96, 32 over 64 97 of 99, those of 2816 x 704 135 of 129.)
   const int subs = kWaves / cut.splits;
   a.share = subs;
   while (static_cast<int64_t>(items) * a.tiles / (2 * a.share) >= (kFp4 || wide ? 1024 : 2048) && a.share < 8 * subs) a.share *= 2;
@@ -847,7 +867,7 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   }
 
   if (int rc = fp4 ? launch_rows<kUpFp4>(a, items, wide, stream) : launch_rows<kUpBf16>(a, items, wide, stream)) return rc;
-  if (fp4 && a.by_pair && tokens <= 4) {
+  if (fp4 && a.by_pair && tokens <= 4) {  // (experts_fp4_tokens_kernel: both sides)
     a.tiles = hidden_size / kRows;
     hipLaunchKernelGGL(experts_fp4_tokens_kernel, dim3(static_cast<unsigned>(a.tiles) * tokens), dim3(kThreads), 0,
                        stream, a);

@@ -25,7 +25,9 @@ __device__ __forceinline__ int quad_max(int v) {
 }
 
 // Lane = eight values of a block, a quad of lanes = the block; largest |v| by
-// integer compare of the bits (a NaN's are above infinity's).
+// integer compare of the bits (a NaN's are above infinity's). One pass at the rate of
+// memory: 403 M values 170 us from BF16 (1.02 GB, 6.0 TB/s), 323 from FP32 (1.83 GB, 5.7).
+// A small call is its launch: 18 us for 6.3 M values, the caller's allocations included.
 template <bool kFp32>
 __global__ __launch_bounds__(kThreads) void quantise_fp4_kernel(const void *weights, uint32_t *codes,
                                                                 uint8_t *scales, int64_t lanes) {
@@ -62,6 +64,7 @@ __global__ __launch_bounds__(kThreads) void quantise_fp4_kernel(const void *weig
   }
 }
 
+// 403 M values 183 us (1.02 GB, 5.6 TB/s).
 __global__ __launch_bounds__(kThreads) void dequantise_fp4_kernel(const uint32_t *codes,
                                                                   const uint8_t *scales, u32x4 *values,
                                                                   int64_t lanes) {

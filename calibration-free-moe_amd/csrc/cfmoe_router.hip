@@ -18,11 +18,9 @@
 namespace cfmoe {
 namespace {
 
-#ifndef BULK
-#define BULK 1024
-#endif
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTop = 64;
+constexpr int kMaxHidden = 65536;  // (offsets into the router's rows are 32 bits)
 constexpr int kTile = 16;          // experts, and tokens, of a matrix instruction
 constexpr int kSplitWaves = 16;    // waves that share a tile's hidden dimension
 constexpr int kBulkWaves = 16;     // of a bulk workgroup, two to an expert tile
@@ -88,7 +86,10 @@ __device__ __forceinline__ void accumulate(const u32x4 *r, const u32x4 *x, int f
 }
 
 // Few tiles: workgroup = 16 experts x 16 tokens, its waves every sixteenth 32 of the
-// hidden dimension.
+// hidden dimension, so that one token's router is read by as many loads at once as it
+// has (one workgroup for all experts, and the selection behind a barrier, took 20.7 us
+// for 128 experts of 2048 where these two launches take 5.2 and 2.7). Latency bounds it:
+// the router is 0.5 MB, 0.1 us of HBM.
 __global__ __launch_bounds__(64 * kSplitWaves) void router_logits_kernel(RouteArgs a) {
   __shared__ f32x4 sums[2][kSplitWaves][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -112,7 +113,11 @@ __global__ __launch_bounds__(64 * kSplitWaves) void router_logits_kernel(RouteAr
 // with half of the hidden dimension. The tokens' rows pass through LDS, 256 values of
 // either half a stage; the loads of all 2048 of a span leave at once and each stage is
 // written when its turn comes, so that only the first is waited for. Each wave streams
-// its experts' rows past them.
+// its experts' rows past them. What bounds it is that each workgroup reads the router's
+// 128 rows and its own tokens' from L2, 640 KB at 2048 values, about 35 GB/s a compute
+// unit: 19 us at 1500 tokens of 256 experts, 23 at 4001, for 3.4 us of matrix products.
+// (64 tokens to a workgroup leave too few workgroups; rows of another stride than
+// 4 KB measured the same.)
 __global__ __launch_bounds__(64 * kBulkWaves, 4) void router_bulk_kernel(RouteArgs a) {
   constexpr int kCols = kBulkTokens / kTile, kStage = 8, kStages = kBulkHidden / 64 / kStage;
   constexpr int kUnits = kStage * 4;                                   // 16 bytes of a half row's stage
@@ -422,7 +427,9 @@ __device__ __forceinline__ void select_token(const RouteArgs &a, int t, const fl
   else static_cast<float *>(a.weights)[at] = weight;
 }
 
-// Wave = one token.
+// Wave = one token. FP32 logits decide almost all orders; the FP64 dot products of those
+// left open are what a call of many tokens pays for ids that do not depend on how a sum
+// was split (9 us of 32 at 4001 tokens of 256 experts).
 template <int kValues>
 __global__ __launch_bounds__(64 * kSelectWaves) void router_select_kernel(RouteArgs a) {
   const int t = blockIdx.x * kSelectWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -447,7 +454,8 @@ CFMOE_API int64_t cfmoe_route_scratch_bytes(int32_t tokens, int32_t experts) {
 CFMOE_API int cfmoe_route(int32_t hidden_size, int32_t experts, int32_t top_k, uint32_t flags, const void *hidden,
                           const void *router, const float *expert_scale, void *ids, void *weights,
                           void *scratch, int32_t tokens, cfmoe_stream stream) {
-  if (hidden_size <= 0 || hidden_size % 128) return fail(CFMOE_EINVAL, "route needs a hidden size that is a multiple of 128");
+  if (hidden_size <= 0 || hidden_size % 128 || hidden_size > kMaxHidden)
+    return fail(CFMOE_EINVAL, "route needs a hidden size that is a multiple of 128, at most 65536");
   if (experts < 1 || experts > kMaxExperts) return fail(CFMOE_EINVAL, "route needs 1 to 1024 experts");
   if (top_k < 1 || top_k > kMaxTop || top_k > experts)
     return fail(CFMOE_EINVAL, "route keeps 1 to 64 experts, no more than there are");
@@ -475,13 +483,18 @@ CFMOE_API int cfmoe_route(int32_t hidden_size, int32_t experts, int32_t top_k, u
   a.renormalise = flags & CFMOE_RENORMALISE;
   const int64_t tiles = static_cast<int64_t>(a.tiles) * ((tokens + kTile - 1) / kTile);
   if (tiles > 0x1fffff) return fail(CFMOE_EINVAL, "route has too many tokens for one launch");
-  // 32 products inside a matrix instruction, one addition for each of a chain of
-  // them, and the waves' sums
-  if (tiles <= BULK) {
+  // The few-tile kernel reads the router's rows once for 16 tokens, the bulk one for 32
+  // from more of the chip's caches, but a workgroup of its takes 18 us however few there
+  // are: at 600 tokens of 256 experts (608 tiles) 20.6 us against 25.4, at 1024 of 128
+  // (512) 18.2 against 25.3, at 2048 of 128 (1024) 25.8 against 26.4, at 1500 of 256
+  // (1504) 33.2 against 27.7, at 3000 of 128 (1504) 33.0 against 26.6, with the selection.
+  // `chain`: 32 products inside a matrix instruction, one addition for each of a chain
+  // of them, and the waves' sums.
+  if (tiles <= 1024) {
     a.chain = 32 + (hidden_size / 32 + kSplitWaves - 1) / kSplitWaves + kSplitWaves;
     hipLaunchKernelGGL(router_logits_kernel, dim3(static_cast<unsigned>(tiles)), dim3(64 * kSplitWaves), 0, stream, a);
   } else {
-    a.chain = 32 + hidden_size / 32;
+    a.chain = 32 + hidden_size / 64 + 1;
     const int groups = (a.tiles + kBulkWaves / 2 - 1) / (kBulkWaves / 2) * ((tokens + kBulkTokens - 1) / kBulkTokens);
     hipLaunchKernelGGL(router_bulk_kernel, dim3(groups), dim3(64 * kBulkWaves), 0, stream, a);
   }

@@ -255,8 +255,8 @@ CFMOE_API int64_t cfmoe_noalloc_scratch_bytes(void);
  * expert, NaN above all; the order is that of the exact logits), their softmax
  * weights, times expert_scale [E] fp32 unless NULL. flags: CFMOE_IDS_INT64,
  * CFMOE_WEIGHTS_BF16, CFMOE_RENORMALISE. ids and weights are [T, top_k], as
- * cfmoe_forward and cfmoe_routed_experts take them. H a multiple of 128, E at
- * most 1024, top_k at most 64. scratch: cfmoe_route_scratch_bytes(T, E) bytes,
+ * cfmoe_forward and cfmoe_routed_experts take them. H a multiple of 128, at most
+ * 65536, E at most 1024, top_k at most 64. scratch: cfmoe_route_scratch_bytes(T, E) bytes,
  * 16-byte aligned like hidden and router; calls that overlap need their own.
  * T = 0 does nothing. The reference leaves routing to its host runtime. */
 CFMOE_API int64_t cfmoe_route_scratch_bytes(int32_t tokens, int32_t experts);
@@ -281,16 +281,17 @@ CFMOE_API int cfmoe_dequantise_fp4(int64_t blocks, const void *codes, const uint
 /* The whole routed part of one layer for a batch of few tokens:
  *   out[t] = sum_k weights[t, k] D_e (phi(G_e x_t) * (U_e x_t)), e = ids[t, k]
  * with FP32 sums; the weighted activations are held as two BF16 numbers each (2^-16
- * off), and out [T, H] is rounded once. gate_up [E, 2I, H] and down are bf16, down channel-major (physical
- * [E, I, H]) as for cfmoe_forward, and the scale pointers are unused; or with
- * CFMOE_FP4 both hold the codes of cfmoe_quantise_fp4 over the rows [E, 2I, H] and
+ * off), and out [T, H] is rounded once. gate_up [E, 2I, H] and down are bf16, down
+ * channel-major (physical [E, I, H]) as for cfmoe_forward, and the scale pointers are
+ * unused; or with CFMOE_FP4 both hold the codes of cfmoe_quantise_fp4 over the rows [E, 2I, H] and
  * [E, H, I], and gate_up_scales [E, 2I, H/32], down_scales [E, H, I/32] their
  * scales. ids outside [0, E) contribute nothing; rows marked in padding uint8 [T]
  * (or NULL) read no weights and come out zero. flags: CFMOE_GELU,
  * CFMOE_IDS_INT64, CFMOE_WEIGHTS_BF16, CFMOE_FP4. H a multiple of 128, I of 16 (of
  * 32 with CFMOE_FP4), both at most 4096; E at most 4096, top_k 64, T top_k 8192.
- * Weights, scales, hidden, out and scratch are 16-byte aligned. scratch: cfmoe_routed_experts_scratch_bytes of the same
- * arguments; calls that overlap need their own. T = 0 does nothing. */
+ * Weights, scales, hidden, out and scratch are 16-byte aligned; out may be hidden
+ * itself. scratch: cfmoe_routed_experts_scratch_bytes of the same arguments; calls
+ * that overlap need their own. T = 0 does nothing. */
 CFMOE_API int64_t cfmoe_routed_experts_scratch_bytes(int32_t hidden_size, int32_t width,
                                                      int32_t experts, int32_t top_k,
                                                      uint32_t flags, int32_t tokens);

@@ -73,6 +73,11 @@ SHAPES = [  # tokens, hidden, width, experts, top-k
     (1, 128, 32, 1, 1), (1, 2048, 768, 16, 8), (2, 256, 96, 4, 4), (3, 2816, 704, 8, 2),
     (5, 512, 160, 32, 6), (13, 384, 64, 3, 2), (16, 640, 352, 8, 3), (31, 256, 512, 64, 8),
     (40, 256, 64, 2, 1), (64, 256, 128, 8, 8), (100, 128, 96, 5, 3), (130, 256, 64, 2, 2),
+    # about the largest batch that is not sorted
+    (64, 256, 64, 70, 1), (65, 256, 64, 70, 1), (16, 256, 64, 20, 4), (13, 256, 64, 100, 5),
+    # long rows and wide layers, few pairs an expert and many
+    (3, 4096, 1056, 3, 2), (70, 4096, 64, 3, 2), (9, 1152, 2080, 2, 2), (60, 1152, 2080, 2, 2),
+    (50, 2816, 96, 4, 2), (2, 128, 4096, 2, 1), (33, 128, 4096, 2, 2), (4, 128, 32, 4096, 64),
 ]
 
 
@@ -198,3 +203,14 @@ def test_offsets_past_32_bits():
                          case.weights.to(DEVICE))
     want, bound = plain.layer(case.x, case.gate_up, case.down, case.ids, case.weights)
     assert bool(((got.cpu().double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("fp4", [False, True], ids=["bf16", "fp4"])
+@pytest.mark.parametrize("tokens", [2, 40])
+def test_out_may_be_the_rows(tokens, fp4):
+    case = Case(tokens, 256, 96, 16, 4, fp4=fp4, seed=8)
+    want = case.run()
+    rows = case.x.to(DEVICE)
+    got = routed_experts(rows, *case.device_weights(), case.ids.to(DEVICE), case.weights.to(DEVICE),
+                         None, rows)
+    assert got is rows and torch.equal(rows, want)

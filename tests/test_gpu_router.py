@@ -38,7 +38,8 @@ def check(x, router, top_k, **options):
 @pytest.mark.parametrize("tokens,hidden,experts,top_k", [
     (1, 128, 1, 1), (1, 2048, 128, 8), (2, 256, 8, 8), (15, 384, 17, 3), (16, 640, 64, 6),
     (17, 2816, 128, 8), (33, 1024, 65, 1), (130, 2048, 256, 8), (300, 512, 250, 10),
-    (5, 256, 1024, 64), (3, 256, 64, 64), (4, 4096, 513, 33),
+    (5, 256, 1024, 64), (3, 256, 64, 64), (4, 4096, 513, 33), (2, 65536, 20, 4),
+    (300, 2176, 1000, 3), (900, 4480, 300, 5),
 ])
 @pytest.mark.parametrize("renormalise", [True, False])
 def test_random_rows(tokens, hidden, experts, top_k, renormalise):

@@ -60,7 +60,7 @@ def call_route(hidden=256, experts=8, top_k=2, x=AT, router=AT, ids=AT, scratch=
 
 @pytest.mark.parametrize("arguments,words", [
     (dict(hidden=200), "multiple of 128"), (dict(hidden=0), "multiple of 128"),
-    (dict(experts=0), "1 to 1024"), (dict(experts=1025), "1 to 1024"),
+    (dict(hidden=65664), "at most 65536"), (dict(experts=0), "1 to 1024"), (dict(experts=1025), "1 to 1024"),
     (dict(top_k=0), "1 to 64"), (dict(top_k=9), "no more than there are"),
     (dict(experts=100, top_k=65), "1 to 64"), (dict(tokens=-1), "zero or more"),
     (dict(x=None), "NULL"), (dict(router=None), "NULL"), (dict(ids=None), "NULL"),
