@@ -23,7 +23,7 @@
 //   1 token, 4 bits                      -     7     7     -     3.3
 //   32 tokens, BF16                      5   124    68     5   179
 //   256 tokens, Zipf(1.2), BF16          5   168   110     7   197
-//   128 tokens, 4 bits                   5    55    43     5    53.6
+//   128 tokens, 4 bits                   5    51    37     5    53.6
 // Large BF16 calls read at 5.4-6.0 TB/s; small ones are the launches and one pass of
 // memory latency each.
 //
@@ -34,8 +34,8 @@
 // all) is held as two BF16 numbers, high = bf16(v) and low = bf16(v - high), 2^-16 of
 // it off at most, and multiplied twice: the output's error stays that of its own
 // rounding (one BF16 activation made it 1.45 times that). It costs BF16 layers nothing
-// to 3 us in 100 and 4-bit ones of many tokens 9 (128 tokens 94 us and 103); one token
-// has columns to spare.
+// to 3 us in 100 and the 4-bit down product of many tokens a third (128 tokens 31 us and
+// 43, since then 37); one token has columns to spare.
 
 #include <algorithm>
 #include <type_traits>
@@ -235,7 +235,8 @@ __device__ __forceinline__ float parts_sum(float v) {
 enum Product { kUpBf16, kUpFp4, kDownFp4 };
 
 // Weight rows times the pairs' vectors. `splits` waves share a row's products, the
-// others take further row tiles, and a round's sums meet in LDS. A wave keeps its
+// others take further row tiles, and the sums of a round, kBatch tiles of each wave, meet
+// in LDS. A wave keeps its
 // piece of the pairs' vectors in registers as matrix operands, kSteps products of 32
 // for kCols x 16 pairs, and multiplies its rows by them (a column past the last pair
 // repeats it; nothing of it is stored).
@@ -250,7 +251,7 @@ enum Product { kUpBf16, kUpFp4, kDownFp4 };
 // Unless kFull a wave may hold fewer loads than the kernel has: it repeats its last
 // one with every bit cleared, weights and vectors both, so that what a row holds
 // cannot reach the sum a second time.
-template <Product kProduct, int kSteps, bool kFull, int kCols>
+template <Product kProduct, int kSteps, bool kFull, int kCols, int kBatch>
 struct RowPass {
   static constexpr bool kFp4 = kProduct != kUpBf16, kDown = kProduct == kDownFp4;
   static constexpr int kLoads = kFp4 ? kSteps / 4 : kSteps;
@@ -266,7 +267,7 @@ struct RowPass {
     const int length = kDown ? a.width : a.hidden;
     const int units = kFp4 ? (length + 127) / 128 : length / 32;
     const int begin = units * split / a.splits, steps = units * (split + 1) / a.splits - begin;
-    const int rounds = (last - first + subs - 1) / subs;
+    const int rounds = (last - first + subs * kBatch - 1) / (subs * kBatch);
     const uint32_t row_bytes = kFp4 ? length / 2 : length * 2, scale_bytes = length / 32;
     // the lane's row of a tile: in the up product gate and up row of a channel in turn
     const uint32_t row = kDown ? lane % 16 : (lane & 1) * a.width + lane % 16 / 2;
@@ -283,19 +284,20 @@ struct RowPass {
     // (steps >= 1: cut_of takes no more waves than there are units)
     auto unit = [&](int i) { return kFull ? i : min(i, steps - 1); };
 
-    u32x4 words[kLoads];
-    auto load = [&](int r) {
-      const int tile = min(first + r * subs + sub, last - 1);
+    u32x4 words[kBatch][kLoads];
+    auto load = [&](int r, int of) {
+      const int tile = min(first + (r * kBatch + of) * subs + sub, last - 1);
       const int64_t row0 = kDown ? static_cast<int64_t>(expert) * a.hidden + tile * kRows
                                  : static_cast<int64_t>(expert) * 2 * a.width + tile * (kRows / 2);
       const uint8_t *w = (kDown ? a.down : a.gate_up) + row0 * row_bytes + begin * 64;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const bool whole = kFull || !kFp4 || own(unit(i));
-        words[i] = load_at<u32x4>(w + unit(i) * 64, whole ? lane_row : lane_row - lane / 16 * 16);
+        words[of][i] = load_at<u32x4>(w + unit(i) * 64, whole ? lane_row : lane_row - lane / 16 * 16);
       }
     };
-    load(0);
+#pragma unroll
+    for (int of = 0; of < kBatch; ++of) load(0, of);
     ready();
     u32x4 b[kCols][kSteps];
 #pragma unroll
@@ -322,14 +324,14 @@ struct RowPass {
     const uint32_t to = kDown ? pair * a.hidden + lane / 16 * 4 : pair * act_row<kFp4>(a.width);
     const float weight = kDown ? 0.0f : pair_weight(a, pair);
 
-    auto product = [&](int r) {
+    auto product = [&](int r, int of) {
       f32x4 d[kCols];
 #pragma unroll
       for (int n = 0; n < kCols; ++n) d[n] = f32x4{0, 0, 0, 0};
-      const int kept = min(r * subs + sub, last - 1 - first) * (kDown ? kRows : kRows / 2) * scale_bytes;
+      const int kept = min((r * kBatch + of) * subs + sub, last - 1 - first) * (kDown ? kRows : kRows / 2) * scale_bytes;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const u32x4 w = words[i] & own(i);
+        const u32x4 w = words[of][i] & own(i);
         if constexpr (kFp4) {
           const uint32_t byte = lane_scales[kept + 4 * unit(i) + (own(unit(i)) ? lane / 16 : 0)];
           const float by = __uint_as_float((byte & own(i)) << 23);
@@ -346,7 +348,7 @@ struct RowPass {
       }
       // (the sums alternate between two buffers: what a round overwrites was read
       // before the last barrier)
-      f32x4 *in = sums + (r & 1) * (kWaves * kSums * 64) + lane;
+      f32x4 *in = sums + ((r & 1) * kBatch + of) * (kWaves * kSums * 64) + lane;
       if constexpr (kDown) {
         f32x4 both;
 #pragma unroll
@@ -363,12 +365,12 @@ struct RowPass {
     };
     auto add = [&](int r) {
       __syncthreads();
-      const f32x4 *in = sums + (r & 1) * (kWaves * kSums * 64) + lane;
-      for (int i = wave; i < subs * kSums; i += kWaves) {
-        const int tile = first + r * subs + i / kSums;
+      for (int i = wave; i < kBatch * subs * kSums; i += kWaves) {
+        const int tile = first + r * kBatch * subs + i / kSums;
         if (!stores || tile >= last) break;
-        f32x4 v = in[(i / kSums * a.splits * kSums + i % kSums) * 64];
-        for (int w = 1; w < a.splits; ++w) v += in[((i / kSums * a.splits + w) * kSums + i % kSums) * 64];
+        const f32x4 *in = sums + ((r & 1) * kBatch + i / (subs * kSums)) * (kWaves * kSums * 64) + lane;
+        f32x4 v = in[(i / kSums % subs * a.splits * kSums + i % kSums) * 64];
+        for (int w = 1; w < a.splits; ++w) v += in[((i / kSums % subs * a.splits + w) * kSums + i % kSums) * 64];
         if (kDown)
           *reinterpret_cast<f32x4 *>(a.partial + (to + tile * kRows)) = v;
         else
@@ -377,15 +379,19 @@ struct RowPass {
       }
     };
     // The rows' registers are free once multiplied: the next round's loads leave before
-    // this one's sums are added up. (More rounds on their way measured the same or worse:
-    // two to eight of one load each over eight waves made the 4-bit down product 41 to
-    // 59 us, 1024 pairs, against 43.)
+    // this one's sums are added up. (Rounds on their way ahead of that, with a barrier
+    // for each, measured the same or worse: two to eight of one load a wave made the
+    // 4-bit down product 41 to 59 us, 1024 pairs, where kBatch 1 made it 43.)
     for (int r = 0; r + 1 < rounds; ++r) {
-      product(r);
-      load(r + 1);
+#pragma unroll
+      for (int of = 0; of < kBatch; ++of) {
+        product(r, of);
+        load(r + 1, of);
+      }
       add(r);
     }
-    product(rounds - 1);
+#pragma unroll
+    for (int of = 0; of < kBatch; ++of) product(rounds - 1, of);
     add(rounds - 1);
     __syncthreads();
   }
@@ -393,10 +399,10 @@ struct RowPass {
 
 // Workgroup = `share` row tiles of one item, for all of its pairs, up to kMaxCols x 16
 // at a time. Dynamic LDS: the scales of its rows.
-template <Product kProduct, int kSteps, bool kFull, int kMaxCols>
+template <Product kProduct, int kSteps, bool kFull, int kMaxCols, int kBatch>
 __global__ __launch_bounds__(kThreads, kMaxCols <= 2 && kSteps <= 8 ? 4 : 2) void experts_rows_kernel(ExpertArgs a) {
   constexpr bool kFp4 = kProduct != kUpBf16, kDown = kProduct == kDownFp4;
-  __shared__ f32x4 sums[2 * kWaves * (kDown ? 1 : kMaxCols) * 64];
+  __shared__ f32x4 sums[2 * kBatch * kWaves * (kDown ? 1 : kMaxCols) * 64];
   __shared__ uint16_t list[kMaxRun];
   extern __shared__ __align__(16) uint8_t lds[];
   const Pairs pairs(a, blockIdx.x / a.groups);
@@ -417,7 +423,7 @@ __global__ __launch_bounds__(kThreads, kMaxCols <= 2 && kSteps <= 8 ? 4 : 2) voi
       reinterpret_cast<u32x4 *>(lds)[i] = load_at<u32x4>(scales, part * a.width * scale_bytes + chunk * 16);
   }
 
-  constexpr int kPairs = RowPass<kProduct, kSteps, kFull, 1>::kPairs;
+  constexpr int kPairs = RowPass<kProduct, kSteps, kFull, 1, kBatch>::kPairs;
   for (int base = 0; base < count;) {
     const int left = count - base;
     auto ready = [&] {
@@ -426,14 +432,14 @@ __global__ __launch_bounds__(kThreads, kMaxCols <= 2 && kSteps <= 8 ? 4 : 2) voi
     };
     if (kMaxCols >= 4 && left > 2 * kPairs) {
       if constexpr (kMaxCols >= 4)
-        RowPass<kProduct, kSteps, kFull, 4>::run(a, expert, first, last, list, count, base, sums, lds, ready);
+        RowPass<kProduct, kSteps, kFull, 4, kBatch>::run(a, expert, first, last, list, count, base, sums, lds, ready);
       base += 4 * kPairs;
     } else if (kMaxCols >= 2 && left > kPairs) {
       if constexpr (kMaxCols >= 2)
-        RowPass<kProduct, kSteps, kFull, 2>::run(a, expert, first, last, list, count, base, sums, lds, ready);
+        RowPass<kProduct, kSteps, kFull, 2, kBatch>::run(a, expert, first, last, list, count, base, sums, lds, ready);
       base += 2 * kPairs;
     } else {
-      RowPass<kProduct, kSteps, kFull, 1>::run(a, expert, first, last, list, count, base, sums, lds, ready);
+      RowPass<kProduct, kSteps, kFull, 1, kBatch>::run(a, expert, first, last, list, count, base, sums, lds, ready);
       base += kPairs;
     }
   }
@@ -720,9 +726,10 @@ int validate(int hidden, int width, int experts, int top_k, uint32_t flags, int 
 
 // How a row of `units` operand loads (32 BF16 values, or 128 in 4 bits) is cut: the
 // waves that share it, and each one's loads, one of the counts that kernels exist
-// for. Fewest idle loads first, then the most waves. The 4-bit down product takes two
-// loads where eight waves can: three want more registers than two workgroups have
-// (width 768, 1024 pairs 43 us against 46).
+// for. Fewest idle loads first, then the most waves. The 4-bit down product takes one
+// load a wave where that leaves none idle (width 1024, 512 pairs of 64 experts, 23 us
+// against 27 of two; width 768 40 against 38), and two where eight waves can: three want
+// more registers than two workgroups have (46 against 43).
 struct Cut {
   int splits, loads;
 };
@@ -730,8 +737,9 @@ struct Cut {
 Cut cut_of(int units, bool fp4, bool down) {
   Cut best = {0, 0};
   for (int splits = kWaves; splits >= 1; splits /= 2)
-    for (int loads : {fp4 ? 2 : 8, fp4 ? 3 : 12, fp4 ? 4 : 16})
-      if (loads * splits >= units && !(down && loads > 2 && units <= 2 * kWaves) && (!best.splits || loads * splits < best.loads * best.splits))
+    for (int loads : {down && splits == units ? 1 : fp4 ? 2 : 8, fp4 ? 2 : 8, fp4 ? 3 : 12, fp4 ? 4 : 16})
+      if (loads * splits >= units && !(down && loads > 2 && units <= 2 * kWaves) &&
+          (!best.splits || loads * splits < best.loads * best.splits))
         best = {splits, loads};
   return best;
 }
@@ -754,16 +762,34 @@ auto down_kernel(bool many, Steps mode) {
                            : experts_down_kernel<kSteps, kHalfStep>;
 }
 
+// Tiles of a wave between two barriers, where its workgroup has as many: what the
+// registers hold with two workgroups to a compute unit, of 4-bit rows only. (128 tokens
+// over 128 experts of 2048 x 768: up product 52 us against 55, down 38 against 43; 64
+// tokens over 64 of 2048 x 1024: 34 against 40, 23 against 28.)
 template <Product kProduct, int kSteps>
-auto rows_kernel(bool full, bool wide) {
+constexpr int batch_tiles(bool wide) {
+  if (kProduct == kUpBf16 || kSteps > 8) return 1;
+  return wide || (kProduct == kDownFp4 && kSteps == 8) ? 2 : 4;
+}
+
+template <Product kProduct, int kSteps>
+auto rows_kernel(bool full, bool wide, int tiles) {
   // Column tiles of a wide kernel. BF16: as many as the registers hold with one
   // workgroup to a compute unit. 4 bits: two, with which there are still two workgroups
   // (four leave room for one: 256 Zipf tokens 103 us against 80).
   constexpr int kWide = kProduct == kUpBf16 ? (kSteps == 8 ? 4 : kSteps == 12 ? 2 : 1)
-                                            : (kProduct == kDownFp4 || kSteps == 8 ? 2 : 1);
+                                            : (kProduct == kDownFp4 || kSteps <= 8 ? 2 : 1);
   constexpr int kNarrow = kProduct == kDownFp4 ? 2 : 1;
-  return wide ? full ? experts_rows_kernel<kProduct, kSteps, true, kWide> : experts_rows_kernel<kProduct, kSteps, false, kWide>
-              : full ? experts_rows_kernel<kProduct, kSteps, true, kNarrow> : experts_rows_kernel<kProduct, kSteps, false, kNarrow>;
+  constexpr int kBatch = batch_tiles<kProduct, kSteps>(false), kWideBatch = batch_tiles<kProduct, kSteps>(true);
+  if (wide)
+    return tiles >= kWideBatch ? full ? experts_rows_kernel<kProduct, kSteps, true, kWide, kWideBatch>
+                                      : experts_rows_kernel<kProduct, kSteps, false, kWide, kWideBatch>
+                               : full ? experts_rows_kernel<kProduct, kSteps, true, kWide, 1>
+                                      : experts_rows_kernel<kProduct, kSteps, false, kWide, 1>;
+  return tiles >= kBatch ? full ? experts_rows_kernel<kProduct, kSteps, true, kNarrow, kBatch>
+                                : experts_rows_kernel<kProduct, kSteps, false, kNarrow, kBatch>
+                         : full ? experts_rows_kernel<kProduct, kSteps, true, kNarrow, 1>
+                                : experts_rows_kernel<kProduct, kSteps, false, kNarrow, 1>;
 }
 
 template <Product kProduct>
@@ -783,9 +809,12 @@ int launch_rows(ExpertArgs a, int items, bool wide, cfmoe_stream stream) {
   a.share = subs;
   while (static_cast<int64_t>(items) * a.tiles / (2 * a.share) >= (kFp4 || wide ? 1024 : 2048) && a.share < 8 * subs) a.share *= 2;
   a.groups = (a.tiles + a.share - 1) / a.share;
-  const auto kernel = steps <= 8    ? rows_kernel<kProduct, 8>(full, wide)
-                      : steps <= 12 ? rows_kernel<kProduct, 12>(full, wide)
-                                    : rows_kernel<kProduct, 16>(full, wide);
+  const int tiles = a.share / subs;  // of a wave
+  auto kernel = steps <= 8    ? rows_kernel<kProduct, 8>(full, wide, tiles)
+                : steps <= 12 ? rows_kernel<kProduct, 12>(full, wide, tiles)
+                              : rows_kernel<kProduct, 16>(full, wide, tiles);
+  if constexpr (kDown)
+    if (steps <= 4) kernel = rows_kernel<kProduct, 4>(full, wide, tiles);
   const unsigned scales = kFp4 ? a.share * kRows * (length / 32) : 0;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.groups) * items), dim3(kThreads), scales, stream, a);
   return check_launch(kDown ? "experts_down" : "experts_up");

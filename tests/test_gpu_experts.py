@@ -133,6 +133,16 @@ def test_skewed_routing_of_many_pairs(fp4):
     Case(300, 128, 64, 12, 4, fp4=fp4, zipf=True).check()
 
 
+@pytest.mark.parametrize("shape", [
+    (1750, 256, 256, 600, 4), (875, 128, 768, 300, 4), (1024, 128, 256, 300, 8),
+    (1024, 128, 224, 300, 8), (800, 256, 512, 600, 4),
+], ids=str)
+@pytest.mark.parametrize("fp4", [False, True], ids=["bf16", "fp4"])
+def test_rounds_of_several_tiles(shape, fp4):
+    """So many runs that a workgroup has several tiles for each of its waves."""
+    Case(*shape, fp4=fp4).check()
+
+
 @pytest.mark.parametrize("fp4", [False, True], ids=["bf16", "fp4"])
 def test_the_largest_call(fp4):
     """8192 pairs; a sample of rows against the reference, more of them are refused."""
