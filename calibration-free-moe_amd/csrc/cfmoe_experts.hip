@@ -236,10 +236,9 @@ enum Product { kUpBf16, kUpFp4, kDownFp4 };
 
 // Weight rows times the pairs' vectors. `splits` waves share a row's products, the
 // others take further row tiles, and the sums of a round, kBatch tiles of each wave, meet
-// in LDS. A wave keeps its
-// piece of the pairs' vectors in registers as matrix operands, kSteps products of 32
-// for kCols x 16 pairs, and multiplies its rows by them (a column past the last pair
-// repeats it; nothing of it is stored).
+// in LDS. A wave keeps its piece of the pairs' vectors in registers as matrix operands,
+// kSteps products of 32 for kCols x kPairs pairs, and multiplies its rows by them (a
+// column past the last pair repeats it; nothing of it is stored).
 //
 // BF16: a lane's 16 bytes are eight values, step j the wave's j-th 32. FP4: they
 // are a whole block of 32, lane group g taking block g of 128 values, so that
@@ -879,8 +878,10 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   // the others' of 16. Wide pays where experts have more than 16 pairs: BF16 from six an
   // expert on average, since skewed routing gains more than uniform loses (128 tokens
   // over 128 experts, top 8: uniform 175 us against 171, Zipf(1.2) 232 against 249; 64
-  // experts' 64 tokens of Zipf(1.2) 164 against 179), 4-bit rows from twelve (128 tokens
-  // 94 and 98 us, 256 tokens' up product 80 and 67).
+  // experts' 64 tokens of Zipf(1.2) 164 against 179), 4-bit rows from twelve (whole calls:
+  // 128 tokens over 128 experts 97 us and 98, 256 tokens 130 and 131, of Zipf(1.2) 152 and
+  // 153, 512 tokens 202 and 213: the up product gains what the down product, one 16 pairs
+  // behind the other, loses; two items of a run for it took longer, 80 us for 74).
   const bool wide = a.pairs >= (fp4 ? 12 : 6) * experts;
   int items = a.by_pair ? a.pairs : experts;
   a.runs = nullptr;
