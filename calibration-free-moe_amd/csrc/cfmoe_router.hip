@@ -341,12 +341,17 @@ __device__ __forceinline__ void select_token(const RouteArgs &a, int t, const fl
   int expert;
   select<kValues>(v, a.experts, most, lane, value32, expert);
   const float next = __shfl_down(value32, 1);
-  // (written so that a NaN or infinity in between counts as open; 64 kept of more:
-  // what follows them was not looked at)
-  const bool unsure = (lane + 1 < most && !(value32 - next > open)) || most < wanted;
+  // (written so that a NaN or infinity in between counts as open, and so does a single
+  // expert's where FP32 may have overflowed; 64 kept of more: what follows them was not
+  // looked at)
+  const bool unsure = (lane + 1 < most && !(value32 - next > open)) || most < wanted || (lane == 0 && !(open < INFINITY));
   const uint64_t unsure_lanes = __ballot(unsure);
   double value = value32;
+  // The softmax over all experts adds up FP32 logits, unless some may have overflowed.
+  // All are open then: their exact values are in the lanes, or v has them less the first.
+  bool overflowed = false;
   if (unsure_lanes != 0) {
+    overflowed = !(open < INFINITY);
     const float cut = __shfl(value32, a.top_k - 1);
     int near = 0;  // experts that are kept or might be
 #pragma unroll
@@ -402,6 +407,9 @@ __device__ __forceinline__ void select_token(const RouteArgs &a, int t, const fl
         }
       }
       select<kValues>(exact, a.experts, a.top_k, lane, value, expert);
+      const double first = __shfl(value, 0);
+#pragma unroll
+      for (int j = 0; j < kValues; ++j) v[j] = overflowed ? static_cast<float>(exact[j] - first) : v[j];
     }
   }
 
@@ -412,9 +420,13 @@ __device__ __forceinline__ void select_token(const RouteArgs &a, int t, const fl
     total = wave_sum(share);
   } else {
     float part = 0.0f;
+    if (overflowed && a.experts <= most) {
+      part = lane < a.experts ? expf(static_cast<float>(value - first)) : 0.0f;
+    } else {
 #pragma unroll
-    for (int j = 0; j < kValues; ++j)
-      part += 64 * j + lane < a.experts ? expf(static_cast<float>(v[j] - first)) : 0.0f;
+      for (int j = 0; j < kValues; ++j)
+        part += 64 * j + lane < a.experts ? expf(overflowed ? v[j] : static_cast<float>(v[j] - first)) : 0.0f;
+    }
     total = wave_sum(part);
   }
   if (lane >= a.top_k) return;
