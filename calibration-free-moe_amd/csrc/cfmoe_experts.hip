@@ -31,7 +31,7 @@
 // expert: nothing computes it, and the join leaves it out.
 //
 // The second product's matrix operand is BF16, so an activation (router weight and
-// all) is held as two BF16 numbers, high = bf16(v) and low = bf16(v - high), 2^-16 of
+// all) is held as two BF16 numbers, high = v cut off and low = bf16(v - high), 2^-16 of
 // it off at most, and multiplied twice: the output's error stays that of its own
 // rounding (one BF16 activation made it 1.45 times that). It costs BF16 layers nothing
 // to 3 us in 100 and the 4-bit down product of many tokens a third (128 tokens 31 us and
@@ -212,15 +212,31 @@ __device__ __forceinline__ uint32_t act_place(uint32_t piece) {
   return 16 * (kFp4 ? (piece & ~15u) + piece % 4 * 4 + piece / 4 % 4 : piece);
 }
 
+// A value's high part: the BF16 number next below it in size, so that the rest is never 0
+// and has its sign. (Against an infinite weight a rest of 0 or of the other sign makes a
+// NaN of what is infinite. To nearest, the high part of a value above 3.39e38 would be
+// infinite; the rest off by 2^-17 of the value where it is 2^-16 now.) An infinity's is
+// the largest number. Below 2^-132 both parts are 2^-133, the least BF16 number.
+__device__ __forceinline__ void split(float v, uint32_t &high, float &low) {
+  const uint32_t sign = __float_as_uint(v) & 0x80000000u, size = __float_as_uint(v) & 0x7fffffffu;
+  const uint32_t least = min(size, 1u) << 16;
+  const uint32_t part = max(__builtin_elementwise_sub_sat(size, 1u) & 0xffff0000u, least);
+  // (a NaN stays in the high part: it is quiet, its bits well above infinity's)
+  const float rest = fmaxf(__uint_as_float(size) - __uint_as_float(part), __uint_as_float(least));
+  high = part | sign;
+  low = __uint_as_float(__float_as_uint(rest) | sign);
+}
+
 // Both parts of a piece at element `to`, of which lane l, l + 16, l + 32 and l + 48 have
 // two channels each: after two swaps, of half waves and of odd with even quarters, two
 // words that stand side by side. (A store for each part took a sixth of the up product's
-// time.) An infinity or NaN has no low part: it would be NaN, and an infinite sum with it.
+// time.)
 __device__ __forceinline__ void store_activations(const ExpertArgs &a, uint32_t to, float first, float second) {
-  const uint32_t high = bf16_pair(first, second);
-  const float high0 = __uint_as_float(high << 16), high1 = __uint_as_float(high & 0xffff0000u);
-  const float low0 = isfinite(high0) ? first - high0 : 0.0f, low1 = isfinite(high1) ? second - high1 : 0.0f;
-  const auto halves = __builtin_amdgcn_permlane32_swap(high, bf16_pair(low0, low1), false, false);
+  uint32_t high0, high1;
+  float low0, low1;
+  split(first, high0, low0);
+  split(second, high1, low1);
+  const auto halves = __builtin_amdgcn_permlane32_swap(high0 >> 16 | high1, bf16_pair(low0, low1), false, false);
   const auto words = __builtin_amdgcn_permlane16_swap(halves[0], halves[1], false, false);
   *reinterpret_cast<u32x2 *>(a.act + (to + (threadIdx.x & 63) / 16 * 4)) = u32x2{words[0], words[1]};
 }
@@ -396,10 +412,18 @@ struct RowPass {
   }
 };
 
+// Waves of a SIMD that the registers have to leave room for: two a workgroup. Three
+// workgroups for the 4-bit up product of few pairs, which holds little (one token of
+// 2048 x 768, three workgroups to a compute unit in all: 14.1 us the call, 15.2 with two).
+constexpr int least_waves(Product product, int steps, bool full, int columns, int batch) {
+  if (product == kUpFp4 && steps <= 8 && full && columns == 1 && batch == 1) return 6;
+  return columns <= 2 && steps <= 8 ? 4 : 2;
+}
+
 // Workgroup = `share` row tiles of one item, for all of its pairs, up to kMaxCols x 16
 // at a time. Dynamic LDS: the scales of its rows.
 template <Product kProduct, int kSteps, bool kFull, int kMaxCols, int kBatch>
-__global__ __launch_bounds__(kThreads, kMaxCols <= 2 && kSteps <= 8 ? 4 : 2) void experts_rows_kernel(ExpertArgs a) {
+__global__ __launch_bounds__(kThreads, least_waves(kProduct, kSteps, kFull, kMaxCols, kBatch)) void experts_rows_kernel(ExpertArgs a) {
   constexpr bool kFp4 = kProduct != kUpBf16, kDown = kProduct == kDownFp4;
   __shared__ f32x4 sums[2 * kBatch * kWaves * (kDown ? 1 : kMaxCols) * 64];
   __shared__ uint16_t list[kMaxRun];

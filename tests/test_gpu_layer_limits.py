@@ -6,8 +6,11 @@ an MI355X).
 import pytest
 import torch
 
+from calibration_free_moe.reader.experts import routed_experts
+from calibration_free_moe.reader.progressive import channel_major_down
 from calibration_free_moe.reader.router import route
 from tests import layer_reference as plain
+from tests.test_gpu_experts import Case
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +44,53 @@ def test_weights_of_logits_beyond_fp32(experts, top_k, renormalise):
     bound[1:3] = exact[1:3]
     assert torch.equal(ids.cpu().long(), want_ids)
     assert bool(((weights.cpu().double() - want).abs() <= bound * want + 2.0 ** -126).all())
+
+
+@pytest.mark.parametrize("fp4", [False, True], ids=["bf16", "fp4"])
+@pytest.mark.parametrize("tokens,experts", [(1, 8), (3, 8), (20, 16), (60, 4)])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -118], ids=["", "small"])
+def test_infinite_down_weights(tokens, experts, fp4, scale):
+    """An infinite weight of `down` makes its output infinite, of the products' sign, NaN
+    where two of them disagree, and leaves the outputs beside it as they are."""
+    case = Case(tokens, 256, 96, experts, 2, fp4=fp4, seed=11)
+    case.weights = case.weights * scale
+    g = torch.Generator().manual_seed(12)
+    for e in range(experts):
+        for h in torch.randperm(256, generator=g)[:40].tolist():
+            channel = int(torch.randint(96, (1,), generator=g))
+            negative = int(torch.randint(2, (1,), generator=g))
+            if fp4:  # 6 2^127, beyond BF16, alone in its block
+                case.down.codes[e, h, channel // 32 * 16:channel // 32 * 16 + 16] = 0
+                case.down.codes[e, h, channel // 2] = (7 + 8 * negative) << 4 * (channel % 2)
+                case.down.scales[e, h, channel // 32] = 254
+            else:
+                case.down[e, h, channel] = -float("inf") if negative else float("inf")
+    gate_up, down = case.values()
+    if fp4:
+        down = down.float().bfloat16()
+    want, bound = plain.layer(case.x, gate_up, down, case.ids, case.weights)
+    assert 20 * tokens < int(want.isinf().sum()) and int(want.isnan().sum()) < 20 * tokens
+    got = case.run().cpu().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+    finite = want.isfinite()
+    # (2^-132: what the smallest activations' second part may be off, times 96 weights
+    # below 2^7)
+    assert bool(((got - want).abs() <= bound + 96 * 2.0 ** -125)[finite].all())
+
+
+@pytest.mark.parametrize("weight", [3.4e38, -3.4e38, 3.2e38])
+def test_activations_next_to_the_largest_number(weight):
+    """3.4e38 lies beyond half a step of the largest BF16 number and is an FP32 one."""
+    x = torch.zeros(1, 128, dtype=torch.bfloat16)
+    gate_up = torch.zeros(1, 64, 128, dtype=torch.bfloat16)
+    down = torch.zeros(1, 128, 32, dtype=torch.bfloat16)
+    x[0, 0], gate_up[0, 0, 0], gate_up[0, 32, 0] = 1, 32, 2.0 ** -5  # silu(32) / 32 = 1 in FP32
+    down[0, :, 0] = 2.0 ** -20
+    got = routed_experts(x.to(DEVICE), gate_up.to(DEVICE), channel_major_down(down.to(DEVICE)),
+                         torch.zeros(1, 1, dtype=torch.int32, device=DEVICE),
+                         torch.tensor([[weight]], device=DEVICE))
+    want = torch.tensor(weight).double() * 2.0 ** -20
+    # an FP32 exponential and quotient, 2^-16 of the activation, one rounding
+    off = 16 * plain.STEP + plain.HALF_BF16 ** 2 + plain.HALF_BF16
+    assert bool(((got.cpu().double() - want).abs() <= 1.01 * off * want.abs()).all())
