@@ -493,7 +493,7 @@ CFMOE_API int cfmoe_route(int32_t hidden_size, int32_t experts, int32_t top_k, u
   a.ids64 = flags & CFMOE_IDS_INT64;
   a.weights16 = flags & CFMOE_WEIGHTS_BF16;
   a.renormalise = flags & CFMOE_RENORMALISE;
-  const int64_t tiles = static_cast<int64_t>(a.tiles) * ((tokens + kTile - 1) / kTile);
+  const int64_t tiles = a.tiles * ((static_cast<int64_t>(tokens) + kTile - 1) / kTile);
   if (tiles > 0x1fffff) return fail(CFMOE_EINVAL, "route has too many tokens for one launch");
   // The few-tile kernel reads the router's rows once for 16 tokens, the bulk one for 32
   // from more of the chip's caches, but a workgroup of its takes 18 us however few there
