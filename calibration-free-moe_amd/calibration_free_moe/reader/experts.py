@@ -36,11 +36,12 @@ def routed_experts(
     hidden BF16 [tokens, H]; ids (int32/int64) and weights (FP32/BF16) [tokens, K];
     padding bool [tokens] marks rows that read no weights and come out zero.
     gate_up BF16 [E, 2 I, H] and down the channel-major logical [E, H, I] (stride
-    (H I, 1, H)), as the reader borrows them (`channel_major_down`), or both
-    `Fp4Weights` of those logical shapes. Ids outside [0, E) contribute nothing; an
-    expert named twice by one token counts twice. Sums are FP32, the weighted
-    activations are held to 2^-16, and the output is rounded once. Results do not
-    depend on the other tokens of the batch in more than the order of FP32 sums.
+    (H I, 1, H), the first of one expert whatever it is), as the reader borrows them
+    (`channel_major_down`), or both `Fp4Weights` of those logical shapes. Ids outside
+    [0, E) contribute nothing; an expert named twice by one token counts twice. Sums are
+    FP32, the weighted activations are held to 2^-16, and the output is rounded once.
+    Results do not depend on the other tokens of the batch in more than the order of
+    FP32 sums.
 
     H is a multiple of 128 and I of 16 (of 32 in 4 bits), both at most 4096; at
     most 4096 experts, 64 ids per token and 8192 pairs per call. Zero tokens give
@@ -69,7 +70,7 @@ def routed_experts(
                 gate_up.dtype != torch.bfloat16
                 or down.dtype != torch.bfloat16
                 or not gate_up.is_contiguous()
-                or down.stride() != (h * i, 1, h)
+                or down.stride() != (h * i if e > 1 else down.stride(0), 1, h)
             )
         )
     ):

@@ -94,3 +94,15 @@ def test_activations_next_to_the_largest_number(weight):
     # an FP32 exponential and quotient, 2^-16 of the activation, one rounding
     off = 16 * plain.STEP + plain.HALF_BF16 ** 2 + plain.HALF_BF16
     assert bool(((got.cpu().double() - want).abs() <= 1.01 * off * want.abs()).all())
+
+
+def test_a_layer_of_one_expert_as_a_view():
+    """The stride of a dimension of size one says nothing: a shared expert's channel-major
+    down [H, I] with a leading dimension is a layer's."""
+    case = Case(5, 256, 96, 1, 1, seed=13)
+    gate_up, down = case.device_weights()
+    one = down[0][None]
+    assert one.stride() == (256, 1, 256) and channel_major_down(one).stride() == one.stride()
+    rest = (case.ids.to(DEVICE), case.weights.to(DEVICE))
+    got = routed_experts(case.x.to(DEVICE), gate_up[0][None], one, *rest)
+    assert torch.equal(got, routed_experts(case.x.to(DEVICE), gate_up, down, *rest))
