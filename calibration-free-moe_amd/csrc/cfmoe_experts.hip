@@ -811,14 +811,17 @@ auto rows_kernel(bool full, bool wide, int tiles) {
                                             : (kProduct == kDownFp4 || kSteps <= 8 ? 2 : 1);
   constexpr int kNarrow = kProduct == kDownFp4 ? 2 : 1;
   constexpr int kBatch = batch_tiles<kProduct, kSteps>(false), kWideBatch = batch_tiles<kProduct, kSteps>(true);
+  // (one width alone fills three loads of eight waves in the 4-bit down product: it takes
+  // the general kernel)
+  constexpr bool kFull = kProduct != kDownFp4 || kSteps != 12;
   if (wide)
-    return tiles >= kWideBatch ? full ? experts_rows_kernel<kProduct, kSteps, true, kWide, kWideBatch>
+    return tiles >= kWideBatch ? full ? experts_rows_kernel<kProduct, kSteps, kFull, kWide, kWideBatch>
                                       : experts_rows_kernel<kProduct, kSteps, false, kWide, kWideBatch>
-                               : full ? experts_rows_kernel<kProduct, kSteps, true, kWide, 1>
+                               : full ? experts_rows_kernel<kProduct, kSteps, kFull, kWide, 1>
                                       : experts_rows_kernel<kProduct, kSteps, false, kWide, 1>;
-  return tiles >= kBatch ? full ? experts_rows_kernel<kProduct, kSteps, true, kNarrow, kBatch>
+  return tiles >= kBatch ? full ? experts_rows_kernel<kProduct, kSteps, kFull, kNarrow, kBatch>
                                 : experts_rows_kernel<kProduct, kSteps, false, kNarrow, kBatch>
-                         : full ? experts_rows_kernel<kProduct, kSteps, true, kNarrow, 1>
+                         : full ? experts_rows_kernel<kProduct, kSteps, kFull, kNarrow, 1>
                                 : experts_rows_kernel<kProduct, kSteps, false, kNarrow, 1>;
 }
 
