@@ -663,9 +663,23 @@ __global__ __launch_bounds__(kThreads, kSteps <= 3 ? 4 : 2) void experts_down_ma
 
 // Few tokens over 4-bit rows: workgroup = 16 outputs of one token, its waves the
 // token's slots (every eighth), so that the slots' sum needs no launch of its own. An
-// expert that several tokens name is read for each of them: 128 experts of 2048 x 768
-// and top 8, one token 7 us, two 7 against 14 with the join, four 12 against 17, eight
-// 23 against 25, sixteen 41 against 32. A pair's high and low parts are columns in turn.
+// expert that several tokens name is read for each of them, and fewer slots than waves
+// leave some idle. A pair's high and low parts are columns in turn.
+//
+// Whole calls in a graph, in us, this kernel against the down and join kernels:
+//                          top 1         top 2         top 4         top 8
+//   128 of 2048 x 768    8:  13, 15   10:  27, 30   12:  40, 43    6:  38, 43
+//                       16:  24, 25   16:  34, 33   16:  49, 48   10:  58, 55
+//   64 of 2048 x 1024    8:  15, 18    8:  22, 24    8:  33, 34    4:  33, 35
+//                       12:  21, 23   10:  29, 28   10:  39, 39    5:  41, 40
+//   64 of 4096 x 2048    3:  21, 21    2:  25, 26    2:  36, 36    1:  37, 39
+//    (top 1 to 4 of 16)  5:  33, 30    4:  34, 33    4:  53, 47    2:  61, 58
+//   1024 of 1024 x 128  16:   8, 10   16:  10, 12   16:  12, 14   16:  22, 24
+//                       32:  12, 11   32:  15, 14   32:  23, 22   32:  33, 29
+// (tokens: us). So it is taken up to 10 MB of rows for each slot a token has, four at the
+// most, and up to 1280 workgroups, what the chip holds at a time.
+constexpr int kFewGroups = 1280;
+constexpr int64_t kFewBytes = 10000000;
 __global__ __launch_bounds__(kThreads) void experts_fp4_tokens_kernel(ExpertArgs a) {
   constexpr int kAhead = 4;
   __shared__ f32x4 sums[kWaves][2][4];
@@ -933,8 +947,9 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   }
 
   if (int rc = fp4 ? launch_rows<kUpFp4>(a, items, wide, stream) : launch_rows<kUpBf16>(a, items, wide, stream)) return rc;
-  if (fp4 && a.by_pair && tokens <= 4) {  // (experts_fp4_tokens_kernel: both sides)
-    a.tiles = hidden_size / kRows;
+  const int64_t read = static_cast<int64_t>(a.pairs) * hidden_size * (width / 2);
+  if (fp4 && a.by_pair && tokens * (hidden_size / kRows) <= kFewGroups && read <= kFewBytes * std::min(top_k, 4)) {
+    a.tiles = hidden_size / kRows;  // (experts_fp4_tokens_kernel: both sides)
     hipLaunchKernelGGL(experts_fp4_tokens_kernel, dim3(static_cast<unsigned>(a.tiles) * tokens), dim3(kThreads), 0,
                        stream, a);
     return check_launch("experts_down");

@@ -88,7 +88,8 @@ def launches(hidden: int, width: int, experts: int, top_k: int, tokens: int, fp4
             found.update((kernel["name"], tiles, len(passes) > 1) for tiles in passes)
 
     rows(rows_kernel(UP_FP4 if fp4 else UP_BF16, hidden, width // 8, items, wide))
-    if fp4 and pairs <= experts and tokens <= 4:
+    few = tokens * (hidden // 16) <= 1280 and pairs * hidden * (width // 2) <= 10_000_000 * min(top_k, 4)
+    if fp4 and pairs <= experts and few:
         found.add(("experts_fp4_tokens_kernel", 0, False))
         return found
     if fp4:
@@ -125,7 +126,11 @@ CASES = [
     (128, 2048, 256, 300, True, MIXED), (256, 1920, 256, 300, True, MIXED), (256, 768, 400, 600, True, MIXED),
     (1024, 96, 512, 600, True, MIXED), (1024, 128, 512, 600, True, MIXED), (256, 480, 512, 600, True, MIXED),
     (256, 1024, 512, 600, True, MIXED),
-    # few tokens, and sorted runs of 64 and 32 pairs
-    (512, 160, 8, 3, True, [2, 1]), (256, 96, 8, 500, False, [100, 70, 17, 16, 1]),
+    # 4-bit rows of few tokens, about the most of them in workgroups and in bytes
+    (512, 160, 8, 3, True, [2, 1]), (512, 160, 64, 40, True, [20, 3, 1]), (512, 160, 64, 41, True, [20, 3, 1]),
+    (128, 4096, 64, 38, True, [20, 3, 1]), (128, 4096, 64, 39, True, [20, 3, 1]),
+    (128, 32, 160, 160, True, [90, 3, 1]),
+    # sorted runs of 64 and 32 pairs
+    (256, 96, 8, 500, False, [100, 70, 17, 16, 1]),
     (256, 96, 8, 500, True, [100, 70, 17, 16, 1]),
 ]
