@@ -818,7 +818,7 @@ constexpr int batch_tiles(bool wide) {
 
 template <Product kProduct, int kSteps>
 auto rows_kernel(bool full, bool wide, int tiles) {
-  // Column tiles of a wide kernel. BF16: as many as the registers hold with one
+  // Column tiles of a wide call's. BF16: as many as the registers hold with one
   // workgroup to a compute unit. 4 bits: two, with which there are still two workgroups
   // (four leave room for one: 256 Zipf tokens 103 us against 80).
   constexpr int kWide = kProduct == kUpBf16 ? (kSteps == 8 ? 4 : kSteps == 12 ? 2 : 1)
@@ -922,15 +922,26 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
   a.weights16 = flags & CFMOE_WEIGHTS_BF16;
   a.gelu = flags & CFMOE_GELU;
   a.by_pair = a.pairs <= experts;
-  // A wide kernel's sorted runs are of 64 pairs over BF16 rows and 32 over 4-bit rows,
-  // the others' of 16. Wide pays where experts have more than 16 pairs: BF16 from six an
-  // expert on average, since skewed routing gains more than uniform loses (128 tokens
-  // over 128 experts, top 8: uniform 175 us against 171, Zipf(1.2) 232 against 249; 64
-  // experts' 64 tokens of Zipf(1.2) 164 against 179), 4-bit rows from twelve (whole calls:
-  // 128 tokens over 128 experts 97 us and 98, 256 tokens 130 and 131, of Zipf(1.2) 152 and
-  // 153, 512 tokens 202 and 213: the up product gains what the down product, one 16 pairs
-  // behind the other, loses; two items of a run for it took longer, 80 us for 74).
-  const bool wide = a.pairs >= (fp4 ? 12 : 6) * experts;
+  // A wide call's sorted runs are of 64 pairs over BF16 rows and 32 over 4-bit rows, the
+  // others' of 16, and its up product takes several column tiles at a time: only where
+  // its registers hold them (rows_kernel). It pays where experts have more than 16 pairs,
+  // and costs where most have few. Whole calls in a graph, wide against narrow, in us, by
+  // pairs an expert on average (uniform routing, and Zipf(1.2)):
+  //   BF16, 64 experts of 2048 x 1024   6: 170, 168 (164, 162)    8: 175, 183 (171, 174)
+  //                                    16: 189, 195 (199, 214)   32: 218, 265 (230, 272)
+  //         128 of 2048 x 768           6: 249, 235 (229, 224)    8: 257, 251 (240, 237)
+  //                                    12: 270, 268 (264, 272)   16: 283, 291 (284, 298)
+  //         64 of 1536 x 768            6: 109, 112 (111, 108)    8: 113, 114 (119, 116)
+  //         32 of 4096 x 1024 (one column tile)                  16: 222, 200 (239, 222)
+  // 4-bit rows' down product has no wide form, so that their calls gain later, and only
+  // where eight waves share an up row:
+  //         128 of 2048 x 768          16: 131, 127 (139, 133)   28: 178, 181 (183, 182)
+  //                                    48: 258, 268 (255, 268)   64: 319, 340 (316, 339)
+  //         64 of 2048 x 1024          24: 104, 103 (106, 102)   64: 191, 206 (190, 206)
+  //         64 of 1024 x 512 (four)    16:  49,  40  (53,  42)   48:  69,  61  (69,  62)
+  const Cut up = cut_of(fp4 ? hidden_size / 128 : hidden_size / 32, fp4, false);
+  const bool wide = fp4 ? up.splits == kWaves && up.loads <= 2 && a.pairs >= 28 * experts
+                        : up.loads <= 12 && a.pairs >= 8 * experts;
   int items = a.by_pair ? a.pairs : experts;
   a.runs = nullptr;
   a.sorted = nullptr;

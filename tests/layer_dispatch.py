@@ -66,7 +66,11 @@ def launches(hidden: int, width: int, experts: int, top_k: int, tokens: int, fp4
     `counts` are the pairs of each expert that has any.
     """
     pairs = tokens * top_k
-    wide = pairs >= (12 if fp4 else 6) * experts
+    splits, loads = cut_of(hidden // (128 if fp4 else 32), fp4, False)
+    if fp4:
+        wide = splits == 8 and loads <= 2 and pairs >= 28 * experts
+    else:
+        wide = loads <= 12 and pairs >= 8 * experts
     items = pairs if pairs <= experts else experts
     runs = list(counts)
     found = set()
@@ -101,8 +105,8 @@ def launches(hidden: int, width: int, experts: int, top_k: int, tokens: int, fp4
 
 
 # hidden, width, experts, pairs (one a token), 4 bits, pairs of each expert that has any;
-# the other pairs name no expert, and the other experts no weights but zeros. Ten experts
-# for these 59 pairs make narrow calls, three wide ones.
+# the other pairs name no expert, and the other experts have no weights but zeros. Ten
+# experts for these 59 pairs make narrow calls, three wide ones over BF16 rows.
 MIXED = [36, 20, 3]
 CASES = [
     # the up product's row lengths
@@ -120,9 +124,12 @@ CASES = [
     *((128, width, 10, 59, True, MIXED)
       for width in (32, 96, 160, 256, 384, 480, 512, 640, 960, 992, 1024, 1056, 1152, 1984, 2016, 2048, 2080,
                     2976, 3104, 4064, 4096)),
+    # wide calls over 4-bit rows, unsorted and sorted
+    *((hidden, 32, 2, 59, True, [39, 20]) for hidden in (1664, 1792, 1920, 2048)),
+    *((hidden, 32, 3, 100, True, MIXED) for hidden in (1920, 2048)),
     # several row tiles of 4-bit rows between two barriers
-    (256, 256, 1024, 1024, True, MIXED), (384, 32, 64, 800, True, MIXED), (2048, 256, 64, 800, True, MIXED),
-    (1792, 256, 64, 800, True, MIXED), (2048, 256, 200, 300, True, MIXED), (1920, 256, 200, 300, True, MIXED),
+    (256, 256, 1024, 1024, True, MIXED), (384, 32, 64, 800, True, MIXED), (2048, 256, 64, 1800, True, MIXED),
+    (1792, 256, 64, 1800, True, MIXED), (2048, 256, 200, 300, True, MIXED), (1920, 256, 200, 300, True, MIXED),
     (128, 2048, 256, 300, True, MIXED), (256, 1920, 256, 300, True, MIXED), (256, 768, 400, 600, True, MIXED),
     (1024, 96, 512, 600, True, MIXED), (1024, 128, 512, 600, True, MIXED), (256, 480, 512, 600, True, MIXED),
     (256, 1024, 512, 600, True, MIXED),
