@@ -41,7 +41,8 @@ def routed_experts(
     [0, E) contribute nothing; an expert named twice by one token counts twice. Sums are
     FP32, the weighted activations are held to 2^-16, and the output is rounded once.
     Results do not depend on the other tokens of the batch in more than the order of
-    FP32 sums.
+    FP32 sums. Infinities and NaN stay in the rows that they reach, and an infinite
+    weight of `down` makes its output infinite.
 
     H is a multiple of 128 and I of 16 (of 32 in 4 bits), both at most 4096; at
     most 4096 experts, 64 ids per token and 8192 pairs per call. Zero tokens give

@@ -89,7 +89,11 @@ def quantise_fp4(weights: Tensor) -> Fp4Weights:
 
 
 def dequantise_fp4(weights: Fp4Weights) -> Tensor:
-    """The BF16 values [..., n] that codes and scales stand for, exactly."""
+    """The BF16 values [..., n] that codes and scales stand for, exactly.
+
+    A scale byte of 254, which `quantise_fp4` never gives, makes magnitudes of 2 and
+    more infinite, 255 every value NaN.
+    """
     if not weights.valid():
         raise ValueError("Expected contiguous CUDA codes [..., n / 2] and scales [..., n / 32]")
     values = torch.empty(weights.shape, dtype=torch.bfloat16, device=weights.device)

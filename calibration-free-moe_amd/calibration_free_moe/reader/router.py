@@ -35,14 +35,18 @@ def route(
     hidden BF16 [tokens, H] and router BF16 [E, H], contiguous; the logits are
     hidden @ router.T. Each token's `top_k` largest logits are kept, largest
     first: equal logits go to the lowest expert, NaN counts as the largest, and
-    the order is that of the exact logits, not of their FP32 sums. Weights are
-    the softmax over the kept experts (`renormalise`) or the kept part of the
-    softmax over all, times `expert_scale` (FP32 [E]) at each kept expert if it
-    is given. Ids are always distinct and inside [0, E), whatever the rows hold.
+    the order is that of the exact logits, not of their FP32 sums (those whose order
+    FP32 leaves open are formed again in FP64). Weights are the softmax over the kept
+    experts (`renormalise`) or the kept part of the softmax over all, times
+    `expert_scale` (FP32 [E]) at each kept expert if it is given; they come from the
+    FP32 sums, or the FP64 ones where there are any, finite logits beyond FP32 among
+    them. Ids are always distinct and inside [0, E), whatever the rows hold.
 
     `out` takes (ids, weights) to write instead of new tensors; their types then
     stand for `ids_dtype` (int32 or int64) and `weights_dtype` (FP32 or BF16).
-    H is a multiple of 128, at most 65536, E at most 1024, top_k at most 64 and E.
+    H is a multiple of 128, at most 65536, E at most 1024, top_k at most 64 and E, and
+    there are fewer than 2^21 tiles of 16 tokens by 16 experts. 64 kept of more experts
+    form all kept logits in FP64, which takes up to three times as long as 63.
     Zero tokens give empty outputs. The work is enqueued on the current stream of the
     tensors' device and can be captured in a graph.
     """

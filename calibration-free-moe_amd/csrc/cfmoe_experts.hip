@@ -24,8 +24,10 @@
 //   32 tokens, BF16                      5   124    68     5   179
 //   256 tokens, Zipf(1.2), BF16          5   168   110     7   197
 //   128 tokens, 4 bits                   5    51    37     5    53.6
-// Large BF16 calls read at 5.4-6.0 TB/s; small ones are the launches and one pass of
-// memory latency each.
+// Large BF16 calls of uniform routing read at 4.5 to 5.1 TB/s over all their launches (up
+// rows at 4.7 to 5.2, down rows at 4.3 to 4.8), the skewed one, whose experts of many
+// pairs take several runs, at 4.2 (4.6 and 3.7), the 4-bit one at 3.3 (4.3 and 2.7). Small
+// calls are the launches and one pass of memory latency each.
 //
 // A pair whose id lies outside [0, E) or whose token is padded belongs to no
 // expert: nothing computes it, and the join leaves it out.
@@ -849,7 +851,9 @@ int launch_rows(ExpertArgs a, int items, bool wide, cfmoe_stream stream) {
   const bool full = units == cut.splits * cut.loads && length % 128 == 0;
   a.splits = cut.splits;
   a.tiles = kDown ? a.hidden / kRows : a.width / (kRows / 2);
-  // Enough workgroups to fill the chip, then fewer loads of the pairs' vectors. (Narrow
+  // Enough workgroups to fill the chip, then fewer loads of the pairs' vectors. Items are
+  // counted as the most runs there can be, all that the host knows of a sorted call: up to
+  // a third of the workgroups find theirs empty and end. (Narrow
   // BF16 kernels, three workgroups to a compute unit: 2048 for 1024 make 16 tokens over
   // 128 experts 94 us of 96, 32 over 64 97 of 99, those of 2816 x 704 135 of 129.)
   const int subs = kWaves / cut.splits;

@@ -252,12 +252,13 @@ CFMOE_API int64_t cfmoe_noalloc_scratch_bytes(void);
 
 /* Router of one layer: logits x router^T of hidden bf16 [T, H] and router
  * bf16 [E, H], the top_k largest per token (largest first, ties to the lowest
- * expert, NaN above all; the order is that of the exact logits), their softmax
- * weights, times expert_scale [E] fp32 unless NULL. flags: CFMOE_IDS_INT64,
- * CFMOE_WEIGHTS_BF16, CFMOE_RENORMALISE. ids and weights are [T, top_k], as
- * cfmoe_forward and cfmoe_routed_experts take them. H a multiple of 128, at most
- * 65536, E at most 1024, top_k at most 64. scratch: cfmoe_route_scratch_bytes(T, E) bytes,
- * 16-byte aligned like hidden and router; calls that overlap need their own.
+ * expert, NaN above all; the order is that of the exact logits, formed again in FP64
+ * where FP32 leaves it open), their softmax weights, times expert_scale [E] fp32 unless
+ * NULL. flags: CFMOE_IDS_INT64, CFMOE_WEIGHTS_BF16, CFMOE_RENORMALISE. ids and weights
+ * are [T, top_k], as cfmoe_forward and cfmoe_routed_experts take them. H a multiple of
+ * 128, at most 65536, E at most 1024, top_k at most 64, fewer than 2^21 tiles of 16 x 16
+ * logits. scratch: cfmoe_route_scratch_bytes(T, E) bytes, 16-byte aligned like hidden and
+ * router; calls that overlap need their own.
  * T = 0 does nothing. The reference leaves routing to its host runtime. */
 CFMOE_API int64_t cfmoe_route_scratch_bytes(int32_t tokens, int32_t experts);
 CFMOE_API int cfmoe_route(int32_t hidden_size, int32_t experts, int32_t top_k, uint32_t flags,
