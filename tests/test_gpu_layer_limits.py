@@ -106,3 +106,20 @@ def test_a_layer_of_one_expert_as_a_view():
     rest = (case.ids.to(DEVICE), case.weights.to(DEVICE))
     got = routed_experts(case.x.to(DEVICE), gate_up[0][None], one, *rest)
     assert torch.equal(got, routed_experts(case.x.to(DEVICE), gate_up, down, *rest))
+
+
+@pytest.mark.parametrize("renormalise", [True, False])
+def test_logits_beyond_fp32_among_many_tokens(renormalise):
+    """The kernel of many tokens: the rows that overflow, and the ordinary ones beside them."""
+    g = torch.Generator().manual_seed(14)
+    x = torch.randn(1400, 256, generator=g).bfloat16()
+    router = (torch.randn(200, 256, generator=g) * 0.1).bfloat16()
+    large = torch.arange(1400) % 9 == 4
+    x[large] = torch.where(x[large] < 0, -3e38, 3e38).bfloat16()
+    ids, weights = route(x.to(DEVICE), router.to(DEVICE), 5, renormalise=renormalise)
+    want_ids, want, bound = plain.routing(x, router, 5, renormalise)
+    assert torch.equal(ids.cpu().long(), want_ids)
+    # (differences of 1e36 and more: the first expert has all the weight)
+    assert bool((want[large, 0] == 1).all()) and torch.equal(weights.cpu()[large].double(), want[large])
+    rest = ~large
+    assert bool(((weights.cpu().double() - want).abs() <= bound * want)[rest].all())
