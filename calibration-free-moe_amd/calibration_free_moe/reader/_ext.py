@@ -17,7 +17,7 @@ import torch
 LIBRARY_NAME = "libcfmoe_reader.so"
 LIBRARY_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIBRARY_NAME)
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 POINT = 1
 GELU = 2
@@ -32,6 +32,12 @@ ENCODER_TILES = 512
 RENORMALISE = 1024
 FP32 = 2048
 FP4 = 4096
+POST_FP32 = 8192
+GATE_FP32 = 16384
+NEXT_FP32 = 32768
+GATE_CHANNEL = 65536
+GATE_ROW = 131072
+GATE_FULL = 262144
 
 EINVAL = 1
 EHIP = 2
@@ -131,6 +137,8 @@ def library() -> ctypes.CDLL:
         )
     lib = ctypes.CDLL(LIBRARY_PATH)
     lib.cfmoe_abi_version.restype = ctypes.c_int
+    if lib.cfmoe_abi_version() != ABI_VERSION:
+        raise RuntimeError(f"{LIBRARY_NAME} ABI mismatch; rebuild the library")
     lib.cfmoe_last_error.restype = ctypes.c_char_p
     lib.cfmoe_workspace_sizes.restype = ctypes.c_int
     lib.cfmoe_workspace_sizes.argtypes = [
@@ -190,8 +198,37 @@ def library() -> ctypes.CDLL:
     lib.cfmoe_routed_experts_scratch_bytes.argtypes = [count] * 4 + [flags, count]
     lib.cfmoe_routed_experts.restype = ctypes.c_int
     lib.cfmoe_routed_experts.argtypes = [count] * 4 + [flags] + [pointer] * 10 + [count, pointer]
-    if lib.cfmoe_abi_version() != ABI_VERSION:
-        raise RuntimeError(f"{LIBRARY_NAME} ABI mismatch; rebuild the library")
+    stride, number = ctypes.c_int64, ctypes.c_float
+    lib.cfmoe_sort_by_expert_scratch_bytes.restype = ctypes.c_int64
+    lib.cfmoe_sort_by_expert_scratch_bytes.argtypes = [count] * 3
+    lib.cfmoe_sort_by_expert.restype = ctypes.c_int
+    lib.cfmoe_sort_by_expert.argtypes = [count, count, flags] + [pointer] * 6 + [count, pointer]
+    lib.cfmoe_gather_rows.restype = ctypes.c_int
+    lib.cfmoe_gather_rows.argtypes = [count, count, flags] + [pointer] * 3 + [count, pointer]
+    lib.cfmoe_combine_rows.restype = ctypes.c_int
+    lib.cfmoe_combine_rows.argtypes = [count, count, flags] + [pointer] * 4 + [count, pointer]
+    lib.cfmoe_combine_rows_backward.restype = ctypes.c_int
+    lib.cfmoe_combine_rows_backward.argtypes = (
+        [count, count, flags] + [pointer] * 6 + [count, pointer]
+    )
+    lib.cfmoe_join_block.restype = ctypes.c_int
+    lib.cfmoe_join_block.argtypes = (
+        [count, flags] + [pointer] * 4 + [number, pointer, number] + [pointer] * 3
+        + [count, pointer]
+    )
+    lib.cfmoe_join_block_backward_scratch_bytes.restype = ctypes.c_int64
+    lib.cfmoe_join_block_backward_scratch_bytes.argtypes = [count] * 3
+    lib.cfmoe_join_block_backward.restype = ctypes.c_int
+    lib.cfmoe_join_block_backward.argtypes = (
+        [count, flags] + [pointer] * 4 + [number] + [pointer] * 10 + [count, pointer]
+    )
+    lib.cfmoe_apply_adapters_scratch_bytes.restype = ctypes.c_int64
+    lib.cfmoe_apply_adapters_scratch_bytes.argtypes = [count] * 3
+    lib.cfmoe_apply_adapters.restype = ctypes.c_int
+    lib.cfmoe_apply_adapters.argtypes = (
+        [count] * 4 + [flags, pointer, stride, pointer, stride] + [pointer] * 5
+        + [stride, pointer, count, pointer]
+    )
     _library = lib
     return lib
 
@@ -244,6 +281,33 @@ def route_scratch_bytes(tokens: int, experts: int) -> int:
 def routed_experts_scratch_bytes(*shape: int) -> int:
     """Bytes for (hidden, width, experts, top_k, flags, tokens); ValueError if refused."""
     size = library().cfmoe_routed_experts_scratch_bytes(*shape)
+    if size < 0:
+        check(-size)
+    return size
+
+
+@functools.lru_cache(maxsize=4096)
+def sort_scratch_bytes(tokens: int, top_k: int, experts: int) -> int:
+    """Bytes for a call of that size; ValueError if refused."""
+    size = library().cfmoe_sort_by_expert_scratch_bytes(tokens, top_k, experts)
+    if size < 0:
+        check(-size)
+    return size
+
+
+@functools.lru_cache(maxsize=4096)
+def join_scratch_bytes(hidden: int, sums: int, tokens: int) -> int:
+    """Bytes for a backward call of that size; ValueError if refused."""
+    size = library().cfmoe_join_block_backward_scratch_bytes(hidden, sums, tokens)
+    if size < 0:
+        check(-size)
+    return size
+
+
+@functools.lru_cache(maxsize=4096)
+def adapters_scratch_bytes(rank: int, adapters: int, tokens: int) -> int:
+    """Bytes for a call of that size; ValueError if refused."""
+    size = library().cfmoe_apply_adapters_scratch_bytes(rank, adapters, tokens)
     if size < 0:
         check(-size)
     return size

@@ -1,0 +1,221 @@
+"""Tokens laid out by expert, and back, with the router's weights and gradients.
+
+What stands between `route` and products over many rows of one expert (a prompt's
+tokens, a training step): the batch's pairs of token and slot are sorted by expert,
+`gather_rows` lays out a row for each, the caller's products take the rows of expert e,
+`offsets[e]` to `offsets[e + 1]`, and `combine_rows` sums what they give. The reference
+has no counterpart; its operator takes the router's ids and weights as they are
+(calibration_free_moe/reader/progressive.py:3876-3885).
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from calibration_free_moe.reader import _ext
+
+MAX_HIDDEN = 1 << 20
+MAX_TOP_K = 64
+
+
+@dataclass(frozen=True)
+class ExpertOrder:
+    """A batch's pairs in expert order, all int32 on one GPU (`sort_by_expert` makes it).
+
+    Rows are the kept pairs by expert, those of one expert in the batch's order, and
+    behind them the dropped pairs. `offsets` [E + 1]: expert e has the rows from
+    offsets[e] to offsets[e + 1], and offsets[E] rows are kept. `places` [tokens, K]: the
+    row of each pair, or -1 - row of a dropped one. `pairs` [tokens K]: t K + k of each row.
+    """
+
+    offsets: Tensor
+    places: Tensor
+    pairs: Tensor
+
+    def valid(self) -> bool:
+        """Whether the three are contiguous int32 of one batch on one GPU."""
+        offsets, places, pairs = self.offsets, self.places, self.pairs
+        return (
+            places.dim() == 2
+            and 1 <= places.shape[1] <= MAX_TOP_K
+            and offsets.dim() == pairs.dim() == 1
+            and offsets.shape[0] >= 2
+            and pairs.shape[0] == places.numel()
+            and offsets.dtype == places.dtype == pairs.dtype == torch.int32
+            and places.is_cuda
+            and offsets.device == places.device == pairs.device
+            and places.is_contiguous()
+            and pairs.is_contiguous()
+            and offsets.is_contiguous()
+        )
+
+
+def sort_by_expert(ids: Tensor, experts: int, padding: Tensor | None = None) -> ExpertOrder:
+    """The order of a batch's pairs by expert, from `route`'s ids (int32/int64) [tokens, K].
+
+    A pair is kept where its id lies in [0, experts) and its token is not marked in
+    `padding` (bool [tokens]); the others (experts of another GPU, a batch padded to its
+    capture size) are dropped and sorted behind. The sort is stable, and its integers are
+    the same for every call. At most 4096 experts, 64 ids per token and 2^30 pairs. Zero
+    tokens give an empty order. One or two HIP launches on the current stream of the ids'
+    device, which the host does not wait for; they can be captured in a graph.
+    """
+    if (
+        ids.dim() != 2
+        or ids.dtype not in (torch.int32, torch.int64)
+        or not ids.is_cuda
+        or not ids.is_contiguous()
+    ):
+        raise ValueError("Expected contiguous int32 or int64 CUDA ids [tokens, K]")
+    tokens, top_k = ids.shape
+    device = ids.device
+    if padding is not None and (
+        padding.shape != (tokens,)
+        or padding.device != device
+        or padding.dtype != torch.bool
+        or not padding.is_contiguous()
+    ):
+        raise ValueError("padding must be contiguous bool [tokens] on the ids' device")
+    size = _ext.sort_scratch_bytes(tokens, top_k, experts)
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
+    places = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
+    pairs = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
+    scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _ext.run(
+        _ext.library().cfmoe_sort_by_expert, device, experts, top_k,
+        _ext.IDS_INT64 if ids.dtype == torch.int64 else 0, ids.data_ptr(),
+        None if padding is None else padding.data_ptr(), offsets.data_ptr(), places.data_ptr(),
+        pairs.data_ptr(), None if scratch is None else scratch.data_ptr(), tokens,
+    )
+    return ExpertOrder(offsets, places, pairs)
+
+
+def _flags(rows: Tensor, weights: Tensor | None = None) -> int:
+    return (_ext.FP32 if rows.dtype == torch.float32 else 0) | (
+        _ext.WEIGHTS_BF16 if weights is not None and weights.dtype == torch.bfloat16 else 0
+    )
+
+
+def _gather(hidden: Tensor, places: Tensor) -> Tensor:
+    tokens, top_k = places.shape
+    rows = hidden.new_empty((tokens * top_k, hidden.shape[1]))
+    _ext.run(
+        _ext.library().cfmoe_gather_rows, hidden.device, hidden.shape[1], top_k, _flags(hidden),
+        hidden.data_ptr(), places.data_ptr(), rows.data_ptr(), tokens,
+    )
+    return rows
+
+
+def _combine(rows: Tensor, places: Tensor, weights: Tensor | None) -> Tensor:
+    tokens, top_k = places.shape
+    out = rows.new_empty((tokens, rows.shape[1]))
+    _ext.run(
+        _ext.library().cfmoe_combine_rows, rows.device, rows.shape[1], top_k,
+        _flags(rows, weights), rows.data_ptr(), places.data_ptr(),
+        None if weights is None else weights.data_ptr(), out.data_ptr(), tokens,
+    )
+    return out
+
+
+class _Gather(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, places):
+        ctx.save_for_backward(places)
+        return _gather(hidden, places)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        (places,) = ctx.saved_tensors
+        return _combine(grad.contiguous(), places, None), None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, places, weights):
+        ctx.save_for_backward(rows, places, weights)
+        return _combine(rows, places, weights)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        rows, places, weights = ctx.saved_tensors
+        tokens, top_k = places.shape
+        grad = grad.contiguous()
+        grad_rows = torch.empty_like(rows) if ctx.needs_input_grad[0] else None
+        grad_weights = torch.empty_like(weights) if ctx.needs_input_grad[2] else None
+        _ext.run(
+            _ext.library().cfmoe_combine_rows_backward, rows.device, rows.shape[1], top_k,
+            _flags(rows, weights), grad.data_ptr(), rows.data_ptr(), places.data_ptr(),
+            None if weights is None else weights.data_ptr(),
+            None if grad_rows is None else grad_rows.data_ptr(),
+            None if grad_weights is None else grad_weights.data_ptr(), tokens,
+        )
+        return grad_rows, None, grad_weights
+
+
+def _check_rows(rows: Tensor, count: int, order: ExpertOrder, what: str) -> None:
+    if (
+        rows.dim() != 2
+        or rows.shape[0] != count
+        or not 1 <= rows.shape[1] <= MAX_HIDDEN
+        or rows.dtype not in (torch.bfloat16, torch.float32)
+        or rows.device != order.places.device
+        or not rows.is_contiguous()
+    ):
+        raise ValueError(
+            f"Expected contiguous BF16 or FP32 {what} of the order's batch on its GPU, "
+            "H from 1 to 2^20"
+        )
+
+
+def gather_rows(hidden: Tensor, order: ExpertOrder) -> Tensor:
+    """Rows [tokens K, H] of the order's pairs, from hidden (BF16 or FP32) [tokens, H].
+
+    Row r is hidden[order.pairs[r] // K]; rows of dropped pairs are zero. The gradient of
+    hidden is the sum of its kept pairs' row gradients in slot order, in FP32, rounded once;
+    gradients of dropped rows are not read. H is any size from 1 to 2^20. One HIP launch on
+    the current stream of the rows' device, for the gradient another; both can be captured
+    in a graph (a backward pass only where no eager graph of the same leaves is alive).
+    """
+    if not order.valid():
+        raise ValueError("Expected an ExpertOrder of contiguous int32 CUDA tensors of one batch")
+    _check_rows(hidden, order.places.shape[0], order, "rows [tokens, H]")
+    if hidden.requires_grad and torch.is_grad_enabled():
+        return _Gather.apply(hidden, order.places)
+    return _gather(hidden, order.places)
+
+
+def combine_rows(rows: Tensor, order: ExpertOrder, weights: Tensor | None = None) -> Tensor:
+    """out [tokens, H]: each token's kept rows, times its weights, summed in slot order.
+
+    rows (BF16 or FP32) [tokens K, H] in the order's rows, weights (FP32 or BF16)
+    [tokens, K] as `route` gives them, or None for ones. Sums are FP32, rounded once to the
+    rows' type; what a dropped pair's row and weight hold is not read, and a token without
+    a kept pair gives zeros. Gradients go to rows (zero in dropped rows) and weights (the
+    FP32 sum of out's gradient times the row; zero for dropped pairs). Launches as
+    `gather_rows`.
+    """
+    if not order.valid():
+        raise ValueError("Expected an ExpertOrder of contiguous int32 CUDA tensors of one batch")
+    places = order.places
+    _check_rows(rows, places.numel(), order, "rows [tokens K, H]")
+    if weights is not None and (
+        weights.shape != places.shape
+        or weights.dtype not in (torch.float32, torch.bfloat16)
+        or weights.device != places.device
+        or not weights.is_contiguous()
+    ):
+        raise ValueError("weights must be contiguous FP32 or BF16 [tokens, K] on the rows' device")
+    if torch.is_grad_enabled() and (
+        rows.requires_grad or (weights is not None and weights.requires_grad)
+    ):
+        return _Combine.apply(rows, places, weights)
+    return _combine(rows, places, weights)
+
+
+__all__ = ["ExpertOrder", "combine_rows", "gather_rows", "sort_by_expert"]

@@ -1,0 +1,202 @@
+"""The norms before and after a block, fused with its gate and the residual's scale.
+
+A block (attention, a layer of experts) takes the normed residual stream, and its output,
+normed again in some models and gated in others, is added to it. `norm_rows` is the first
+norm of a stack; `join_block` is all that stands between one block's output and the next
+block's input, in one pass over both. The reference leaves these to its host runtime.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from calibration_free_moe.reader import _ext
+
+MAX_HIDDEN = 8192
+
+
+def _pointer(t: Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _gate_flag(gate: Tensor | None, hidden: Tensor) -> int:
+    if gate is None:
+        return 0
+    if gate.dim() == 1:
+        return _ext.GATE_CHANNEL
+    return _ext.GATE_ROW if gate.shape[1] == 1 else _ext.GATE_FULL
+
+
+def _flags(hidden: Tensor, post: Tensor | None, gate: Tensor | None, following: Tensor | None) -> int:
+    flags = _gate_flag(gate, hidden)
+    if hidden.dtype == torch.float32:
+        return flags | _ext.FP32
+    fp32 = torch.float32
+    if post is not None and post.dtype == fp32:
+        flags |= _ext.POST_FP32
+    if gate is not None and gate.dtype == fp32:
+        flags |= _ext.GATE_FP32
+    if following is not None and following.dtype == fp32:
+        flags |= _ext.NEXT_FP32
+    return flags
+
+
+def _forward(hidden, block, post, gate, following, scale, epsilon, train):
+    """(joined, next, statistics): None where not asked for."""
+    tokens, size = hidden.shape
+    joined = None if block is None else torch.empty_like(hidden)
+    out = None if following is None else torch.empty_like(hidden)
+    statistics = None
+    if train:
+        statistics = torch.empty((tokens, 2), dtype=torch.float32, device=hidden.device)
+    _ext.run(
+        _ext.library().cfmoe_join_block, hidden.device, size,
+        _flags(hidden, post, gate, following), hidden.data_ptr(), _pointer(block), _pointer(post),
+        _pointer(gate), scale, _pointer(following), epsilon, _pointer(joined), _pointer(out),
+        _pointer(statistics), tokens,
+    )
+    return joined, out, statistics
+
+
+class _Join(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, block, post, gate, following, scale, epsilon):
+        joined, out, statistics = _forward(
+            hidden, block, post, gate, following, scale, epsilon, True
+        )
+        ctx.save_for_backward(hidden, block, post, gate, following, statistics)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        if joined is None:
+            return out
+        return joined if out is None else (joined, out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        hidden, block, post, gate, following, statistics = ctx.saved_tensors
+        grad_joined = None if block is None else grads[0]
+        grad_out = None if following is None else grads[-1]
+        needs = list(ctx.needs_input_grad[:5])
+        if grad_joined is None and grad_out is None:
+            return (None,) * 7
+        # (a weight of an output that nothing was made of has no gradient)
+        needs[4] = needs[4] and grad_out is not None
+        tokens, size = hidden.shape
+        inputs = (hidden, block, post, gate, following)
+        made = [torch.empty_like(t) if need else None for t, need in zip(inputs, needs)]
+        sums = needs[2] + needs[4] + (needs[3] and gate.dim() == 1)
+        scratch = None
+        if sums:
+            scratch = torch.empty(
+                _ext.join_scratch_bytes(size, sums, tokens), dtype=torch.uint8, device=hidden.device
+            )
+        if grad_joined is not None:
+            grad_joined = grad_joined.contiguous()
+        if grad_out is not None:
+            grad_out = grad_out.contiguous()
+        _ext.run(
+            _ext.library().cfmoe_join_block_backward, hidden.device, size,
+            _flags(hidden, post, gate, following), hidden.data_ptr(), _pointer(block),
+            _pointer(post), _pointer(gate), ctx.scale, _pointer(following), _pointer(statistics),
+            _pointer(grad_joined), _pointer(grad_out), _pointer(made[0]), _pointer(made[1]),
+            _pointer(made[2]), _pointer(made[3]), _pointer(made[4]), _pointer(scratch), tokens,
+        )
+        return (*made, None, None)
+
+
+def _check_hidden(hidden: Tensor, epsilon: float) -> None:
+    if (
+        hidden.dim() != 2
+        or not 1 <= hidden.shape[1] <= MAX_HIDDEN
+        or hidden.dtype not in (torch.bfloat16, torch.float32)
+        or not hidden.is_cuda
+        or not hidden.is_contiguous()
+    ):
+        raise ValueError("Expected contiguous BF16 or FP32 CUDA rows [tokens, H], H from 1 to 8192")
+    if not 1e-30 <= epsilon <= 1e30:
+        raise ValueError("epsilon must lie between 1e-30 and 1e30")
+
+
+def _check_weight(weight: Tensor, hidden: Tensor, name: str) -> None:
+    if (
+        weight.shape != hidden.shape[1:]
+        or weight.dtype not in (hidden.dtype, torch.float32)
+        or weight.device != hidden.device
+        or not weight.is_contiguous()
+    ):
+        raise ValueError(f"{name} must be contiguous [H] of the rows' type or FP32, on their device")
+
+
+def norm_rows(hidden: Tensor, weight: Tensor, *, epsilon: float = 1e-6) -> Tensor:
+    """hidden / sqrt(mean(hidden^2) + epsilon) * weight, of each row [H] of hidden.
+
+    hidden BF16 or FP32 [tokens, H], H any size from 1 to 8192; weight [H] of that type or
+    FP32; epsilon from 1e-30 to 1e30. Sums are FP32, the output is rounded once to the rows'
+    type; rows whose squares pass FP32 are scaled first. Gradients go to both, the weight's
+    summed over rows in FP32 in an order that depends on sizes alone. One HIP launch on the
+    current stream of the rows' device (for the gradient two), which can be captured in a
+    graph (a backward pass only where no eager graph of the same leaves is alive).
+    """
+    _check_hidden(hidden, epsilon)
+    _check_weight(weight, hidden, "weight")
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _Join.apply(hidden, None, None, None, weight, 1.0, epsilon)
+    return _forward(hidden, None, None, None, weight, 1.0, epsilon, False)[1]
+
+
+def join_block(
+    hidden: Tensor,
+    block: Tensor,
+    *,
+    post_weight: Tensor | None = None,
+    gate: Tensor | None = None,
+    residual_scale: float = 1.0,
+    next_weight: Tensor | None = None,
+    epsilon: float = 1e-6,
+) -> Tensor | tuple[Tensor, Tensor]:
+    """joined = residual_scale hidden + gate n, and with `next_weight` (joined, next).
+
+    n is the block's output `block`, or with `post_weight` its norm as of `norm_rows`; next is
+    the norm of joined, before joined is rounded, with `next_weight`: what the next block
+    takes. hidden and block BF16 or FP32 [tokens, H], of one type; weights [H] of that type or
+    FP32; gate, if given, per channel [H] or per row [tokens, 1] of that type or FP32, or
+    per value [tokens, H] of that type. H any size from 1 to 8192.
+
+    Gradients go to all tensors, those of weights and of a gate that is spread over rows or
+    columns summed in FP32 in an order that depends on sizes alone; they are formed from the
+    inputs again, with no other rounding than their own. Numbers and launches as `norm_rows`.
+    """
+    _check_hidden(hidden, epsilon)
+    if (
+        block.shape != hidden.shape
+        or block.dtype != hidden.dtype
+        or block.device != hidden.device
+        or not block.is_contiguous()
+    ):
+        raise ValueError("block must be contiguous rows of hidden's shape, type and device")
+    if post_weight is not None:
+        _check_weight(post_weight, hidden, "post_weight")
+    if next_weight is not None:
+        _check_weight(next_weight, hidden, "next_weight")
+    if gate is not None and (
+        gate.shape not in (hidden.shape[1:], (hidden.shape[0], 1), hidden.shape)
+        or gate.dtype not in (hidden.dtype, torch.float32)
+        or (_gate_flag(gate, hidden) == _ext.GATE_FULL and gate.dtype != hidden.dtype)
+        or gate.device != hidden.device
+        or not gate.is_contiguous()
+    ):
+        raise ValueError(
+            "gate must be contiguous [H] or [tokens, 1] of the rows' type or FP32, or [tokens, H] "
+            "of their type, on their device"
+        )
+    inputs = (hidden, block, post_weight, gate, next_weight)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+        return _Join.apply(*inputs, residual_scale, epsilon)
+    joined, out, _ = _forward(*inputs, residual_scale, epsilon, False)
+    return joined if out is None else (joined, out)
+
+
+__all__ = ["join_block", "norm_rows"]

@@ -1,0 +1,470 @@
+// MI355X (gfx950): tokens laid out by expert, and back.
+//
+// A token t has K pairs (t, k) with expert ids[t, k]. A pair is kept where its id lies in
+// [0, E) and its token is not padding. Rows are the kept pairs by expert, pairs of one
+// expert in the batch's order, and behind them the dropped pairs, in that order too:
+//
+//   offsets[e]    first row of expert e; offsets[E] rows are kept
+//   pairs[row]    t K + k of the row's pair
+//   places[t, k]  row of the pair, or -1 - row of a dropped one
+//
+//   gather    rows[row] = x[t], 0 for dropped pairs
+//   combine   out[t] = sum_k w[t, k] rows[place], kept pairs in slot order, FP32, rounded once
+//   backward  of gather: dx[t] = sum_k drows[place], which is combine without weights
+//             of combine: drows[place] = w[t, k] dout[t], 0 for dropped pairs,
+//                         dw[t, k] = sum_h dout[t, h] rows[place, h]
+//
+// What a dropped pair's row or weight holds is never read, so it may hold a NaN.
+
+#include "cfmoe_rows.h"
+
+namespace cfmoe {
+namespace {
+
+constexpr int kMaxExperts = 4096;
+constexpr int kMaxTop = 64;
+constexpr int64_t kMaxPairs = INT64_C(1) << 30;
+constexpr int kSortWaves = 16;
+constexpr int kSortBlocks = 64;       // workgroups that share the pairs of a large call
+constexpr int kCountBytes = 63 << 10; // a workgroup's counts, per wave and expert
+constexpr int kHeld = 4;              // keys of a lane that stay in registers
+constexpr int kThreads = 256;
+constexpr int kSlots = 8;             // rows of a token in flight at once
+
+// ---------------------------------------------------------------------------
+// order of the pairs
+
+struct OrderArgs {
+  const void *ids;
+  const uint8_t *padding;
+  int32_t *offsets, *places, *pairs;
+  int32_t *counts;  // [workgroups, E + 1], or NULL where one workgroup has all pairs
+  int pairs_total, top_k, experts;
+  int range;  // pairs of one wave
+  bool ids64;
+};
+
+__device__ __forceinline__ int key_of(const OrderArgs &a, int pair) {
+  int64_t id = a.ids64 ? static_cast<const int64_t *>(a.ids)[pair] : static_cast<const int32_t *>(a.ids)[pair];
+  if (a.padding && a.padding[pair / a.top_k]) id = a.experts;
+  return id >= 0 && id < a.experts ? static_cast<int>(id) : a.experts;
+}
+
+// counts[w][e]: pairs of key e in wave w's range.
+__device__ __forceinline__ void count_range(const OrderArgs &a, int *counts, int waves, int low, int high,
+                                            int (&held)[kHeld]) {
+  const int width = a.experts + 1, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int i = threadIdx.x; i < waves * width; i += blockDim.x) counts[i] = 0;
+  // (before the barrier: the first keys and the zeros are on their way together)
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) held[j] = low + 64 * j + lane < high ? key_of(a, low + 64 * j + lane) : -1;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if (held[j] >= 0) atomicAdd(&counts[wave * width + held[j]], 1);
+  for (int p = low + 64 * kHeld + lane; p < high; p += 64) atomicAdd(&counts[wave * width + key_of(a, p)], 1);
+  __syncthreads();
+}
+
+__device__ __forceinline__ void range_of(const OrderArgs &a, int waves, int &low, int &high) {
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * waves + (threadIdx.x >> 6)) * a.range;
+  low = static_cast<int>(first < a.pairs_total ? first : a.pairs_total);
+  high = static_cast<int>(first + a.range < a.pairs_total ? first + a.range : a.pairs_total);
+}
+
+// The keys' counts of each workgroup's pairs, for a call of several.
+__global__ __launch_bounds__(64 * kSortWaves) void order_count_kernel(OrderArgs a) {
+  extern __shared__ int counts[];
+  const int width = a.experts + 1, waves = blockDim.x >> 6;
+  int low, high, held[kHeld];
+  range_of(a, waves, low, high);
+  count_range(a, counts, waves, low, high, held);
+  for (int e = threadIdx.x; e < width; e += blockDim.x) {
+    int total = 0;
+    for (int w = 0; w < waves; ++w) total += counts[w * width + e];
+    a.counts[static_cast<int64_t>(blockIdx.x) * width + e] = total;
+  }
+}
+
+// Stable counting sort. A wave has a range of consecutive pairs: it counts their keys in
+// LDS, the counts become first rows (a scan over the keys, then over workgroups and waves),
+// and the wave walks its range again, 64 pairs at a time. Pairs of one key among the 64
+// find each other by one ballot for each bit of the key, so that a pair's row is its key's
+// next row and the number of its fellows in lower lanes. No atomic's order shows.
+__global__ __launch_bounds__(64 * kSortWaves) void order_kernel(OrderArgs a) {
+  extern __shared__ int shared[];
+  __shared__ int wave_sums[kSortWaves];
+  const int width = a.experts + 1, waves = blockDim.x >> 6;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  volatile int *counts = shared;
+  int low, high, held[kHeld];
+  range_of(a, waves, low, high);
+  count_range(a, shared, waves, low, high, held);
+
+  // thread i scans `each` consecutive keys
+  const int each = (width + blockDim.x - 1) / blockDim.x;
+  const int first = threadIdx.x * each, last = min(first + each, width);
+  int sum = 0;
+  for (int e = first; e < last; ++e) {
+    if (a.counts) {
+      for (int b = 0; b < static_cast<int>(gridDim.x); ++b) sum += a.counts[static_cast<int64_t>(b) * width + e];
+    } else {
+      for (int w = 0; w < waves; ++w) sum += counts[w * width + e];
+    }
+  }
+  int scan = sum;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int below = __shfl_up(scan, m);
+    if (lane >= m) scan += below;
+  }
+  if (lane == 63) wave_sums[wave] = scan;
+  __syncthreads();
+  int row = scan - sum;
+  for (int w = 0; w < wave; ++w) row += wave_sums[w];
+  for (int e = first; e < last; ++e) {
+    if (blockIdx.x == 0) a.offsets[e] = row;
+    int next = row, total = 0;
+    if (a.counts) {
+      for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
+        const int c = a.counts[static_cast<int64_t>(b) * width + e];
+        if (b < static_cast<int>(blockIdx.x)) next += c;
+        total += c;
+      }
+    }
+    for (int w = 0; w < waves; ++w) {
+      const int c = counts[w * width + e];
+      counts[w * width + e] = next;
+      next += c;
+    }
+    row = a.counts ? row + total : next;
+  }
+  __syncthreads();
+
+  const int bits = 32 - __builtin_clz(a.experts);
+  auto place = [&](int p, int key, bool live) {
+    uint64_t fellows = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot((key >> b) & 1);
+      fellows &= (key >> b) & 1 ? set : ~set;
+    }
+    const int below = __builtin_popcountll(fellows & ((UINT64_C(1) << lane) - 1));
+    if (!live) return;
+    const int at = wave * width + key;
+    const int r = counts[at] + below;
+    __builtin_amdgcn_wave_barrier();
+    if (below + 1 == __builtin_popcountll(fellows)) counts[at] = r + 1;
+    __builtin_amdgcn_wave_barrier();
+    a.places[p] = key < a.experts ? r : -1 - r;
+    a.pairs[r] = p;
+  };
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if (low + 64 * j < high) place(low + 64 * j + lane, held[j], held[j] >= 0);
+  for (int p = low + 64 * kHeld; p < high; p += 64) {
+    const bool live = p + lane < high;
+    place(p + lane, live ? key_of(a, p + lane) : -1, live);
+  }
+}
+
+// Waves of a sorting workgroup: 16, fewer where the counts of many experts need the LDS.
+int sort_waves(int experts) {
+  int waves = kSortWaves;
+  while (waves * (experts + 1) * 4 > kCountBytes) waves /= 2;
+  return waves;
+}
+
+// One workgroup up to this many pairs (kHeld for each lane of 16 waves), else up to 64.
+int sort_blocks(int64_t pairs, int experts) {
+  const int64_t each = 64 * kHeld * sort_waves(experts);
+  const int64_t blocks = (pairs + each - 1) / each;
+  return static_cast<int>(blocks < kSortBlocks ? blocks : kSortBlocks);
+}
+
+// ---------------------------------------------------------------------------
+// rows of the pairs, and back
+
+struct RowsArgs {
+  const void *from;     // [T, H] (gather, combine's backward) or [T K, H] (combine)
+  const void *rows;     // combine's backward: [T K, H]
+  const int32_t *places;
+  const void *weights;  // [T, K] or NULL
+  void *out;            // gather and combine's backward: [T K, H], combine: [T, H]
+  void *grad_weights;   // [T, K]
+  int tokens, top_k, hidden;
+  bool weights16;
+};
+
+// A pair's row, and whether the pair is kept; -1 for what no order holds.
+__device__ __forceinline__ int place_of(const RowsArgs &a, int64_t pair, bool &kept) {
+  const int place = a.places[pair];
+  kept = place >= 0;
+  const int row = kept ? place : -1 - place;
+  return static_cast<int64_t>(row) < static_cast<int64_t>(a.tokens) * a.top_k ? row : -1;
+}
+
+__device__ __forceinline__ float weight_of(const RowsArgs &a, int64_t pair) {
+  return a.weights16 ? bf16_value(static_cast<const uint16_t *>(a.weights)[pair])
+                     : static_cast<const float *>(a.weights)[pair];
+}
+
+// A token's lanes: all of a workgroup, or one wave of it where the rows are short.
+template <typename F>
+__device__ __forceinline__ void for_tokens(const RowsArgs &a, int waves, F f) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / 64 / waves);
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / 64 / waves) + wave / waves; t < a.tokens; t += step)
+    f(static_cast<int>(t), static_cast<int>(threadIdx.x) & (64 * waves - 1));
+}
+
+// rows[place] = x[t]: a token's row is read once and written K times.
+template <bool kFp32, bool kVector, int kWaves>
+__global__ __launch_bounds__(kThreads) void gather_kernel(RowsArgs a) {
+  constexpr int kValues = Lane<kFp32, kVector>::kValues;
+  for_tokens(a, kWaves, [&](int t, int lane) {
+    for (int h = lane * kValues; h < a.hidden; h += 64 * kWaves * kValues) {
+      float v[kValues], zero[kValues] = {};
+      load_values<kFp32, kVector>(a.from, static_cast<int64_t>(t) * a.hidden + h, v);
+      for (int k = 0; k < a.top_k; ++k) {
+        bool kept;
+        const int row = place_of(a, static_cast<int64_t>(t) * a.top_k + k, kept);
+        if (row >= 0) store_values<kFp32, kVector>(a.out, static_cast<int64_t>(row) * a.hidden + h, kept ? v : zero);
+      }
+    }
+  });
+}
+
+// out[t] = sum over kept slots of w rows[place]: kSlots rows are on their way together.
+template <bool kFp32, bool kVector, int kWaves>
+__global__ __launch_bounds__(kThreads) void combine_kernel(RowsArgs a) {
+  constexpr int kValues = Lane<kFp32, kVector>::kValues;
+  for_tokens(a, kWaves, [&](int t, int lane) {
+    for (int h = lane * kValues; h < a.hidden; h += 64 * kWaves * kValues) {
+      float sum[kValues] = {};
+      for (int k0 = 0; k0 < a.top_k; k0 += kSlots) {
+        float v[kSlots][kValues], w[kSlots];
+        bool kept[kSlots];
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) {
+          kept[j] = false;
+          if (k0 + j < a.top_k) {
+            const int64_t pair = static_cast<int64_t>(t) * a.top_k + k0 + j;
+            const int row = place_of(a, pair, kept[j]);
+            kept[j] = kept[j] && row >= 0;
+            if (kept[j]) {
+              w[j] = a.weights ? weight_of(a, pair) : 1.0f;
+              load_values<kFp32, kVector>(a.from, static_cast<int64_t>(row) * a.hidden + h, v[j]);
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) {
+          if (!kept[j]) continue;
+#pragma unroll
+          for (int i = 0; i < kValues; ++i) sum[i] = a.weights ? fmaf(w[j], v[j][i], sum[i]) : sum[i] + v[j][i];
+        }
+      }
+      store_values<kFp32, kVector>(a.out, static_cast<int64_t>(t) * a.hidden + h, sum);
+    }
+  });
+}
+
+// drows[place] = w dout[t] and dw = dout[t] . rows[place], kSlots slots at a time.
+template <bool kFp32, bool kVector, int kWaves>
+__global__ __launch_bounds__(kThreads) void combine_backward_kernel(RowsArgs a) {
+  constexpr int kValues = Lane<kFp32, kVector>::kValues;
+  __shared__ float parts[kThreads / 64][kSlots];
+  const int wave = threadIdx.x >> 6;
+  for_tokens(a, kWaves, [&](int t, int lane) {
+    for (int k0 = 0; k0 < a.top_k; k0 += kSlots) {
+      float dot[kSlots] = {};
+      for (int h = lane * kValues; h < a.hidden; h += 64 * kWaves * kValues) {
+        float grad[kValues];
+        load_values<kFp32, kVector>(a.from, static_cast<int64_t>(t) * a.hidden + h, grad);
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) {
+          if (k0 + j >= a.top_k) continue;
+          const int64_t pair = static_cast<int64_t>(t) * a.top_k + k0 + j;
+          bool kept;
+          const int row = place_of(a, pair, kept);
+          if (row < 0) continue;
+          const int64_t at = static_cast<int64_t>(row) * a.hidden + h;
+          if (kept && a.grad_weights) {
+            float v[kValues];
+            load_values<kFp32, kVector>(a.rows, at, v);
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) dot[j] = fmaf(grad[i], v[i], dot[j]);
+          }
+          if (a.out) {
+            float v[kValues];
+            const float w = !kept ? 0.0f : a.weights ? weight_of(a, pair) : 1.0f;
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) v[i] = kept ? w * grad[i] : 0.0f;
+            store_values<kFp32, kVector>(a.out, at, v);
+          }
+        }
+      }
+      if (!a.grad_weights) continue;
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) dot[j] = wave_total(dot[j]);
+      if (kWaves > 1) {
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j)
+          if ((lane & 63) == j) parts[wave][j] = dot[j];
+        __syncthreads();
+      }
+      if (lane < kSlots && k0 + lane < a.top_k) {
+        float total = 0.0f;
+        if (kWaves > 1) {
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) total += parts[w][lane];
+        } else {
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j) total = lane == j ? dot[j] : total;
+        }
+        const int64_t pair = static_cast<int64_t>(t) * a.top_k + k0 + lane;
+        if (a.weights16) static_cast<uint16_t *>(a.grad_weights)[pair] = bf16_bits(total);
+        else static_cast<float *>(a.grad_weights)[pair] = total;
+      }
+      if (kWaves > 1) __syncthreads();
+    }
+  });
+}
+
+int check_rows(const RowsArgs &a) {
+  if (a.hidden < 1 || a.hidden > (1 << 20)) return fail(CFMOE_EINVAL, "rows need a hidden size from 1 to 2^20");
+  if (a.top_k < 1 || a.top_k > kMaxTop) return fail(CFMOE_EINVAL, "rows need 1 to 64 pairs a token");
+  if (a.tokens < 0 || static_cast<int64_t>(a.tokens) * a.top_k > kMaxPairs)
+    return fail(CFMOE_EINVAL, "rows need 0 to 2^30 pairs");
+  return 0;
+}
+
+// Whole 16-byte vectors where every row starts at one.
+#define CFMOE_ROWS_LAUNCH(KERNEL, fp32, vector, a, stream)                                              \
+  do {                                                                                                  \
+    const int lanes = (a).hidden / ((vector) ? ((fp32) ? 4 : 8) : 1);                                   \
+    const bool wide = lanes > 64;                                                                       \
+    const int64_t groups = wide ? (a).tokens : (static_cast<int64_t>((a).tokens) + 3) / 4;              \
+    const dim3 grid(static_cast<unsigned>(groups < (1 << 20) ? groups : (1 << 20)));                    \
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a); }; \
+    if (fp32) {                                                                                         \
+      if (vector) launch(wide ? KERNEL<true, true, 4> : KERNEL<true, true, 1>);                         \
+      else launch(wide ? KERNEL<true, false, 4> : KERNEL<true, false, 1>);                              \
+    } else {                                                                                            \
+      if (vector) launch(wide ? KERNEL<false, true, 4> : KERNEL<false, true, 1>);                       \
+      else launch(wide ? KERNEL<false, false, 4> : KERNEL<false, false, 1>);                            \
+    }                                                                                                   \
+  } while (0)
+
+bool whole_vectors(int hidden, bool fp32) { return hidden % (fp32 ? 4 : 8) == 0; }
+
+}  // namespace
+}  // namespace cfmoe
+
+extern "C" {
+
+using namespace cfmoe;
+
+CFMOE_API int64_t cfmoe_sort_by_expert_scratch_bytes(int32_t tokens, int32_t top_k, int32_t experts) {
+  if (tokens < 0 || top_k < 1 || top_k > kMaxTop || static_cast<int64_t>(tokens) * top_k > kMaxPairs)
+    return -fail(CFMOE_EINVAL, "sort_by_expert needs 0 to 2^30 pairs, 1 to 64 a token");
+  if (experts < 1 || experts > kMaxExperts) return -fail(CFMOE_EINVAL, "sort_by_expert needs 1 to 4096 experts");
+  const int blocks = sort_blocks(static_cast<int64_t>(tokens) * top_k, experts);
+  return blocks <= 1 ? 0 : static_cast<int64_t>(blocks) * (experts + 1) * 4;
+}
+
+CFMOE_API int cfmoe_sort_by_expert(int32_t experts, int32_t top_k, uint32_t flags, const void *ids,
+                                   const uint8_t *padding, int32_t *offsets, int32_t *places, int32_t *pairs,
+                                   void *scratch, int32_t tokens, cfmoe_stream stream) {
+  const int64_t bytes = cfmoe_sort_by_expert_scratch_bytes(tokens, top_k, experts);
+  if (bytes < 0) return static_cast<int>(-bytes);
+  if (!offsets || (tokens && (!ids || !places || !pairs)) || (bytes && !scratch)) return fail(CFMOE_EINVAL, "NULL argument");
+  OrderArgs a;
+  a.ids = ids;
+  a.padding = padding;
+  a.offsets = offsets;
+  a.places = places;
+  a.pairs = pairs;
+  a.counts = bytes ? static_cast<int32_t *>(scratch) : nullptr;
+  a.pairs_total = tokens * top_k;
+  a.top_k = top_k;
+  a.experts = experts;
+  a.ids64 = flags & CFMOE_IDS_INT64;
+  // (no pairs: one workgroup writes the offsets, all zero)
+  const int blocks = bytes ? sort_blocks(a.pairs_total, experts) : 1, waves = sort_waves(experts);
+  const int64_t share = (a.pairs_total + static_cast<int64_t>(blocks) * waves - 1) / (static_cast<int64_t>(blocks) * waves);
+  a.range = static_cast<int>((share + 63) / 64 * 64);
+  const unsigned lds = static_cast<unsigned>(waves * (experts + 1) * 4);
+  if (a.counts) {
+    hipLaunchKernelGGL(order_count_kernel, dim3(blocks), dim3(64 * waves), lds, stream, a);
+    if (int rc = check_launch("order_count")) return rc;
+  }
+  hipLaunchKernelGGL(order_kernel, dim3(blocks), dim3(64 * waves), lds, stream, a);
+  return check_launch("order");
+}
+
+CFMOE_API int cfmoe_gather_rows(int32_t hidden_size, int32_t top_k, uint32_t flags, const void *hidden,
+                                const int32_t *places, void *rows, int32_t tokens, cfmoe_stream stream) {
+  RowsArgs a = {};
+  a.from = hidden;
+  a.places = places;
+  a.out = rows;
+  a.tokens = tokens;
+  a.top_k = top_k;
+  a.hidden = hidden_size;
+  if (int rc = check_rows(a)) return rc;
+  if (tokens == 0) return 0;
+  if (!hidden || !places || !rows) return fail(CFMOE_EINVAL, "NULL argument");
+  const bool fp32 = flags & CFMOE_FP32;
+  const bool vector = whole_vectors(hidden_size, fp32) && !misaligned16(hidden) && !misaligned16(rows);
+  CFMOE_ROWS_LAUNCH(gather_kernel, fp32, vector, a, stream);
+  return check_launch("gather_rows");
+}
+
+CFMOE_API int cfmoe_combine_rows(int32_t hidden_size, int32_t top_k, uint32_t flags, const void *rows,
+                                 const int32_t *places, const void *weights, void *out, int32_t tokens,
+                                 cfmoe_stream stream) {
+  RowsArgs a = {};
+  a.from = rows;
+  a.places = places;
+  a.weights = weights;
+  a.out = out;
+  a.tokens = tokens;
+  a.top_k = top_k;
+  a.hidden = hidden_size;
+  a.weights16 = flags & CFMOE_WEIGHTS_BF16;
+  if (int rc = check_rows(a)) return rc;
+  if (tokens == 0) return 0;
+  if (!rows || !places || !out) return fail(CFMOE_EINVAL, "NULL argument");
+  const bool fp32 = flags & CFMOE_FP32;
+  const bool vector = whole_vectors(hidden_size, fp32) && !misaligned16(rows) && !misaligned16(out);
+  CFMOE_ROWS_LAUNCH(combine_kernel, fp32, vector, a, stream);
+  return check_launch("combine_rows");
+}
+
+CFMOE_API int cfmoe_combine_rows_backward(int32_t hidden_size, int32_t top_k, uint32_t flags, const void *grad_out,
+                                          const void *rows, const int32_t *places, const void *weights,
+                                          void *grad_rows, void *grad_weights, int32_t tokens,
+                                          cfmoe_stream stream) {
+  RowsArgs a = {};
+  a.from = grad_out;
+  a.rows = rows;
+  a.places = places;
+  a.weights = weights;
+  a.out = grad_rows;
+  a.grad_weights = grad_weights;
+  a.tokens = tokens;
+  a.top_k = top_k;
+  a.hidden = hidden_size;
+  a.weights16 = flags & CFMOE_WEIGHTS_BF16;
+  if (int rc = check_rows(a)) return rc;
+  if (tokens == 0 || (!grad_rows && !grad_weights)) return 0;
+  if (!grad_out || !places || (grad_weights && !rows)) return fail(CFMOE_EINVAL, "NULL argument");
+  const bool fp32 = flags & CFMOE_FP32;
+  const bool vector = whole_vectors(hidden_size, fp32) && !misaligned16(grad_out) &&
+                      !misaligned16(grad_weights ? rows : nullptr) && !misaligned16(grad_rows);
+  CFMOE_ROWS_LAUNCH(combine_backward_kernel, fp32, vector, a, stream);
+  return check_launch("combine_rows_backward");
+}
+
+}  // extern "C"

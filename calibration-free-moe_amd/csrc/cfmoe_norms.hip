@@ -1,0 +1,499 @@
+// MI355X (gfx950): the norms before and after a block, its gate and the residual's scale.
+//
+// Of rows x (the residual stream) and b (a block's output), with i(v) = 1 / sqrt(mean(v^2) + eps):
+//
+//   n = b i(b) p        behind the block, p its weights; n = b without them
+//   j = s x + g n       s a number, g nothing, [H], [T, 1] or [T, H]
+//   y = j i(j) w        before the next block, w its weights
+//
+// and backward, with G = dL/dj of both outputs, b^ = b i(b), j^ = j i(j), means over a row:
+//
+//   G  = dj + i(j) (dy w - j^ mean(dy w j^))      dw = sum_t dy j^
+//   dx = s G      dg = G n, summed where g was spread
+//   dn = G g      dp = sum_t dn b^
+//   db = i(b) (dn p - b^ mean(dn p b^))           db = dn without p
+//
+// A norm alone is the case without b: j = x, and only y is written. A row is read once and
+// stays in registers between the sums; y is of j before it is rounded, and the backward
+// pass forms j again from what forward read, so that no rounding but the outputs' own is in
+// them. Squares are summed in FP32; a row whose sum passes FP32 is summed again 2^-80 times
+// as large, which leaves no number to overflow (epsilon is then below what a sum of FP32
+// holds, as it is in the exact one).
+
+#include <type_traits>
+
+#include "cfmoe_rows.h"
+
+namespace cfmoe {
+namespace {
+
+constexpr int kMaxHidden = 8192;
+constexpr int kEach = 8;  // values of a row that a thread holds
+constexpr float kSmall = 0x1p-80f;
+
+enum Gate { kNone, kChannel, kRow, kFull };
+
+struct JoinArgs {
+  const void *hidden, *block, *post, *gate, *next;
+  void *joined, *out;
+  float *statistics;  // [T, 2]: i(b) and i(j); -v stands for 2^-80 v
+  const void *grad_joined, *grad_out;
+  void *grad_hidden, *grad_block, *grad_gate;
+  float *partial;  // [workgroups, sums, H]: dw, dp and the channel gate's dg, those there are
+  int tokens, size, sums;
+  float scale, epsilon;
+  Gate form;
+  bool post32, gate32, next32, grad_post, grad_next;
+};
+
+template <bool kFp32, bool kVector, int kWaves>
+struct Row {
+  static constexpr int kValues = Lane<kFp32, kVector>::kValues;
+  static constexpr int kParts = kEach / kValues;
+  static constexpr int kThreads = 64 * kWaves;
+
+  // First column of a thread's part p; its values follow one another.
+  __device__ static int column(int p) { return (p * kThreads + static_cast<int>(threadIdx.x)) * kValues; }
+
+  __device__ static void load(const void *rows, int64_t row, int size, float *v) {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      if (column(p) < size) {
+        load_values<kFp32, kVector>(rows, row * size + column(p), v + p * kValues);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) v[p * kValues + i] = 0.0f;
+      }
+    }
+  }
+
+  __device__ static void store(void *rows, int64_t row, int size, const float *v) {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p)
+      if (column(p) < size) store_values<kFp32, kVector>(rows, row * size + column(p), v + p * kValues);
+  }
+
+  // Weights [H] of the rows' type or FP32; zero past the end.
+  __device__ static void weights(const void *w, bool fp32, int size, float *v) {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      float *part = v + p * kValues;
+      if (column(p) >= size) {
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) part[i] = 0.0f;
+      } else if (!kFp32 && fp32) {
+        if constexpr (kVector) {
+          load_values<true, true>(w, column(p), part);
+          load_values<true, true>(w, column(p) + kValues / 2, part + kValues / 2);
+        } else {
+          load_values<true, false>(w, column(p), part);
+        }
+      } else {
+        load_values<kFp32, kVector>(w, column(p), part);
+      }
+    }
+  }
+
+  // The gate's values for the thread's columns.
+  __device__ static void gates(const JoinArgs &a, int64_t row, float *v) {
+    if (a.form == kChannel) {
+      weights(a.gate, a.gate32, a.size, v);
+    } else if (a.form == kRow) {
+      float g;
+      if (kFp32 || a.gate32) g = static_cast<const float *>(a.gate)[row];
+      else g = bf16_value(static_cast<const uint16_t *>(a.gate)[row]);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) v[i] = g;
+    } else {
+      load(a.gate, row, a.size, v);
+    }
+  }
+};
+
+// Sums over the workgroup, in every thread, always in the same order. `turn` changes with
+// each call, so that one barrier is enough: who writes a half again has passed the barrier
+// of the call between, which all reach after they read it.
+template <int kWaves, int kSums>
+__device__ __forceinline__ void group_totals(float (&v)[kSums], float (*shared)[2][kWaves], int &turn) {
+#pragma unroll
+  for (int s = 0; s < kSums; ++s) v[s] = wave_total(v[s]);
+  if constexpr (kWaves > 1) {
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int s = 0; s < kSums; ++s) shared[turn][s][threadIdx.x >> 6] = v[s];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < kSums; ++s) {
+      v[s] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) v[s] += shared[turn][s][w];
+    }
+  }
+}
+
+// 1 / sqrt(mean(v^2) + eps); negative, it is that of 2^-80 v.
+template <int kWaves>
+__device__ __forceinline__ float inverse_root(const float *v, const JoinArgs &a, float (*shared)[2][kWaves], int &turn) {
+  float sum[1] = {0.0f};
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) sum[0] = fmaf(v[i], v[i], sum[0]);
+  group_totals<kWaves, 1>(sum, shared, turn);
+  const float size = static_cast<float>(a.size);
+  if (sum[0] <= 3.4e38f) return 1.0f / sqrtf(sum[0] / size + a.epsilon);
+  sum[0] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) sum[0] = fmaf(v[i] * kSmall, v[i] * kSmall, sum[0]);
+  group_totals<kWaves, 1>(sum, shared, turn);
+  return -1.0f / sqrtf(sum[0] / size);
+}
+
+__device__ __forceinline__ float unit(float v, float inverse) {
+  return inverse < 0.0f ? v * kSmall * -inverse : v * inverse;
+}
+
+// times 1 / sqrt(...) itself
+__device__ __forceinline__ float times_inverse(float v, float inverse) {
+  return inverse < 0.0f ? v * -inverse * kSmall : v * inverse;
+}
+
+// Workgroup = a row, a thread eight of its values.
+template <bool kFp32, bool kVector, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void join_kernel(JoinArgs a) {
+  using R = Row<kFp32, kVector, kWaves>;
+  __shared__ float shared[2][2][kWaves];
+  int turn = 0;
+  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    float j[kEach], w[kEach], first = 0.0f, second = 0.0f;
+    R::load(a.hidden, t, a.size, j);
+    if (a.block) {
+      float n[kEach];
+      R::load(a.block, t, a.size, n);
+      if (a.post) {
+        R::weights(a.post, a.post32, a.size, w);
+        first = inverse_root<kWaves>(n, a, shared, turn);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) n[i] = unit(n[i], first) * w[i];
+      }
+      if (a.form != kNone) {
+        R::gates(a, t, w);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) n[i] *= w[i];
+      }
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) j[i] = fmaf(a.scale, j[i], n[i]);
+      R::store(a.joined, t, a.size, j);
+    }
+    if (a.next) {
+      R::weights(a.next, a.next32, a.size, w);
+      second = inverse_root<kWaves>(j, a, shared, turn);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) w[i] *= unit(j[i], second);
+      R::store(a.out, t, a.size, w);
+    }
+    if (a.statistics && threadIdx.x == 0) {
+      a.statistics[2 * t] = first;
+      a.statistics[2 * t + 1] = second;
+    }
+  }
+}
+
+// Workgroup = rows in steps of the grid; the sums over rows stay in registers and leave as
+// one partial row each, which join_sums_kernel adds up: no atomics, so that a call gives
+// the same bits every time.
+template <bool kFp32, bool kVector, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void join_backward_kernel(JoinArgs a) {
+  using R = Row<kFp32, kVector, kWaves>;
+  __shared__ float shared[2][2][kWaves];
+  int turn = 0;
+  const float part = 1.0f / static_cast<float>(a.size);
+  float sum_next[kEach] = {}, sum_post[kEach] = {}, sum_gate[kEach] = {};
+  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    float j[kEach], unit_block[kEach], n[kEach], gate[kEach], grad[kEach], w[kEach], first = 0.0f;
+    R::load(a.hidden, t, a.size, j);
+    if (a.grad_joined) {
+      R::load(a.grad_joined, t, a.size, grad);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) grad[i] = 0.0f;
+    }
+    if (a.block) {
+      R::load(a.block, t, a.size, unit_block);
+      if (a.form != kNone) {
+        R::gates(a, t, gate);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) gate[i] = 1.0f;
+      }
+      if (a.post) {
+        first = a.statistics[2 * t];
+        R::weights(a.post, a.post32, a.size, w);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          unit_block[i] = unit(unit_block[i], first);
+          n[i] = unit_block[i] * w[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) n[i] = unit_block[i];
+      }
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) j[i] = fmaf(a.scale, j[i], a.form != kNone ? gate[i] * n[i] : n[i]);
+    }
+    if (a.grad_out) {
+      const float second = a.statistics[2 * t + 1];
+      float y[kEach], mean[1] = {0.0f};
+      R::load(a.grad_out, t, a.size, y);
+      R::weights(a.next, a.next32, a.size, w);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        j[i] = unit(j[i], second);
+        sum_next[i] = fmaf(y[i], j[i], sum_next[i]);
+        y[i] *= w[i];
+        mean[0] = fmaf(y[i], j[i], mean[0]);
+      }
+      group_totals<kWaves, 1>(mean, shared, turn);
+      mean[0] *= part;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) grad[i] += times_inverse(fmaf(-j[i], mean[0], y[i]), second);
+    }
+    if (a.grad_hidden) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) w[i] = a.scale * grad[i];
+      R::store(a.grad_hidden, t, a.size, w);
+    }
+    if (!a.block) continue;
+    float totals[2] = {0.0f, 0.0f};
+    if (a.grad_gate) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        n[i] *= grad[i];
+        totals[0] += n[i];
+        sum_gate[i] += n[i];
+      }
+      if (a.grad_gate && a.form == kFull) R::store(a.grad_gate, t, a.size, n);
+    }
+    if (a.form != kNone) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) grad[i] *= gate[i];
+    }
+    if (a.post) {
+      R::weights(a.post, a.post32, a.size, w);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        sum_post[i] = fmaf(grad[i], unit_block[i], sum_post[i]);
+        grad[i] *= w[i];
+        totals[1] = fmaf(grad[i], unit_block[i], totals[1]);
+      }
+    }
+    const bool row_gate = a.grad_gate && a.form == kRow;
+    if (a.post || row_gate) group_totals<kWaves, 2>(totals, shared, turn);
+    if (row_gate && threadIdx.x == 0) {
+      if (kFp32 || a.gate32) static_cast<float *>(a.grad_gate)[t] = totals[0];
+      else static_cast<uint16_t *>(a.grad_gate)[t] = bf16_bits(totals[0]);
+    }
+    if (!a.grad_block) continue;
+    if (a.post) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        grad[i] = times_inverse(fmaf(-unit_block[i], totals[1] * part, grad[i]), first);
+    }
+    R::store(a.grad_block, t, a.size, grad);
+  }
+  if (!a.partial) return;
+  float *rows = a.partial + static_cast<int64_t>(blockIdx.x) * a.sums * a.size;
+  auto leave = [&](const float *v) {
+#pragma unroll
+    for (int p = 0; p < R::kParts; ++p) {
+      const int c = R::column(p);
+      if (c >= a.size) continue;
+#pragma unroll
+      for (int i = 0; i < R::kValues; ++i) rows[c + i] = v[p * R::kValues + i];
+    }
+    rows += a.size;
+  };
+  if (a.grad_next) leave(sum_next);
+  if (a.grad_post) leave(sum_post);
+  if (a.grad_gate && a.form == kChannel) leave(sum_gate);
+}
+
+struct SumsArgs {
+  const float *partial;
+  void *to[3];
+  bool fp32[3];
+  int groups, sums, size;
+};
+
+constexpr int kSumWaves = 16;
+
+// Wave = some of the partial rows of 64 columns, in order; the waves' sums are added in order.
+__global__ __launch_bounds__(64 * kSumWaves) void join_sums_kernel(SumsArgs a) {
+  __shared__ float sums[kSumWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane, which = blockIdx.y;
+  float sum = 0.0f;
+  if (c < a.size) {
+    const float *from = a.partial + static_cast<int64_t>(which) * a.size + c;
+    const int64_t step = static_cast<int64_t>(a.sums) * a.size;
+#pragma unroll 8
+    for (int g = wave; g < a.groups; g += kSumWaves) sum += from[g * step];
+  }
+  sums[wave][lane] = sum;
+  __syncthreads();
+  if (wave || c >= a.size) return;
+#pragma unroll
+  for (int w = 1; w < kSumWaves; ++w) sum += sums[w][lane];
+  if (a.fp32[which]) static_cast<float *>(a.to[which])[c] = sum;
+  else static_cast<uint16_t *>(a.to[which])[c] = bf16_bits(sum);
+}
+
+int backward_groups(int tokens) { return tokens < 1024 ? tokens : 1024; }
+
+int check_join(int hidden_size, int tokens, float epsilon) {
+  if (hidden_size < 1 || hidden_size > kMaxHidden) return fail(CFMOE_EINVAL, "join_block needs a hidden size from 1 to 8192");
+  if (tokens < 0) return fail(CFMOE_EINVAL, "join_block needs a token count of zero or more");
+  if (!(epsilon >= 1e-30f && epsilon <= 1e30f)) return fail(CFMOE_EINVAL, "join_block needs an epsilon from 1e-30 to 1e30");
+  return 0;
+}
+
+// Waves of a row: the fewest whose threads hold it.
+template <typename F>
+int dispatch_row(int size, bool fp32, bool vector, F f) {
+  auto typed = [&](auto waves) {
+    constexpr int kWaves = decltype(waves)::value;
+    if (fp32) return vector ? f(Row<true, true, kWaves>()) : f(Row<true, false, kWaves>());
+    return vector ? f(Row<false, true, kWaves>()) : f(Row<false, false, kWaves>());
+  };
+  if (size <= 64 * kEach) return typed(std::integral_constant<int, 1>());
+  if (size <= 256 * kEach) return typed(std::integral_constant<int, 4>());
+  if (size <= 512 * kEach) return typed(std::integral_constant<int, 8>());
+  return typed(std::integral_constant<int, 16>());
+}
+
+template <bool kFp32, bool kVector, int kWaves>
+int launch_join(Row<kFp32, kVector, kWaves>, const JoinArgs &a, hipStream_t stream) {
+  const unsigned groups = a.tokens < (1 << 20) ? a.tokens : (1 << 20);
+  hipLaunchKernelGGL((join_kernel<kFp32, kVector, kWaves>), dim3(groups), dim3(64 * kWaves), 0, stream, a);
+  return check_launch("join_block");
+}
+
+template <bool kFp32, bool kVector, int kWaves>
+int launch_backward(Row<kFp32, kVector, kWaves>, const JoinArgs &a, hipStream_t stream) {
+  hipLaunchKernelGGL((join_backward_kernel<kFp32, kVector, kWaves>), dim3(backward_groups(a.tokens)), dim3(64 * kWaves), 0,
+                     stream, a);
+  return check_launch("join_block_backward");
+}
+
+Gate gate_of(uint32_t flags) {
+  return flags & CFMOE_GATE_CHANNEL ? kChannel : flags & CFMOE_GATE_ROW ? kRow : flags & CFMOE_GATE_FULL ? kFull : kNone;
+}
+
+}  // namespace
+}  // namespace cfmoe
+
+extern "C" {
+
+using namespace cfmoe;
+
+CFMOE_API int cfmoe_join_block(int32_t hidden_size, uint32_t flags, const void *hidden, const void *block,
+                               const void *post_weight, const void *gate, float residual_scale,
+                               const void *next_weight, float epsilon, void *joined, void *next, float *statistics,
+                               int32_t tokens, cfmoe_stream stream) {
+  if (int rc = check_join(hidden_size, tokens, epsilon)) return rc;
+  if (tokens == 0) return 0;
+  JoinArgs a = {};
+  a.form = gate_of(flags);
+  if (!hidden || (block ? !joined : !next_weight) || (next_weight && !next) || (a.form != kNone && !gate))
+    return fail(CFMOE_EINVAL, "NULL argument");
+  if (!block && (post_weight || a.form != kNone)) return fail(CFMOE_EINVAL, "join_block takes a post weight or a gate with a block only");
+  a.hidden = hidden;
+  a.block = block;
+  a.post = post_weight;
+  a.gate = a.form != kNone ? gate : nullptr;
+  a.next = next_weight;
+  a.joined = joined;
+  a.out = next;
+  a.statistics = statistics;
+  a.tokens = tokens;
+  a.size = hidden_size;
+  a.scale = residual_scale;
+  a.epsilon = epsilon;
+  const bool fp32 = flags & CFMOE_FP32;
+  a.post32 = fp32 || flags & CFMOE_POST_FP32;
+  a.gate32 = fp32 || flags & CFMOE_GATE_FP32;
+  a.next32 = fp32 || flags & CFMOE_NEXT_FP32;
+  if (a.form == kFull && !fp32 && flags & CFMOE_GATE_FP32)
+    return fail(CFMOE_EINVAL, "join_block needs a gate per value in the rows' type");
+  const bool vector = hidden_size % (fp32 ? 4 : 8) == 0 && !misaligned16(hidden) && !misaligned16(block) &&
+                      !misaligned16(a.post) && !misaligned16(a.form == kRow ? nullptr : a.gate) && !misaligned16(a.next) &&
+                      !misaligned16(joined) && !misaligned16(next);
+  return dispatch_row(hidden_size, fp32, vector, [&](auto row) { return launch_join(row, a, stream); });
+}
+
+CFMOE_API int64_t cfmoe_join_block_backward_scratch_bytes(int32_t hidden_size, int32_t sums, int32_t tokens) {
+  if (hidden_size < 1 || hidden_size > kMaxHidden || sums < 0 || sums > 3 || tokens < 0)
+    return -fail(CFMOE_EINVAL, "join_block needs a hidden size from 1 to 8192, up to 3 sums and 0 or more tokens");
+  return static_cast<int64_t>(backward_groups(tokens)) * sums * hidden_size * 4;
+}
+
+CFMOE_API int cfmoe_join_block_backward(int32_t hidden_size, uint32_t flags, const void *hidden, const void *block,
+                                        const void *post_weight, const void *gate, float residual_scale,
+                                        const void *next_weight, const float *statistics, const void *grad_joined,
+                                        const void *grad_next, void *grad_hidden, void *grad_block,
+                                        void *grad_post_weight, void *grad_gate, void *grad_next_weight, void *scratch,
+                                        int32_t tokens, cfmoe_stream stream) {
+  if (int rc = check_join(hidden_size, tokens, 1.0f)) return rc;
+  JoinArgs a = {};
+  a.form = gate_of(flags);
+  const bool fp32 = flags & CFMOE_FP32;
+  SumsArgs s = {};
+  if (grad_next_weight) s.fp32[s.sums] = fp32 || flags & CFMOE_NEXT_FP32, s.to[s.sums++] = grad_next_weight;
+  if (grad_post_weight) s.fp32[s.sums] = fp32 || flags & CFMOE_POST_FP32, s.to[s.sums++] = grad_post_weight;
+  if (grad_gate && a.form == kChannel) s.fp32[s.sums] = fp32 || flags & CFMOE_GATE_FP32, s.to[s.sums++] = grad_gate;
+  if ((tokens && (!hidden || (a.form != kNone && !gate) || (grad_next && !next_weight) ||
+                  ((post_weight || grad_next) && !statistics) || (s.sums && !scratch))) ||
+      (grad_next_weight && tokens && !grad_next) || (grad_post_weight && !post_weight) || (grad_gate && a.form == kNone))
+    return fail(CFMOE_EINVAL, "NULL argument");
+  if (tokens && !block && (post_weight || a.form != kNone || grad_block || grad_joined))
+    return fail(CFMOE_EINVAL, "join_block takes a post weight or a gate with a block only");
+  if (a.form == kFull && !fp32 && flags & CFMOE_GATE_FP32)
+    return fail(CFMOE_EINVAL, "join_block needs a gate per value in the rows' type");
+  a.hidden = hidden;
+  a.block = block;
+  a.post = post_weight;
+  a.gate = a.form != kNone ? gate : nullptr;
+  a.next = next_weight;
+  a.statistics = const_cast<float *>(statistics);
+  a.grad_joined = grad_joined;
+  a.grad_out = grad_next;
+  a.grad_hidden = grad_hidden;
+  a.grad_block = grad_block;
+  a.grad_gate = grad_gate;
+  a.partial = s.sums ? static_cast<float *>(scratch) : nullptr;
+  a.tokens = tokens;
+  a.size = hidden_size;
+  a.sums = s.sums;
+  a.scale = residual_scale;
+  a.post32 = fp32 || flags & CFMOE_POST_FP32;
+  a.gate32 = fp32 || flags & CFMOE_GATE_FP32;
+  a.next32 = fp32 || flags & CFMOE_NEXT_FP32;
+  a.grad_post = grad_post_weight;
+  a.grad_next = grad_next_weight;
+  if (tokens) {
+    const bool vector = hidden_size % (fp32 ? 4 : 8) == 0 && !misaligned16(hidden) && !misaligned16(block) &&
+                        !misaligned16(a.post) && !misaligned16(a.form == kRow ? nullptr : a.gate) &&
+                        !misaligned16(a.next) && !misaligned16(grad_joined) && !misaligned16(grad_next) &&
+                        !misaligned16(grad_hidden) && !misaligned16(grad_block) &&
+                        !misaligned16(a.form == kFull ? grad_gate : nullptr);
+    if (int rc = dispatch_row(hidden_size, fp32, vector, [&](auto row) { return launch_backward(row, a, stream); })) return rc;
+  }
+  if (!s.sums) return 0;
+  s.partial = a.partial;
+  s.groups = backward_groups(tokens);
+  s.size = hidden_size;
+  hipLaunchKernelGGL(join_sums_kernel, dim3((hidden_size + 63) / 64, s.sums), dim3(64 * kSumWaves), 0, stream, s);
+  return check_launch("join_block_sums");
+}
+
+}  // extern "C"

@@ -36,7 +36,7 @@ extern "C" {
 
 typedef struct ihipStream_t *cfmoe_stream;
 
-#define CFMOE_ABI_VERSION 11
+#define CFMOE_ABI_VERSION 12
 
 /* cfmoe_dims.flags */
 #define CFMOE_POINT 1u          /* point score (else five-node Gauss-Hermite) */
@@ -56,8 +56,15 @@ typedef struct ihipStream_t *cfmoe_stream;
 
 #define CFMOE_RENORMALISE 1024u /* cfmoe_route: weights sum to 1 over the kept experts (else
                                    they are the kept part of the softmax over all) */
-#define CFMOE_FP32 2048u        /* cfmoe_quantise_fp4: FP32 weights (else BF16) */
+#define CFMOE_FP32 2048u        /* cfmoe_quantise_fp4: FP32 weights (else BF16); rows of the
+                                   entry points around the experts: FP32 (else BF16) */
 #define CFMOE_FP4 4096u         /* cfmoe_routed_experts: microscaled 4-bit weights (else BF16) */
+#define CFMOE_POST_FP32 8192u    /* cfmoe_join_block with BF16 rows: FP32 post_weight, */
+#define CFMOE_GATE_FP32 16384u   /* FP32 gate (of a channel or a row), */
+#define CFMOE_NEXT_FP32 32768u   /* FP32 next_weight (each else BF16) */
+#define CFMOE_GATE_CHANNEL 65536u /* cfmoe_join_block: gate is [H], */
+#define CFMOE_GATE_ROW 131072u   /* [T, 1] */
+#define CFMOE_GATE_FULL 262144u  /* or [T, H] (else there is none) */
 
 /* Stages of one call, in launch order (cfmoe_launch_stage). */
 #define CFMOE_STAGE_PREPARE 0 /* route, rotate, mask, grid quantisation */
@@ -301,6 +308,85 @@ CFMOE_API int cfmoe_routed_experts(int32_t hidden_size, int32_t width, int32_t e
                                    const uint8_t *gate_up_scales, const void *down,
                                    const uint8_t *down_scales, const void *hidden, const void *ids,
                                    const void *weights, const uint8_t *padding, void *out,
+                                   void *scratch, int32_t tokens, cfmoe_stream stream);
+
+/* Tokens laid out by expert. A pair (t, k) is kept where ids[t, k] lies in [0, E) and t is
+ * not marked in padding uint8 [T] (or NULL). Rows are the kept pairs by expert, in the
+ * batch's order, then the dropped ones: offsets [E + 1] (offsets[E] rows are kept), pairs
+ * [T top_k] (t top_k + k of each row) and places [T, top_k] (row of each pair, -1 - row of
+ * a dropped one). flags: CFMOE_IDS_INT64. E at most 4096, top_k 64, T top_k 2^30. T = 0
+ * writes offsets only. scratch: cfmoe_sort_by_expert_scratch_bytes bytes (NULL where 0),
+ * 4-byte aligned; calls that overlap need their own. No reference counterpart. */
+CFMOE_API int64_t cfmoe_sort_by_expert_scratch_bytes(int32_t tokens, int32_t top_k, int32_t experts);
+CFMOE_API int cfmoe_sort_by_expert(int32_t experts, int32_t top_k, uint32_t flags, const void *ids,
+                                   const uint8_t *padding, int32_t *offsets, int32_t *places,
+                                   int32_t *pairs, void *scratch, int32_t tokens,
+                                   cfmoe_stream stream);
+
+/* Rows of the pairs: rows [T top_k, H] of hidden [T, H], zero for dropped pairs; back, out
+ * [T, H] = the kept pairs' rows summed in slot order with weights [T, top_k] (NULL: 1), FP32
+ * sums rounded once, which without weights is also the gradient of the first; and the
+ * gradient of the second: grad_rows (or NULL) and grad_weights (or NULL; needs rows). Rows
+ * of dropped pairs and their weights are not read. places as cfmoe_sort_by_expert writes
+ * them; a place past T top_k is skipped. flags: CFMOE_FP32 (rows), CFMOE_WEIGHTS_BF16. H
+ * from 1 to 2^20; rows 16-byte aligned with H a multiple of 8 (FP32: 4) are faster. */
+CFMOE_API int cfmoe_gather_rows(int32_t hidden_size, int32_t top_k, uint32_t flags,
+                                const void *hidden, const int32_t *places, void *rows,
+                                int32_t tokens, cfmoe_stream stream);
+CFMOE_API int cfmoe_combine_rows(int32_t hidden_size, int32_t top_k, uint32_t flags,
+                                 const void *rows, const int32_t *places, const void *weights,
+                                 void *out, int32_t tokens, cfmoe_stream stream);
+CFMOE_API int cfmoe_combine_rows_backward(int32_t hidden_size, int32_t top_k, uint32_t flags,
+                                          const void *grad_out, const void *rows,
+                                          const int32_t *places, const void *weights,
+                                          void *grad_rows, void *grad_weights, int32_t tokens,
+                                          cfmoe_stream stream);
+
+/* A block joined to the residual stream, with the norms around it, of rows [T, H]:
+ *   n = block / sqrt(mean(block^2) + epsilon) * post_weight   (block itself where NULL)
+ *   joined = residual_scale * hidden + gate * n
+ *   next = joined / sqrt(mean(joined^2) + epsilon) * next_weight  (not written where NULL)
+ * with block NULL: next is the norm of hidden, and joined is not written. gate is [H], [T, 1]
+ * or [T, H] by CFMOE_GATE_CHANNEL, _ROW, _FULL, of the rows' type or with CFMOE_GATE_FP32
+ * FP32 (not per value); weights [H] likewise. statistics [T, 2] fp32 (or NULL) is what the
+ * backward call takes. FP32 sums; next is of joined before its rounding. joined may be hidden
+ * or block. H from 1 to 8192, epsilon 1e-30 to 1e30. flags: CFMOE_FP32 and those named.
+ * The backward call takes the same inputs, the gradients of joined and next (either may be
+ * NULL) and writes those asked for (not NULL); scratch: ..._backward_scratch_bytes of the
+ * number of gradients summed over rows that are asked for (post_weight, next_weight, a
+ * channel gate), 16-byte aligned; calls that overlap need their own. A call repeated
+ * gives the same bits. No reference counterpart. */
+CFMOE_API int cfmoe_join_block(int32_t hidden_size, uint32_t flags, const void *hidden,
+                               const void *block, const void *post_weight, const void *gate,
+                               float residual_scale, const void *next_weight, float epsilon,
+                               void *joined, void *next, float *statistics, int32_t tokens,
+                               cfmoe_stream stream);
+CFMOE_API int64_t cfmoe_join_block_backward_scratch_bytes(int32_t hidden_size, int32_t sums,
+                                                          int32_t tokens);
+CFMOE_API int cfmoe_join_block_backward(
+    int32_t hidden_size, uint32_t flags, const void *hidden, const void *block,
+    const void *post_weight, const void *gate, float residual_scale, const void *next_weight,
+    const float *statistics, const void *grad_joined, const void *grad_next, void *grad_hidden,
+    void *grad_block, void *grad_post_weight, void *grad_gate, void *grad_next_weight,
+    void *scratch, int32_t tokens, cfmoe_stream stream);
+
+/* Low-rank adapters of a batch's requests beside a shared projection, whose product base
+ * is given: out[t] = base[t] + scales[a] decoder[a] (encoder[a] hidden[t]), a = slots[t], and
+ * base[t] itself, bit for bit, where a lies outside [0, N). bf16 rows base and out [T, O]
+ * and hidden [T, H] with row strides in values; contiguous bf16 encoder [N, R, H] and
+ * decoder [N, O, R]; slots int32 (CFMOE_IDS_INT64: int64) [T], scales fp32 [N] or NULL
+ * (1). FP32 sums; the inner values are held as two BF16 numbers (2^-16 off), and out is
+ * rounded once. out may be base, with its stride, or hidden; no other overlap. H and O
+ * multiples of 8 up to 65536, R of 8 up to 256, strides of 8; N at most 4096, T 2^24. All
+ * 16-byte aligned but slots and scales. scratch: cfmoe_apply_adapters_scratch_bytes; calls
+ * that overlap need their own. No reference counterpart. */
+CFMOE_API int64_t cfmoe_apply_adapters_scratch_bytes(int32_t rank, int32_t adapters,
+                                                     int32_t tokens);
+CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t rank,
+                                   int32_t adapters, uint32_t flags, const void *base,
+                                   int64_t base_stride, const void *hidden, int64_t hidden_stride,
+                                   const void *encoder, const void *decoder, const void *slots,
+                                   const float *scales, void *out, int64_t out_stride,
                                    void *scratch, int32_t tokens, cfmoe_stream stream);
 
 /* Thread-local message of the last failing call. */
