@@ -73,7 +73,7 @@ def apply_adapters(
     16-byte aligned). `out` may be `base`, whose rows without an adapter are then left
     alone, or `hidden`; no other overlap. H and O are multiples of 8 up to 65536, R of 8 up
     to 256, N up to 4096, tokens up to 2^24; zero tokens give an empty output. Two HIP launches
-    on the current stream of the tensors' device, up to four for more than 1024 tokens, with
+    on the current stream of the tensors' device, up to four for more than 256 tokens, with
     scratch allocated per call; they can be captured in a graph. Tensors that require
     gradients are refused while gradients are on.
     """
@@ -129,7 +129,7 @@ def apply_adapters(
         raise ValueError("out must be BF16 rows [tokens, O] on the rows' device, one behind another")
     elif tokens and (_overlap(out, base) or _overlap(out, hidden)):
         raise ValueError("out overlaps base or hidden and is not the same rows")
-    size = _ext.adapters_scratch_bytes(rank, n, tokens)
+    size = _ext.adapters_scratch_bytes(h, rank, n, tokens)
     scratch = torch.empty(size, dtype=torch.uint8, device=device)
     _ext.run(
         _ext.library().cfmoe_apply_adapters, device, h, o, rank, n,

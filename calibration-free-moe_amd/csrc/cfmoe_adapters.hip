@@ -6,14 +6,15 @@
 // a token whose slot names none keeps its row of `base`, bit for bit.
 //
 // Tokens of one adapter share its weights: they form tiles, and a tile's products are
-// matrix instructions, C_a x over the hidden dimension (adapter_inner_kernel, waves share
-// it and add up in LDS) and D_a v over the rank (adapter_out_kernel). A decode step's tiles
-// hold a token or two, which leaves most columns of an instruction empty: what bounds it
-// is the weights' reading, once for each tile.
+// matrix instructions, v = s_a C_a x over the hidden dimension and D_a v over the rank. A
+// decode step's tiles hold a token or two, which leaves most columns of an instruction
+// empty: what bounds it is the weights' reading, once for each tile. The hidden dimension
+// and the ranks are spread over workgroups (adapter_inner_kernel), and the second launch
+// (adapter_out_kernel) adds up their parts of v. Many tokens are sorted by adapter first.
 //
-// v = s_a C_a x is FP32 in memory between the two. As operand of the second product it is
-// the sum of two BF16 numbers (2^-16 off: the first cut off, so that the second has its
-// sign and an infinite weight meets no zero where v is not one), and out is rounded once.
+// As operand of the second product v is the sum of two BF16 numbers (2^-16 off: the first
+// cut off, so that the second has its sign and an infinite weight meets no zero where v is
+// not one), and out is rounded once.
 
 #include "cfmoe_rows.h"
 
@@ -23,22 +24,28 @@ namespace {
 constexpr int kMaxAdapters = 4096;
 constexpr int kMaxRank = 256;
 constexpr int kMaxSize = 65536;
-constexpr int kInnerTokens = 16;  // of a tile of the first product
-constexpr int kInnerWaves = 16;
-constexpr int kOutWaves = 4;
-constexpr int kOutColumns = 64;   // outputs of one wave
-constexpr int kFewTokens = 1024;  // up to which a workgroup finds its tile by itself
+constexpr int kFewTokens = 256;    // up to which a workgroup finds its tile by itself
+constexpr int kTokens = 16;        // of a tile, few tokens
+constexpr int kManyTokens = 32;    // of a tile, many tokens
+constexpr int kWaves = 4;
+constexpr int kUnit = 8;           // values of 16 bytes
+constexpr int kColumns = 64;       // outputs of one wave
+constexpr int kTurn = 64 * kWaves; // hidden values that the waves take at a time
+constexpr int kFewSplits = 16;     // of the hidden dimension at most
+constexpr int kManySplits = 2;
+constexpr int kMostGroups = 2048;  // workgroups of the second launch, from which each takes more outputs
 
 struct AdapterArgs {
   const uint16_t *base, *x, *encoder, *decoder;
   const void *slots;
   const float *scales;
   uint16_t *out;
-  float *inner;            // [T, R]
+  float *inner;            // [splits, T, R]: parts of v, tokens in sorted order where they are sorted
   const int32_t *offsets;  // [N + 1] and
   const int32_t *pairs;    // [T]: tokens by adapter (many tokens only)
   int64_t base_stride, x_stride, out_stride;
   int tokens, hidden, outputs, rank, adapters;
+  int splits, share;       // of the hidden dimension, and values of one
   bool slots64;
 };
 
@@ -48,192 +55,322 @@ __device__ __forceinline__ int slot_of(const AdapterArgs &a, int t) {
   return s >= 0 && s < a.adapters ? static_cast<int>(s) : a.adapters;
 }
 
-// Tokens of one adapter, up to kTile: tile `index` of the call. False for a workgroup that
-// has none. Few tokens (kSorted false): tile t is led by token t, if a whole number of
-// tiles' tokens of its adapter come before it; the workgroup reads all slots. Many: the
-// tokens are sorted, and the tile is found from the adapters' offsets. All threads of the
-// workgroup call it; it ends with a barrier.
-template <bool kSorted, int kTile, int kWaves>
-__device__ __forceinline__ bool find_tile(const AdapterArgs &a, int index, int *members, int &adapter, int &count) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if constexpr (kSorted) {
-    int before = 0;  // tiles of earlier adapters
-    for (int first = 0; first <= a.adapters; first += 64) {
-      const int n = first + lane;
-      int from = 0, to = 0;
-      if (n <= a.adapters) {
-        from = a.offsets[n];
-        to = n < a.adapters ? a.offsets[n + 1] : a.tokens;
-      }
-      const int tiles = (to - from + kTile - 1) / kTile;
-      int scan = tiles;
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) {
-        const int below = __shfl_up(scan, m);
-        if (lane >= m) scan += below;
-      }
-      const uint64_t past = __ballot(before + scan > index);
-      if (past) {
-        const int owner = __builtin_ctzll(past);
-        const int start = __shfl(from, owner) + (index - before - __shfl(scan - tiles, owner)) * kTile;
-        adapter = __builtin_amdgcn_readfirstlane(first + owner);
-        count = __builtin_amdgcn_readfirstlane(min(kTile, __shfl(to, owner) - start));
-        for (int i = threadIdx.x; i < count; i += 64 * kWaves) members[i] = a.pairs[start + i];
-        __syncthreads();
-        return true;
-      }
-      before += __shfl(scan, 63);
-    }
-    return false;
-  } else {
-    __shared__ uint64_t masks[kFewTokens / 64];
-    adapter = __builtin_amdgcn_readfirstlane(slot_of(a, index));
-    for (int first = wave * 64; first < a.tokens; first += 64 * kWaves) {
-      const int t = first + lane;
-      const uint64_t same = __ballot(t < a.tokens && slot_of(a, t) == adapter);
-      if (lane == 0) masks[first / 64] = same;
-    }
-    __syncthreads();
-    int before = 0;
-    for (int w = 0; w < index / 64; ++w) before += __builtin_popcountll(masks[w]);
-    before += __builtin_popcountll(masks[index / 64] & ((UINT64_C(1) << (index % 64)) - 1));
-    if (before % kTile) return false;
-    // each token from `index` on takes its place
-    int total = before;
-    for (int w = index / 64; w < (a.tokens + 63) / 64; ++w) total += __builtin_popcountll(w == index / 64 ? masks[w] >> (index % 64) : masks[w]);
-    count = min(kTile, total - before);
-    int place = 0;
-    for (int w = 0; w < (a.tokens + 63) / 64; ++w) {
-      if (w % kWaves == wave && (masks[w] >> lane) & 1) {
-        const int rank = place + __builtin_popcountll(masks[w] & ((UINT64_C(1) << lane) - 1)) - before;
-        if (rank >= 0 && rank < kTile) members[rank] = 64 * w + lane;
-      }
-      place += __builtin_popcountll(masks[w]);
-    }
-    __syncthreads();
-    return true;
+// Tokens of one adapter, up to kTokens, of a call of few: tile t is led by token t, if a
+// whole number of tiles' tokens of its adapter come before it; the workgroup reads all
+// slots. False where no tile is. All threads of the workgroup call it.
+__device__ __forceinline__ bool find_tile(const AdapterArgs &a, int leader, int *members, int &adapter, int &count) {
+  __shared__ uint64_t masks[kFewTokens / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, words = (a.tokens + 63) / 64;
+  adapter = __builtin_amdgcn_readfirstlane(slot_of(a, leader));
+  for (int w = wave; w < words; w += kWaves) {
+    const int t = 64 * w + lane;
+    const uint64_t same = __ballot(t < a.tokens && slot_of(a, min(t, a.tokens - 1)) == adapter);
+    if (lane == 0) masks[w] = same;
   }
+  __syncthreads();
+  int before = __builtin_popcountll(masks[leader / 64] & ((UINT64_C(1) << (leader % 64)) - 1));
+  for (int w = 0; w < leader / 64; ++w) before += __builtin_popcountll(masks[w]);
+  if (before % kTokens) return false;
+  int passed = 0;
+  for (int w = 0; w < words; ++w) {
+    const uint64_t same = masks[w];
+    const int rank = passed - before + __builtin_popcountll(same & ((UINT64_C(1) << lane) - 1));
+    if (wave == 0 && (same >> lane & 1) && rank >= 0 && rank < kTokens) members[rank] = 64 * w + lane;
+    passed += __builtin_popcountll(same);
+  }
+  count = __builtin_amdgcn_readfirstlane(min(kTokens, passed - before));
+  __syncthreads();
+  return true;
+}
+
+// The same of a call whose tokens are sorted by adapter: tile `index`, tiles counted
+// through the adapters' offsets by each wave for itself.
+template <int kTile>
+__device__ __forceinline__ bool find_sorted_tile(const AdapterArgs &a, int index, int &adapter, int &start, int &count) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;  // tiles of earlier adapters
+  for (int first = 0; first <= a.adapters; first += 64) {
+    const int n = first + lane;
+    int from = 0, to = 0;
+    if (n <= a.adapters) {
+      from = a.offsets[n];
+      to = n < a.adapters ? a.offsets[n + 1] : a.tokens;
+    }
+    const int tiles = (to - from + kTile - 1) / kTile;
+    int scan = tiles;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int below = __shfl_up(scan, m);
+      if (lane >= m) scan += below;
+    }
+    const uint64_t past = __ballot(before + scan > index);
+    if (past) {
+      const int owner = __builtin_ctzll(past);
+      adapter = first + owner;
+      start = __builtin_amdgcn_readlane(from, owner) +
+              (index - before - __builtin_amdgcn_readlane(scan - tiles, owner)) * kTile;
+      count = min(kTile, __builtin_amdgcn_readlane(to, owner) - start);
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(scan, 63);
+  }
+  return false;
 }
 
 __device__ __forceinline__ u32x4 load16(const uint16_t *p) { return *reinterpret_cast<const u32x4 *>(p); }
 
-// inner[t, r] = s sum_h C[r, h] x[t, h] for a tile of 16 tokens and kTiles tiles of 16
-// ranks. The waves take the hidden dimension in turns of 64; a lane's operands are 16
-// values that follow one another (the order of products in a sum is free, and both
-// operands have the same), so that four lanes read 128 bytes of a row.
-template <bool kSorted, int kTiles>
-__global__ __launch_bounds__(64 * kInnerWaves) void adapter_inner_kernel(AdapterArgs a) {
-  __shared__ int members[kInnerTokens];
-  __shared__ float sums[kInnerWaves][kTiles][256];
-  int adapter, count;
-  if (!find_tile<kSorted, kInnerTokens, kInnerWaves>(a, blockIdx.x, members, adapter, count)) return;
-  if (adapter >= a.adapters) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q = lane >> 4;
-  const int r0 = blockIdx.y * 16 * kTiles;
-  const uint16_t *x = a.x + members[min(m, count - 1)] * a.x_stride;
-  const uint16_t *c[kTiles];
+// Pairs of BF16 numbers whose sums are v to 2^-16, the first cut off.
+__device__ __forceinline__ void split(f32x4 v, u32x2 &high, u32x2 &low) {
 #pragma unroll
-  for (int i = 0; i < kTiles; ++i)
-    c[i] = a.encoder + (static_cast<int64_t>(adapter) * a.rank + min(r0 + 16 * i + m, a.rank - 1)) * a.hidden;
-  f32x4 d[kTiles] = {};
-  for (int h = 64 * wave + 16 * q; h - 16 * q < a.hidden; h += 64 * kInnerWaves) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const bool in = h + 8 * s < a.hidden;
-      const u32x4 zero = {0, 0, 0, 0};
-      const u32x4 xv = in ? load16(x + h + 8 * s) : zero;
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) d[i] = mma(in ? load16(c[i] + h + 8 * s) : zero, xv, d[i]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) sums[wave][i][m * 16 + 4 * q + r] = d[i][r];
-  __syncthreads();
-  const float scale = a.scales ? a.scales[adapter] : 1.0f;
-  for (int i = threadIdx.x; i < 256 * kTiles; i += 64 * kInnerWaves) {
-    const int tile = i / 256, token = i % 256 / 16, r = r0 + 16 * tile + i % 16;
-    if (token >= count || r >= a.rank) continue;
-    float total = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kInnerWaves; ++w) total += sums[w][tile][i % 256];
-    a.inner[static_cast<int64_t>(members[token]) * a.rank + r] = scale * total;
-  }
-}
-
-// Two BF16 numbers whose sum is v to 2^-16, the first cut off: high and low halves of eight.
-__device__ __forceinline__ void split(const float *v, u32x4 &high, u32x4 &low) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const uint32_t a = __float_as_uint(v[2 * i]) & 0xffff0000u, b = __float_as_uint(v[2 * i + 1]) & 0xffff0000u;
     high[i] = a >> 16 | b;
     low[i] = bf16_pair(v[2 * i] - __uint_as_float(a), v[2 * i + 1] - __uint_as_float(b));
   }
 }
 
-// out = base + D v for a tile of tokens, a wave 64 outputs of them. Row 4 q + r of the i-th
-// matrix tile is output 16 q + 4 i + r, so that a lane ends with 16 outputs that follow one
-// another, and four lanes with 128 bytes of a row.
-template <bool kSorted, int kGroups>
-__global__ __launch_bounds__(64 * kOutWaves) void adapter_out_kernel(AdapterArgs a) {
-  __shared__ int members[16 * kGroups];
-  int adapter, count;
-  if (!find_tile<kSorted, 16 * kGroups, kOutWaves>(a, blockIdx.x, members, adapter, count)) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q = lane >> 4;
-  const int o0 = (blockIdx.y * kOutWaves + wave) * kOutColumns;
-  if (o0 >= a.outputs) return;
-  const bool bare = adapter >= a.adapters;
-  if (bare && a.out == a.base) return;
-  const uint16_t *d[4];
+// Values of a row of v in LDS: whole steps of 32, and a unit for the banks.
+__host__ __device__ __forceinline__ int parts_row(int rank) { return (rank + 31) / 32 * 32 + kUnit; }
+
+// inner[split, token, r] = a split's part of s sum_h C[r, h] x[token, h], of a tile of
+// tokens and kTiles tiles of 16 ranks. The waves take the split's hidden values in turns of
+// 64 and add up in LDS. The operands pass through LDS, each wave's through its own part of
+// it: eight lanes read 128 bytes of a row from memory, where the matrix instruction's own
+// layout has neighbouring lanes read from different rows. Rows of LDS are an odd number of
+// 16-byte units long, so that the 16 rows of an operand lie in different banks.
+template <bool kSorted, int kTiles>
+__global__ __launch_bounds__(64 * kWaves) void adapter_inner_kernel(AdapterArgs a) {
+  constexpr int kTile = kSorted ? kManyTokens : kTokens, kGroups = kTile / 16;
+  constexpr int kRows = 16 * kTiles + kTile, kLoads = kRows / 8, kRankLoads = 2 * kTiles;
+  __shared__ __attribute__((aligned(16))) uint16_t stage[kWaves][kRows][64 + kUnit];
+  __shared__ int members[kTokens];
+  static_assert(sizeof(float) * kWaves * kGroups * kTiles * 256 <= sizeof(stage), "the sums take the stage's place");
+  float(*sums)[kGroups][kTiles][256] = reinterpret_cast<float(*)[kGroups][kTiles][256]>(stage);
+  int adapter, start = 0, count;
+  if constexpr (kSorted) {
+    if (!find_sorted_tile<kTile>(a, blockIdx.x, adapter, start, count)) return;
+  } else {
+    if (!find_tile(a, blockIdx.x, members, adapter, count)) return;
+  }
+  if (adapter >= a.adapters) return;
+  const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r0 = blockIdx.y * 16 * kTiles;
+  // this lane's unit of every eighth row: C's, then the tokens' (those past the end are the
+  // last again, and what they give is not stored)
+  const uint16_t *row[kLoads];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    d[i] = a.decoder + (static_cast<int64_t>(bare ? 0 : adapter) * a.outputs + min(o0 + m / 4 * 16 + 4 * i + m % 4, a.outputs - 1)) * a.rank;
+  for (int j = 0; j < kLoads; ++j) {
+    const int r = min(r0 + 8 * j + lane / 8, a.rank - 1), t = min(8 * (j - kRankLoads) + lane / 8, count - 1);
+    if (j < kRankLoads) row[j] = a.encoder + (static_cast<int64_t>(adapter) * a.rank + r) * a.hidden;
+    else row[j] = a.x + static_cast<int64_t>(kSorted ? a.pairs[start + t] : members[t]) * a.x_stride;
+    row[j] += kUnit * (lane % 8);
+  }
+  f32x4 d[kGroups][kTiles] = {};
+  const int first = blockIdx.z * a.share, last = min(first + a.share, a.hidden);
+  u32x4 raw[kLoads];
+  auto fetch = [&](int h0) {
+    if (h0 + 64 <= last) {
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    if (16 * g >= count) break;
-    const int64_t t = members[min(16 * g + m, count - 1)];
-    f32x4 sum[4] = {};
-    if (!bare) {
-      for (int k = 8 * q; k - 8 * q < a.rank; k += 32) {
-        const bool in = k < a.rank;
-        u32x4 high = {0, 0, 0, 0}, low = {0, 0, 0, 0};
-        if (in) {
-          float v[8];
-          load_values<true, true>(a.inner, t * a.rank + k, v);
-          load_values<true, true>(a.inner, t * a.rank + k + 4, v + 4);
-          split(v, high, low);
-        }
+      for (int j = 0; j < kLoads; ++j) raw[j] = load16(row[j] + h0);
+    } else if (h0 < last) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const u32x4 w = in ? load16(d[i] + k) : u32x4{0, 0, 0, 0};
-          sum[i] = mma(w, low, mma(w, high, sum[i]));
-        }
+      for (int j = 0; j < kLoads; ++j) {
+        raw[j] = u32x4{0, 0, 0, 0};
+        if (h0 + kUnit * (lane % 8) < last) raw[j] = load16(row[j] + h0);
       }
     }
-    if (16 * g + m >= count) continue;
+  };
+  fetch(first + 64 * wave);
+  for (int h0 = first + 64 * wave; h0 < last; h0 += kTurn) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+      *reinterpret_cast<u32x4 *>(&stage[wave][8 * j + lane / 8][kUnit * (lane % 8)]) = raw[j];
+    fetch(h0 + kTurn);
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int o = o0 + 16 * q + 8 * s;
-      if (o >= a.outputs) continue;
-      u32x4 row = load16(a.base + t * a.base_stride + o);
-      if (!bare) {
-        float v[8];
+      u32x4 xv[kGroups];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[2 * i] = __uint_as_float(row[i] << 16) + sum[2 * s + i / 2][2 * i % 4];
-          v[2 * i + 1] = __uint_as_float(row[i] & 0xffff0000u) + sum[2 * s + i / 2][2 * i % 4 + 1];
-        }
-        row = u32x4{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])};
+      for (int g = 0; g < kGroups; ++g) xv[g] = load16(&stage[wave][16 * (kTiles + g) + m][32 * s + kUnit * q]);
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        const u32x4 cv = load16(&stage[wave][16 * i + m][32 * s + kUnit * q]);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) d[g][i] = mma(cv, xv[g], d[g][i]);
       }
-      *reinterpret_cast<u32x4 *>(a.out + t * a.out_stride + o) = row;
     }
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) *reinterpret_cast<f32x4 *>(&sums[wave][g][i][m * 16 + 4 * q]) = d[g][i];
+  __syncthreads();
+  const float scale = a.scales ? a.scales[adapter] : 1.0f;
+  const int n = threadIdx.x % 16;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    const int t = 16 * g + threadIdx.x / 16;
+    if (t >= count) return;
+    float *to = a.inner + (static_cast<int64_t>(blockIdx.z) * a.tokens + (kSorted ? start + t : members[t])) * a.rank + r0 + n;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      if (r0 + 16 * i + n >= a.rank) break;
+      float total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) total += sums[w][g][i][threadIdx.x];
+      to[16 * i] = scale * total;
+    }
+  }
+}
+
+// Output of matrix row n of tile i, behind a wave's first: lane 16 q + m ends with outputs
+// 8 q .. 8 q + 7 and 32 + 8 q .. of token m, so that four lanes take 64 bytes of a row.
+__device__ __forceinline__ int output_of(int i, int n) { return i / 2 * 32 + n / 4 * 8 + i % 2 * 4 + n % 4; }
+
+// out = base + D v for a tile of tokens, a wave 64 outputs of them at a time: rows of base
+// and D on their way first, then v from its parts, as two BF16 numbers in LDS. kShort is for
+// ranks up to 32, whose rows of D the next 64 outputs' are read ahead of.
+template <bool kSorted, bool kShort>
+__global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a) {
+  constexpr int kTile = kSorted ? kManyTokens : kTokens, kGroups = kTile / 16;
+  extern __shared__ __attribute__((aligned(16))) uint16_t parts[];  // [2, kTile, parts_row(R)]
+  __shared__ int members[kTokens];
+  int adapter, start = 0, count;
+  if constexpr (kSorted) {
+    if (!find_sorted_tile<kTile>(a, blockIdx.x, adapter, start, count)) return;
+  } else {
+    if (!find_tile(a, blockIdx.x, members, adapter, count)) return;
+  }
+  const bool bare = adapter >= a.adapters;
+  if (bare && a.out == a.base) return;
+  const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int step = gridDim.y * kWaves * kColumns, stride = parts_row(a.rank);
+  int o0 = (blockIdx.y * kWaves + wave) * kColumns;
+  // this lane's unit of its tokens' rows (a token past the end is the last again)
+  const uint16_t *from[kGroups];
+  uint16_t *to[kGroups];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    const int at = min(16 * g + m, count - 1);
+    const int64_t token = kSorted ? a.pairs[start + at] : members[at];
+    from[g] = a.base + token * a.base_stride + kUnit * q;
+    to[g] = a.out + token * a.out_stride + kUnit * q;
+  }
+  u32x4 base[kGroups][2], w[4];
+  auto fetch_base = [&](int first) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (first + 32 * s + kUnit * q >= a.outputs) continue;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) base[g][s] = load16(from[g] + first + 32 * s);
+    }
+  };
+  const uint16_t *decoder = a.decoder + static_cast<int64_t>(bare ? 0 : adapter) * a.outputs * a.rank;
+  unsigned unit[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unit[i] = output_of(i, m) * a.rank + kUnit * q;
+  // rows of D, zero past the last rank (rows past the last output are not stored)
+  auto fetch_rows = [&](int first, int r0, u32x4 *rows) {
+    const uint16_t *at = decoder + static_cast<int64_t>(first) * a.rank + r0;
+    if (first + kColumns <= a.outputs && r0 + 32 <= a.rank) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rows[i] = load16(at + unit[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        rows[i] = u32x4{0, 0, 0, 0};
+        if (first + output_of(i, m) < a.outputs && r0 + kUnit * q < a.rank) rows[i] = load16(at + unit[i]);
+      }
+    }
+  };
+  auto fetch = [&](int first) {
+    if (first >= a.outputs) return;
+    fetch_base(first);
+    if (kShort && !bare) fetch_rows(first, 0, w);
+  };
+  fetch(o0);
+  if (!bare) {
+    // (zeros behind the last rank: the matrix instructions take 32 at a time)
+    const int fours = (stride - kUnit) / 4;
+    for (int i = threadIdx.x; i < count * fours; i += 64 * kWaves) {
+      const int t = i / fours, r = i % fours * 4;
+      const float *inner = a.inner + static_cast<int64_t>(kSorted ? start + t : members[t]) * a.rank + r;
+      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (r < a.rank) {
+        v = *reinterpret_cast<const f32x4 *>(inner);
+#pragma unroll 4
+        for (int s = 1; s < a.splits; ++s)
+          v += *reinterpret_cast<const f32x4 *>(inner + static_cast<int64_t>(s) * a.tokens * a.rank);
+      }
+      u32x2 high, low;
+      split(v, high, low);
+      *reinterpret_cast<u32x2 *>(parts + t * stride + r) = high;
+      *reinterpret_cast<u32x2 *>(parts + (kTile + t) * stride + r) = low;
+    }
+    __syncthreads();
+  }
+  // (rows of `parts` past the last token hold what they held: their columns of the products
+  // are not stored)
+  const uint16_t *v = parts + m * stride + kUnit * q;
+  for (; o0 < a.outputs; o0 += step) {
+    f32x4 sum[kGroups][4] = {};
+    auto multiply = [&](int r0, const u32x4 *rows) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const u32x4 high = load16(v + 16 * g * stride + r0), low = load16(v + (kTile + 16 * g) * stride + r0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[g][i] = mma(rows[i], low, mma(rows[i], high, sum[g][i]));
+      }
+    };
+    if (!bare) {
+      if constexpr (kShort) {
+        multiply(0, w);
+      } else {
+#pragma unroll 2
+        for (int r0 = 0; r0 < a.rank; r0 += 32) {
+          u32x4 rows[4];
+          fetch_rows(o0, r0, rows);
+          multiply(r0, rows);
+        }
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        u32x4 row = base[g][s];
+        if (!bare) {
+          float value[kUnit];
+          Lane<false, true>::values(row, value);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            row[i] = bf16_pair(value[2 * i] + sum[g][2 * s + i / 2][2 * i % 4],
+                               value[2 * i + 1] + sum[g][2 * s + i / 2][2 * i % 4 + 1]);
+        }
+        if (16 * g + m < count && o0 + 32 * s + kUnit * q < a.outputs)
+          *reinterpret_cast<u32x4 *>(to[g] + o0 + 32 * s) = row;
+      }
+    }
+    fetch(o0 + step);
   }
 }
 
 int64_t rounded(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
+// A workgroup of few tokens reads all slots to find its tile, and one is launched for every
+// token; the sort is a launch of its own.
 bool sorts(int tokens) { return tokens > kFewTokens; }
+
+// Workgroups share the hidden dimension: of few tokens 256 values each or a sixteenth, of
+// many two halves, whose parts the second launch reads again for every 256 outputs.
+int splits_of(int tokens, int hidden) {
+  const int turns = (hidden + kTurn - 1) / kTurn, most = sorts(tokens) ? kManySplits : kFewSplits;
+  return turns < most ? turns : most;
+}
 
 }  // namespace
 }  // namespace cfmoe
@@ -242,11 +379,13 @@ extern "C" {
 
 using namespace cfmoe;
 
-CFMOE_API int64_t cfmoe_apply_adapters_scratch_bytes(int32_t rank, int32_t adapters, int32_t tokens) {
+CFMOE_API int64_t cfmoe_apply_adapters_scratch_bytes(int32_t hidden_size, int32_t rank, int32_t adapters, int32_t tokens) {
   if (rank < 8 || rank > kMaxRank || rank % 8) return -fail(CFMOE_EINVAL, "apply_adapters needs a rank that is a multiple of 8, at most 256");
   if (adapters < 1 || adapters > kMaxAdapters) return -fail(CFMOE_EINVAL, "apply_adapters needs 1 to 4096 adapters");
   if (tokens < 0 || tokens > (1 << 24)) return -fail(CFMOE_EINVAL, "apply_adapters needs 0 to 2^24 tokens");
-  int64_t bytes = static_cast<int64_t>(tokens) * rank * 4;
+  if (hidden_size < 8 || hidden_size > kMaxSize || hidden_size % 8)
+    return -fail(CFMOE_EINVAL, "apply_adapters needs hidden and output sizes that are multiples of 8, at most 65536");
+  int64_t bytes = splits_of(tokens, hidden_size) * static_cast<int64_t>(tokens) * rank * 4;
   if (sorts(tokens))
     bytes += rounded(4 * (adapters + 1)) + 2 * rounded(4 * static_cast<int64_t>(tokens)) +
              cfmoe_sort_by_expert_scratch_bytes(tokens, 1, adapters);
@@ -257,9 +396,9 @@ CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t
                                    const void *base, int64_t base_stride, const void *hidden, int64_t hidden_stride,
                                    const void *encoder, const void *decoder, const void *slots, const float *scales,
                                    void *out, int64_t out_stride, void *scratch, int32_t tokens, cfmoe_stream stream) {
-  const int64_t bytes = cfmoe_apply_adapters_scratch_bytes(rank, adapters, tokens);
+  const int64_t bytes = cfmoe_apply_adapters_scratch_bytes(hidden_size, rank, adapters, tokens);
   if (bytes < 0) return static_cast<int>(-bytes);
-  if (hidden_size < 8 || hidden_size > kMaxSize || hidden_size % 8 || outputs < 8 || outputs > kMaxSize || outputs % 8)
+  if (outputs < 8 || outputs > kMaxSize || outputs % 8)
     return fail(CFMOE_EINVAL, "apply_adapters needs hidden and output sizes that are multiples of 8, at most 65536");
   if (base_stride % 8 || hidden_stride % 8 || out_stride % 8 || base_stride < 0 || hidden_stride < 0 || out_stride < outputs)
     return fail(CFMOE_EINVAL, "apply_adapters needs row strides that are multiples of 8");
@@ -286,37 +425,49 @@ CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t
   a.rank = rank;
   a.adapters = adapters;
   a.slots64 = flags & CFMOE_IDS_INT64;
-  const unsigned columns = (outputs + kOutWaves * kOutColumns - 1) / (kOutWaves * kOutColumns);
-  const unsigned ranks = (rank + 15) / 16;
-  if (!sorts(tokens)) {
-    hipLaunchKernelGGL((adapter_inner_kernel<false, 1>), dim3(tokens, ranks), dim3(64 * kInnerWaves), 0, stream, a);
-    if (int rc = check_launch("adapter_inner")) return rc;
-    hipLaunchKernelGGL((adapter_out_kernel<false, 1>), dim3(tokens, columns), dim3(64 * kOutWaves), 0, stream, a);
-    return check_launch("adapter_out");
+  a.splits = splits_of(tokens, hidden_size);
+  // (whole turns: a split ends where the next begins)
+  a.share = (hidden_size + a.splits * kTurn - 1) / (a.splits * kTurn) * kTurn;
+  const bool sorted = sorts(tokens);
+  const int tile = sorted ? kManyTokens : kTokens;
+  int most = tokens;  // tiles there can be
+  if (sorted) {
+    char *at = static_cast<char *>(scratch) + static_cast<int64_t>(a.splits) * tokens * rank * 4;
+    auto take = [&](int64_t size) {
+      void *p = at;
+      at += rounded(size);
+      return static_cast<int32_t *>(p);
+    };
+    int32_t *offsets = take(4 * (adapters + 1)), *pairs = take(4 * static_cast<int64_t>(tokens));
+    int32_t *places = take(4 * static_cast<int64_t>(tokens));
+    if (int rc = cfmoe_sort_by_expert(adapters, 1, flags & CFMOE_IDS_INT64, slots, nullptr, offsets, places, pairs, at, tokens, stream))
+      return rc;
+    a.offsets = offsets;
+    a.pairs = pairs;
+    // one more than whole ones for each adapter, and for the tokens without one
+    most = tokens / tile + (adapters + 1 < tokens ? adapters + 1 : tokens);
+    if (most > tokens) most = tokens;
   }
-  char *at = static_cast<char *>(scratch) + static_cast<int64_t>(tokens) * rank * 4;
-  auto take = [&](int64_t size) {
-    void *p = at;
-    at += rounded(size);
-    return static_cast<int32_t *>(p);
+  const dim3 block(64 * kWaves);
+  const int tiles = (rank + 15) / 16, held = !sorted || tiles == 1 ? 1 : tiles == 2 ? 2 : 4;
+  auto start = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(most, (tiles + held - 1) / held, a.splits), block, 0, stream, a);
+    return check_launch("adapter_inner");
   };
-  int32_t *offsets = take(4 * (adapters + 1)), *pairs = take(4 * static_cast<int64_t>(tokens));
-  int32_t *places = take(4 * static_cast<int64_t>(tokens));
-  if (int rc = cfmoe_sort_by_expert(adapters, 1, flags & CFMOE_IDS_INT64, slots, nullptr, offsets, places, pairs, at, tokens, stream))
+  if (int rc = !sorted     ? start(adapter_inner_kernel<false, 1>)
+               : held == 1 ? start(adapter_inner_kernel<true, 1>)
+               : held == 2 ? start(adapter_inner_kernel<true, 2>)
+                           : start(adapter_inner_kernel<true, 4>))
     return rc;
-  a.offsets = offsets;
-  a.pairs = pairs;
-  // tiles there can be at most: one more for each adapter, and for the tokens without one
-  auto tiles = [&](int tile) {
-    return static_cast<unsigned>((tokens + tile - 1) / tile + (adapters + 1 < tokens ? adapters + 1 : tokens));
+  int columns = (outputs + kWaves * kColumns - 1) / (kWaves * kColumns);
+  while (columns > 1 && static_cast<int64_t>(most) * columns > kMostGroups) columns = (columns + 1) / 2;
+  const unsigned lds = 2 * tile * parts_row(rank) * 2;
+  auto finish = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(most, columns), block, lds, stream, a);
+    return check_launch("adapter_out");
   };
-  if (ranks > 1)
-    hipLaunchKernelGGL((adapter_inner_kernel<true, 4>), dim3(tiles(kInnerTokens), (ranks + 3) / 4), dim3(64 * kInnerWaves), 0, stream, a);
-  else
-    hipLaunchKernelGGL((adapter_inner_kernel<true, 1>), dim3(tiles(kInnerTokens), 1), dim3(64 * kInnerWaves), 0, stream, a);
-  if (int rc = check_launch("adapter_inner")) return rc;
-  hipLaunchKernelGGL((adapter_out_kernel<true, 4>), dim3(tiles(64), columns), dim3(64 * kOutWaves), 0, stream, a);
-  return check_launch("adapter_out");
+  if (rank <= 32) return finish(sorted ? adapter_out_kernel<true, true> : adapter_out_kernel<false, true>);
+  return finish(sorted ? adapter_out_kernel<true, false> : adapter_out_kernel<false, false>);
 }
 
 }  // extern "C"

@@ -50,67 +50,107 @@ __device__ __forceinline__ int key_of(const OrderArgs &a, int pair) {
   return id >= 0 && id < a.experts ? static_cast<int>(id) : a.experts;
 }
 
-// counts[w][e]: pairs of key e in wave w's range.
-__device__ __forceinline__ void count_range(const OrderArgs &a, int *counts, int waves, int low, int high,
-                                            int (&held)[kHeld]) {
-  const int width = a.experts + 1, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int i = threadIdx.x; i < waves * width; i += blockDim.x) counts[i] = 0;
-  // (before the barrier: the first keys and the zeros are on their way together)
-#pragma unroll
-  for (int j = 0; j < kHeld; ++j) held[j] = low + 64 * j + lane < high ? key_of(a, low + 64 * j + lane) : -1;
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < kHeld; ++j)
-    if (held[j] >= 0) atomicAdd(&counts[wave * width + held[j]], 1);
-  for (int p = low + 64 * kHeld + lane; p < high; p += 64) atomicAdd(&counts[wave * width + key_of(a, p)], 1);
-  __syncthreads();
-}
-
+// Pairs of this wave: [low, high).
 __device__ __forceinline__ void range_of(const OrderArgs &a, int waves, int &low, int &high) {
   const int64_t first = (static_cast<int64_t>(blockIdx.x) * waves + (threadIdx.x >> 6)) * a.range;
   low = static_cast<int>(first < a.pairs_total ? first : a.pairs_total);
   high = static_cast<int>(first + a.range < a.pairs_total ? first + a.range : a.pairs_total);
 }
 
+// The first keys of the wave's range, -1 past its end.
+__device__ __forceinline__ void hold_keys(const OrderArgs &a, int low, int high, int (&held)[kHeld]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) held[j] = low + 64 * j + lane < high ? key_of(a, low + 64 * j + lane) : -1;
+}
+
+// Takes 64 keys, one a lane (-1: none), into the wave's running `next` rows of each key:
+// lanes of one key find each other by a ballot for each of its bits, and each gets its key's
+// next row and the number of its fellows in lower lanes. No atomic, so no order but the lanes'.
+__device__ __forceinline__ int take_keys(const OrderArgs &a, volatile int *next, int key) {
+  const int lane = threadIdx.x & 63, bits = 32 - __builtin_clz(a.experts);
+  const bool live = key >= 0;
+  uint64_t fellows = __ballot(live);
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t set = __ballot((key >> b) & 1);
+    fellows &= (key >> b) & 1 ? set : ~set;
+  }
+  const int below = __builtin_popcountll(fellows & ((UINT64_C(1) << lane) - 1));
+  int row = 0;
+  // (the lanes of a wave read before its last fellow writes, in program order)
+  if (live) row = next[key] + below;
+  __builtin_amdgcn_wave_barrier();
+  if (live && below + 1 == __builtin_popcountll(fellows)) next[key] = row + 1;
+  __builtin_amdgcn_wave_barrier();
+  return row;
+}
+
 // The keys' counts of each workgroup's pairs, for a call of several.
 __global__ __launch_bounds__(64 * kSortWaves) void order_count_kernel(OrderArgs a) {
-  extern __shared__ int counts[];
-  const int width = a.experts + 1, waves = blockDim.x >> 6;
+  extern __shared__ int shared[];
+  const int width = a.experts + 1, waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   int low, high, held[kHeld];
   range_of(a, waves, low, high);
-  count_range(a, counts, waves, low, high, held);
+  hold_keys(a, low, high, held);
+  for (int i = threadIdx.x; i < waves * width; i += blockDim.x) shared[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if (low + 64 * j < high) take_keys(a, shared + wave * width, held[j]);
+  for (int p = low + 64 * kHeld; p < high; p += 64) take_keys(a, shared + wave * width, p + lane < high ? key_of(a, p + lane) : -1);
+  __syncthreads();
   for (int e = threadIdx.x; e < width; e += blockDim.x) {
     int total = 0;
-    for (int w = 0; w < waves; ++w) total += counts[w * width + e];
+    for (int w = 0; w < waves; ++w) total += shared[w * width + e];
     a.counts[static_cast<int64_t>(blockIdx.x) * width + e] = total;
   }
 }
 
 // Stable counting sort. A wave has a range of consecutive pairs: it counts their keys in
 // LDS, the counts become first rows (a scan over the keys, then over workgroups and waves),
-// and the wave walks its range again, 64 pairs at a time. Pairs of one key among the 64
-// find each other by one ballot for each bit of the key, so that a pair's row is its key's
-// next row and the number of its fellows in lower lanes. No atomic's order shows.
+// and a pair's row is its key's first row of the wave and its rank there, which the counting
+// gave; pairs that the lanes do not hold from then are ranked again.
 __global__ __launch_bounds__(64 * kSortWaves) void order_kernel(OrderArgs a) {
   extern __shared__ int shared[];
   __shared__ int wave_sums[kSortWaves];
   const int width = a.experts + 1, waves = blockDim.x >> 6;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  volatile int *counts = shared;
-  int low, high, held[kHeld];
+  int *totals = shared, *before = shared + width, *counts = shared + 2 * width + wave * width;
+  int low, high, held[kHeld], rank[kHeld];
   range_of(a, waves, low, high);
-  count_range(a, shared, waves, low, high, held);
+  hold_keys(a, low, high, held);
+  for (int i = threadIdx.x; i < (waves + 2) * width; i += blockDim.x) shared[i] = 0;
+  __syncthreads();
+  if (a.counts) {  // (a wave some of the workgroups, all their loads on the way together)
+    for (int e = lane; e < width; e += 64) {
+      int total = 0, earlier = 0;
+#pragma unroll 4
+      for (int b = wave; b < static_cast<int>(gridDim.x); b += waves) {
+        const int c = a.counts[static_cast<int64_t>(b) * width + e];
+        total += c;
+        earlier += b < static_cast<int>(blockIdx.x) ? c : 0;
+      }
+      if (total) atomicAdd(&totals[e], total);
+      if (earlier) atomicAdd(&before[e], earlier);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if (low + 64 * j < high) rank[j] = take_keys(a, counts, held[j]);
+  for (int p = low + 64 * kHeld; p < high; p += 64) take_keys(a, counts, p + lane < high ? key_of(a, p + lane) : -1);
+  __syncthreads();
 
   // thread i scans `each` consecutive keys
   const int each = (width + blockDim.x - 1) / blockDim.x;
   const int first = threadIdx.x * each, last = min(first + each, width);
   int sum = 0;
   for (int e = first; e < last; ++e) {
-    if (a.counts) {
-      for (int b = 0; b < static_cast<int>(gridDim.x); ++b) sum += a.counts[static_cast<int64_t>(b) * width + e];
-    } else {
-      for (int w = 0; w < waves; ++w) sum += counts[w * width + e];
+    if (!a.counts) {
+      int total = 0;
+      for (int w = 0; w < waves; ++w) total += shared[(2 + w) * width + e];
+      totals[e] = total;
     }
+    sum += totals[e];
   }
   int scan = sum;
 #pragma unroll
@@ -124,60 +164,48 @@ __global__ __launch_bounds__(64 * kSortWaves) void order_kernel(OrderArgs a) {
   for (int w = 0; w < wave; ++w) row += wave_sums[w];
   for (int e = first; e < last; ++e) {
     if (blockIdx.x == 0) a.offsets[e] = row;
-    int next = row, total = 0;
-    if (a.counts) {
-      for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
-        const int c = a.counts[static_cast<int64_t>(b) * width + e];
-        if (b < static_cast<int>(blockIdx.x)) next += c;
-        total += c;
-      }
-    }
+    int next = row + before[e];
     for (int w = 0; w < waves; ++w) {
-      const int c = counts[w * width + e];
-      counts[w * width + e] = next;
+      const int c = shared[(2 + w) * width + e];
+      shared[(2 + w) * width + e] = next;
       next += c;
     }
-    row = a.counts ? row + total : next;
+    row += totals[e];
   }
   __syncthreads();
 
-  const int bits = 32 - __builtin_clz(a.experts);
-  auto place = [&](int p, int key, bool live) {
-    uint64_t fellows = __ballot(live);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t set = __ballot((key >> b) & 1);
-      fellows &= (key >> b) & 1 ? set : ~set;
-    }
-    const int below = __builtin_popcountll(fellows & ((UINT64_C(1) << lane) - 1));
-    if (!live) return;
-    const int at = wave * width + key;
-    const int r = counts[at] + below;
-    __builtin_amdgcn_wave_barrier();
-    if (below + 1 == __builtin_popcountll(fellows)) counts[at] = r + 1;
-    __builtin_amdgcn_wave_barrier();
+  auto place = [&](int p, int key, int r) {
     a.places[p] = key < a.experts ? r : -1 - r;
     a.pairs[r] = p;
   };
+  // (all of a wave's ranks are read before its later pairs move the rows on)
 #pragma unroll
   for (int j = 0; j < kHeld; ++j)
-    if (low + 64 * j < high) place(low + 64 * j + lane, held[j], held[j] >= 0);
+    if (held[j] >= 0) place(low + 64 * j + lane, held[j], counts[held[j]] + rank[j]);
+  if (low + 64 * kHeld >= high) return;
+  // rows of the pairs not held: behind the wave's held ones
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) take_keys(a, counts, held[j]);
   for (int p = low + 64 * kHeld; p < high; p += 64) {
-    const bool live = p + lane < high;
-    place(p + lane, live ? key_of(a, p + lane) : -1, live);
+    const int key = p + lane < high ? key_of(a, p + lane) : -1;
+    const int r = take_keys(a, counts, key);
+    if (key >= 0) place(p + lane, key, r);
   }
 }
 
-// Waves of a sorting workgroup: 16, fewer where the counts of many experts need the LDS.
-int sort_waves(int experts) {
+// Waves of a sorting workgroup at most: 16, fewer where the counts of many experts need the LDS.
+int most_waves(int experts) {
   int waves = kSortWaves;
-  while (waves * (experts + 1) * 4 > kCountBytes) waves /= 2;
+  while ((waves + 2) * (experts + 1) * 4 > kCountBytes) waves /= 2;
   return waves;
 }
 
-// One workgroup up to this many pairs (kHeld for each lane of 16 waves), else up to 64.
+// One workgroup while its lanes hold all keys, else up to 64 of a key a lane.
 int sort_blocks(int64_t pairs, int experts) {
-  const int64_t each = 64 * kHeld * sort_waves(experts);
-  const int64_t blocks = (pairs + each - 1) / each;
+  const int64_t lanes = 64 * most_waves(experts);
+  if (pairs <= lanes * kHeld) return 1;
+  const int64_t blocks = (pairs + lanes - 1) / lanes;
   return static_cast<int>(blocks < kSortBlocks ? blocks : kSortBlocks);
 }
 
@@ -195,18 +223,31 @@ struct RowsArgs {
   bool weights16;
 };
 
-// A pair's row, and whether the pair is kept; -1 for what no order holds.
-__device__ __forceinline__ int place_of(const RowsArgs &a, int64_t pair, bool &kept) {
-  const int place = a.places[pair];
-  kept = place >= 0;
-  const int row = kept ? place : -1 - place;
-  return static_cast<int64_t>(row) < static_cast<int64_t>(a.tokens) * a.top_k ? row : -1;
-}
+// The slots of one token: lane k of each of its waves reads slot k's place and weight, and
+// hands them to all lanes, so that a token's rows are on their way after one round trip.
+struct Slots {
+  int place;
+  float weight;
 
-__device__ __forceinline__ float weight_of(const RowsArgs &a, int64_t pair) {
-  return a.weights16 ? bf16_value(static_cast<const uint16_t *>(a.weights)[pair])
-                     : static_cast<const float *>(a.weights)[pair];
-}
+  __device__ __forceinline__ Slots(const RowsArgs &a, int t) : place(INT32_MAX), weight(1.0f) {
+    const int k = threadIdx.x & 63;
+    if (k >= a.top_k) return;
+    const int64_t pair = static_cast<int64_t>(t) * a.top_k + k;
+    place = a.places[pair];
+    if (a.weights)
+      weight = a.weights16 ? bf16_value(static_cast<const uint16_t *>(a.weights)[pair])
+                           : static_cast<const float *>(a.weights)[pair];
+    // (a place past the rows, which no order holds, is skipped)
+    const int row = place >= 0 ? place : -1 - place;
+    if (row >= static_cast<int64_t>(a.tokens) * a.top_k) place = INT32_MAX;
+  }
+  __device__ __forceinline__ int at(int k) const { return __builtin_amdgcn_readlane(place, k); }
+  __device__ __forceinline__ float weight_at(int k) const {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), k));
+  }
+};
+
+__device__ __forceinline__ bool kept(int place) { return place >= 0 && place != INT32_MAX; }
 
 // A token's lanes: all of a workgroup, or one wave of it where the rows are short.
 template <typename F>
@@ -222,13 +263,15 @@ template <bool kFp32, bool kVector, int kWaves>
 __global__ __launch_bounds__(kThreads) void gather_kernel(RowsArgs a) {
   constexpr int kValues = Lane<kFp32, kVector>::kValues;
   for_tokens(a, kWaves, [&](int t, int lane) {
+    const Slots slots(a, t);
     for (int h = lane * kValues; h < a.hidden; h += 64 * kWaves * kValues) {
       float v[kValues], zero[kValues] = {};
       load_values<kFp32, kVector>(a.from, static_cast<int64_t>(t) * a.hidden + h, v);
       for (int k = 0; k < a.top_k; ++k) {
-        bool kept;
-        const int row = place_of(a, static_cast<int64_t>(t) * a.top_k + k, kept);
-        if (row >= 0) store_values<kFp32, kVector>(a.out, static_cast<int64_t>(row) * a.hidden + h, kept ? v : zero);
+        const int place = slots.at(k);
+        if (place == INT32_MAX) continue;
+        const int64_t row = place >= 0 ? place : -1 - place;
+        store_values<kFp32, kVector>(a.out, row * a.hidden + h, place >= 0 ? v : zero);
       }
     }
   });
@@ -239,29 +282,22 @@ template <bool kFp32, bool kVector, int kWaves>
 __global__ __launch_bounds__(kThreads) void combine_kernel(RowsArgs a) {
   constexpr int kValues = Lane<kFp32, kVector>::kValues;
   for_tokens(a, kWaves, [&](int t, int lane) {
+    const Slots slots(a, t);
     for (int h = lane * kValues; h < a.hidden; h += 64 * kWaves * kValues) {
       float sum[kValues] = {};
       for (int k0 = 0; k0 < a.top_k; k0 += kSlots) {
-        float v[kSlots][kValues], w[kSlots];
-        bool kept[kSlots];
+        float v[kSlots][kValues];
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
-          kept[j] = false;
-          if (k0 + j < a.top_k) {
-            const int64_t pair = static_cast<int64_t>(t) * a.top_k + k0 + j;
-            const int row = place_of(a, pair, kept[j]);
-            kept[j] = kept[j] && row >= 0;
-            if (kept[j]) {
-              w[j] = a.weights ? weight_of(a, pair) : 1.0f;
-              load_values<kFp32, kVector>(a.from, static_cast<int64_t>(row) * a.hidden + h, v[j]);
-            }
-          }
+          const int place = k0 + j < a.top_k ? slots.at(k0 + j) : -1;
+          if (kept(place)) load_values<kFp32, kVector, true>(a.from, static_cast<int64_t>(place) * a.hidden + h, v[j]);
         }
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
-          if (!kept[j]) continue;
+          if (k0 + j >= a.top_k || !kept(slots.at(k0 + j))) continue;
+          const float w = slots.weight_at(k0 + j);
 #pragma unroll
-          for (int i = 0; i < kValues; ++i) sum[i] = a.weights ? fmaf(w[j], v[j][i], sum[i]) : sum[i] + v[j][i];
+          for (int i = 0; i < kValues; ++i) sum[i] = fmaf(w, v[j][i], sum[i]);
         }
       }
       store_values<kFp32, kVector>(a.out, static_cast<int64_t>(t) * a.hidden + h, sum);
@@ -276,32 +312,35 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(RowsArgs a) 
   __shared__ float parts[kThreads / 64][kSlots];
   const int wave = threadIdx.x >> 6;
   for_tokens(a, kWaves, [&](int t, int lane) {
+    const Slots slots(a, t);
     for (int k0 = 0; k0 < a.top_k; k0 += kSlots) {
       float dot[kSlots] = {};
       for (int h = lane * kValues; h < a.hidden; h += 64 * kWaves * kValues) {
-        float grad[kValues];
+        float grad[kValues], v[kSlots][kValues];
         load_values<kFp32, kVector>(a.from, static_cast<int64_t>(t) * a.hidden + h, grad);
+        if (a.grad_weights) {
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j) {
+            const int place = k0 + j < a.top_k ? slots.at(k0 + j) : -1;
+            if (kept(place)) load_values<kFp32, kVector, true>(a.rows, static_cast<int64_t>(place) * a.hidden + h, v[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j) {
+            if (k0 + j >= a.top_k || !kept(slots.at(k0 + j))) continue;
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) dot[j] = fmaf(grad[i], v[j][i], dot[j]);
+          }
+        }
+        if (!a.out) continue;
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
-          if (k0 + j >= a.top_k) continue;
-          const int64_t pair = static_cast<int64_t>(t) * a.top_k + k0 + j;
-          bool kept;
-          const int row = place_of(a, pair, kept);
-          if (row < 0) continue;
-          const int64_t at = static_cast<int64_t>(row) * a.hidden + h;
-          if (kept && a.grad_weights) {
-            float v[kValues];
-            load_values<kFp32, kVector>(a.rows, at, v);
+          const int place = k0 + j < a.top_k ? slots.at(k0 + j) : INT32_MAX;
+          if (place == INT32_MAX) continue;
+          const float w = slots.weight_at(k0 + j);
+          float g[kValues];
 #pragma unroll
-            for (int i = 0; i < kValues; ++i) dot[j] = fmaf(grad[i], v[i], dot[j]);
-          }
-          if (a.out) {
-            float v[kValues];
-            const float w = !kept ? 0.0f : a.weights ? weight_of(a, pair) : 1.0f;
-#pragma unroll
-            for (int i = 0; i < kValues; ++i) v[i] = kept ? w * grad[i] : 0.0f;
-            store_values<kFp32, kVector>(a.out, at, v);
-          }
+          for (int i = 0; i < kValues; ++i) g[i] = place >= 0 ? w * grad[i] : 0.0f;
+          store_values<kFp32, kVector>(a.out, static_cast<int64_t>(place >= 0 ? place : -1 - place) * a.hidden + h, g);
         }
       }
       if (!a.grad_weights) continue;
@@ -391,10 +430,13 @@ CFMOE_API int cfmoe_sort_by_expert(int32_t experts, int32_t top_k, uint32_t flag
   a.experts = experts;
   a.ids64 = flags & CFMOE_IDS_INT64;
   // (no pairs: one workgroup writes the offsets, all zero)
-  const int blocks = bytes ? sort_blocks(a.pairs_total, experts) : 1, waves = sort_waves(experts);
+  const int blocks = sort_blocks(a.pairs_total, experts);
+  int waves = most_waves(experts);
+  if (blocks == 1)
+    while (waves > 1 && a.pairs_total <= 32 * waves) waves /= 2;
   const int64_t share = (a.pairs_total + static_cast<int64_t>(blocks) * waves - 1) / (static_cast<int64_t>(blocks) * waves);
   a.range = static_cast<int>((share + 63) / 64 * 64);
-  const unsigned lds = static_cast<unsigned>(waves * (experts + 1) * 4);
+  const unsigned lds = static_cast<unsigned>((waves + 2) * (experts + 1) * 4);
   if (a.counts) {
     hipLaunchKernelGGL(order_count_kernel, dim3(blocks), dim3(64 * waves), lds, stream, a);
     if (int rc = check_launch("order_count")) return rc;

@@ -20,8 +20,6 @@
 // as large, which leaves no number to overflow (epsilon is then below what a sum of FP32
 // holds, as it is in the exact one).
 
-#include <type_traits>
-
 #include "cfmoe_rows.h"
 
 namespace cfmoe {
@@ -29,6 +27,8 @@ namespace {
 
 constexpr int kMaxHidden = 8192;
 constexpr int kEach = 8;  // values of a row that a thread holds
+constexpr int kForwardWaves = 6144;   // of a launch at most: 24 to a compute unit
+constexpr int kBackwardWaves = 3072;  // 12, and at most 1024 workgroups
 constexpr float kSmall = 0x1p-80f;
 
 enum Gate { kNone, kChannel, kRow, kFull };
@@ -48,22 +48,32 @@ struct JoinArgs {
 
 template <bool kFp32, bool kVector, int kWaves>
 struct Row {
-  static constexpr int kValues = Lane<kFp32, kVector>::kValues;
+  using L = Lane<kFp32, kVector>;
+  static constexpr int kValues = L::kValues;
   static constexpr int kParts = kEach / kValues;
   static constexpr int kThreads = 64 * kWaves;
+
+  // Eight values of a row on their way.
+  struct Raw {
+    typename L::Raw part[kParts];
+  };
 
   // First column of a thread's part p; its values follow one another.
   __device__ static int column(int p) { return (p * kThreads + static_cast<int>(threadIdx.x)) * kValues; }
 
-  __device__ static void load(const void *rows, int64_t row, int size, float *v) {
+  __device__ static void load(const void *rows, int64_t row, int size, Raw &raw) {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p)
+      if (column(p) < size) raw.part[p] = L::load(rows, row * size + column(p));
+  }
+
+  // Zero past the end.
+  __device__ static void values(const Raw &raw, int size, float *v) {
 #pragma unroll
     for (int p = 0; p < kParts; ++p) {
-      if (column(p) < size) {
-        load_values<kFp32, kVector>(rows, row * size + column(p), v + p * kValues);
-      } else {
+      L::values(raw.part[p], v + p * kValues);
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) v[p * kValues + i] = 0.0f;
-      }
+      for (int i = 0; i < kValues; ++i) v[p * kValues + i] = column(p) < size ? v[p * kValues + i] : 0.0f;
     }
   }
 
@@ -93,22 +103,14 @@ struct Row {
       }
     }
   }
-
-  // The gate's values for the thread's columns.
-  __device__ static void gates(const JoinArgs &a, int64_t row, float *v) {
-    if (a.form == kChannel) {
-      weights(a.gate, a.gate32, a.size, v);
-    } else if (a.form == kRow) {
-      float g;
-      if (kFp32 || a.gate32) g = static_cast<const float *>(a.gate)[row];
-      else g = bf16_value(static_cast<const uint16_t *>(a.gate)[row]);
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) v[i] = g;
-    } else {
-      load(a.gate, row, a.size, v);
-    }
-  }
 };
+
+// A row's gate, [T, 1].
+template <bool kFp32>
+__device__ __forceinline__ float row_gate(const JoinArgs &a, int64_t row) {
+  return kFp32 || a.gate32 ? static_cast<const float *>(a.gate)[row]
+                           : bf16_value(static_cast<const uint16_t *>(a.gate)[row]);
+}
 
 // Sums over the workgroup, in every thread, always in the same order. `turn` changes with
 // each call, so that one barrier is enough: who writes a half again has passed the barrier
@@ -158,39 +160,55 @@ __device__ __forceinline__ float times_inverse(float v, float inverse) {
   return inverse < 0.0f ? v * -inverse * kSmall : v * inverse;
 }
 
-// Workgroup = a row, a thread eight of its values.
+// Workgroup = rows in steps of the grid, a thread eight values of each. The weights are
+// read once, and the next row is on its way while this one's sums are formed.
 template <bool kFp32, bool kVector, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void join_kernel(JoinArgs a) {
   using R = Row<kFp32, kVector, kWaves>;
   __shared__ float shared[2][2][kWaves];
   int turn = 0;
+  typename R::Raw x = {}, b = {}, g = {};
+  float spread = 0.0f;
+  auto fetch = [&](int64_t t) {
+    R::load(a.hidden, t, a.size, x);
+    if (a.block) R::load(a.block, t, a.size, b);
+    if (a.form == kFull) R::load(a.gate, t, a.size, g);
+    if (a.form == kRow) spread = row_gate<kFp32>(a, t);
+  };
+  fetch(blockIdx.x);
+  float post[kEach], next[kEach], gate[kEach];
+  if (a.post) R::weights(a.post, a.post32, a.size, post);
+  if (a.next) R::weights(a.next, a.next32, a.size, next);
+  if (a.form == kChannel) R::weights(a.gate, a.gate32, a.size, gate);
   for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    float j[kEach], w[kEach], first = 0.0f, second = 0.0f;
-    R::load(a.hidden, t, a.size, j);
+    float j[kEach], n[kEach], first = 0.0f, second = 0.0f;
+    R::values(x, a.size, j);
+    if (a.block) R::values(b, a.size, n);
+    if (a.form == kFull) R::values(g, a.size, gate);
+    if (a.form == kRow) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) gate[i] = spread;
+    }
+    if (t + gridDim.x < a.tokens) fetch(t + gridDim.x);
     if (a.block) {
-      float n[kEach];
-      R::load(a.block, t, a.size, n);
       if (a.post) {
-        R::weights(a.post, a.post32, a.size, w);
         first = inverse_root<kWaves>(n, a, shared, turn);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) n[i] = unit(n[i], first) * w[i];
+        for (int i = 0; i < kEach; ++i) n[i] = unit(n[i], first) * post[i];
       }
       if (a.form != kNone) {
-        R::gates(a, t, w);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) n[i] *= w[i];
+        for (int i = 0; i < kEach; ++i) n[i] *= gate[i];
       }
 #pragma unroll
       for (int i = 0; i < kEach; ++i) j[i] = fmaf(a.scale, j[i], n[i]);
       R::store(a.joined, t, a.size, j);
     }
     if (a.next) {
-      R::weights(a.next, a.next32, a.size, w);
       second = inverse_root<kWaves>(j, a, shared, turn);
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) w[i] *= unit(j[i], second);
-      R::store(a.out, t, a.size, w);
+      for (int i = 0; i < kEach; ++i) n[i] = next[i] * unit(j[i], second);
+      R::store(a.out, t, a.size, n);
     }
     if (a.statistics && threadIdx.x == 0) {
       a.statistics[2 * t] = first;
@@ -208,88 +226,97 @@ __global__ __launch_bounds__(64 * kWaves) void join_backward_kernel(JoinArgs a) 
   __shared__ float shared[2][2][kWaves];
   int turn = 0;
   const float part = 1.0f / static_cast<float>(a.size);
+  typename R::Raw x = {}, b = {}, g = {}, dj = {}, dy = {};
+  float spread = 0.0f, first = 0.0f, second = 0.0f;
+  auto fetch = [&](int64_t t) {
+    R::load(a.hidden, t, a.size, x);
+    if (a.block) R::load(a.block, t, a.size, b);
+    if (a.grad_joined) R::load(a.grad_joined, t, a.size, dj);
+    if (a.grad_out) R::load(a.grad_out, t, a.size, dy);
+    if (a.form == kFull) R::load(a.gate, t, a.size, g);
+    if (a.form == kRow) spread = row_gate<kFp32>(a, t);
+    if (a.post) first = a.statistics[2 * t];
+    if (a.grad_out) second = a.statistics[2 * t + 1];
+  };
+  fetch(blockIdx.x);
+  float post[kEach], next[kEach], gate[kEach];
+  if (a.post) R::weights(a.post, a.post32, a.size, post);
+  if (a.grad_out) R::weights(a.next, a.next32, a.size, next);
+  if (a.form == kChannel) R::weights(a.gate, a.gate32, a.size, gate);
   float sum_next[kEach] = {}, sum_post[kEach] = {}, sum_gate[kEach] = {};
   for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    float j[kEach], unit_block[kEach], n[kEach], gate[kEach], grad[kEach], w[kEach], first = 0.0f;
-    R::load(a.hidden, t, a.size, j);
+    // (unit: the block's rows over their root, or as they are)
+    float j[kEach], unit_block[kEach], grad[kEach], y[kEach];
+    const float inverse_block = first, inverse = second;
+    R::values(x, a.size, j);
+    if (a.block) R::values(b, a.size, unit_block);
+    if (a.form == kFull) R::values(g, a.size, gate);
+    if (a.form == kRow) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) gate[i] = spread;
+    }
+    if (a.grad_out) R::values(dy, a.size, y);
     if (a.grad_joined) {
-      R::load(a.grad_joined, t, a.size, grad);
+      R::values(dj, a.size, grad);
     } else {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) grad[i] = 0.0f;
     }
+    if (t + gridDim.x < a.tokens) fetch(t + gridDim.x);
     if (a.block) {
-      R::load(a.block, t, a.size, unit_block);
-      if (a.form != kNone) {
-        R::gates(a, t, gate);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) gate[i] = 1.0f;
-      }
-      if (a.post) {
-        first = a.statistics[2 * t];
-        R::weights(a.post, a.post32, a.size, w);
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-          unit_block[i] = unit(unit_block[i], first);
-          n[i] = unit_block[i] * w[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) n[i] = unit_block[i];
-      }
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) j[i] = fmaf(a.scale, j[i], a.form != kNone ? gate[i] * n[i] : n[i]);
-    }
-    if (a.grad_out) {
-      const float second = a.statistics[2 * t + 1];
-      float y[kEach], mean[1] = {0.0f};
-      R::load(a.grad_out, t, a.size, y);
-      R::weights(a.next, a.next32, a.size, w);
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        j[i] = unit(j[i], second);
+        if (a.post) unit_block[i] = unit(unit_block[i], inverse_block);
+        float n = a.post ? unit_block[i] * post[i] : unit_block[i];
+        if (a.form != kNone) n *= gate[i];
+        j[i] = fmaf(a.scale, j[i], n);
+      }
+    }
+    if (a.grad_out) {
+      float mean[1] = {0.0f};
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        j[i] = unit(j[i], inverse);
         sum_next[i] = fmaf(y[i], j[i], sum_next[i]);
-        y[i] *= w[i];
+        y[i] *= next[i];
         mean[0] = fmaf(y[i], j[i], mean[0]);
       }
       group_totals<kWaves, 1>(mean, shared, turn);
       mean[0] *= part;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) grad[i] += times_inverse(fmaf(-j[i], mean[0], y[i]), second);
+      for (int i = 0; i < kEach; ++i) grad[i] += times_inverse(fmaf(-j[i], mean[0], y[i]), inverse);
     }
     if (a.grad_hidden) {
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) w[i] = a.scale * grad[i];
-      R::store(a.grad_hidden, t, a.size, w);
+      for (int i = 0; i < kEach; ++i) y[i] = a.scale * grad[i];
+      R::store(a.grad_hidden, t, a.size, y);
     }
     if (!a.block) continue;
     float totals[2] = {0.0f, 0.0f};
     if (a.grad_gate) {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        n[i] *= grad[i];
-        totals[0] += n[i];
-        sum_gate[i] += n[i];
+        y[i] = grad[i] * (a.post ? unit_block[i] * post[i] : unit_block[i]);
+        totals[0] += y[i];
+        sum_gate[i] += y[i];
       }
-      if (a.grad_gate && a.form == kFull) R::store(a.grad_gate, t, a.size, n);
+      if (a.form == kFull) R::store(a.grad_gate, t, a.size, y);
     }
     if (a.form != kNone) {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) grad[i] *= gate[i];
     }
     if (a.post) {
-      R::weights(a.post, a.post32, a.size, w);
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
         sum_post[i] = fmaf(grad[i], unit_block[i], sum_post[i]);
-        grad[i] *= w[i];
+        grad[i] *= post[i];
         totals[1] = fmaf(grad[i], unit_block[i], totals[1]);
       }
     }
-    const bool row_gate = a.grad_gate && a.form == kRow;
-    if (a.post || row_gate) group_totals<kWaves, 2>(totals, shared, turn);
-    if (row_gate && threadIdx.x == 0) {
+    const bool row_sum = a.grad_gate && a.form == kRow;
+    if (a.post || row_sum) group_totals<kWaves, 2>(totals, shared, turn);
+    if (row_sum && threadIdx.x == 0) {
       if (kFp32 || a.gate32) static_cast<float *>(a.grad_gate)[t] = totals[0];
       else static_cast<uint16_t *>(a.grad_gate)[t] = bf16_bits(totals[0]);
     }
@@ -297,7 +324,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_backward_kernel(JoinArgs a) 
     if (a.post) {
 #pragma unroll
       for (int i = 0; i < kEach; ++i)
-        grad[i] = times_inverse(fmaf(-unit_block[i], totals[1] * part, grad[i]), first);
+        grad[i] = times_inverse(fmaf(-unit_block[i], totals[1] * part, grad[i]), inverse_block);
     }
     R::store(a.grad_block, t, a.size, grad);
   }
@@ -348,8 +375,6 @@ __global__ __launch_bounds__(64 * kSumWaves) void join_sums_kernel(SumsArgs a) {
   else static_cast<uint16_t *>(a.to[which])[c] = bf16_bits(sum);
 }
 
-int backward_groups(int tokens) { return tokens < 1024 ? tokens : 1024; }
-
 int check_join(int hidden_size, int tokens, float epsilon) {
   if (hidden_size < 1 || hidden_size > kMaxHidden) return fail(CFMOE_EINVAL, "join_block needs a hidden size from 1 to 8192");
   if (tokens < 0) return fail(CFMOE_EINVAL, "join_block needs a token count of zero or more");
@@ -357,7 +382,20 @@ int check_join(int hidden_size, int tokens, float epsilon) {
   return 0;
 }
 
-// Waves of a row: the fewest whose threads hold it.
+// Waves of a row: the fewest of these whose threads hold it.
+int row_waves(int size) {
+  for (int waves : {1, 2, 4, 8})
+    if (size <= 64 * kEach * waves) return waves;
+  return 16;
+}
+
+// Workgroups of a backward call. Each leaves a partial row of every sum.
+int backward_groups(int size, int tokens) {
+  const int waves = row_waves(size);
+  const int groups = waves < 3 ? 1024 : kBackwardWaves / waves;
+  return tokens < groups ? tokens : groups;
+}
+
 template <typename F>
 int dispatch_row(int size, bool fp32, bool vector, F f) {
   auto typed = [&](auto waves) {
@@ -365,22 +403,26 @@ int dispatch_row(int size, bool fp32, bool vector, F f) {
     if (fp32) return vector ? f(Row<true, true, kWaves>()) : f(Row<true, false, kWaves>());
     return vector ? f(Row<false, true, kWaves>()) : f(Row<false, false, kWaves>());
   };
-  if (size <= 64 * kEach) return typed(std::integral_constant<int, 1>());
-  if (size <= 256 * kEach) return typed(std::integral_constant<int, 4>());
-  if (size <= 512 * kEach) return typed(std::integral_constant<int, 8>());
-  return typed(std::integral_constant<int, 16>());
+  switch (row_waves(size)) {
+    case 1: return typed(std::integral_constant<int, 1>());
+    case 2: return typed(std::integral_constant<int, 2>());
+    case 4: return typed(std::integral_constant<int, 4>());
+    case 8: return typed(std::integral_constant<int, 8>());
+    default: return typed(std::integral_constant<int, 16>());
+  }
 }
 
 template <bool kFp32, bool kVector, int kWaves>
 int launch_join(Row<kFp32, kVector, kWaves>, const JoinArgs &a, hipStream_t stream) {
-  const unsigned groups = a.tokens < (1 << 20) ? a.tokens : (1 << 20);
+  constexpr int kGroups = kForwardWaves / kWaves;
+  const int groups = a.tokens < kGroups ? a.tokens : kGroups;
   hipLaunchKernelGGL((join_kernel<kFp32, kVector, kWaves>), dim3(groups), dim3(64 * kWaves), 0, stream, a);
   return check_launch("join_block");
 }
 
 template <bool kFp32, bool kVector, int kWaves>
 int launch_backward(Row<kFp32, kVector, kWaves>, const JoinArgs &a, hipStream_t stream) {
-  hipLaunchKernelGGL((join_backward_kernel<kFp32, kVector, kWaves>), dim3(backward_groups(a.tokens)), dim3(64 * kWaves), 0,
+  hipLaunchKernelGGL((join_backward_kernel<kFp32, kVector, kWaves>), dim3(backward_groups(a.size, a.tokens)), dim3(64 * kWaves), 0,
                      stream, a);
   return check_launch("join_block_backward");
 }
@@ -434,7 +476,7 @@ CFMOE_API int cfmoe_join_block(int32_t hidden_size, uint32_t flags, const void *
 CFMOE_API int64_t cfmoe_join_block_backward_scratch_bytes(int32_t hidden_size, int32_t sums, int32_t tokens) {
   if (hidden_size < 1 || hidden_size > kMaxHidden || sums < 0 || sums > 3 || tokens < 0)
     return -fail(CFMOE_EINVAL, "join_block needs a hidden size from 1 to 8192, up to 3 sums and 0 or more tokens");
-  return static_cast<int64_t>(backward_groups(tokens)) * sums * hidden_size * 4;
+  return static_cast<int64_t>(backward_groups(hidden_size, tokens)) * sums * hidden_size * 4;
 }
 
 CFMOE_API int cfmoe_join_block_backward(int32_t hidden_size, uint32_t flags, const void *hidden, const void *block,
@@ -490,7 +532,7 @@ CFMOE_API int cfmoe_join_block_backward(int32_t hidden_size, uint32_t flags, con
   }
   if (!s.sums) return 0;
   s.partial = a.partial;
-  s.groups = backward_groups(tokens);
+  s.groups = backward_groups(hidden_size, tokens);
   s.size = hidden_size;
   hipLaunchKernelGGL(join_sums_kernel, dim3((hidden_size + 63) / 64, s.sums), dim3(64 * kSumWaves), 0, stream, s);
   return check_launch("join_block_sums");

@@ -380,8 +380,8 @@ CFMOE_API int cfmoe_join_block_backward(
  * multiples of 8 up to 65536, R of 8 up to 256, strides of 8; N at most 4096, T 2^24. All
  * 16-byte aligned but slots and scales. scratch: cfmoe_apply_adapters_scratch_bytes; calls
  * that overlap need their own. No reference counterpart. */
-CFMOE_API int64_t cfmoe_apply_adapters_scratch_bytes(int32_t rank, int32_t adapters,
-                                                     int32_t tokens);
+CFMOE_API int64_t cfmoe_apply_adapters_scratch_bytes(int32_t hidden_size, int32_t rank,
+                                                     int32_t adapters, int32_t tokens);
 CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t rank,
                                    int32_t adapters, uint32_t flags, const void *base,
                                    int64_t base_stride, const void *hidden, int64_t hidden_stride,

@@ -145,8 +145,8 @@ def call_adapters(hidden=64, outputs=64, rank=8, adapters=2, base=AT, x=AT, enco
     (dict(tokens=-1), "2^24"), (dict(tokens=(1 << 24) + 1), "2^24"),
     (dict(base=None), "NULL"), (dict(x=None), "NULL"), (dict(encoder=None), "NULL"),
     (dict(decoder=None), "NULL"), (dict(slots=None), "NULL"), (dict(out=None), "NULL"),
-    (dict(scratch=None), "NULL"), (dict(x=AT + 2), "16-byte"), (dict(base=AT + 8), "16-byte"),
-    (dict(out=AT + 4), "16-byte"), (dict(decoder=AT + 8), "16-byte"),
+    (dict(scratch=None), "NULL"), (dict(x=AT + 2), "16-byte"),
+    (dict(base=AT + 8), "16-byte"), (dict(scratch=AT + 8), "16-byte"), (dict(out=AT + 4), "16-byte"), (dict(decoder=AT + 8), "16-byte"),
     (dict(strides=(60, 64, 64)), "strides"), (dict(strides=(64, 68, 64)), "strides"),
     (dict(strides=(64, 64, 56)), "strides"), (dict(strides=(-64, 64, 64)), "strides"),
 ])
@@ -169,9 +169,12 @@ def test_scratch_sizes():
     assert lib.cfmoe_sort_by_expert_scratch_bytes(1, 65, 8) == -_ext.EINVAL
     assert lib.cfmoe_join_block_backward_scratch_bytes(100, 2, 5) == 5 * 2 * 100 * 4
     assert lib.cfmoe_join_block_backward_scratch_bytes(9000, 2, 5) == -_ext.EINVAL
-    assert lib.cfmoe_apply_adapters_scratch_bytes(16, 4, 3) >= 3 * 16 * 4
-    assert lib.cfmoe_apply_adapters_scratch_bytes(16, 4, 1 << 24) >= (1 << 24) * 16 * 4
-    assert lib.cfmoe_apply_adapters_scratch_bytes(15, 4, 3) == -_ext.EINVAL
+    assert lib.cfmoe_apply_adapters_scratch_bytes(64, 16, 4, 3) >= 3 * 16 * 4
+    assert lib.cfmoe_apply_adapters_scratch_bytes(2048, 16, 4, 3) >= 8 * 3 * 16 * 4
+    assert lib.cfmoe_apply_adapters_scratch_bytes(64, 16, 4, 5000) >= 5000 * (16 * 4 + 8) + 5 * 4
+    assert lib.cfmoe_apply_adapters_scratch_bytes(64, 16, 4, 1 << 24) >= (1 << 24) * 16 * 4
+    assert lib.cfmoe_apply_adapters_scratch_bytes(64, 15, 4, 3) == -_ext.EINVAL
+    assert lib.cfmoe_apply_adapters_scratch_bytes(60, 16, 4, 3) == -_ext.EINVAL
 
 
 def test_overlaps_of_out():
