@@ -15,6 +15,11 @@ from torch import Tensor
 
 from calibration_free_moe.reader import _ext
 
+MAX_SIZE = 65536
+MAX_RANK = 256
+MAX_ADAPTERS = 4096
+MAX_TOKENS = 1 << 24
+
 
 def _stride(t: Tensor) -> int:
     """Values from one row to the next; of a single row, which has none, its length."""
@@ -85,6 +90,20 @@ def apply_adapters(
     n, rank, _ = encoder.shape
     o, device = base.shape[1], hidden.device
     if (
+        h % 8
+        or not 8 <= h <= MAX_SIZE
+        or o % 8
+        or not 8 <= o <= MAX_SIZE
+        or rank % 8
+        or not 8 <= rank <= MAX_RANK
+        or not 1 <= n <= MAX_ADAPTERS
+        or tokens > MAX_TOKENS
+    ):
+        raise ValueError(
+            "Expected hidden and output sizes that are multiples of 8 up to 65536, a rank that is "
+            "one up to 256, 1 to 4096 adapters and at most 2^24 tokens"
+        )
+    if (
         encoder.shape != (n, rank, h)
         or decoder.shape != (n, o, rank)
         or not hidden.is_cuda
@@ -119,8 +138,12 @@ def apply_adapters(
         raise ValueError(
             "Expected contiguous int32/int64 slots [tokens] and FP32 scales [N] on the rows' device"
         )
-    if torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (base, hidden, encoder, decoder, scales)
+    if torch.is_grad_enabled() and (
+        base.requires_grad
+        or hidden.requires_grad
+        or encoder.requires_grad
+        or decoder.requires_grad
+        or (scales is not None and scales.requires_grad)
     ):
         raise ValueError("apply_adapters is forward only: detach its inputs or call it in no_grad")
     if out is None:

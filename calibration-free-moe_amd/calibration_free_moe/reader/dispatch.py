@@ -19,7 +19,9 @@ from torch.autograd.function import once_differentiable
 from calibration_free_moe.reader import _ext
 
 MAX_HIDDEN = 1 << 20
+MAX_EXPERTS = 4096
 MAX_TOP_K = 64
+MAX_PAIRS = 1 << 30
 
 
 @dataclass(frozen=True)
@@ -36,22 +38,23 @@ class ExpertOrder:
     places: Tensor
     pairs: Tensor
 
-    def valid(self) -> bool:
-        """Whether the three are contiguous int32 of one batch on one GPU."""
+    def __post_init__(self) -> None:
         offsets, places, pairs = self.offsets, self.places, self.pairs
-        return (
-            places.dim() == 2
-            and 1 <= places.shape[1] <= MAX_TOP_K
-            and offsets.dim() == pairs.dim() == 1
-            and offsets.shape[0] >= 2
-            and pairs.shape[0] == places.numel()
-            and offsets.dtype == places.dtype == pairs.dtype == torch.int32
-            and places.is_cuda
-            and offsets.device == places.device == pairs.device
-            and places.is_contiguous()
-            and pairs.is_contiguous()
-            and offsets.is_contiguous()
-        )
+        if (
+            places.dim() != 2
+            or not 1 <= places.shape[1] <= MAX_TOP_K
+            or offsets.dim() != 1
+            or pairs.dim() != 1
+            or offsets.shape[0] < 2
+            or pairs.shape[0] != places.numel()
+            or places.numel() > MAX_PAIRS
+            or not offsets.dtype == places.dtype == pairs.dtype == torch.int32
+            or not offsets.device == places.device == pairs.device
+            or not places.is_contiguous()
+            or not pairs.is_contiguous()
+            or not offsets.is_contiguous()
+        ):
+            raise ValueError("Expected contiguous int32 tensors of one batch for an ExpertOrder")
 
 
 def sort_by_expert(ids: Tensor, experts: int, padding: Tensor | None = None) -> ExpertOrder:
@@ -73,6 +76,8 @@ def sort_by_expert(ids: Tensor, experts: int, padding: Tensor | None = None) -> 
         raise ValueError("Expected contiguous int32 or int64 CUDA ids [tokens, K]")
     tokens, top_k = ids.shape
     device = ids.device
+    if not 1 <= experts <= MAX_EXPERTS or not 1 <= top_k <= MAX_TOP_K or ids.numel() > MAX_PAIRS:
+        raise ValueError("Expected 1 to 4096 experts, 1 to 64 ids per token and at most 2^30 pairs")
     if padding is not None and (
         padding.shape != (tokens,)
         or padding.device != device
@@ -164,11 +169,12 @@ def _check_rows(rows: Tensor, count: int, order: ExpertOrder, what: str) -> None
         or rows.shape[0] != count
         or not 1 <= rows.shape[1] <= MAX_HIDDEN
         or rows.dtype not in (torch.bfloat16, torch.float32)
+        or not rows.is_cuda
         or rows.device != order.places.device
         or not rows.is_contiguous()
     ):
         raise ValueError(
-            f"Expected contiguous BF16 or FP32 {what} of the order's batch on its GPU, "
+            f"Expected contiguous BF16 or FP32 CUDA {what} of the order's batch on its GPU, "
             "H from 1 to 2^20"
         )
 
@@ -182,8 +188,6 @@ def gather_rows(hidden: Tensor, order: ExpertOrder) -> Tensor:
     the current stream of the rows' device, for the gradient another; both can be captured
     in a graph (a backward pass only where no eager graph of the same leaves is alive).
     """
-    if not order.valid():
-        raise ValueError("Expected an ExpertOrder of contiguous int32 CUDA tensors of one batch")
     _check_rows(hidden, order.places.shape[0], order, "rows [tokens, H]")
     if hidden.requires_grad and torch.is_grad_enabled():
         return _Gather.apply(hidden, order.places)
@@ -200,8 +204,6 @@ def combine_rows(rows: Tensor, order: ExpertOrder, weights: Tensor | None = None
     FP32 sum of out's gradient times the row; zero for dropped pairs). Launches as
     `gather_rows`.
     """
-    if not order.valid():
-        raise ValueError("Expected an ExpertOrder of contiguous int32 CUDA tensors of one batch")
     places = order.places
     _check_rows(rows, places.numel(), order, "rows [tokens K, H]")
     if weights is not None and (

@@ -15,6 +15,7 @@ from torch.autograd.function import once_differentiable
 from calibration_free_moe.reader import _ext
 
 MAX_HIDDEN = 8192
+MAX_TOKENS = 2 ** 31 - 1
 
 
 def _pointer(t: Tensor | None) -> int | None:
@@ -111,13 +112,14 @@ def _check_hidden(hidden: Tensor, epsilon: float) -> None:
     if (
         hidden.dim() != 2
         or not 1 <= hidden.shape[1] <= MAX_HIDDEN
+        or hidden.shape[0] > MAX_TOKENS
         or hidden.dtype not in (torch.bfloat16, torch.float32)
         or not hidden.is_cuda
         or not hidden.is_contiguous()
     ):
         raise ValueError("Expected contiguous BF16 or FP32 CUDA rows [tokens, H], H from 1 to 8192")
-    if not 1e-30 <= epsilon <= 1e30:
-        raise ValueError("epsilon must lie between 1e-30 and 1e30")
+    if not isinstance(epsilon, (int, float)) or not 1e-30 <= epsilon <= 1e30:
+        raise ValueError("epsilon must be a number between 1e-30 and 1e30")
 
 
 def _check_weight(weight: Tensor, hidden: Tensor, name: str) -> None:
@@ -192,8 +194,16 @@ def join_block(
             "gate must be contiguous [H] or [tokens, 1] of the rows' type or FP32, or [tokens, H] "
             "of their type, on their device"
         )
+    if not isinstance(residual_scale, (int, float)):
+        raise ValueError("residual_scale must be a number")
     inputs = (hidden, block, post_weight, gate, next_weight)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+    if torch.is_grad_enabled() and (
+        hidden.requires_grad
+        or block.requires_grad
+        or (post_weight is not None and post_weight.requires_grad)
+        or (gate is not None and gate.requires_grad)
+        or (next_weight is not None and next_weight.requires_grad)
+    ):
         return _Join.apply(*inputs, residual_scale, epsilon)
     joined, out, _ = _forward(*inputs, residual_scale, epsilon, False)
     return joined if out is None else (joined, out)

@@ -12,9 +12,8 @@
 // and the ranks are spread over workgroups (adapter_inner_kernel), and the second launch
 // (adapter_out_kernel) adds up their parts of v. Many tokens are sorted by adapter first.
 //
-// As operand of the second product v is the sum of two BF16 numbers (2^-16 off: the first
-// cut off, so that the second has its sign and an infinite weight meets no zero where v is
-// not one), and out is rounded once.
+// As operand of the second product v is the sum of two BF16 numbers (2^-16 off; one would
+// leave out 2^-8 off v's largest terms, more than out's own rounding), and out is rounded once.
 
 #include "cfmoe_rows.h"
 
@@ -119,13 +118,20 @@ __device__ __forceinline__ bool find_sorted_tile(const AdapterArgs &a, int index
 
 __device__ __forceinline__ u32x4 load16(const uint16_t *p) { return *reinterpret_cast<const u32x4 *>(p); }
 
-// Pairs of BF16 numbers whose sums are v to 2^-16, the first cut off.
+// Pairs of BF16 numbers whose sums are v to 2^-16. The first is cut off from the number
+// below v, so that neither is zero where v is not (down to 2^-132): an infinite weight times
+// them is that infinity, and where v is infinite the second is.
 __device__ __forceinline__ void split(f32x4 v, u32x2 &high, u32x2 &low) {
+  uint32_t cut[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t bits = __float_as_uint(v[i]), size = bits & 0x7fffffffu;
+    cut[i] = ((size - (size != 0)) | (bits & 0x80000000u)) & 0xffff0000u;
+  }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const uint32_t a = __float_as_uint(v[2 * i]) & 0xffff0000u, b = __float_as_uint(v[2 * i + 1]) & 0xffff0000u;
-    high[i] = a >> 16 | b;
-    low[i] = bf16_pair(v[2 * i] - __uint_as_float(a), v[2 * i + 1] - __uint_as_float(b));
+    high[i] = cut[2 * i] >> 16 | cut[2 * i + 1];
+    low[i] = bf16_pair(v[2 * i] - __uint_as_float(cut[2 * i]), v[2 * i + 1] - __uint_as_float(cut[2 * i + 1]));
   }
 }
 

@@ -145,6 +145,29 @@ def test_infinities_and_nan_stay_in_their_rows(tokens):
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("tokens", [3, 300])
+def test_infinite_weights_and_inner_values_of_any_kind(tokens):
+    """Inner values that are BF16 numbers themselves, and infinite ones: infinities where the
+    sum has one, not NaN."""
+    made = make(tokens, 64, 64, 1, 8)
+    made["slots"][:] = 0
+    made["hidden"][:] = 0
+    made["hidden"][:, 5] = 0.5
+    made["encoder"][:] = 0
+    made["encoder"][0, :, 5] = 1.0
+    made["decoder"][0, 3, 2], made["decoder"][0, 4, 2] = float("inf"), float("-inf")
+    out = apply_adapters(**{k: v.to(DEVICE) for k, v in made.items()}).cpu()
+    assert bool((out[:, 3] == float("inf")).all()) and bool((out[:, 4] == float("-inf")).all())
+    assert bool(out[:, 5:].isfinite().all())
+    made = make(tokens, 64, 64, 1, 8)
+    made["slots"][:] = 0
+    made["hidden"][0, 5] = float("inf")
+    made["encoder"][0] = made["encoder"][0].abs() + 0.01
+    made["decoder"] = made["decoder"].abs() + 0.01
+    out = apply_adapters(**{k: v.to(DEVICE) for k, v in made.items()}).cpu()
+    assert bool((out[0] == float("inf")).all()) and bool(out[1:].isfinite().all())
+
+
 def test_the_batch_does_not_matter():
     """A token alone and among others: the same value to the order of the sums."""
     made = make(40, 256, 128, 4, 32)
@@ -184,6 +207,7 @@ def test_refusals():
     refuse(slots=on["slots"][:3])
     refuse(scales=on["scales"].bfloat16())
     refuse(scales=on["scales"][:1])
+    refuse("multiples of 8", base=on["base"][:, :68], decoder=on["decoder"][:, :68].contiguous())
     refuse("rank", encoder=on["encoder"][:, :12].contiguous(), decoder=on["decoder"][..., :12].contiguous())
     refuse("out must", out=torch.zeros(4, 64, dtype=BF16, device=DEVICE))
     refuse("out must", out=torch.zeros(1, 72, dtype=BF16, device=DEVICE).expand(4, 72))

@@ -33,7 +33,6 @@ def make_ids(tokens, top_k, experts, seed, skew=False, outside=True):
 def check_order(ids, experts, padding=None):
     order = sort_by_expert(ids.to(DEVICE), experts, None if padding is None else padding.to(DEVICE))
     offsets, places, pairs = plain.order(ids, experts, padding)
-    assert order.valid()
     assert order.offsets.tolist() == offsets
     assert order.places.flatten().tolist() == places and order.places.shape == ids.shape
     assert order.pairs.tolist() == pairs
@@ -70,7 +69,7 @@ def test_order_without_kept_pairs(tokens):
 
 def test_empty_batches():
     order = sort_by_expert(torch.empty(0, 8, dtype=torch.int32, device=DEVICE), 5)
-    assert order.offsets.tolist() == [0] * 6 and order.valid()
+    assert order.offsets.tolist() == [0] * 6
     x = torch.empty(0, 16, device=DEVICE, requires_grad=True)
     rows = gather_rows(x, order)
     weights = torch.empty(0, 8, device=DEVICE, requires_grad=True)
@@ -197,6 +196,27 @@ def test_gradients_against_differences():
         c_out, rows, places, weights)[1::2]]
     allowed = sum(float((b * d.abs()).sum()) for b, d in zip(bounds, along)) + 1e-10
     assert abs(sum(float((v.cpu().double() * d).sum()) for v, d in zip(got, along)) - slope) <= allowed
+
+
+def test_a_batch_without_kept_pairs():
+    """All experts elsewhere: rows, sums and gradients are zeros, whatever the inputs hold."""
+    order = sort_by_expert(torch.full((6, 3), -1, device=DEVICE), 4)
+    x = torch.randn(6, 520, device=DEVICE, requires_grad=True)
+    rows = torch.full((18, 520), float("nan"), device=DEVICE, requires_grad=True)
+    weights = torch.full((6, 3), float("nan"), device=DEVICE, requires_grad=True)
+    laid, out = gather_rows(x, order), combine_rows(rows, order, weights)
+    grads = torch.autograd.grad((laid, out), (x, rows, weights),
+                                (torch.full_like(laid, float("nan")), torch.ones_like(out)))
+    for t in (laid, out, *grads):
+        assert bool((t == 0).all())
+
+
+def test_second_derivatives_are_refused():
+    order = sort_by_expert(torch.zeros(2, 1, dtype=torch.int32, device=DEVICE), 1)
+    x = torch.randn(2, 8, device=DEVICE, requires_grad=True)
+    (grad,) = torch.autograd.grad((gather_rows(x, order) ** 2).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        grad.sum().backward()
 
 
 def test_infinities_and_nan_stay_where_they_are():

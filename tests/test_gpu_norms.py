@@ -141,6 +141,13 @@ def test_norm(tokens, dtype, weights32):
     check_norm(made["hidden"], made["next"])
 
 
+@pytest.mark.parametrize("tokens,size", [(700, 2056), (400, 4100), (1500, 520)])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_more_rows_than_workgroups(tokens, size, dtype):
+    """Sums over rows of which a workgroup has several, at every width of one."""
+    check(make(tokens, size, dtype, True, "channel", True), 0.9)
+
+
 @pytest.mark.parametrize("epsilon", [1e-30, 1e-12, 0.5, 1e30])
 def test_norm_epsilon(epsilon):
     made = make(6, 200, FP32, True, "none", True)
@@ -312,6 +319,11 @@ def test_refusals():
             norm_rows(x, w, epsilon=epsilon)
         with pytest.raises(ValueError, match="epsilon"):
             join_block(x, x, epsilon=epsilon)
+    for number in (torch.tensor(0.5), "1"):
+        with pytest.raises(ValueError, match="number"):
+            join_block(x, x, residual_scale=number)
+        with pytest.raises(ValueError, match="number"):
+            norm_rows(x, w, epsilon=number)
     for bad in (x[:3], x.bfloat16(), x.cpu()):
         with pytest.raises(ValueError, match="block"):
             join_block(x, bad)
