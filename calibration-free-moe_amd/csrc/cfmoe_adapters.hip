@@ -351,7 +351,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a)
         u32x4 row = base[g][s];
         if (!bare) {
           float value[kUnit];
-          Lane<false, true>::values(row, value);
+          Lane<false, kWhole>::values(row, value);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             row[i] = bf16_pair(value[2 * i] + sum[g][2 * s + i / 2][2 * i % 4],

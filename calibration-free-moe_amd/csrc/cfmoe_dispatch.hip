@@ -250,85 +250,97 @@ struct Slots {
 __device__ __forceinline__ bool kept(int place) { return place >= 0 && place != INT32_MAX; }
 
 // A token's lanes: all of a workgroup, or one wave of it where the rows are short.
-template <typename F>
-__device__ __forceinline__ void for_tokens(const RowsArgs &a, int waves, F f) {
+template <int kWaves, typename F>
+__device__ __forceinline__ void for_tokens(const RowsArgs &a, F f) {
+  constexpr int kTokens = kThreads / 64 / kWaves;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / 64 / waves);
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / 64 / waves) + wave / waves; t < a.tokens; t += step)
-    f(static_cast<int>(t), static_cast<int>(threadIdx.x) & (64 * waves - 1));
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kTokens;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + wave / kWaves; t < a.tokens; t += step)
+    f(static_cast<int>(t), static_cast<int>(threadIdx.x) & (64 * kWaves - 1));
 }
 
 // rows[place] = x[t]: a token's row is read once and written K times.
-template <bool kFp32, bool kVector, int kWaves>
+template <bool kFp32, Rows kRows, int kWaves>
 __global__ __launch_bounds__(kThreads) void gather_kernel(RowsArgs a) {
-  constexpr int kValues = Lane<kFp32, kVector>::kValues;
-  for_tokens(a, kWaves, [&](int t, int lane) {
+  using L = Lane<kFp32, kRows>;
+  for_tokens<kWaves>(a, [&](int t, int lane) {
     const Slots slots(a, t);
-    for (int h = lane * kValues; h < a.hidden; h += 64 * kWaves * kValues) {
-      float v[kValues], zero[kValues] = {};
-      load_values<kFp32, kVector>(a.from, static_cast<int64_t>(t) * a.hidden + h, v);
+    for (int column = lane * L::kValues; column < a.hidden; column += 64 * kWaves * L::kValues) {
+      const int h = L::first(column, a.hidden);
+      float v[L::kValues], zero[L::kValues] = {};
+      L::values(L::load(a.from, static_cast<int64_t>(t) * a.hidden + h), v);
       for (int k = 0; k < a.top_k; ++k) {
         const int place = slots.at(k);
         if (place == INT32_MAX) continue;
         const int64_t row = place >= 0 ? place : -1 - place;
-        store_values<kFp32, kVector>(a.out, row * a.hidden + h, place >= 0 ? v : zero);
+        L::store(a.out, row * a.hidden + h, place >= 0 ? v : zero);
       }
     }
   });
 }
 
 // out[t] = sum over kept slots of w rows[place]: kSlots rows are on their way together.
-template <bool kFp32, bool kVector, int kWaves>
+template <bool kFp32, Rows kRows, int kWaves>
 __global__ __launch_bounds__(kThreads) void combine_kernel(RowsArgs a) {
-  constexpr int kValues = Lane<kFp32, kVector>::kValues;
-  for_tokens(a, kWaves, [&](int t, int lane) {
+  using L = Lane<kFp32, kRows>;
+  for_tokens<kWaves>(a, [&](int t, int lane) {
     const Slots slots(a, t);
-    for (int h = lane * kValues; h < a.hidden; h += 64 * kWaves * kValues) {
-      float sum[kValues] = {};
+    for (int column = lane * L::kValues; column < a.hidden; column += 64 * kWaves * L::kValues) {
+      const int h = L::first(column, a.hidden);
+      float sum[L::kValues] = {};
       for (int k0 = 0; k0 < a.top_k; k0 += kSlots) {
-        float v[kSlots][kValues];
+        typename L::Raw raw[kSlots] = {};
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
           const int place = k0 + j < a.top_k ? slots.at(k0 + j) : -1;
-          if (kept(place)) load_values<kFp32, kVector, true>(a.from, static_cast<int64_t>(place) * a.hidden + h, v[j]);
+          if (kept(place)) raw[j] = L::template load<true>(a.from, static_cast<int64_t>(place) * a.hidden + h);
         }
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
           if (k0 + j >= a.top_k || !kept(slots.at(k0 + j))) continue;
           const float w = slots.weight_at(k0 + j);
+          float v[L::kValues];
+          L::values(raw[j], v);
 #pragma unroll
-          for (int i = 0; i < kValues; ++i) sum[i] = fmaf(w, v[j][i], sum[i]);
+          for (int i = 0; i < L::kValues; ++i) sum[i] = fmaf(w, v[i], sum[i]);
         }
       }
-      store_values<kFp32, kVector>(a.out, static_cast<int64_t>(t) * a.hidden + h, sum);
+      L::store(a.out, static_cast<int64_t>(t) * a.hidden + h, sum);
     }
   });
 }
 
 // drows[place] = w dout[t] and dw = dout[t] . rows[place], kSlots slots at a time.
-template <bool kFp32, bool kVector, int kWaves>
+template <bool kFp32, Rows kRows, int kWaves>
 __global__ __launch_bounds__(kThreads) void combine_backward_kernel(RowsArgs a) {
-  constexpr int kValues = Lane<kFp32, kVector>::kValues;
-  __shared__ float parts[kThreads / 64][kSlots];
+  using L = Lane<kFp32, kRows>;
+  __shared__ float parts[kWaves][kSlots];
   const int wave = threadIdx.x >> 6;
-  for_tokens(a, kWaves, [&](int t, int lane) {
+  for_tokens<kWaves>(a, [&](int t, int lane) {
     const Slots slots(a, t);
     for (int k0 = 0; k0 < a.top_k; k0 += kSlots) {
       float dot[kSlots] = {};
-      for (int h = lane * kValues; h < a.hidden; h += 64 * kWaves * kValues) {
-        float grad[kValues], v[kSlots][kValues];
-        load_values<kFp32, kVector>(a.from, static_cast<int64_t>(t) * a.hidden + h, grad);
+      for (int column = lane * L::kValues; column < a.hidden; column += 64 * kWaves * L::kValues) {
+        const int h = L::first(column, a.hidden), others = L::others(column, a.hidden);
+        float grad[L::kValues];
+        typename L::Raw raw[kSlots] = {};
+        L::values(L::load(a.from, static_cast<int64_t>(t) * a.hidden + h), grad);
         if (a.grad_weights) {
 #pragma unroll
           for (int j = 0; j < kSlots; ++j) {
             const int place = k0 + j < a.top_k ? slots.at(k0 + j) : -1;
-            if (kept(place)) load_values<kFp32, kVector, true>(a.rows, static_cast<int64_t>(place) * a.hidden + h, v[j]);
+            if (kept(place)) raw[j] = L::template load<true>(a.rows, static_cast<int64_t>(place) * a.hidden + h);
           }
 #pragma unroll
           for (int j = 0; j < kSlots; ++j) {
             if (k0 + j >= a.top_k || !kept(slots.at(k0 + j))) continue;
+            float v[L::kValues];
+            L::values(raw[j], v);
 #pragma unroll
-            for (int i = 0; i < kValues; ++i) dot[j] = fmaf(grad[i], v[j][i], dot[j]);
+            for (int i = 0; i < L::kValues; ++i) {
+              const float more = fmaf(grad[i], v[i], dot[j]);
+              dot[j] = kRows == kRagged && i < others ? dot[j] : more;
+            }
           }
         }
         if (!a.out) continue;
@@ -337,10 +349,10 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(RowsArgs a) 
           const int place = k0 + j < a.top_k ? slots.at(k0 + j) : INT32_MAX;
           if (place == INT32_MAX) continue;
           const float w = slots.weight_at(k0 + j);
-          float g[kValues];
+          float g[L::kValues];
 #pragma unroll
-          for (int i = 0; i < kValues; ++i) g[i] = place >= 0 ? w * grad[i] : 0.0f;
-          store_values<kFp32, kVector>(a.out, static_cast<int64_t>(place >= 0 ? place : -1 - place) * a.hidden + h, g);
+          for (int i = 0; i < L::kValues; ++i) g[i] = place >= 0 ? w * grad[i] : 0.0f;
+          L::store(a.out, static_cast<int64_t>(place >= 0 ? place : -1 - place) * a.hidden + h, g);
         }
       }
       if (!a.grad_weights) continue;
@@ -378,24 +390,25 @@ int check_rows(const RowsArgs &a) {
   return 0;
 }
 
-// Whole 16-byte vectors where every row starts at one.
-#define CFMOE_ROWS_LAUNCH(KERNEL, fp32, vector, a, stream)                                              \
-  do {                                                                                                  \
-    const int lanes = (a).hidden / ((vector) ? ((fp32) ? 4 : 8) : 1);                                   \
-    const bool wide = lanes > 64;                                                                       \
-    const int64_t groups = wide ? (a).tokens : (static_cast<int64_t>((a).tokens) + 3) / 4;              \
-    const dim3 grid(static_cast<unsigned>(groups < (1 << 20) ? groups : (1 << 20)));                    \
-    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a); }; \
-    if (fp32) {                                                                                         \
-      if (vector) launch(wide ? KERNEL<true, true, 4> : KERNEL<true, true, 1>);                         \
-      else launch(wide ? KERNEL<true, false, 4> : KERNEL<true, false, 1>);                              \
-    } else {                                                                                            \
-      if (vector) launch(wide ? KERNEL<false, true, 4> : KERNEL<false, true, 1>);                       \
-      else launch(wide ? KERNEL<false, false, 4> : KERNEL<false, false, 1>);                            \
-    }                                                                                                   \
+// A wave takes a token of up to two lane's worths, a workgroup of four a longer one. 8192
+// tokens of 8 rows, BF16, one wave and four: the sum of rows of 1024 32 and 37 us, its
+// gradients 52 and 82, of rows of 2048 76 and 60, 120 and 106; laying out either way is the
+// same to 1024 (24 us), 58 and 50 at 2048.
+#define CFMOE_ROWS_LAUNCH(KERNEL, fp32, a, stream)                                                          \
+  do {                                                                                                      \
+    const Rows rows = rows_of((a).hidden, fp32);                                                            \
+    const int values = rows == kSingle ? 1 : (fp32) ? 4 : 8;                                                \
+    const bool wide = (a).hidden > 128 * values;                                                            \
+    const int64_t groups = wide ? (a).tokens : (static_cast<int64_t>((a).tokens) + 3) / 4;                  \
+    const dim3 grid(static_cast<unsigned>(groups < (1 << 20) ? groups : (1 << 20)));                        \
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a); };     \
+    auto typed = [&](auto narrow, auto full) { launch(wide ? full : narrow); };                             \
+    if (rows == kSingle) launch((fp32) ? KERNEL<true, kSingle, 1> : KERNEL<false, kSingle, 1>);             \
+    else if ((fp32) && rows == kWhole) typed(KERNEL<true, kWhole, 1>, KERNEL<true, kWhole, 4>);             \
+    else if (fp32) typed(KERNEL<true, kRagged, 1>, KERNEL<true, kRagged, 4>);                               \
+    else if (rows == kWhole) typed(KERNEL<false, kWhole, 1>, KERNEL<false, kWhole, 4>);                     \
+    else typed(KERNEL<false, kRagged, 1>, KERNEL<false, kRagged, 4>);                                       \
   } while (0)
-
-bool whole_vectors(int hidden, bool fp32) { return hidden % (fp32 ? 4 : 8) == 0; }
 
 }  // namespace
 }  // namespace cfmoe
@@ -457,9 +470,7 @@ CFMOE_API int cfmoe_gather_rows(int32_t hidden_size, int32_t top_k, uint32_t fla
   if (int rc = check_rows(a)) return rc;
   if (tokens == 0) return 0;
   if (!hidden || !places || !rows) return fail(CFMOE_EINVAL, "NULL argument");
-  const bool fp32 = flags & CFMOE_FP32;
-  const bool vector = whole_vectors(hidden_size, fp32) && !misaligned16(hidden) && !misaligned16(rows);
-  CFMOE_ROWS_LAUNCH(gather_kernel, fp32, vector, a, stream);
+  CFMOE_ROWS_LAUNCH(gather_kernel, (flags & CFMOE_FP32) != 0, a, stream);
   return check_launch("gather_rows");
 }
 
@@ -478,9 +489,7 @@ CFMOE_API int cfmoe_combine_rows(int32_t hidden_size, int32_t top_k, uint32_t fl
   if (int rc = check_rows(a)) return rc;
   if (tokens == 0) return 0;
   if (!rows || !places || !out) return fail(CFMOE_EINVAL, "NULL argument");
-  const bool fp32 = flags & CFMOE_FP32;
-  const bool vector = whole_vectors(hidden_size, fp32) && !misaligned16(rows) && !misaligned16(out);
-  CFMOE_ROWS_LAUNCH(combine_kernel, fp32, vector, a, stream);
+  CFMOE_ROWS_LAUNCH(combine_kernel, (flags & CFMOE_FP32) != 0, a, stream);
   return check_launch("combine_rows");
 }
 
@@ -502,10 +511,7 @@ CFMOE_API int cfmoe_combine_rows_backward(int32_t hidden_size, int32_t top_k, ui
   if (int rc = check_rows(a)) return rc;
   if (tokens == 0 || (!grad_rows && !grad_weights)) return 0;
   if (!grad_out || !places || (grad_weights && !rows)) return fail(CFMOE_EINVAL, "NULL argument");
-  const bool fp32 = flags & CFMOE_FP32;
-  const bool vector = whole_vectors(hidden_size, fp32) && !misaligned16(grad_out) &&
-                      !misaligned16(grad_weights ? rows : nullptr) && !misaligned16(grad_rows);
-  CFMOE_ROWS_LAUNCH(combine_backward_kernel, fp32, vector, a, stream);
+  CFMOE_ROWS_LAUNCH(combine_backward_kernel, (flags & CFMOE_FP32) != 0, a, stream);
   return check_launch("combine_rows_backward");
 }
 

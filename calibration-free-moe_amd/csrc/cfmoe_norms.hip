@@ -46,9 +46,9 @@ struct JoinArgs {
   bool post32, gate32, next32, grad_post, grad_next;
 };
 
-template <bool kFp32, bool kVector, int kWaves>
+template <bool kFp32, Rows kRows, int kWaves>
 struct Row {
-  using L = Lane<kFp32, kVector>;
+  using L = Lane<kFp32, kRows>;
   static constexpr int kValues = L::kValues;
   static constexpr int kParts = kEach / kValues;
   static constexpr int kThreads = 64 * kWaves;
@@ -58,13 +58,19 @@ struct Row {
     typename L::Raw part[kParts];
   };
 
-  // First column of a thread's part p; its values follow one another.
+  // Column from which a thread's part p counts its values, and the one its values begin at.
   __device__ static int column(int p) { return (p * kThreads + static_cast<int>(threadIdx.x)) * kValues; }
+  __device__ static int first(int p, int size) { return L::first(column(p), size); }
+
+  // Whether the thread counts its value i in a sum.
+  __device__ static bool counts(int i, int size) {
+    return kRows != kRagged || i % kValues >= L::others(column(i / kValues), size);
+  }
 
   __device__ static void load(const void *rows, int64_t row, int size, Raw &raw) {
 #pragma unroll
     for (int p = 0; p < kParts; ++p)
-      if (column(p) < size) raw.part[p] = L::load(rows, row * size + column(p));
+      if (column(p) < size) raw.part[p] = L::load(rows, row * size + first(p, size));
   }
 
   // Zero past the end.
@@ -80,7 +86,7 @@ struct Row {
   __device__ static void store(void *rows, int64_t row, int size, const float *v) {
 #pragma unroll
     for (int p = 0; p < kParts; ++p)
-      if (column(p) < size) store_values<kFp32, kVector>(rows, row * size + column(p), v + p * kValues);
+      if (column(p) < size) L::store(rows, row * size + first(p, size), v + p * kValues);
   }
 
   // Weights [H] of the rows' type or FP32; zero past the end.
@@ -92,14 +98,11 @@ struct Row {
 #pragma unroll
         for (int i = 0; i < kValues; ++i) part[i] = 0.0f;
       } else if (!kFp32 && fp32) {
-        if constexpr (kVector) {
-          load_values<true, true>(w, column(p), part);
-          load_values<true, true>(w, column(p) + kValues / 2, part + kValues / 2);
-        } else {
-          load_values<true, false>(w, column(p), part);
-        }
+        using F = Lane<true, kRows>;
+#pragma unroll
+        for (int i = 0; i < kValues; i += F::kValues) F::values(F::load(w, first(p, size) + i), part + i);
       } else {
-        load_values<kFp32, kVector>(w, column(p), part);
+        L::values(L::load(w, first(p, size)), part);
       }
     }
   }
@@ -136,9 +139,11 @@ __device__ __forceinline__ void group_totals(float (&v)[kSums], float (*shared)[
 }
 
 // 1 / sqrt(mean(v^2) + eps); negative, it is that of 2^-80 v.
-template <int kWaves>
-__device__ __forceinline__ float inverse_root(const float *v, const JoinArgs &a, float (*shared)[2][kWaves], int &turn) {
-  float sum[1] = {0.0f};
+template <typename R, int kWaves>
+__device__ __forceinline__ float inverse_root(const float *values, const JoinArgs &a, float (*shared)[2][kWaves], int &turn) {
+  float sum[1] = {0.0f}, v[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) v[i] = R::counts(i, a.size) ? values[i] : 0.0f;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) sum[0] = fmaf(v[i], v[i], sum[0]);
   group_totals<kWaves, 1>(sum, shared, turn);
@@ -162,9 +167,9 @@ __device__ __forceinline__ float times_inverse(float v, float inverse) {
 
 // Workgroup = rows in steps of the grid, a thread eight values of each. The weights are
 // read once, and the next row is on its way while this one's sums are formed.
-template <bool kFp32, bool kVector, int kWaves>
+template <bool kFp32, Rows kRows, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void join_kernel(JoinArgs a) {
-  using R = Row<kFp32, kVector, kWaves>;
+  using R = Row<kFp32, kRows, kWaves>;
   __shared__ float shared[2][2][kWaves];
   int turn = 0;
   typename R::Raw x = {}, b = {}, g = {};
@@ -192,7 +197,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(JoinArgs a) {
     if (t + gridDim.x < a.tokens) fetch(t + gridDim.x);
     if (a.block) {
       if (a.post) {
-        first = inverse_root<kWaves>(n, a, shared, turn);
+        first = inverse_root<R, kWaves>(n, a, shared, turn);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) n[i] = unit(n[i], first) * post[i];
       }
@@ -205,7 +210,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(JoinArgs a) {
       R::store(a.joined, t, a.size, j);
     }
     if (a.next) {
-      second = inverse_root<kWaves>(j, a, shared, turn);
+      second = inverse_root<R, kWaves>(j, a, shared, turn);
 #pragma unroll
       for (int i = 0; i < kEach; ++i) n[i] = next[i] * unit(j[i], second);
       R::store(a.out, t, a.size, n);
@@ -220,9 +225,9 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(JoinArgs a) {
 // Workgroup = rows in steps of the grid; the sums over rows stay in registers and leave as
 // one partial row each, which join_sums_kernel adds up: no atomics, so that a call gives
 // the same bits every time.
-template <bool kFp32, bool kVector, int kWaves>
+template <bool kFp32, Rows kRows, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void join_backward_kernel(JoinArgs a) {
-  using R = Row<kFp32, kVector, kWaves>;
+  using R = Row<kFp32, kRows, kWaves>;
   __shared__ float shared[2][2][kWaves];
   int turn = 0;
   const float part = 1.0f / static_cast<float>(a.size);
@@ -279,7 +284,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_backward_kernel(JoinArgs a) 
         j[i] = unit(j[i], inverse);
         sum_next[i] = fmaf(y[i], j[i], sum_next[i]);
         y[i] *= next[i];
-        mean[0] = fmaf(y[i], j[i], mean[0]);
+        if (R::counts(i, a.size)) mean[0] = fmaf(y[i], j[i], mean[0]);
       }
       group_totals<kWaves, 1>(mean, shared, turn);
       mean[0] *= part;
@@ -297,7 +302,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_backward_kernel(JoinArgs a) 
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
         y[i] = grad[i] * (a.post ? unit_block[i] * post[i] : unit_block[i]);
-        totals[0] += y[i];
+        if (R::counts(i, a.size)) totals[0] += y[i];
         sum_gate[i] += y[i];
       }
       if (a.form == kFull) R::store(a.grad_gate, t, a.size, y);
@@ -311,7 +316,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_backward_kernel(JoinArgs a) 
       for (int i = 0; i < kEach; ++i) {
         sum_post[i] = fmaf(grad[i], unit_block[i], sum_post[i]);
         grad[i] *= post[i];
-        totals[1] = fmaf(grad[i], unit_block[i], totals[1]);
+        if (R::counts(i, a.size)) totals[1] = fmaf(grad[i], unit_block[i], totals[1]);
       }
     }
     const bool row_sum = a.grad_gate && a.form == kRow;
@@ -332,11 +337,9 @@ __global__ __launch_bounds__(64 * kWaves) void join_backward_kernel(JoinArgs a) 
   float *rows = a.partial + static_cast<int64_t>(blockIdx.x) * a.sums * a.size;
   auto leave = [&](const float *v) {
 #pragma unroll
-    for (int p = 0; p < R::kParts; ++p) {
-      const int c = R::column(p);
-      if (c >= a.size) continue;
-#pragma unroll
-      for (int i = 0; i < R::kValues; ++i) rows[c + i] = v[p * R::kValues + i];
+    for (int i = 0; i < kEach; ++i) {
+      const int p = i / R::kValues;
+      if (R::column(p) < a.size && R::counts(i, a.size)) rows[R::first(p, a.size) + i % R::kValues] = v[i];
     }
     rows += a.size;
   };
@@ -397,11 +400,13 @@ int backward_groups(int size, int tokens) {
 }
 
 template <typename F>
-int dispatch_row(int size, bool fp32, bool vector, F f) {
+int dispatch_row(int size, bool fp32, F f) {
+  const Rows rows = rows_of(size, fp32);
+  if (rows == kSingle) return fp32 ? f(Row<true, kSingle, 1>()) : f(Row<false, kSingle, 1>());
   auto typed = [&](auto waves) {
     constexpr int kWaves = decltype(waves)::value;
-    if (fp32) return vector ? f(Row<true, true, kWaves>()) : f(Row<true, false, kWaves>());
-    return vector ? f(Row<false, true, kWaves>()) : f(Row<false, false, kWaves>());
+    if (fp32) return rows == kWhole ? f(Row<true, kWhole, kWaves>()) : f(Row<true, kRagged, kWaves>());
+    return rows == kWhole ? f(Row<false, kWhole, kWaves>()) : f(Row<false, kRagged, kWaves>());
   };
   switch (row_waves(size)) {
     case 1: return typed(std::integral_constant<int, 1>());
@@ -412,17 +417,17 @@ int dispatch_row(int size, bool fp32, bool vector, F f) {
   }
 }
 
-template <bool kFp32, bool kVector, int kWaves>
-int launch_join(Row<kFp32, kVector, kWaves>, const JoinArgs &a, hipStream_t stream) {
+template <bool kFp32, Rows kRows, int kWaves>
+int launch_join(Row<kFp32, kRows, kWaves>, const JoinArgs &a, hipStream_t stream) {
   constexpr int kGroups = kForwardWaves / kWaves;
   const int groups = a.tokens < kGroups ? a.tokens : kGroups;
-  hipLaunchKernelGGL((join_kernel<kFp32, kVector, kWaves>), dim3(groups), dim3(64 * kWaves), 0, stream, a);
+  hipLaunchKernelGGL((join_kernel<kFp32, kRows, kWaves>), dim3(groups), dim3(64 * kWaves), 0, stream, a);
   return check_launch("join_block");
 }
 
-template <bool kFp32, bool kVector, int kWaves>
-int launch_backward(Row<kFp32, kVector, kWaves>, const JoinArgs &a, hipStream_t stream) {
-  hipLaunchKernelGGL((join_backward_kernel<kFp32, kVector, kWaves>), dim3(backward_groups(a.size, a.tokens)), dim3(64 * kWaves), 0,
+template <bool kFp32, Rows kRows, int kWaves>
+int launch_backward(Row<kFp32, kRows, kWaves>, const JoinArgs &a, hipStream_t stream) {
+  hipLaunchKernelGGL((join_backward_kernel<kFp32, kRows, kWaves>), dim3(backward_groups(a.size, a.tokens)), dim3(64 * kWaves), 0,
                      stream, a);
   return check_launch("join_block_backward");
 }
@@ -467,10 +472,7 @@ CFMOE_API int cfmoe_join_block(int32_t hidden_size, uint32_t flags, const void *
   a.next32 = fp32 || flags & CFMOE_NEXT_FP32;
   if (a.form == kFull && !fp32 && flags & CFMOE_GATE_FP32)
     return fail(CFMOE_EINVAL, "join_block needs a gate per value in the rows' type");
-  const bool vector = hidden_size % (fp32 ? 4 : 8) == 0 && !misaligned16(hidden) && !misaligned16(block) &&
-                      !misaligned16(a.post) && !misaligned16(a.form == kRow ? nullptr : a.gate) && !misaligned16(a.next) &&
-                      !misaligned16(joined) && !misaligned16(next);
-  return dispatch_row(hidden_size, fp32, vector, [&](auto row) { return launch_join(row, a, stream); });
+  return dispatch_row(hidden_size, fp32, [&](auto row) { return launch_join(row, a, stream); });
 }
 
 CFMOE_API int64_t cfmoe_join_block_backward_scratch_bytes(int32_t hidden_size, int32_t sums, int32_t tokens) {
@@ -523,12 +525,7 @@ CFMOE_API int cfmoe_join_block_backward(int32_t hidden_size, uint32_t flags, con
   a.grad_post = grad_post_weight;
   a.grad_next = grad_next_weight;
   if (tokens) {
-    const bool vector = hidden_size % (fp32 ? 4 : 8) == 0 && !misaligned16(hidden) && !misaligned16(block) &&
-                        !misaligned16(a.post) && !misaligned16(a.form == kRow ? nullptr : a.gate) &&
-                        !misaligned16(a.next) && !misaligned16(grad_joined) && !misaligned16(grad_next) &&
-                        !misaligned16(grad_hidden) && !misaligned16(grad_block) &&
-                        !misaligned16(a.form == kFull ? grad_gate : nullptr);
-    if (int rc = dispatch_row(hidden_size, fp32, vector, [&](auto row) { return launch_backward(row, a, stream); })) return rc;
+    if (int rc = dispatch_row(hidden_size, fp32, [&](auto row) { return launch_backward(row, a, stream); })) return rc;
   }
   if (!s.sums) return 0;
   s.partial = a.partial;

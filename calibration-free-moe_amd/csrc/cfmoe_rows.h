@@ -7,35 +7,50 @@
 
 namespace cfmoe {
 
-template <bool kOnce, typename T>
-__device__ __forceinline__ T load_from(const T *p) {
-  return kOnce ? __builtin_nontemporal_load(p) : *p;
-}
+// 16 bytes at any address of 4-byte or 2-byte values.
+typedef uint32_t vector_of_4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t vector_of_2 __attribute__((ext_vector_type(4), aligned(2)));
 
-template <bool kOnce, typename T>
-__device__ __forceinline__ void store_to(T *p, T v) {
-  if (kOnce) __builtin_nontemporal_store(v, p);
-  else *p = v;
-}
+// What one lane takes of a row at a time: 16 bytes, or one value of rows that are shorter.
+// Memory takes 16 bytes from any value's address, so that rows need no alignment of their
+// own. A row's last lane takes its last 16 bytes: where the row is no whole number of them,
+// it has values that the lane before has too, which stores them alike and is the one that
+// counts them in a sum. kOnce is for what no later load finds in a cache.
+enum Rows { kSingle, kWhole, kRagged };
 
-// What one lane takes of a row at a time: 16 bytes, or one value where sizes or addresses
-// do not allow whole vectors. kOnce is for what no later load finds in a cache.
-template <bool kFp32, bool kVector>
+template <bool kFp32, Rows kRows>
 struct Lane {
   using Value = std::conditional_t<kFp32, float, uint16_t>;
-  using Raw = std::conditional_t<kVector, u32x4, Value>;
-  static constexpr int kValues = kVector ? (kFp32 ? 4 : 8) : 1;
+  using Raw = std::conditional_t<kRows != kSingle, u32x4, Value>;
+  static constexpr int kValues = kRows != kSingle ? (kFp32 ? 4 : 8) : 1;
+
+  // First element of the lane whose values would begin at `column`, and how many of the
+  // values from there are another lane's.
+  static __device__ __forceinline__ int first(int column, int size) {
+    return kRows == kRagged ? min(column, size - kValues) : column;
+  }
+  static __device__ __forceinline__ int others(int column, int size) { return column - first(column, size); }
 
   template <bool kOnce = false>
   static __device__ __forceinline__ Raw load(const void *row, int64_t at) {
-    return load_from<kOnce>(reinterpret_cast<const Raw *>(static_cast<const Value *>(row) + at));
+    const Value *from = static_cast<const Value *>(row) + at;
+    // (the types by name: as a template's argument they would lose their alignment)
+    if constexpr (kRows == kSingle) {
+      return *from;
+    } else if constexpr (kFp32) {
+      const vector_of_4 *p = reinterpret_cast<const vector_of_4 *>(from);
+      return kOnce ? __builtin_nontemporal_load(p) : *p;
+    } else {
+      const vector_of_2 *p = reinterpret_cast<const vector_of_2 *>(from);
+      return kOnce ? __builtin_nontemporal_load(p) : *p;
+    }
   }
 
   static __device__ __forceinline__ void values(Raw raw, float *v) {
-    if constexpr (kFp32 && kVector) {
+    if constexpr (kFp32 && kRows != kSingle) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(raw[i]);
-    } else if constexpr (kVector) {
+    } else if constexpr (kRows != kSingle) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         v[2 * i] = __uint_as_float(raw[i] << 16);
@@ -47,32 +62,36 @@ struct Lane {
       v[0] = bf16_value(raw);
     }
   }
+
+  // Each value is rounded here, once, to the row's type.
+  static __device__ __forceinline__ void store(void *row, int64_t at, const float *v) {
+    Raw raw;
+    if constexpr (kFp32 && kRows != kSingle) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = __float_as_uint(v[i]);
+    } else if constexpr (kRows != kSingle) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
+    } else if constexpr (kFp32) {
+      raw = v[0];
+    } else {
+      raw = bf16_bits(v[0]);
+    }
+    Value *to = static_cast<Value *>(row) + at;
+    if constexpr (kRows == kSingle) *to = raw;
+    else if constexpr (kFp32) *reinterpret_cast<vector_of_4 *>(to) = raw;
+    else *reinterpret_cast<vector_of_2 *>(to) = raw;
+  }
 };
 
-// The values of a row from element `at`.
-template <bool kFp32, bool kVector, bool kOnce = false>
-__device__ __forceinline__ void load_values(const void *row, int64_t at, float *v) {
-  Lane<kFp32, kVector>::values(Lane<kFp32, kVector>::template load<kOnce>(row, at), v);
+inline Rows rows_of(int size, bool fp32) {
+  const int values = fp32 ? 4 : 8;
+  return size < values ? kSingle : size % values ? kRagged : kWhole;
 }
 
-// Each value is rounded here, once, to the row's type.
-template <bool kFp32, bool kVector, bool kOnce = false>
-__device__ __forceinline__ void store_values(void *row, int64_t at, const float *v) {
-  if constexpr (kFp32 && kVector) {
-    store_to<kOnce>(reinterpret_cast<f32x4 *>(static_cast<float *>(row) + at), f32x4{v[0], v[1], v[2], v[3]});
-  } else if constexpr (kFp32) {
-    store_to<kOnce>(static_cast<float *>(row) + at, v[0]);
-  } else if constexpr (kVector) {
-    store_to<kOnce>(reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(row) + at),
-                    u32x4{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])});
-  } else {
-    store_to<kOnce>(static_cast<uint16_t *>(row) + at, bf16_bits(v[0]));
-  }
-}
-
-template <int kControl, int kRows = 0xf>
+template <int kControl, int kLanes = 0xf>
 __device__ __forceinline__ float lane_moved(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kControl, kRows, 0xf, false));
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kControl, kLanes, 0xf, false));
 }
 
 // Sum over the wave, the same in every lane, always in the same order: pairs, quads, halves

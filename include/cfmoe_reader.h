@@ -329,7 +329,7 @@ CFMOE_API int cfmoe_sort_by_expert(int32_t experts, int32_t top_k, uint32_t flag
  * gradient of the second: grad_rows (or NULL) and grad_weights (or NULL; needs rows). Rows
  * of dropped pairs and their weights are not read. places as cfmoe_sort_by_expert writes
  * them; a place past T top_k is skipped. flags: CFMOE_FP32 (rows), CFMOE_WEIGHTS_BF16. H
- * from 1 to 2^20; rows 16-byte aligned with H a multiple of 8 (FP32: 4) are faster. */
+ * from 1 to 2^20; rows need no alignment but their type's. */
 CFMOE_API int cfmoe_gather_rows(int32_t hidden_size, int32_t top_k, uint32_t flags,
                                 const void *hidden, const int32_t *places, void *rows,
                                 int32_t tokens, cfmoe_stream stream);
@@ -349,8 +349,8 @@ CFMOE_API int cfmoe_combine_rows_backward(int32_t hidden_size, int32_t top_k, ui
  * with block NULL: next is the norm of hidden, and joined is not written. gate is [H], [T, 1]
  * or [T, H] by CFMOE_GATE_CHANNEL, _ROW, _FULL, of the rows' type or with CFMOE_GATE_FP32
  * FP32 (not per value); weights [H] likewise. statistics [T, 2] fp32 (or NULL) is what the
- * backward call takes. FP32 sums; next is of joined before its rounding. joined may be hidden
- * or block. H from 1 to 8192, epsilon 1e-30 to 1e30. flags: CFMOE_FP32 and those named.
+ * backward call takes. FP32 sums; next is of joined before its rounding. No output
+ * may overlap an input. H from 1 to 8192, epsilon 1e-30 to 1e30. flags: CFMOE_FP32 and those named.
  * The backward call takes the same inputs, the gradients of joined and next (either may be
  * NULL) and writes those asked for (not NULL); scratch: ..._backward_scratch_bytes of the
  * number of gradients summed over rows that are asked for (post_weight, next_weight, a
