@@ -77,8 +77,8 @@ def apply_adapters(
     base, hidden and out may be column slices of wider rows (first stride a multiple of 8,
     16-byte aligned). `out` may be `base`, whose rows without an adapter are then left
     alone, or `hidden`; no other overlap. H and O are multiples of 8 up to 65536, R of 8 up
-    to 256, N up to 4096, tokens up to 2^24; zero tokens give an empty output. Two HIP launches
-    on the current stream of the tensors' device, up to four for more than 256 tokens, with
+    to 256, N up to 4096, tokens up to 2^24; zero tokens give an empty output. One or two HIP
+    launches on the current stream of the tensors' device, up to four for more than 256 tokens, with
     scratch allocated per call; they can be captured in a graph. Tensors that require
     gradients are refused while gradients are on.
     """

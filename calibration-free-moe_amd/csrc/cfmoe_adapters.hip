@@ -8,9 +8,11 @@
 // Tokens of one adapter share its weights: they form tiles, and a tile's products are
 // matrix instructions, v = s_a C_a x over the hidden dimension and D_a v over the rank. A
 // decode step's tiles hold a token or two, which leaves most columns of an instruction
-// empty: what bounds it is the weights' reading, once for each tile. The hidden dimension
-// and the ranks are spread over workgroups (adapter_inner_kernel), and the second launch
-// (adapter_out_kernel) adds up their parts of v. Many tokens are sorted by adapter first.
+// empty: what bounds it is the weights' reading, once for each tile, and a compute unit
+// takes about 25 GB/s from memory. So the hidden dimension and the ranks are spread over
+// workgroups (adapter_inner_kernel), and the second launch (adapter_out_kernel) adds up
+// their parts of v; of few ranks one workgroup reads all (adapter_one_kernel). Many tokens
+// are sorted by adapter first.
 //
 // As operand of the second product v is the sum of two BF16 numbers (2^-16 off; one would
 // leave out 2^-8 off v's largest terms, more than out's own rounding), and out is rounded once.
@@ -27,6 +29,9 @@ constexpr int kFewTokens = 256;    // up to which a workgroup finds its tile by 
 constexpr int kTokens = 16;        // of a tile, few tokens
 constexpr int kManyTokens = 32;    // of a tile, many tokens
 constexpr int kWaves = 4;
+constexpr int kOneWaves = 16;      // of the kernel of both products, and what it takes of
+constexpr int kOneRank = 32;       // ranks
+constexpr int kOneValues = 65536;  // and values of C
 constexpr int kUnit = 8;           // values of 16 bytes
 constexpr int kColumns = 64;       // outputs of one wave
 constexpr int kTurn = 64 * kWaves; // hidden values that the waves take at a time
@@ -57,6 +62,7 @@ __device__ __forceinline__ int slot_of(const AdapterArgs &a, int t) {
 // Tokens of one adapter, up to kTokens, of a call of few: tile t is led by token t, if a
 // whole number of tiles' tokens of its adapter come before it; the workgroup reads all
 // slots. False where no tile is. All threads of the workgroup call it.
+template <int kWaves>
 __device__ __forceinline__ bool find_tile(const AdapterArgs &a, int leader, int *members, int &adapter, int &count) {
   __shared__ uint64_t masks[kFewTokens / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, words = (a.tokens + 63) / 64;
@@ -156,7 +162,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_inner_kernel(AdapterArgs 
   if constexpr (kSorted) {
     if (!find_sorted_tile<kTile>(a, blockIdx.x, adapter, start, count)) return;
   } else {
-    if (!find_tile(a, blockIdx.x, members, adapter, count)) return;
+    if (!find_tile<kWaves>(a, blockIdx.x, members, adapter, count)) return;
   }
   if (adapter >= a.adapters) return;
   const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
@@ -236,6 +242,16 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_inner_kernel(AdapterArgs 
 // 8 q .. 8 q + 7 and 32 + 8 q .. of token m, so that four lanes take 64 bytes of a row.
 __device__ __forceinline__ int output_of(int i, int n) { return i / 2 * 32 + n / 4 * 8 + i % 2 * 4 + n % 4; }
 
+// Half s of a lane's outputs, rounded once.
+__device__ __forceinline__ u32x4 added(u32x4 base, const f32x4 *sum, int s) {
+  float v[kUnit];
+  Lane<false, kWhole>::values(base, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    base[i] = bf16_pair(v[2 * i] + sum[2 * s + i / 2][2 * i % 4], v[2 * i + 1] + sum[2 * s + i / 2][2 * i % 4 + 1]);
+  return base;
+}
+
 // out = base + D v for a tile of tokens, a wave 64 outputs of them at a time: rows of base
 // and D on their way first, then v from its parts, as two BF16 numbers in LDS. kShort is for
 // ranks up to 32, whose rows of D the next 64 outputs' are read ahead of.
@@ -248,7 +264,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a)
   if constexpr (kSorted) {
     if (!find_sorted_tile<kTile>(a, blockIdx.x, adapter, start, count)) return;
   } else {
-    if (!find_tile(a, blockIdx.x, members, adapter, count)) return;
+    if (!find_tile<kWaves>(a, blockIdx.x, members, adapter, count)) return;
   }
   const bool bare = adapter >= a.adapters;
   if (bare && a.out == a.base) return;
@@ -348,15 +364,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a)
     for (int g = 0; g < kGroups; ++g) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        u32x4 row = base[g][s];
-        if (!bare) {
-          float value[kUnit];
-          Lane<false, kWhole>::values(row, value);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            row[i] = bf16_pair(value[2 * i] + sum[g][2 * s + i / 2][2 * i % 4],
-                               value[2 * i + 1] + sum[g][2 * s + i / 2][2 * i % 4 + 1]);
-        }
+        const u32x4 row = bare ? base[g][s] : added(base[g][s], sum[g], s);
         if (16 * g + m < count && o0 + 32 * s + kUnit * q < a.outputs)
           *reinterpret_cast<u32x4 *>(to[g] + o0 + 32 * s) = row;
       }
@@ -365,10 +373,102 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a)
   }
 }
 
+// Both products of a few tokens and ranks in one launch: workgroup = a tile and 1024 of its
+// outputs, v formed again for each. The waves take the hidden dimension in turns of 64 (a
+// lane 16 values that follow one another: the order of products in a sum is free, and both
+// operands have the same); rows of base and D are on their way meanwhile.
+template <int kTiles>
+__global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(AdapterArgs a) {
+  constexpr int kRow = 32 + kUnit;
+  __shared__ __attribute__((aligned(16))) float sums[kOneWaves][kTiles][256];
+  __shared__ __attribute__((aligned(16))) uint16_t parts[2][kTokens][kRow];
+  __shared__ int members[kTokens];
+  int adapter, count;
+  if (!find_tile<kOneWaves>(a, blockIdx.x, members, adapter, count)) return;
+  const bool bare = adapter >= a.adapters;
+  if (bare && a.out == a.base) return;
+  const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t token = members[min(m, count - 1)];
+  const int o0 = (blockIdx.y * kOneWaves + wave) * kColumns;
+  const u32x4 zero = {0, 0, 0, 0};
+  u32x4 base[2], w[4] = {};
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int o = o0 + 32 * s + kUnit * q;
+    if (o < a.outputs) base[s] = load16(a.base + token * a.base_stride + o);
+  }
+  f32x4 sum[4] = {};
+  if (!bare) {
+    // (outputs past the last are its again, and not stored)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t o = min(o0 + output_of(i, m), a.outputs - 1);
+      if (kUnit * q < a.rank) w[i] = load16(a.decoder + (static_cast<int64_t>(adapter) * a.outputs + o) * a.rank + kUnit * q);
+    }
+    const uint16_t *x = a.x + token * a.x_stride, *c[kTiles];
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i)
+      c[i] = a.encoder + (static_cast<int64_t>(adapter) * a.rank + min(16 * i + m, a.rank - 1)) * a.hidden;
+    f32x4 d[kTiles] = {};
+#pragma unroll 2
+    for (int h0 = 64 * wave; h0 < a.hidden; h0 += 64 * kOneWaves) {
+      u32x4 xv[2], cv[2][kTiles];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int h = h0 + 16 * q + kUnit * s, at = min(h, a.hidden - kUnit);
+        xv[s] = load16(x + at);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) cv[s][i] = load16(c[i] + at);
+        if (h >= a.hidden) {
+          xv[s] = zero;
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) cv[s][i] = zero;
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) d[i] = mma(cv[s][i], xv[s], d[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) *reinterpret_cast<f32x4 *>(&sums[wave][i][m * 16 + 4 * q]) = d[i];
+    __syncthreads();
+    if (threadIdx.x < 8 * kTokens) {
+      // thread = four ranks of a token; zeros behind the last rank
+      const int t = threadIdx.x / 8, r = threadIdx.x % 8 * 4;
+      const float scale = a.scales ? a.scales[adapter] : 1.0f;
+      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (r < a.rank) {
+#pragma unroll
+        for (int k = 0; k < kOneWaves; ++k) v += *reinterpret_cast<const f32x4 *>(&sums[k][r / 16][t * 16 + r % 16]);
+        v *= scale;
+      }
+      u32x2 high, low;
+      split(v, high, low);
+      *reinterpret_cast<u32x2 *>(&parts[0][t][r]) = high;
+      *reinterpret_cast<u32x2 *>(&parts[1][t][r]) = low;
+    }
+    __syncthreads();
+    const u32x4 high = load16(&parts[0][m][kUnit * q]), low = load16(&parts[1][m][kUnit * q]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = mma(w[i], low, mma(w[i], high, sum[i]));
+  }
+  if (m >= count) return;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int o = o0 + 32 * s + kUnit * q;
+    if (o < a.outputs)
+      *reinterpret_cast<u32x4 *>(a.out + token * a.out_stride + o) = bare ? base[s] : added(base[s], sum, s);
+  }
+}
+
 int64_t rounded(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 // A workgroup of few tokens reads all slots to find its tile, and one is launched for every
-// token; the sort is a launch of its own.
+// token; the sort is a launch of its own. 250 tokens of 8 adapters of rank 64 (2816 to 1408
+// values) take 19 us either way, 200 of as many adapters of rank 16 12.5 and 19 sorted, 512 of
+// 8 adapters of rank 32 26 and 17.
 bool sorts(int tokens) { return tokens > kFewTokens; }
 
 // Workgroups share the hidden dimension: of few tokens 256 values each or a sixteenth, of
@@ -454,8 +554,20 @@ CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t
     most = tokens / tile + (adapters + 1 < tokens ? adapters + 1 : tokens);
     if (most > tokens) most = tokens;
   }
+  const int tiles = (rank + 15) / 16;
+  // Few tokens: what one compute unit takes from memory bounds the kernel of both products,
+  // a launch's end and start the two. A token of 2048 values, rank 8 / 16 / 32, 2048 outputs:
+  // 6.8 / 7.3 / 9.4 us against 8.2 / 8.4 / 8.7, of 4096 values and rank 16 9.5 against 8.9; 64
+  // tokens of as many adapters, rank 16 / 32, 1024 outputs: 7.7 / 9.9 against 9.0 / 8.9; rank 64,
+  // a token: 15.7 against 9.5. On the host a launch is 2.5 us. (Its workgroups read rows of
+  // hidden while others of the same rows write out.)
+  if (!sorted && rank <= kOneRank && hidden_size * rank <= kOneValues && a.out != a.x) {
+    const dim3 grid(tokens, (outputs + kOneWaves * kColumns - 1) / (kOneWaves * kColumns));
+    hipLaunchKernelGGL(tiles == 1 ? adapter_one_kernel<1> : adapter_one_kernel<2>, grid, dim3(64 * kOneWaves), 0, stream, a);
+    return check_launch("adapter_one");
+  }
   const dim3 block(64 * kWaves);
-  const int tiles = (rank + 15) / 16, held = !sorted || tiles == 1 ? 1 : tiles == 2 ? 2 : 4;
+  const int held = !sorted || tiles == 1 ? 1 : tiles == 2 ? 2 : 4;
   auto start = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(most, (tiles + held - 1) / held, a.splits), block, 0, stream, a);
     return check_launch("adapter_inner");
