@@ -15,6 +15,12 @@
 //                         dw[t, k] = sum_h dout[t, h] rows[place, h]
 //
 // What a dropped pair's row or weight holds is never read, so it may hold a NaN.
+//
+// All but the order is one pass over rows, bound by memory. 4096 and 8191 tokens of eight
+// BF16 rows of 2048: laid out 24 and 50 to 59 us (151 and 302 MB, 5.1 to 6.3 TB/s), summed 27
+// and 58 (5.2 to 5.6), the sum's gradients 112 (570 MB, 5.1 TB/s). Rows that are read once
+// are loaded past the caches: 62 -> 59 us the sum, 121 -> 109 its gradients; stores past them
+// made a sum that follows slower (104 -> 112 both).
 
 #include "cfmoe_rows.h"
 
@@ -109,7 +115,10 @@ __global__ __launch_bounds__(64 * kSortWaves) void order_count_kernel(OrderArgs 
 // Stable counting sort. A wave has a range of consecutive pairs: it counts their keys in
 // LDS, the counts become first rows (a scan over the keys, then over workgroups and waves),
 // and a pair's row is its key's first row of the wave and its rank there, which the counting
-// gave; pairs that the lanes do not hold from then are ranked again.
+// gave; pairs that the lanes do not hold from then are ranked again. Round trips and barriers
+// bound it: 3.6 us for one token, 4.8 for 1048 pairs in one workgroup, 4.6 and 6.4 in two
+// launches for 32768 in 32. (Counting by LDS atomics took 9.3 us for 4001 pairs of five
+// keys, which now take 6.1.)
 __global__ __launch_bounds__(64 * kSortWaves) void order_kernel(OrderArgs a) {
   extern __shared__ int shared[];
   __shared__ int wave_sums[kSortWaves];
@@ -201,7 +210,8 @@ int most_waves(int experts) {
   return waves;
 }
 
-// One workgroup while its lanes hold all keys, else up to 64 of a key a lane.
+// One workgroup while its lanes hold all keys, else up to 64 of a key a lane: 4096 pairs are
+// 6.1 us in one, 32768 took 4.7 and 10.5 in eight of four keys a lane.
 int sort_blocks(int64_t pairs, int experts) {
   const int64_t lanes = 64 * most_waves(experts);
   if (pairs <= lanes * kHeld) return 1;
@@ -390,10 +400,10 @@ int check_rows(const RowsArgs &a) {
   return 0;
 }
 
-// A wave takes a token of up to two lane's worths, a workgroup of four a longer one. 8192
-// tokens of 8 rows, BF16, one wave and four: the sum of rows of 1024 32 and 37 us, its
-// gradients 52 and 82, of rows of 2048 76 and 60, 120 and 106; laying out either way is the
-// same to 1024 (24 us), 58 and 50 at 2048.
+// A wave takes a token of up to two lanes' worth, a workgroup of four a longer one. 8192
+// tokens of 8 rows, BF16, one wave against four: laying out rows of 264 / 1024 / 2048 9.1 / 23.6
+// / 58.5 us and 10.0 / 23.9 / 50.1, their sum 10.0 / 27.3 / 62.2 and 11.4 / 26.8 / 52.4, its
+// gradients 19.8 / 48.0 / 107.6 and 31.6 / 48.7 / 95.6.
 #define CFMOE_ROWS_LAUNCH(KERNEL, fp32, a, stream)                                                          \
   do {                                                                                                      \
     const Rows rows = rows_of((a).hidden, fp32);                                                            \
