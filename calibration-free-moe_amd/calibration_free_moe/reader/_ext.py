@@ -263,7 +263,8 @@ def trit_plane_bytes(dims: Dims) -> int:
 def run(function: Callable[..., int], device: torch.device, *arguments: object) -> None:
     """Call `function(*arguments, stream)` on `device` and its current stream; check its status."""
     index = device.index
-    if torch.cuda.current_device() != index:
+    # (the tensors' device is initialised: torch.cuda.current_device() looks for that again)
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
             return run(function, device, *arguments)
     # (the raw handle: a torch.cuda.Stream object costs 2 us more than the lookup)

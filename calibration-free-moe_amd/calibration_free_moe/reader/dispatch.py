@@ -96,7 +96,10 @@ def sort_by_expert(ids: Tensor, experts: int, padding: Tensor | None = None) -> 
         None if padding is None else padding.data_ptr(), offsets.data_ptr(), places.data_ptr(),
         pairs.data_ptr(), None if scratch is None else scratch.data_ptr(), tokens,
     )
-    return ExpertOrder(offsets, places, pairs)
+    # (as made here the three need no check)
+    order = ExpertOrder.__new__(ExpertOrder)
+    order.__dict__.update(offsets=offsets, places=places, pairs=pairs)
+    return order
 
 
 def _flags(rows: Tensor, weights: Tensor | None = None) -> int:

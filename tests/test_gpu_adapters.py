@@ -43,7 +43,9 @@ def check(made, **change):
     (1, 8, 8, 1, 8), (1, 2048, 2048, 8, 16), (2, 64, 72, 1, 24), (16, 128, 256, 1, 32),
     (17, 120, 264, 1, 40), (33, 264, 1000, 3, 64), (64, 2048, 512, 64, 32), (100, 1024, 320, 5, 128),
     (70, 72, 136, 2, 256), (48, 2816, 64, 7, 8), (250, 512, 96, 300, 16), (5, 1032, 8, 2, 248),
-    (3, 8192, 64, 2, 16), (1024, 64, 64, 3, 16), (1023, 64, 64, 900, 8),
+    (3, 8192, 64, 2, 16), (1024, 64, 64, 3, 16), (1023, 64, 64, 900, 8), (256, 64, 72, 9, 16),
+    (256, 4104, 64, 3, 16), (7, 4096, 1032, 3, 16), (200, 1024, 2056, 40, 40), (4, 65536, 8, 2, 8),
+    (2, 8, 65536, 2, 256),
 ])
 @pytest.mark.parametrize("scaled", [False, True])
 def test_few_tokens(tokens, hidden, outputs, adapters, rank, scaled):
@@ -54,7 +56,8 @@ def test_few_tokens(tokens, hidden, outputs, adapters, rank, scaled):
 @pytest.mark.parametrize("tokens,hidden,outputs,adapters,rank", [
     (1025, 64, 64, 1, 8), (1030, 128, 264, 5, 16), (1500, 264, 72, 2, 24), (1200, 512, 320, 70, 64),
     (2000, 72, 136, 3, 128), (1100, 64, 64, 4096, 8), (1400, 136, 96, 63, 40), (1300, 64, 200, 64, 256),
-    (4100, 64, 64, 65, 72), (5000, 96, 64, 10, 16),
+    (4100, 64, 64, 65, 72), (5000, 96, 64, 10, 16), (257, 64, 72, 9, 16), (300, 2048, 1024, 300, 8),
+    (260, 4096, 2056, 2, 40),
 ])
 @pytest.mark.parametrize("runs", [False, True])
 def test_many_tokens(tokens, hidden, outputs, adapters, rank, runs):
@@ -176,6 +179,24 @@ def test_the_batch_does_not_matter():
     for t in (0, 13, 39):
         alone = {k: on[k][t:t + 1] if k in ("base", "hidden", "slots") else on[k] for k in on}
         assert torch.equal(apply_adapters(**alone)[0], out[t])
+
+
+@pytest.mark.parametrize("tokens", [2, 300])
+def test_more_weights_than_32_bits_count(tokens):
+    """The last of many adapters, 5 GB of either weight, as the only one of a short list."""
+    n, rank, size = 300, 128, 65536
+    assert n * rank * size > 2 ** 31
+    g = torch.Generator(device=DEVICE).manual_seed(3)
+    x = torch.randn(tokens, size, generator=g, device=DEVICE).bfloat16()
+    base = torch.randn(tokens, size, generator=g, device=DEVICE).bfloat16()
+    encoder = torch.empty(n, rank, size, dtype=BF16, device=DEVICE)
+    decoder = torch.empty(n, size, rank, dtype=BF16, device=DEVICE)
+    encoder[-1] = (torch.randn(rank, size, generator=g, device=DEVICE) / 256).bfloat16()
+    decoder[-1] = torch.randn(size, rank, generator=g, device=DEVICE).bfloat16()
+    slots = torch.full((tokens,), n - 1, dtype=torch.int32, device=DEVICE)
+    got = apply_adapters(base, x, encoder, decoder, slots)
+    want = apply_adapters(base, x, encoder[-1:].clone(), decoder[-1:].clone(), torch.zeros_like(slots))
+    assert torch.equal(got, want) and not torch.equal(got, base)
 
 
 def test_empty_batches():
