@@ -266,24 +266,28 @@ __device__ __forceinline__ void for_tokens(const RowsArgs &a, F f) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t step = static_cast<int64_t>(gridDim.x) * kTokens;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + wave / kWaves; t < a.tokens; t += step)
-    f(static_cast<int>(t), static_cast<int>(threadIdx.x) & (64 * kWaves - 1));
+    f(static_cast<int>(t), wave % kWaves, static_cast<int>(threadIdx.x & 63));
 }
+
+// In the kernels below all lanes of a wave go through a row together, those past its end
+// with the row's last values, which they neither store nor count: a slot's place is read
+// from its lane by the others while that lane is at work.
 
 // rows[place] = x[t]: a token's row is read once and written K times.
 template <bool kFp32, Rows kRows, int kWaves>
 __global__ __launch_bounds__(kThreads) void gather_kernel(RowsArgs a) {
   using L = Lane<kFp32, kRows>;
-  for_tokens<kWaves>(a, [&](int t, int lane) {
+  for_tokens<kWaves>(a, [&](int t, int part, int lane) {
     const Slots slots(a, t);
-    for (int column = lane * L::kValues; column < a.hidden; column += 64 * kWaves * L::kValues) {
-      const int h = L::first(column, a.hidden);
+    for (int base = 64 * part * L::kValues; base < a.hidden; base += 64 * kWaves * L::kValues) {
+      const int column = base + lane * L::kValues, h = L::first(column, a.hidden);
       float v[L::kValues], zero[L::kValues] = {};
       L::values(L::load(a.from, static_cast<int64_t>(t) * a.hidden + h), v);
       for (int k = 0; k < a.top_k; ++k) {
         const int place = slots.at(k);
         if (place == INT32_MAX) continue;
         const int64_t row = place >= 0 ? place : -1 - place;
-        L::store(a.out, row * a.hidden + h, place >= 0 ? v : zero);
+        if (column < a.hidden) L::store(a.out, row * a.hidden + h, place >= 0 ? v : zero);
       }
     }
   });
@@ -293,10 +297,10 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(RowsArgs a) {
 template <bool kFp32, Rows kRows, int kWaves>
 __global__ __launch_bounds__(kThreads) void combine_kernel(RowsArgs a) {
   using L = Lane<kFp32, kRows>;
-  for_tokens<kWaves>(a, [&](int t, int lane) {
+  for_tokens<kWaves>(a, [&](int t, int part, int lane) {
     const Slots slots(a, t);
-    for (int column = lane * L::kValues; column < a.hidden; column += 64 * kWaves * L::kValues) {
-      const int h = L::first(column, a.hidden);
+    for (int base = 64 * part * L::kValues; base < a.hidden; base += 64 * kWaves * L::kValues) {
+      const int column = base + lane * L::kValues, h = L::first(column, a.hidden);
       float sum[L::kValues] = {};
       for (int k0 = 0; k0 < a.top_k; k0 += kSlots) {
         typename L::Raw raw[kSlots] = {};
@@ -315,7 +319,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(RowsArgs a) {
           for (int i = 0; i < L::kValues; ++i) sum[i] = fmaf(w, v[i], sum[i]);
         }
       }
-      L::store(a.out, static_cast<int64_t>(t) * a.hidden + h, sum);
+      if (column < a.hidden) L::store(a.out, static_cast<int64_t>(t) * a.hidden + h, sum);
     }
   });
 }
@@ -325,13 +329,15 @@ template <bool kFp32, Rows kRows, int kWaves>
 __global__ __launch_bounds__(kThreads) void combine_backward_kernel(RowsArgs a) {
   using L = Lane<kFp32, kRows>;
   __shared__ float parts[kWaves][kSlots];
-  const int wave = threadIdx.x >> 6;
-  for_tokens<kWaves>(a, [&](int t, int lane) {
+  for_tokens<kWaves>(a, [&](int t, int part, int lane) {
     const Slots slots(a, t);
     for (int k0 = 0; k0 < a.top_k; k0 += kSlots) {
       float dot[kSlots] = {};
-      for (int column = lane * L::kValues; column < a.hidden; column += 64 * kWaves * L::kValues) {
-        const int h = L::first(column, a.hidden), others = L::others(column, a.hidden);
+      // (whole: no lane of the wave is past the row's end)
+      auto take = [&](int column, auto whole) {
+        constexpr bool kInside = decltype(whole)::value;
+        const int h = kInside ? column : L::first(column, a.hidden), others = column - h;
+        const bool in = kInside || column < a.hidden;
         float grad[L::kValues];
         typename L::Raw raw[kSlots] = {};
         L::values(L::load(a.from, static_cast<int64_t>(t) * a.hidden + h), grad);
@@ -344,16 +350,17 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(RowsArgs a) 
 #pragma unroll
           for (int j = 0; j < kSlots; ++j) {
             if (k0 + j >= a.top_k || !kept(slots.at(k0 + j))) continue;
-            float v[L::kValues];
+            float v[L::kValues], more = dot[j];
             L::values(raw[j], v);
 #pragma unroll
             for (int i = 0; i < L::kValues; ++i) {
-              const float more = fmaf(grad[i], v[i], dot[j]);
-              dot[j] = kRows == kRagged && i < others ? dot[j] : more;
+              const float next = fmaf(grad[i], v[i], more);
+              more = !kInside && i < others ? more : next;
             }
+            dot[j] = in ? more : dot[j];
           }
         }
-        if (!a.out) continue;
+        if (!a.out) return;
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
           const int place = k0 + j < a.top_k ? slots.at(k0 + j) : INT32_MAX;
@@ -362,8 +369,14 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(RowsArgs a) 
           float g[L::kValues];
 #pragma unroll
           for (int i = 0; i < L::kValues; ++i) g[i] = place >= 0 ? w * grad[i] : 0.0f;
-          L::store(a.out, static_cast<int64_t>(place >= 0 ? place : -1 - place) * a.hidden + h, g);
+          const int64_t row = place >= 0 ? place : -1 - place;
+          if (in) L::store(a.out, row * a.hidden + h, g);
         }
+      };
+      for (int base = 64 * part * L::kValues; base < a.hidden; base += 64 * kWaves * L::kValues) {
+        const int column = base + lane * L::kValues;
+        if (base + 64 * L::kValues <= a.hidden) take(column, std::true_type());
+        else take(column, std::false_type());
       }
       if (!a.grad_weights) continue;
 #pragma unroll
@@ -371,10 +384,10 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(RowsArgs a) 
       if (kWaves > 1) {
 #pragma unroll
         for (int j = 0; j < kSlots; ++j)
-          if ((lane & 63) == j) parts[wave][j] = dot[j];
+          if (lane == j) parts[part][j] = dot[j];
         __syncthreads();
       }
-      if (lane < kSlots && k0 + lane < a.top_k) {
+      if (part == 0 && lane < kSlots && k0 + lane < a.top_k) {
         float total = 0.0f;
         if (kWaves > 1) {
 #pragma unroll

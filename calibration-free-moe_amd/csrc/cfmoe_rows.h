@@ -24,11 +24,9 @@ struct Lane {
   using Raw = std::conditional_t<kRows != kSingle, u32x4, Value>;
   static constexpr int kValues = kRows != kSingle ? (kFp32 ? 4 : 8) : 1;
 
-  // First element of the lane whose values would begin at `column`, and how many of the
-  // values from there are another lane's.
-  static __device__ __forceinline__ int first(int column, int size) {
-    return kRows == kRagged ? min(column, size - kValues) : column;
-  }
+  // First element of the lane whose values would begin at `column` (the row's last ones past
+  // its end), and how many of the values from there are another lane's.
+  static __device__ __forceinline__ int first(int column, int size) { return min(column, size - kValues); }
   static __device__ __forceinline__ int others(int column, int size) { return column - first(column, size); }
 
   template <bool kOnce = false>
