@@ -9,7 +9,7 @@
 // matrix instructions, v = s_a C_a x over the hidden dimension and D_a v over the rank. A
 // decode step's tiles hold a token or two, which leaves most columns of an instruction
 // empty: what bounds it is the weights' reading, once for each tile, and a compute unit
-// takes about 25 GB/s from memory. So the hidden dimension and the ranks are spread over
+// takes about 75 GB/s from memory. So the hidden dimension and the ranks are spread over
 // workgroups (adapter_inner_kernel), and the second launch (adapter_out_kernel) adds up
 // their parts of v; of few ranks one workgroup reads all (adapter_one_kernel). Many tokens
 // are sorted by adapter first.
@@ -31,7 +31,7 @@ constexpr int kManyTokens = 32;    // of a tile, many tokens
 constexpr int kWaves = 4;
 constexpr int kOneWaves = 16;      // of the kernel of both products, and what it takes of
 constexpr int kOneRank = 32;       // ranks
-constexpr int kOneValues = 65536;  // and values of C
+constexpr int kOneValues = 131072; // and values of C
 constexpr int kUnit = 8;           // values of 16 bytes
 constexpr int kColumns = 64;       // outputs of one wave
 constexpr int kTurn = 64 * kWaves; // hidden values that the waves take at a time
@@ -144,44 +144,21 @@ __device__ __forceinline__ void split(f32x4 v, u32x2 &high, u32x2 &low) {
 // Values of a row of v in LDS: whole steps of 32, and a unit for the banks.
 __host__ __device__ __forceinline__ int parts_row(int rank) { return (rank + 31) / 32 * 32 + kUnit; }
 
-// inner[split, token, r] = a split's part of s sum_h C[r, h] x[token, h], of a tile of
-// tokens and kTiles tiles of 16 ranks. The waves take the split's hidden values in turns of
-// 64 and add up in LDS. The operands pass through LDS, each wave's through its own part of
-// it: eight lanes read 128 bytes of a row from memory, where the matrix instruction's own
-// layout has neighbouring lanes read from different rows (4001 tokens of 2048 values, rank
-// 64: 14.5 us so, 10.5 through LDS). Rows of LDS are an odd number of 16-byte units long, so
-// that the 16 rows of an operand lie in different banks. What bounds it then is the chain
-// of offsets, tokens and rows in memory, four turns of them for a wave.
-template <bool kSorted, int kTiles>
-__global__ __launch_bounds__(64 * kWaves) void adapter_inner_kernel(AdapterArgs a) {
-  constexpr int kTile = kSorted ? kManyTokens : kTokens, kGroups = kTile / 16;
-  constexpr int kRows = 16 * kTiles + kTile, kLoads = kRows / 8, kRankLoads = 2 * kTiles;
-  __shared__ __attribute__((aligned(16))) uint16_t stage[kWaves][kRows][64 + kUnit];
-  __shared__ int members[kTokens];
-  static_assert(sizeof(float) * kWaves * kGroups * kTiles * 256 <= sizeof(stage), "the sums take the stage's place");
-  float(*sums)[kGroups][kTiles][256] = reinterpret_cast<float(*)[kGroups][kTiles][256]>(stage);
-  int adapter, start = 0, count;
-  if constexpr (kSorted) {
-    if (!find_sorted_tile<kTile>(a, blockIdx.x, adapter, start, count)) return;
-  } else {
-    if (!find_tile<kWaves>(a, blockIdx.x, members, adapter, count)) return;
-  }
-  if (adapter >= a.adapters) return;
+// d[g][i] += C x of a wave's part of the hidden dimension: its turns of 64 values from `first`
+// on, in steps of `step`, of kTiles tiles of 16 rows of C and kGroups of 16 tokens. The
+// operands pass through the wave's own part of LDS: eight lanes read 128 bytes of a row from
+// memory, where the matrix instruction's own layout has neighbouring lanes read from
+// different rows, a quarter as fast (4001 tokens of 2048 values, rank 64: 14.5 us so, 10.5
+// through LDS). Rows of LDS are an odd number of 16-byte units long, so that the 16 rows of
+// an operand lie in different banks. row[j]: this lane's unit of every eighth row, C's, then
+// the tokens' (past the end any, what they give is not stored).
+constexpr int kStageRow = 64 + kUnit;
+
+template <int kTiles, int kGroups>
+__device__ __forceinline__ void staged_product(uint16_t (*stage)[kStageRow], const uint16_t *const *row, int first,
+                                               int last, int step, f32x4 (*d)[kTiles]) {
+  constexpr int kLoads = 2 * (kTiles + kGroups);
   const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r0 = blockIdx.y * 16 * kTiles;
-  // this lane's unit of every eighth row: C's, then the tokens' (those past the end are the
-  // last again, and what they give is not stored)
-  const uint16_t *row[kLoads];
-#pragma unroll
-  for (int j = 0; j < kLoads; ++j) {
-    const int r = min(r0 + 8 * j + lane / 8, a.rank - 1), t = min(8 * (j - kRankLoads) + lane / 8, count - 1);
-    if (j < kRankLoads) row[j] = a.encoder + (static_cast<int64_t>(adapter) * a.rank + r) * a.hidden;
-    else row[j] = a.x + static_cast<int64_t>(kSorted ? a.pairs[start + t] : members[t]) * a.x_stride;
-    row[j] += kUnit * (lane % 8);
-  }
-  f32x4 d[kGroups][kTiles] = {};
-  const int first = blockIdx.z * a.share, last = min(first + a.share, a.hidden);
   u32x4 raw[kLoads];
   auto fetch = [&](int h0) {
     if (h0 + 64 <= last) {
@@ -195,27 +172,61 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_inner_kernel(AdapterArgs 
       }
     }
   };
-  fetch(first + 64 * wave);
-  for (int h0 = first + 64 * wave; h0 < last; h0 += kTurn) {
+  fetch(first);
+  for (int h0 = first; h0 < last; h0 += step) {
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j)
-      *reinterpret_cast<u32x4 *>(&stage[wave][8 * j + lane / 8][kUnit * (lane % 8)]) = raw[j];
-    fetch(h0 + kTurn);
+    for (int j = 0; j < kLoads; ++j) *reinterpret_cast<u32x4 *>(&stage[8 * j + lane / 8][kUnit * (lane % 8)]) = raw[j];
+    fetch(h0 + step);
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       u32x4 xv[kGroups];
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) xv[g] = load16(&stage[wave][16 * (kTiles + g) + m][32 * s + kUnit * q]);
+      for (int g = 0; g < kGroups; ++g) xv[g] = load16(&stage[16 * (kTiles + g) + m][32 * s + kUnit * q]);
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
-        const u32x4 cv = load16(&stage[wave][16 * i + m][32 * s + kUnit * q]);
+        const u32x4 cv = load16(&stage[16 * i + m][32 * s + kUnit * q]);
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) d[g][i] = mma(cv, xv[g], d[g][i]);
       }
     }
     __builtin_amdgcn_wave_barrier();
   }
+}
+
+// inner[split, token, r] = a split's part of s sum_h C[r, h] x[token, h], of a tile of
+// tokens and kTiles tiles of 16 ranks. The waves take the split's hidden values in turns of
+// 64 and add up in LDS. What bounds it is the chain of offsets, tokens and rows in memory,
+// four turns of them for a wave.
+template <bool kSorted, int kTiles>
+__global__ __launch_bounds__(64 * kWaves) void adapter_inner_kernel(AdapterArgs a) {
+  constexpr int kTile = kSorted ? kManyTokens : kTokens, kGroups = kTile / 16;
+  constexpr int kRows = 16 * kTiles + kTile, kLoads = kRows / 8, kRankLoads = 2 * kTiles;
+  __shared__ __attribute__((aligned(16))) uint16_t stage[kWaves][kRows][kStageRow];
+  __shared__ int members[kTokens];
+  static_assert(sizeof(float) * kWaves * kGroups * kTiles * 256 <= sizeof(stage), "the sums take the stage's place");
+  float(*sums)[kGroups][kTiles][256] = reinterpret_cast<float(*)[kGroups][kTiles][256]>(stage);
+  int adapter, start = 0, count;
+  if constexpr (kSorted) {
+    if (!find_sorted_tile<kTile>(a, blockIdx.x, adapter, start, count)) return;
+  } else {
+    if (!find_tile<kWaves>(a, blockIdx.x, members, adapter, count)) return;
+  }
+  if (adapter >= a.adapters) return;
+  const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r0 = blockIdx.y * 16 * kTiles;
+  const uint16_t *row[kLoads];
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    const int r = min(r0 + 8 * j + lane / 8, a.rank - 1), t = min(8 * (j - kRankLoads) + lane / 8, count - 1);
+    if (j < kRankLoads) row[j] = a.encoder + (static_cast<int64_t>(adapter) * a.rank + r) * a.hidden;
+    else row[j] = a.x + static_cast<int64_t>(kSorted ? a.pairs[start + t] : members[t]) * a.x_stride;
+    row[j] += kUnit * (lane % 8);
+  }
+  f32x4 d[kGroups][kTiles] = {};
+  const int first = blockIdx.z * a.share, last = min(first + a.share, a.hidden);
+  staged_product<kTiles, kGroups>(stage[wave], row, first + 64 * wave, last, kTurn, d);
   __syncthreads();
 #pragma unroll
   for (int g = 0; g < kGroups; ++g)
@@ -358,7 +369,6 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a)
       if constexpr (kShort) {
         multiply(0, w);
       } else {
-#pragma unroll 2
         for (int r0 = 0; r0 < a.rank; r0 += 32) {
           u32x4 rows[4];
           fetch_rows(o0, r0, rows);
@@ -380,15 +390,16 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a)
 }
 
 // Both products of a few tokens and ranks in one launch: workgroup = a tile and 1024 of its
-// outputs, v formed again for each. The waves take the hidden dimension in turns of 64 (a
-// lane 16 values that follow one another: the order of products in a sum is free, and both
-// operands have the same); rows of base and D are on their way meanwhile.
+// outputs, v formed again for each. The waves take the hidden dimension in turns of 64; rows
+// of base and D are on their way meanwhile.
 template <int kTiles>
 __global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(AdapterArgs a) {
-  constexpr int kRow = 32 + kUnit;
-  __shared__ __attribute__((aligned(16))) float sums[kOneWaves][kTiles][256];
+  constexpr int kRow = 32 + kUnit, kLoads = 2 * (kTiles + 1);
+  __shared__ __attribute__((aligned(16))) uint16_t stage[kOneWaves][16 * (kTiles + 1)][kStageRow];
   __shared__ __attribute__((aligned(16))) uint16_t parts[2][kTokens][kRow];
   __shared__ int members[kTokens];
+  static_assert(sizeof(float) * kOneWaves * kTiles * 256 <= sizeof(stage), "the sums take the stage's place");
+  float(*sums)[kTiles][256] = reinterpret_cast<float(*)[kTiles][256]>(stage);
   int adapter, count;
   if (!find_tile<kOneWaves>(a, blockIdx.x, members, adapter, count)) return;
   const bool bare = adapter >= a.adapters;
@@ -397,7 +408,6 @@ __global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(AdapterArgs
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t token = members[min(m, count - 1)];
   const int o0 = (blockIdx.y * kOneWaves + wave) * kColumns;
-  const u32x4 zero = {0, 0, 0, 0};
   u32x4 base[2], w[4] = {};
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
@@ -412,33 +422,19 @@ __global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(AdapterArgs
       const int64_t o = min(o0 + output_of(i, m), a.outputs - 1);
       if (kUnit * q < a.rank) w[i] = load16(a.decoder + (static_cast<int64_t>(adapter) * a.outputs + o) * a.rank + kUnit * q);
     }
-    const uint16_t *x = a.x + token * a.x_stride, *c[kTiles];
+    const uint16_t *row[kLoads];
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i)
-      c[i] = a.encoder + (static_cast<int64_t>(adapter) * a.rank + min(16 * i + m, a.rank - 1)) * a.hidden;
-    f32x4 d[kTiles] = {};
-#pragma unroll 2
-    for (int h0 = 64 * wave; h0 < a.hidden; h0 += 64 * kOneWaves) {
-      u32x4 xv[2], cv[2][kTiles];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int h = h0 + 16 * q + kUnit * s, at = min(h, a.hidden - kUnit);
-        xv[s] = load16(x + at);
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) cv[s][i] = load16(c[i] + at);
-        if (h >= a.hidden) {
-          xv[s] = zero;
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i) cv[s][i] = zero;
-        }
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) d[i] = mma(cv[s][i], xv[s], d[i]);
+    for (int j = 0; j < kLoads; ++j) {
+      const int r = min(8 * j + lane / 8, a.rank - 1), t = min(8 * (j - 2 * kTiles) + lane / 8, count - 1);
+      if (j < 2 * kTiles) row[j] = a.encoder + (static_cast<int64_t>(adapter) * a.rank + r) * a.hidden;
+      else row[j] = a.x + static_cast<int64_t>(members[t]) * a.x_stride;
+      row[j] += kUnit * (lane % 8);
     }
+    f32x4 d[1][kTiles] = {};
+    staged_product<kTiles, 1>(stage[wave], row, 64 * wave, a.hidden, 64 * kOneWaves, d);
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) *reinterpret_cast<f32x4 *>(&sums[wave][i][m * 16 + 4 * q]) = d[i];
+    for (int i = 0; i < kTiles; ++i) *reinterpret_cast<f32x4 *>(&sums[wave][i][m * 16 + 4 * q]) = d[0][i];
     __syncthreads();
     if (threadIdx.x < 8 * kTokens) {
       // thread = four ranks of a token; zeros behind the last rank
@@ -565,10 +561,11 @@ CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t
   const int tiles = (rank + 15) / 16;
   // Few tokens: what one compute unit takes from memory bounds the kernel of both products,
   // a launch's end and start the two. A token of 2048 values, rank 8 / 16 / 32, 2048 outputs:
-  // 6.8 / 7.3 / 9.4 us against 8.2 / 8.4 / 8.7, of 4096 values and rank 16 9.5 against 8.9; 64
-  // tokens of as many adapters, rank 16 / 32, 1024 outputs: 7.7 / 9.9 against 9.0 / 8.9; rank 64,
-  // a token: 15.7 against 9.5. On the host a launch is 2.5 us. (Its workgroups read rows of
-  // hidden while others of the same rows write out.)
+  // 7.0 / 6.9 / 8.2 us against 8.2 / 8.4 / 8.8, of 4096 values and rank 32 10.0 against 9.3, of
+  // 8192 13.3 against 9.5; 64 tokens of as many adapters, rank 16 / 32, 1024 outputs: 7.1 / 8.5
+  // against 9.0 / 8.9; 256 tokens of 8 adapters, rank 16, 2048 outputs 9.2 against 13.4. Rank
+  // 64 in two passes: 14.8 against 9.6. On the host a launch is 2.5 us. (Its workgroups read
+  // rows of hidden while others of the same rows write out.)
   if (!sorted && rank <= kOneRank && hidden_size * rank <= kOneValues && a.out != a.x) {
     const dim3 grid(tokens, (outputs + kOneWaves * kColumns - 1) / (kOneWaves * kColumns));
     hipLaunchKernelGGL(tiles == 1 ? adapter_one_kernel<1> : adapter_one_kernel<2>, grid, dim3(64 * kOneWaves), 0, stream, a);

@@ -44,7 +44,7 @@ def check(made, **change):
     (17, 120, 264, 1, 40), (33, 264, 1000, 3, 64), (64, 2048, 512, 64, 32), (100, 1024, 320, 5, 128),
     (70, 72, 136, 2, 256), (48, 2816, 64, 7, 8), (250, 512, 96, 300, 16), (5, 1032, 8, 2, 248),
     (3, 8192, 64, 2, 16), (1024, 64, 64, 3, 16), (1023, 64, 64, 900, 8), (256, 64, 72, 9, 16),
-    (256, 4104, 64, 3, 16), (7, 4096, 1032, 3, 16), (200, 1024, 2056, 40, 40), (4, 65536, 8, 2, 8),
+    (256, 4104, 64, 3, 16), (7, 4096, 1032, 3, 32), (9, 4104, 1032, 3, 32), (200, 1024, 2056, 40, 40), (4, 65536, 8, 2, 8),
     (2, 8, 65536, 2, 256),
 ])
 @pytest.mark.parametrize("scaled", [False, True])
