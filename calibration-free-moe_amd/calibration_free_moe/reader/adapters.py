@@ -79,7 +79,7 @@ def apply_adapters(
     alone, or `hidden`; no other overlap. H and O are multiples of 8 up to 65536, R of 8 up
     to 256, N up to 4096, tokens up to 2^24; zero tokens give an empty output. One or two HIP
     launches on the current stream of the tensors' device, up to four for more than 256 tokens, with
-    scratch allocated per call; they can be captured in a graph. Tensors that require
+    scratch allocated per call; `out` counts as written in place; they can be captured in a graph. Tensors that require
     gradients are refused while gradients are on.
     """
     if hidden.dim() != 2 or base.dim() != 2 or encoder.dim() != 3 or decoder.dim() != 3:
@@ -146,7 +146,8 @@ def apply_adapters(
         or (scales is not None and scales.requires_grad)
     ):
         raise ValueError("apply_adapters is forward only: detach its inputs or call it in no_grad")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((tokens, o), dtype=torch.bfloat16, device=device)
     elif not _rows(out, tokens, o, device) or _stride(out) < o:
         raise ValueError("out must be BF16 rows [tokens, O] on the rows' device, one behind another")
@@ -161,6 +162,9 @@ def apply_adapters(
         slots.data_ptr(), None if scales is None else scales.data_ptr(), out.data_ptr(),
         _stride(out), scratch.data_ptr(), tokens,
     )
+    if given and not out.is_inference():
+        # (what saved the tensor for a backward pass is to see that it changed)
+        torch.autograd.graph.increment_version(out)
     return out
 
 

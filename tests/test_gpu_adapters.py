@@ -240,3 +240,39 @@ def test_refusals():
     refuse("forward only", decoder=on["decoder"].clone().requires_grad_())
     with torch.no_grad():
         apply_adapters(**{**on, "hidden": on["hidden"].clone().requires_grad_()})
+
+
+def test_out_saved_for_a_backward_pass_is_seen_to_have_changed():
+    made = make(20, 64, 64, 2, 8)
+    on = {k: v.to(DEVICE) for k, v in made.items()}
+    factor = torch.ones(64, device=DEVICE, dtype=BF16, requires_grad=True)
+    product = on["base"] * factor
+    apply_adapters(**on)
+    (product * 1).sum().backward(retain_graph=True)
+    apply_adapters(**on, out=on["base"])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    with torch.inference_mode():
+        base = on["base"].clone()
+        apply_adapters(**{**on, "base": base}, out=base)
+
+
+@pytest.mark.parametrize("tokens,hidden,outputs,adapters,rank", [
+    (1024, 64, 64, 3, 32), (512, 64, 1032, 4, 24), (513, 64, 1032, 4, 24), (700, 64, 64, 460, 8),
+    (700, 64, 64, 500, 8), (900, 4096, 264, 180, 32), (900, 4096, 264, 300, 32), (1000, 72, 1024, 1, 16),
+    (257, 2048, 4096, 8, 16), (64, 512, 8192, 64, 16), (64, 512, 8200, 64, 16), (16, 64, 65536, 2, 8),
+])
+@pytest.mark.parametrize("ids64", [False, True])
+def test_sizes_at_which_the_launches_change(tokens, hidden, outputs, adapters, rank, ids64):
+    made = make(tokens, hidden, outputs, adapters, rank, seed=tokens + rank)
+    check(made, **({"slots": made["slots"].long()} if ids64 else {}))
+
+
+@pytest.mark.parametrize("tokens", [257, 700, 1024])
+def test_out_is_hidden_of_few_ranks(tokens):
+    made = make(tokens, 128, 128, 3, 16)
+    on = {k: v.to(DEVICE) for k, v in made.items()}
+    want = check(made)[0]
+    got = apply_adapters(**on, out=on["hidden"])
+    plain.within(got, *plain.adapters(**made))
+    assert torch.equal(got.isnan(), want.isnan())
