@@ -25,13 +25,14 @@ namespace {
 constexpr int kMaxAdapters = 4096;
 constexpr int kMaxRank = 256;
 constexpr int kMaxSize = 65536;
-constexpr int kFewTokens = 256;    // up to which a workgroup finds its tile by itself
+constexpr int kFewTokens = 256;    // up to which two launches find their tiles by themselves
 constexpr int kTokens = 16;        // of a tile, few tokens
 constexpr int kManyTokens = 32;    // of a tile, many tokens
 constexpr int kWaves = 4;
 constexpr int kOneWaves = 16;      // of the kernel of both products, and what it takes of
-constexpr int kOneRank = 32;       // ranks
-constexpr int kOneValues = 131072; // and values of C
+constexpr int kOneRank = 32;       // ranks,
+constexpr int kOneValues = 131072; // values of C
+constexpr int kOneGroups = 1024;   // and workgroups, so tokens too
 constexpr int kUnit = 8;           // values of 16 bytes
 constexpr int kColumns = 64;       // outputs of one wave
 constexpr int kTurn = 64 * kWaves; // hidden values that the waves take at a time
@@ -64,7 +65,7 @@ __device__ __forceinline__ int slot_of(const AdapterArgs &a, int t) {
 // slots. False where no tile is. All threads of the workgroup call it.
 template <int kWaves>
 __device__ __forceinline__ bool find_tile(const AdapterArgs &a, int leader, int *members, int &adapter, int &count) {
-  __shared__ uint64_t masks[kFewTokens / 64];
+  __shared__ uint64_t masks[kOneGroups / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, words = (a.tokens + 63) / 64;
   adapter = __builtin_amdgcn_readfirstlane(slot_of(a, leader));
   for (int w = wave; w < words; w += kWaves) {
@@ -177,7 +178,7 @@ __device__ __forceinline__ void staged_product(uint16_t (*stage)[kStageRow], con
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) *reinterpret_cast<u32x4 *>(&stage[8 * j + lane / 8][kUnit * (lane % 8)]) = raw[j];
     fetch(h0 + step);
-    __builtin_amdgcn_wave_barrier();
+    wave_in_step();
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       u32x4 xv[kGroups];
@@ -190,7 +191,7 @@ __device__ __forceinline__ void staged_product(uint16_t (*stage)[kStageRow], con
         for (int g = 0; g < kGroups; ++g) d[g][i] = mma(cv, xv[g], d[g][i]);
       }
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_in_step();
   }
 }
 
@@ -389,8 +390,8 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a)
   }
 }
 
-// Both products of a few tokens and ranks in one launch: workgroup = a tile and 1024 of its
-// outputs, v formed again for each. The waves take the hidden dimension in turns of 64; rows
+// Both products of few tokens and ranks in one launch: workgroup = a tile and 1024 of its
+// outputs, v formed again for each (so out cannot be x, which others still read). The waves take the hidden dimension in turns of 64; rows
 // of base and D are on their way meanwhile.
 template <int kTiles>
 __global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(AdapterArgs a) {
@@ -467,10 +468,29 @@ __global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(AdapterArgs
 
 int64_t rounded(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
-// A workgroup of few tokens reads all slots to find its tile, and one is launched for every
-// token; the sort is a launch of its own. 250 tokens of 8 adapters of rank 64 (2816 to 1408
-// values) take 19 us either way, 200 of as many adapters of rank 16 12.5 and 19 sorted, 512 of
-// 8 adapters of rank 32 26 and 17.
+// Workgroups of a tile in the kernel of both products.
+int one_pieces(int outputs) { return (outputs + kOneWaves * kColumns - 1) / (kOneWaves * kColumns); }
+
+// Both products in one launch: what one compute unit takes from memory bounds it, a
+// launch's end and start the two. A token of 2048 values, rank 8 / 16 / 32, 2048 outputs:
+// 7.0 / 6.9 / 8.2 us against 8.2 / 8.4 / 8.8, of 4096 values and rank 32 10.0 against 9.3, of
+// 8192 13.3 against 9.5. Rank 64 in two passes: 14.8 against 9.6. On the host a launch is
+// 2.5 us.
+//
+// Its workgroups at work are to have room on the card together, two of rank 16 on a compute
+// unit, one of rank 32: each forms v again. 64 tokens of as many adapters, rank 32, to 4096 /
+// 8192 / 16384 outputs: 9.3 / 16.8 / 29 us against 10.6 / 14.3 / 18; rank 16 7.3 / 12.3 / 22
+// against 9.7 / 13.0 / 15.4. The others only find no tile: 300 / 700 / 1000 tokens of 16
+// adapters, rank 16, 1024 values and outputs 7.7 / 10.1 / 13.5 against 12.6 / 13.2 / 13.3.
+bool one_launch(int tokens, int hidden, int outputs, int rank, int adapters) {
+  if (rank > kOneRank || hidden * rank > kOneValues) return false;
+  const int64_t pieces = one_pieces(outputs), tiles = tokens / kTokens + adapters + 1;
+  return tokens * pieces <= kOneGroups && (tokens < tiles ? tokens : tiles) * pieces <= (rank <= 16 ? 512 : 256);
+}
+
+// With two launches a workgroup of few tokens reads all slots to find its tile, and one is
+// launched for every token; the sort is a launch of its own. 250 tokens of 8 adapters of rank
+// 64 (2816 to 1408 values) take 19 us either way, 512 of 8 adapters of rank 32 26 and 17.
 bool sorts(int tokens) { return tokens > kFewTokens; }
 
 // Workgroups share the hidden dimension: of few tokens 256 values each or a sixteenth, of
@@ -538,6 +558,12 @@ CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t
   a.splits = splits_of(tokens, hidden_size);
   // (whole turns: a split ends where the next begins)
   a.share = (hidden_size + a.splits * kTurn - 1) / (a.splits * kTurn) * kTurn;
+  const int tiles = (rank + 15) / 16;
+  if (one_launch(tokens, hidden_size, outputs, rank, adapters) && a.out != a.x) {
+    const dim3 grid(tokens, one_pieces(outputs));
+    hipLaunchKernelGGL(tiles == 1 ? adapter_one_kernel<1> : adapter_one_kernel<2>, grid, dim3(64 * kOneWaves), 0, stream, a);
+    return check_launch("adapter_one");
+  }
   const bool sorted = sorts(tokens);
   const int tile = sorted ? kManyTokens : kTokens;
   int most = tokens;  // tiles there can be
@@ -557,19 +583,6 @@ CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t
     // one more than whole ones for each adapter, and for the tokens without one
     most = tokens / tile + (adapters + 1 < tokens ? adapters + 1 : tokens);
     if (most > tokens) most = tokens;
-  }
-  const int tiles = (rank + 15) / 16;
-  // Few tokens: what one compute unit takes from memory bounds the kernel of both products,
-  // a launch's end and start the two. A token of 2048 values, rank 8 / 16 / 32, 2048 outputs:
-  // 7.0 / 6.9 / 8.2 us against 8.2 / 8.4 / 8.8, of 4096 values and rank 32 10.0 against 9.3, of
-  // 8192 13.3 against 9.5; 64 tokens of as many adapters, rank 16 / 32, 1024 outputs: 7.1 / 8.5
-  // against 9.0 / 8.9; 256 tokens of 8 adapters, rank 16, 2048 outputs 9.2 against 13.4. Rank
-  // 64 in two passes: 14.8 against 9.6. On the host a launch is 2.5 us. (Its workgroups read
-  // rows of hidden while others of the same rows write out.)
-  if (!sorted && rank <= kOneRank && hidden_size * rank <= kOneValues && a.out != a.x) {
-    const dim3 grid(tokens, (outputs + kOneWaves * kColumns - 1) / (kOneWaves * kColumns));
-    hipLaunchKernelGGL(tiles == 1 ? adapter_one_kernel<1> : adapter_one_kernel<2>, grid, dim3(64 * kOneWaves), 0, stream, a);
-    return check_launch("adapter_one");
   }
   const dim3 block(64 * kWaves);
   const int held = !sorted || tiles == 1 ? 1 : tiles == 2 ? 2 : 4;

@@ -73,7 +73,7 @@ __device__ __forceinline__ void hold_keys(const OrderArgs &a, int low, int high,
 // Takes 64 keys, one a lane (-1: none), into the wave's running `next` rows of each key:
 // lanes of one key find each other by a ballot for each of its bits, and each gets its key's
 // next row and the number of its fellows in lower lanes. No atomic, so no order but the lanes'.
-__device__ __forceinline__ int take_keys(const OrderArgs &a, volatile int *next, int key) {
+__device__ __forceinline__ int take_keys(const OrderArgs &a, int *next, int key) {
   const int lane = threadIdx.x & 63, bits = 32 - __builtin_clz(a.experts);
   const bool live = key >= 0;
   uint64_t fellows = __ballot(live);
@@ -85,9 +85,9 @@ __device__ __forceinline__ int take_keys(const OrderArgs &a, volatile int *next,
   int row = 0;
   // (the lanes of a wave read before its last fellow writes, in program order)
   if (live) row = next[key] + below;
-  __builtin_amdgcn_wave_barrier();
+  wave_in_step();
   if (live && below + 1 == __builtin_popcountll(fellows)) next[key] = row + 1;
-  __builtin_amdgcn_wave_barrier();
+  wave_in_step();
   return row;
 }
 
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void order_kernel(OrderArgs a) {
     if (held[j] >= 0) place(low + 64 * j + lane, held[j], counts[held[j]] + rank[j]);
   if (low + 64 * kHeld >= high) return;
   // rows of the pairs not held: behind the wave's held ones
-  __builtin_amdgcn_wave_barrier();
+  wave_in_step();
 #pragma unroll
   for (int j = 0; j < kHeld; ++j) take_keys(a, counts, held[j]);
   for (int p = low + 64 * kHeld; p < high; p += 64) {

@@ -104,6 +104,14 @@ __device__ __forceinline__ float wave_total(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// What lanes of a wave wrote to LDS before is what its lanes read after: their accesses are
+// done in order, and the compiler keeps them so. No instruction of its own.
+__device__ __forceinline__ void wave_in_step() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 inline bool misaligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
 
 }  // namespace cfmoe
