@@ -68,7 +68,7 @@ class _Join(torch.autograd.Function):
             hidden, block, post, gate, following, scale, epsilon, True
         )
         ctx.save_for_backward(hidden, block, post, gate, following, statistics)
-        ctx.scale = scale
+        ctx.scale, ctx.flags = scale, _flags(hidden, post, gate, following)
         ctx.set_materialize_grads(False)
         if joined is None:
             return out
@@ -79,16 +79,18 @@ class _Join(torch.autograd.Function):
     def backward(ctx, *grads):
         hidden, block, post, gate, following, statistics = ctx.saved_tensors
         grad_joined = None if block is None else grads[0]
+        # (a weight of an output that nothing was made of has no gradient)
         grad_out = None if following is None else grads[-1]
-        needs = list(ctx.needs_input_grad[:5])
         if grad_joined is None and grad_out is None:
             return (None,) * 7
-        # (a weight of an output that nothing was made of has no gradient)
-        needs[4] = needs[4] and grad_out is not None
+        need_hidden, need_block, need_post, need_gate, need_next, _, _ = ctx.needs_input_grad
+        made_hidden = torch.empty_like(hidden) if need_hidden else None
+        made_block = torch.empty_like(block) if need_block else None
+        made_post = torch.empty_like(post) if need_post else None
+        made_gate = torch.empty_like(gate) if need_gate else None
+        made_next = torch.empty_like(following) if need_next and grad_out is not None else None
         tokens, size = hidden.shape
-        inputs = (hidden, block, post, gate, following)
-        made = [torch.empty_like(t) if need else None for t, need in zip(inputs, needs)]
-        sums = needs[2] + needs[4] + (needs[3] and gate.dim() == 1)
+        sums = (made_post is not None) + (made_next is not None) + (need_gate and gate.dim() == 1)
         scratch = None
         if sums:
             scratch = torch.empty(
@@ -99,13 +101,13 @@ class _Join(torch.autograd.Function):
         if grad_out is not None:
             grad_out = grad_out.contiguous()
         _ext.run(
-            _ext.library().cfmoe_join_block_backward, hidden.device, size,
-            _flags(hidden, post, gate, following), hidden.data_ptr(), _pointer(block),
-            _pointer(post), _pointer(gate), ctx.scale, _pointer(following), _pointer(statistics),
-            _pointer(grad_joined), _pointer(grad_out), _pointer(made[0]), _pointer(made[1]),
-            _pointer(made[2]), _pointer(made[3]), _pointer(made[4]), _pointer(scratch), tokens,
+            _ext.library().cfmoe_join_block_backward, hidden.device, size, ctx.flags,
+            hidden.data_ptr(), _pointer(block), _pointer(post), _pointer(gate), ctx.scale,
+            _pointer(following), statistics.data_ptr(), _pointer(grad_joined), _pointer(grad_out),
+            _pointer(made_hidden), _pointer(made_block), _pointer(made_post), _pointer(made_gate),
+            _pointer(made_next), _pointer(scratch), tokens,
         )
-        return (*made, None, None)
+        return made_hidden, made_block, made_post, made_gate, made_next, None, None
 
 
 def _check_hidden(hidden: Tensor, epsilon: float) -> None:
