@@ -223,7 +223,7 @@ def library() -> ctypes.CDLL:
         [count, flags] + [pointer] * 4 + [number] + [pointer] * 10 + [count, pointer]
     )
     lib.cfmoe_apply_adapters_scratch_bytes.restype = ctypes.c_int64
-    lib.cfmoe_apply_adapters_scratch_bytes.argtypes = [count] * 4
+    lib.cfmoe_apply_adapters_scratch_bytes.argtypes = [count] * 6
     lib.cfmoe_apply_adapters.restype = ctypes.c_int
     lib.cfmoe_apply_adapters.argtypes = (
         [count] * 4 + [flags, pointer, stride, pointer, stride] + [pointer] * 5
@@ -306,9 +306,9 @@ def join_scratch_bytes(hidden: int, sums: int, tokens: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096)
-def adapters_scratch_bytes(hidden: int, rank: int, adapters: int, tokens: int) -> int:
-    """Bytes for a call of that size; ValueError if refused."""
-    size = library().cfmoe_apply_adapters_scratch_bytes(hidden, rank, adapters, tokens)
+def adapters_scratch_bytes(*shape: int) -> int:
+    """Bytes for a call of that shape; ValueError if refused."""
+    size = library().cfmoe_apply_adapters_scratch_bytes(*shape)
     if size < 0:
         check(-size)
     return size

@@ -26,14 +26,14 @@ def _stride(t: Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _rows(t: Tensor, tokens: int, size: int, device: torch.device) -> bool:
-    """Whether t is BF16 rows [tokens, size] of consecutive values, 16-byte aligned."""
+def _rows(t: Tensor, device: torch.device) -> bool:
+    """Whether t is BF16 rows on the device, of consecutive values, 16-byte aligned."""
+    step, one = t.stride()
     return (
-        t.shape == (tokens, size)
-        and t.dtype == torch.bfloat16
+        t.dtype == torch.bfloat16
         and t.device == device
-        and t.stride(1) == 1
-        and _stride(t) % 8 == 0
+        and one == 1
+        and (step % 8 == 0 or t.shape[0] < 2)
         and t.data_ptr() % 16 == 0
     )
 
@@ -78,17 +78,19 @@ def apply_adapters(
     16-byte aligned). `out` may be `base`, whose rows without an adapter are then left
     alone, or `hidden`; no other overlap. H and O are multiples of 8 up to 65536, R of 8 up
     to 256, N up to 4096, tokens up to 2^24; zero tokens give an empty output. One or two HIP
-    launches on the current stream of the tensors' device, up to four for more than 256 tokens, with
-    scratch allocated per call; `out` counts as written in place; they can be captured in a graph. Tensors that require
-    gradients are refused while gradients are on.
+    launches on the current stream of the tensors' device, up to four for more than 256 tokens,
+    with scratch allocated per call where they need any; they can be captured in a graph. `out`
+    counts as written in place. Tensors that require gradients are refused while gradients are
+    on.
     """
     if hidden.dim() != 2 or base.dim() != 2 or encoder.dim() != 3 or decoder.dim() != 3:
         raise ValueError(
             "Expected base [tokens, O], hidden [tokens, H], encoder [N, R, H] and decoder [N, O, R]"
         )
     tokens, h = hidden.shape
-    n, rank, _ = encoder.shape
-    o, device = base.shape[1], hidden.device
+    n, rank, encoded = encoder.shape
+    device = hidden.device
+    o = base.shape[1]
     if (
         h % 8
         or not 8 <= h <= MAX_SIZE
@@ -104,8 +106,9 @@ def apply_adapters(
             "one up to 256, 1 to 4096 adapters and at most 2^24 tokens"
         )
     if (
-        encoder.shape != (n, rank, h)
+        encoded != h
         or decoder.shape != (n, o, rank)
+        or base.shape[0] != tokens
         or not hidden.is_cuda
         or encoder.dtype != torch.bfloat16
         or decoder.dtype != torch.bfloat16
@@ -113,16 +116,17 @@ def apply_adapters(
         or decoder.device != device
         or not encoder.is_contiguous()
         or not decoder.is_contiguous()
-        or not _rows(hidden, tokens, h, device)
-        or not _rows(base, tokens, o, device)
+        or not _rows(hidden, device)
+        or not _rows(base, device)
     ):
         raise ValueError(
             "Expected BF16 CUDA rows [tokens, H] and [tokens, O], 16-byte aligned with a first "
             "stride of a multiple of 8, and contiguous BF16 encoder [N, R, H] and decoder [N, O, R]"
         )
+    wide = slots.dtype == torch.int64
     if (
         slots.shape != (tokens,)
-        or slots.dtype not in (torch.int32, torch.int64)
+        or not (wide or slots.dtype == torch.int32)
         or slots.device != device
         or not slots.is_contiguous()
         or (
@@ -148,19 +152,20 @@ def apply_adapters(
         raise ValueError("apply_adapters is forward only: detach its inputs or call it in no_grad")
     given = out is not None
     if not given:
-        out = torch.empty((tokens, o), dtype=torch.bfloat16, device=device)
-    elif not _rows(out, tokens, o, device) or _stride(out) < o:
+        out = hidden.new_empty((tokens, o))
+    elif out.shape != base.shape or not _rows(out, device) or _stride(out) < o:
         raise ValueError("out must be BF16 rows [tokens, O] on the rows' device, one behind another")
     elif tokens and (_overlap(out, base) or _overlap(out, hidden)):
         raise ValueError("out overlaps base or hidden and is not the same rows")
-    size = _ext.adapters_scratch_bytes(h, rank, n, tokens)
-    scratch = torch.empty(size, dtype=torch.uint8, device=device)
+    pointer, x = out.data_ptr(), hidden.data_ptr()
+    size = _ext.adapters_scratch_bytes(h, o, rank, n, tokens, pointer == x)
+    scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _ext.run(
         _ext.library().cfmoe_apply_adapters, device, h, o, rank, n,
-        _ext.IDS_INT64 if slots.dtype == torch.int64 else 0, base.data_ptr(), _stride(base),
-        hidden.data_ptr(), _stride(hidden), encoder.data_ptr(), decoder.data_ptr(),
-        slots.data_ptr(), None if scales is None else scales.data_ptr(), out.data_ptr(),
-        _stride(out), scratch.data_ptr(), tokens,
+        _ext.IDS_INT64 if wide else 0, base.data_ptr(), _stride(base), x, _stride(hidden),
+        encoder.data_ptr(), decoder.data_ptr(), slots.data_ptr(),
+        None if scales is None else scales.data_ptr(), pointer, _stride(out) if given else o,
+        None if scratch is None else scratch.data_ptr(), tokens,
     )
     if given and not out.is_inference():
         # (what saved the tensor for a backward pass is to see that it changed)

@@ -509,12 +509,14 @@ extern "C" {
 
 using namespace cfmoe;
 
-CFMOE_API int64_t cfmoe_apply_adapters_scratch_bytes(int32_t hidden_size, int32_t rank, int32_t adapters, int32_t tokens) {
+CFMOE_API int64_t cfmoe_apply_adapters_scratch_bytes(int32_t hidden_size, int32_t outputs, int32_t rank, int32_t adapters,
+                                                     int32_t tokens, int32_t out_is_hidden) {
   if (rank < 8 || rank > kMaxRank || rank % 8) return -fail(CFMOE_EINVAL, "apply_adapters needs a rank that is a multiple of 8, at most 256");
   if (adapters < 1 || adapters > kMaxAdapters) return -fail(CFMOE_EINVAL, "apply_adapters needs 1 to 4096 adapters");
   if (tokens < 0 || tokens > (1 << 24)) return -fail(CFMOE_EINVAL, "apply_adapters needs 0 to 2^24 tokens");
-  if (hidden_size < 8 || hidden_size > kMaxSize || hidden_size % 8)
+  if (hidden_size < 8 || hidden_size > kMaxSize || hidden_size % 8 || outputs < 8 || outputs > kMaxSize || outputs % 8)
     return -fail(CFMOE_EINVAL, "apply_adapters needs hidden and output sizes that are multiples of 8, at most 65536");
+  if (!out_is_hidden && one_launch(tokens, hidden_size, outputs, rank, adapters)) return 0;
   int64_t bytes = splits_of(tokens, hidden_size) * static_cast<int64_t>(tokens) * rank * 4;
   if (sorts(tokens))
     bytes += rounded(4 * (adapters + 1)) + 2 * rounded(4 * static_cast<int64_t>(tokens)) +
@@ -526,14 +528,12 @@ CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t
                                    const void *base, int64_t base_stride, const void *hidden, int64_t hidden_stride,
                                    const void *encoder, const void *decoder, const void *slots, const float *scales,
                                    void *out, int64_t out_stride, void *scratch, int32_t tokens, cfmoe_stream stream) {
-  const int64_t bytes = cfmoe_apply_adapters_scratch_bytes(hidden_size, rank, adapters, tokens);
+  const int64_t bytes = cfmoe_apply_adapters_scratch_bytes(hidden_size, outputs, rank, adapters, tokens, out == hidden);
   if (bytes < 0) return static_cast<int>(-bytes);
-  if (outputs < 8 || outputs > kMaxSize || outputs % 8)
-    return fail(CFMOE_EINVAL, "apply_adapters needs hidden and output sizes that are multiples of 8, at most 65536");
   if (base_stride % 8 || hidden_stride % 8 || out_stride % 8 || base_stride < 0 || hidden_stride < 0 || out_stride < outputs)
     return fail(CFMOE_EINVAL, "apply_adapters needs row strides that are multiples of 8");
   if (tokens == 0) return 0;
-  if (!base || !hidden || !encoder || !decoder || !slots || !out || !scratch) return fail(CFMOE_EINVAL, "NULL argument");
+  if (!base || !hidden || !encoder || !decoder || !slots || !out || (bytes && !scratch)) return fail(CFMOE_EINVAL, "NULL argument");
   if (misaligned16(base) || misaligned16(hidden) || misaligned16(encoder) || misaligned16(decoder) || misaligned16(out) ||
       misaligned16(scratch))
     return fail(CFMOE_EINVAL, "apply_adapters needs 16-byte aligned rows, weights and scratch");
@@ -559,7 +559,7 @@ CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t
   // (whole turns: a split ends where the next begins)
   a.share = (hidden_size + a.splits * kTurn - 1) / (a.splits * kTurn) * kTurn;
   const int tiles = (rank + 15) / 16;
-  if (one_launch(tokens, hidden_size, outputs, rank, adapters) && a.out != a.x) {
+  if (bytes == 0) {
     const dim3 grid(tokens, one_pieces(outputs));
     hipLaunchKernelGGL(tiles == 1 ? adapter_one_kernel<1> : adapter_one_kernel<2>, grid, dim3(64 * kOneWaves), 0, stream, a);
     return check_launch("adapter_one");

@@ -378,10 +378,12 @@ CFMOE_API int cfmoe_join_block_backward(
  * (1). FP32 sums; the inner values are held as two BF16 numbers (2^-16 off), and out is
  * rounded once. out may be base, with its stride, or hidden; no other overlap. H and O
  * multiples of 8 up to 65536, R of 8 up to 256, strides of 8; N at most 4096, T 2^24. All
- * 16-byte aligned but slots and scales. scratch: cfmoe_apply_adapters_scratch_bytes; calls
- * that overlap need their own. No reference counterpart. */
-CFMOE_API int64_t cfmoe_apply_adapters_scratch_bytes(int32_t hidden_size, int32_t rank,
-                                                     int32_t adapters, int32_t tokens);
+ * 16-byte aligned but slots and scales. scratch: cfmoe_apply_adapters_scratch_bytes (NULL
+ * where 0, as it is for few tokens of few ranks whose out is not hidden); calls that overlap
+ * need their own. No reference counterpart. */
+CFMOE_API int64_t cfmoe_apply_adapters_scratch_bytes(int32_t hidden_size, int32_t outputs,
+                                                     int32_t rank, int32_t adapters,
+                                                     int32_t tokens, int32_t out_is_hidden);
 CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t rank,
                                    int32_t adapters, uint32_t flags, const void *base,
                                    int64_t base_stride, const void *hidden, int64_t hidden_stride,

@@ -169,12 +169,16 @@ def test_scratch_sizes():
     assert lib.cfmoe_sort_by_expert_scratch_bytes(1, 65, 8) == -_ext.EINVAL
     assert lib.cfmoe_join_block_backward_scratch_bytes(100, 2, 5) == 5 * 2 * 100 * 4
     assert lib.cfmoe_join_block_backward_scratch_bytes(9000, 2, 5) == -_ext.EINVAL
-    assert lib.cfmoe_apply_adapters_scratch_bytes(64, 16, 4, 3) >= 3 * 16 * 4
-    assert lib.cfmoe_apply_adapters_scratch_bytes(2048, 16, 4, 3) >= 8 * 3 * 16 * 4
-    assert lib.cfmoe_apply_adapters_scratch_bytes(64, 16, 4, 5000) >= 5000 * (16 * 4 + 8) + 5 * 4
-    assert lib.cfmoe_apply_adapters_scratch_bytes(64, 16, 4, 1 << 24) >= (1 << 24) * 16 * 4
-    assert lib.cfmoe_apply_adapters_scratch_bytes(64, 15, 4, 3) == -_ext.EINVAL
-    assert lib.cfmoe_apply_adapters_scratch_bytes(60, 16, 4, 3) == -_ext.EINVAL
+    adapters = lib.cfmoe_apply_adapters_scratch_bytes
+    assert adapters(64, 64, 40, 4, 3, 0) >= 3 * 40 * 4
+    assert adapters(2048, 64, 40, 4, 3, 0) >= 8 * 3 * 40 * 4
+    assert adapters(64, 64, 16, 4, 5000, 0) >= 5000 * (16 * 4 + 8) + 5 * 4
+    assert adapters(64, 64, 16, 4, 1 << 24, 0) >= (1 << 24) * 16 * 4
+    assert adapters(64, 64, 16, 4, 3, 0) == 0  # one launch, unless out is what others still read
+    assert adapters(64, 64, 16, 4, 3, 1) >= 3 * 16 * 4
+    assert adapters(64, 64, 15, 4, 3, 0) == -_ext.EINVAL
+    assert adapters(60, 64, 16, 4, 3, 0) == -_ext.EINVAL
+    assert adapters(64, 60, 16, 4, 3, 0) == -_ext.EINVAL
 
 
 def test_overlaps_of_out():
