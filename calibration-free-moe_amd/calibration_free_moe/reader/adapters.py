@@ -152,7 +152,7 @@ def apply_adapters(
         raise ValueError("apply_adapters is forward only: detach its inputs or call it in no_grad")
     given = out is not None
     if not given:
-        out = hidden.new_empty((tokens, o))
+        out = hidden.new_empty(tokens, o)
     elif out.shape != base.shape or not _rows(out, device) or _stride(out) < o:
         raise ValueError("out must be BF16 rows [tokens, O] on the rows' device, one behind another")
     elif tokens and (_overlap(out, base) or _overlap(out, hidden)):

@@ -87,7 +87,7 @@ def sort_by_expert(ids: Tensor, experts: int, padding: Tensor | None = None) -> 
         raise ValueError("padding must be contiguous bool [tokens] on the ids' device")
     size = _ext.sort_scratch_bytes(tokens, top_k, experts)
     offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
-    places = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
+    places = torch.empty(tokens, top_k, dtype=torch.int32, device=device)
     pairs = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
     scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _ext.run(
@@ -110,7 +110,7 @@ def _flags(rows: Tensor, weights: Tensor | None = None) -> int:
 
 def _gather(hidden: Tensor, places: Tensor) -> Tensor:
     tokens, top_k = places.shape
-    rows = hidden.new_empty((tokens * top_k, hidden.shape[1]))
+    rows = hidden.new_empty(tokens * top_k, hidden.shape[1])
     _ext.run(
         _ext.library().cfmoe_gather_rows, hidden.device, hidden.shape[1], top_k, _flags(hidden),
         hidden.data_ptr(), places.data_ptr(), rows.data_ptr(), tokens,
@@ -120,7 +120,7 @@ def _gather(hidden: Tensor, places: Tensor) -> Tensor:
 
 def _combine(rows: Tensor, places: Tensor, weights: Tensor | None) -> Tensor:
     tokens, top_k = places.shape
-    out = rows.new_empty((tokens, rows.shape[1]))
+    out = rows.new_empty(tokens, rows.shape[1])
     _ext.run(
         _ext.library().cfmoe_combine_rows, rows.device, rows.shape[1], top_k,
         _flags(rows, weights), rows.data_ptr(), places.data_ptr(),

@@ -84,8 +84,12 @@ class _Join(torch.autograd.Function):
         if grad_joined is None and grad_out is None:
             return (None,) * 7
         need_hidden, need_block, need_post, need_gate, need_next, _, _ = ctx.needs_input_grad
+        # (both terms of a plain sum have one gradient, written once as by torch's own sum)
+        shared = (
+            need_hidden and need_block and post is None and gate is None and ctx.scale == 1.0
+        )
         made_hidden = torch.empty_like(hidden) if need_hidden else None
-        made_block = torch.empty_like(block) if need_block else None
+        made_block = torch.empty_like(block) if need_block and not shared else None
         made_post = torch.empty_like(post) if need_post else None
         made_gate = torch.empty_like(gate) if need_gate else None
         made_next = torch.empty_like(following) if need_next and grad_out is not None else None
@@ -107,6 +111,8 @@ class _Join(torch.autograd.Function):
             _pointer(made_hidden), _pointer(made_block), _pointer(made_post), _pointer(made_gate),
             _pointer(made_next), _pointer(scratch), tokens,
         )
+        if shared:
+            made_block = made_hidden
         return made_hidden, made_block, made_post, made_gate, made_next, None, None
 
 

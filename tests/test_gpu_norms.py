@@ -333,3 +333,37 @@ def test_refusals():
             join_block(x, x, gate=bad)
     with pytest.raises(ValueError, match="gate"):
         join_block(x.bfloat16(), x.bfloat16(), gate=x)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("following", [False, True])
+def test_gradients_of_a_plain_sum_are_each_terms_own(dtype, following):
+    """Of joined = hidden + block both terms have one gradient: sums of them, of leaves and of
+    a tensor that is both terms, stay apart."""
+    made = make(33, 264, dtype, False, "none", following)
+    on = {k: None if v is None else v.to(DEVICE).requires_grad_() for k, v in made.items()}
+    scaled = join_block(on["hidden"] * 1, on["block"] * 1, residual_scale=1,
+                        next_weight=on["next"])
+    outputs = scaled if following else (scaled,)
+    grads = [torch.randn_like(o) for o in outputs]
+    torch.autograd.backward(outputs, grads, retain_graph=True)
+    assert torch.equal(on["hidden"].grad, on["block"].grad)
+    one = on["hidden"].grad.clone()
+    on["hidden"].grad.zero_()
+    assert torch.equal(on["block"].grad, one)
+    torch.autograd.backward(outputs, grads)
+    assert torch.equal(on["hidden"].grad, one) and torch.equal(on["block"].grad, one + one)
+
+    leaves = [on["hidden"].detach().requires_grad_(), on["block"].detach().requires_grad_()]
+    out = join_block(*leaves, next_weight=on["next"])
+    torch.autograd.backward(out if following else (out,), grads)
+    leaves[0].grad.zero_()
+    assert torch.equal(leaves[1].grad, one)
+
+    both = on["hidden"].detach().requires_grad_()
+    out = join_block(both, both, next_weight=on["next"])
+    torch.autograd.backward(out if following else (out,), grads)
+    apart = [both.detach().clone().requires_grad_() for _ in range(2)]
+    out = join_block(*apart, next_weight=on["next"])
+    torch.autograd.backward(out if following else (out,), grads)
+    assert torch.equal(both.grad, apart[0].grad + apart[1].grad)
