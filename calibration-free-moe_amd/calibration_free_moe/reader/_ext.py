@@ -11,10 +11,12 @@ import ctypes
 import functools
 import os
 from collections.abc import Callable
+from types import ModuleType
 
 import torch
 
 LIBRARY_NAME = "libcfmoe_reader.so"
+AUTOGRAD_NAME = "_autograd.so"
 LIBRARY_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIBRARY_NAME)
 
 ABI_VERSION = 12
@@ -287,19 +289,25 @@ def routed_experts_scratch_bytes(*shape: int) -> int:
     return size
 
 
+@functools.cache
+def autograd() -> ModuleType:
+    """The operators that have gradients, which torch's autograd engine calls (cfmoe_autograd.cpp)."""
+    library()
+    try:
+        from calibration_free_moe.reader import _autograd
+    except ImportError as error:
+        raise RuntimeError(
+            f"{AUTOGRAD_NAME} is missing; run build() of __graft_entry__.py ({error})"
+        ) from error
+    if _autograd.ABI_VERSION != ABI_VERSION:
+        raise RuntimeError(f"{AUTOGRAD_NAME} ABI mismatch; rebuild the library")
+    return _autograd
+
+
 @functools.lru_cache(maxsize=4096)
 def sort_scratch_bytes(tokens: int, top_k: int, experts: int) -> int:
     """Bytes for a call of that size; ValueError if refused."""
     size = library().cfmoe_sort_by_expert_scratch_bytes(tokens, top_k, experts)
-    if size < 0:
-        check(-size)
-    return size
-
-
-@functools.lru_cache(maxsize=4096)
-def join_scratch_bytes(hidden: int, sums: int, tokens: int) -> int:
-    """Bytes for a backward call of that size; ValueError if refused."""
-    size = library().cfmoe_join_block_backward_scratch_bytes(hidden, sums, tokens)
     if size < 0:
         check(-size)
     return size

@@ -14,7 +14,6 @@ from dataclasses import dataclass
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from calibration_free_moe.reader import _ext
 
@@ -102,70 +101,6 @@ def sort_by_expert(ids: Tensor, experts: int, padding: Tensor | None = None) -> 
     return order
 
 
-def _flags(rows: Tensor, weights: Tensor | None = None) -> int:
-    return (_ext.FP32 if rows.dtype == torch.float32 else 0) | (
-        _ext.WEIGHTS_BF16 if weights is not None and weights.dtype == torch.bfloat16 else 0
-    )
-
-
-def _gather(hidden: Tensor, places: Tensor) -> Tensor:
-    tokens, top_k = places.shape
-    rows = hidden.new_empty(tokens * top_k, hidden.shape[1])
-    _ext.run(
-        _ext.library().cfmoe_gather_rows, hidden.device, hidden.shape[1], top_k, _flags(hidden),
-        hidden.data_ptr(), places.data_ptr(), rows.data_ptr(), tokens,
-    )
-    return rows
-
-
-def _combine(rows: Tensor, places: Tensor, weights: Tensor | None) -> Tensor:
-    tokens, top_k = places.shape
-    out = rows.new_empty(tokens, rows.shape[1])
-    _ext.run(
-        _ext.library().cfmoe_combine_rows, rows.device, rows.shape[1], top_k,
-        _flags(rows, weights), rows.data_ptr(), places.data_ptr(),
-        None if weights is None else weights.data_ptr(), out.data_ptr(), tokens,
-    )
-    return out
-
-
-class _Gather(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, places):
-        ctx.save_for_backward(places)
-        return _gather(hidden, places)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        (places,) = ctx.saved_tensors
-        return _combine(grad.contiguous(), places, None), None
-
-
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, rows, places, weights):
-        ctx.save_for_backward(rows, places, weights)
-        return _combine(rows, places, weights)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        rows, places, weights = ctx.saved_tensors
-        tokens, top_k = places.shape
-        grad = grad.contiguous()
-        grad_rows = torch.empty_like(rows) if ctx.needs_input_grad[0] else None
-        grad_weights = torch.empty_like(weights) if ctx.needs_input_grad[2] else None
-        _ext.run(
-            _ext.library().cfmoe_combine_rows_backward, rows.device, rows.shape[1], top_k,
-            _flags(rows, weights), grad.data_ptr(), rows.data_ptr(), places.data_ptr(),
-            None if weights is None else weights.data_ptr(),
-            None if grad_rows is None else grad_rows.data_ptr(),
-            None if grad_weights is None else grad_weights.data_ptr(), tokens,
-        )
-        return grad_rows, None, grad_weights
-
-
 def _check_rows(rows: Tensor, count: int, order: ExpertOrder, what: str) -> None:
     if (
         rows.dim() != 2
@@ -192,9 +127,7 @@ def gather_rows(hidden: Tensor, order: ExpertOrder) -> Tensor:
     in a graph (a backward pass only where no eager graph of the same leaves is alive).
     """
     _check_rows(hidden, order.places.shape[0], order, "rows [tokens, H]")
-    if hidden.requires_grad and torch.is_grad_enabled():
-        return _Gather.apply(hidden, order.places)
-    return _gather(hidden, order.places)
+    return _ext.autograd().gather_rows(hidden, order.places)
 
 
 def combine_rows(rows: Tensor, order: ExpertOrder, weights: Tensor | None = None) -> Tensor:
@@ -216,11 +149,7 @@ def combine_rows(rows: Tensor, order: ExpertOrder, weights: Tensor | None = None
         or not weights.is_contiguous()
     ):
         raise ValueError("weights must be contiguous FP32 or BF16 [tokens, K] on the rows' device")
-    if torch.is_grad_enabled() and (
-        rows.requires_grad or (weights is not None and weights.requires_grad)
-    ):
-        return _Combine.apply(rows, places, weights)
-    return _combine(rows, places, weights)
+    return _ext.autograd().combine_rows(rows, places, weights)
 
 
 __all__ = ["ExpertOrder", "combine_rows", "gather_rows", "sort_by_expert"]

@@ -10,16 +10,11 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from calibration_free_moe.reader import _ext
 
 MAX_HIDDEN = 8192
 MAX_TOKENS = 2 ** 31 - 1
-
-
-def _pointer(t: Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
 
 
 def _gate_flag(gate: Tensor | None, hidden: Tensor) -> int:
@@ -42,78 +37,6 @@ def _flags(hidden: Tensor, post: Tensor | None, gate: Tensor | None, following: 
     if following is not None and following.dtype == fp32:
         flags |= _ext.NEXT_FP32
     return flags
-
-
-def _forward(hidden, block, post, gate, following, scale, epsilon, train):
-    """(joined, next, statistics): None where not asked for."""
-    tokens, size = hidden.shape
-    joined = None if block is None else torch.empty_like(hidden)
-    out = None if following is None else torch.empty_like(hidden)
-    statistics = None
-    if train:
-        statistics = torch.empty((tokens, 2), dtype=torch.float32, device=hidden.device)
-    _ext.run(
-        _ext.library().cfmoe_join_block, hidden.device, size,
-        _flags(hidden, post, gate, following), hidden.data_ptr(), _pointer(block), _pointer(post),
-        _pointer(gate), scale, _pointer(following), epsilon, _pointer(joined), _pointer(out),
-        _pointer(statistics), tokens,
-    )
-    return joined, out, statistics
-
-
-class _Join(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, block, post, gate, following, scale, epsilon):
-        joined, out, statistics = _forward(
-            hidden, block, post, gate, following, scale, epsilon, True
-        )
-        ctx.save_for_backward(hidden, block, post, gate, following, statistics)
-        ctx.scale, ctx.flags = scale, _flags(hidden, post, gate, following)
-        ctx.set_materialize_grads(False)
-        if joined is None:
-            return out
-        return joined if out is None else (joined, out)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
-        hidden, block, post, gate, following, statistics = ctx.saved_tensors
-        grad_joined = None if block is None else grads[0]
-        # (a weight of an output that nothing was made of has no gradient)
-        grad_out = None if following is None else grads[-1]
-        if grad_joined is None and grad_out is None:
-            return (None,) * 7
-        need_hidden, need_block, need_post, need_gate, need_next, _, _ = ctx.needs_input_grad
-        # (both terms of a plain sum have one gradient, written once as by torch's own sum)
-        shared = (
-            need_hidden and need_block and post is None and gate is None and ctx.scale == 1.0
-        )
-        made_hidden = torch.empty_like(hidden) if need_hidden else None
-        made_block = torch.empty_like(block) if need_block and not shared else None
-        made_post = torch.empty_like(post) if need_post else None
-        made_gate = torch.empty_like(gate) if need_gate else None
-        made_next = torch.empty_like(following) if need_next and grad_out is not None else None
-        tokens, size = hidden.shape
-        sums = (made_post is not None) + (made_next is not None) + (need_gate and gate.dim() == 1)
-        scratch = None
-        if sums:
-            scratch = torch.empty(
-                _ext.join_scratch_bytes(size, sums, tokens), dtype=torch.uint8, device=hidden.device
-            )
-        if grad_joined is not None:
-            grad_joined = grad_joined.contiguous()
-        if grad_out is not None:
-            grad_out = grad_out.contiguous()
-        _ext.run(
-            _ext.library().cfmoe_join_block_backward, hidden.device, size, ctx.flags,
-            hidden.data_ptr(), _pointer(block), _pointer(post), _pointer(gate), ctx.scale,
-            _pointer(following), statistics.data_ptr(), _pointer(grad_joined), _pointer(grad_out),
-            _pointer(made_hidden), _pointer(made_block), _pointer(made_post), _pointer(made_gate),
-            _pointer(made_next), _pointer(scratch), tokens,
-        )
-        if shared:
-            made_block = made_hidden
-        return made_hidden, made_block, made_post, made_gate, made_next, None, None
 
 
 def _check_hidden(hidden: Tensor, epsilon: float) -> None:
@@ -152,9 +75,9 @@ def norm_rows(hidden: Tensor, weight: Tensor, *, epsilon: float = 1e-6) -> Tenso
     """
     _check_hidden(hidden, epsilon)
     _check_weight(weight, hidden, "weight")
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        return _Join.apply(hidden, None, None, None, weight, 1.0, epsilon)
-    return _forward(hidden, None, None, None, weight, 1.0, epsilon, False)[1]
+    return _ext.autograd().join_block(
+        hidden, None, None, None, weight, 1.0, epsilon, _flags(hidden, None, None, weight)
+    )[0]
 
 
 def join_block(
@@ -204,17 +127,11 @@ def join_block(
         )
     if not isinstance(residual_scale, (int, float)):
         raise ValueError("residual_scale must be a number")
-    inputs = (hidden, block, post_weight, gate, next_weight)
-    if torch.is_grad_enabled() and (
-        hidden.requires_grad
-        or block.requires_grad
-        or (post_weight is not None and post_weight.requires_grad)
-        or (gate is not None and gate.requires_grad)
-        or (next_weight is not None and next_weight.requires_grad)
-    ):
-        return _Join.apply(*inputs, residual_scale, epsilon)
-    joined, out, _ = _forward(*inputs, residual_scale, epsilon, False)
-    return joined if out is None else (joined, out)
+    made = _ext.autograd().join_block(
+        hidden, block, post_weight, gate, next_weight, residual_scale, epsilon,
+        _flags(hidden, post_weight, gate, next_weight),
+    )
+    return made[0] if next_weight is None else tuple(made)
 
 
 __all__ = ["join_block", "norm_rows"]

@@ -4,6 +4,8 @@ The Python checks see CPU tensors (never a launch); the C entry points are calle
 with addresses that are never read, because the arguments are refused first.
 """
 
+import sys
+
 import pytest
 import torch
 
@@ -195,3 +197,19 @@ def test_overlaps_of_out():
     assert not _overlap(out, torch.zeros(6, 16, dtype=torch.bfloat16))
     assert _overlap(wide[:1, :16], wide[:1, 8:24])
     assert not _overlap(wide[:1, :16], wide[:1, 16:32])
+
+
+def test_gradients_module_is_of_this_library(monkeypatch):
+    module = _ext.autograd()
+    assert module.ABI_VERSION == _ext.ABI_VERSION
+    _ext.autograd.cache_clear()
+    with monkeypatch.context() as patch:
+        patch.setattr(module, "ABI_VERSION", _ext.ABI_VERSION - 1)
+        with pytest.raises(RuntimeError, match="ABI mismatch"):
+            _ext.autograd()
+    with monkeypatch.context() as patch:
+        patch.setitem(sys.modules, "calibration_free_moe.reader._autograd", None)
+        patch.delattr("calibration_free_moe.reader._autograd")
+        with pytest.raises(RuntimeError, match="_autograd.so is missing"):
+            _ext.autograd()
+    assert _ext.autograd() is module
