@@ -29,8 +29,8 @@ constexpr int kMaxHidden = 8192;
 constexpr int kEach = 8;  // values of a row that a thread holds
 // Waves of a launch at most: 24 to a compute unit (16 / 24 / 32: 27.5 / 26.5 / 27.7 us), and 12
 // in at most 1024 workgroups.
-constexpr int kForwardWaves = 6144;
-constexpr int kBackwardWaves = 3072;
+constexpr int kForwardWaves = 24 * 256;
+constexpr int kBackwardWaves = 12 * 256;
 constexpr float kSmall = 0x1p-80f;
 
 enum Gate { kNone, kChannel, kRow, kFull };
