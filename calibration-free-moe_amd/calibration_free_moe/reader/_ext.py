@@ -16,7 +16,7 @@ from types import ModuleType
 import torch
 
 LIBRARY_NAME = "libcfmoe_reader.so"
-AUTOGRAD_NAME = "_autograd.so"
+OPERATORS_NAME = "_torch.so"
 LIBRARY_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIBRARY_NAME)
 
 ABI_VERSION = 12
@@ -290,33 +290,15 @@ def routed_experts_scratch_bytes(*shape: int) -> int:
 
 
 @functools.cache
-def autograd() -> ModuleType:
-    """The operators that have gradients, which torch's autograd engine calls (cfmoe_autograd.cpp)."""
+def operators() -> ModuleType:
+    """The operators around a layer's experts, with their gradients (cfmoe_torch.cpp)."""
     library()
     try:
-        from calibration_free_moe.reader import _autograd
+        from calibration_free_moe.reader import _torch
     except ImportError as error:
         raise RuntimeError(
-            f"{AUTOGRAD_NAME} is missing; run build() of __graft_entry__.py ({error})"
+            f"{OPERATORS_NAME} is missing; run build() of __graft_entry__.py ({error})"
         ) from error
-    if _autograd.ABI_VERSION != ABI_VERSION:
-        raise RuntimeError(f"{AUTOGRAD_NAME} ABI mismatch; rebuild the library")
-    return _autograd
-
-
-@functools.lru_cache(maxsize=4096)
-def sort_scratch_bytes(tokens: int, top_k: int, experts: int) -> int:
-    """Bytes for a call of that size; ValueError if refused."""
-    size = library().cfmoe_sort_by_expert_scratch_bytes(tokens, top_k, experts)
-    if size < 0:
-        check(-size)
-    return size
-
-
-@functools.lru_cache(maxsize=4096)
-def adapters_scratch_bytes(*shape: int) -> int:
-    """Bytes for a call of that shape; ValueError if refused."""
-    size = library().cfmoe_apply_adapters_scratch_bytes(*shape)
-    if size < 0:
-        check(-size)
-    return size
+    if _torch.ABI_VERSION != ABI_VERSION:
+        raise RuntimeError(f"{OPERATORS_NAME} ABI mismatch; rebuild the library")
+    return _torch

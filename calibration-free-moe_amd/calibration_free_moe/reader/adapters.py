@@ -123,10 +123,9 @@ def apply_adapters(
             "Expected BF16 CUDA rows [tokens, H] and [tokens, O], 16-byte aligned with a first "
             "stride of a multiple of 8, and contiguous BF16 encoder [N, R, H] and decoder [N, O, R]"
         )
-    wide = slots.dtype == torch.int64
     if (
         slots.shape != (tokens,)
-        or not (wide or slots.dtype == torch.int32)
+        or slots.dtype not in (torch.int32, torch.int64)
         or slots.device != device
         or not slots.is_contiguous()
         or (
@@ -150,27 +149,14 @@ def apply_adapters(
         or (scales is not None and scales.requires_grad)
     ):
         raise ValueError("apply_adapters is forward only: detach its inputs or call it in no_grad")
-    given = out is not None
-    if not given:
-        out = hidden.new_empty(tokens, o)
-    elif out.shape != base.shape or not _rows(out, device) or _stride(out) < o:
-        raise ValueError("out must be BF16 rows [tokens, O] on the rows' device, one behind another")
-    elif tokens and (_overlap(out, base) or _overlap(out, hidden)):
-        raise ValueError("out overlaps base or hidden and is not the same rows")
-    pointer, x = out.data_ptr(), hidden.data_ptr()
-    size = _ext.adapters_scratch_bytes(h, o, rank, n, tokens, pointer == x)
-    scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    _ext.run(
-        _ext.library().cfmoe_apply_adapters, device, h, o, rank, n,
-        _ext.IDS_INT64 if wide else 0, base.data_ptr(), _stride(base), x, _stride(hidden),
-        encoder.data_ptr(), decoder.data_ptr(), slots.data_ptr(),
-        None if scales is None else scales.data_ptr(), pointer, _stride(out) if given else o,
-        None if scratch is None else scratch.data_ptr(), tokens,
-    )
-    if given and not out.is_inference():
-        # (what saved the tensor for a backward pass is to see that it changed)
-        torch.autograd.graph.increment_version(out)
-    return out
+    if out is not None:
+        if out.shape != base.shape or not _rows(out, device) or _stride(out) < o:
+            raise ValueError(
+                "out must be BF16 rows [tokens, O] on the rows' device, one behind another"
+            )
+        if tokens and (_overlap(out, base) or _overlap(out, hidden)):
+            raise ValueError("out overlaps base or hidden and is not the same rows")
+    return _ext.operators().apply_adapters(base, hidden, encoder, decoder, slots, scales, out)
 
 
 __all__ = ["apply_adapters"]

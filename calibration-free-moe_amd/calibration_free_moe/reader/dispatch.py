@@ -84,17 +84,7 @@ def sort_by_expert(ids: Tensor, experts: int, padding: Tensor | None = None) -> 
         or not padding.is_contiguous()
     ):
         raise ValueError("padding must be contiguous bool [tokens] on the ids' device")
-    size = _ext.sort_scratch_bytes(tokens, top_k, experts)
-    offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
-    places = torch.empty(tokens, top_k, dtype=torch.int32, device=device)
-    pairs = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
-    scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    _ext.run(
-        _ext.library().cfmoe_sort_by_expert, device, experts, top_k,
-        _ext.IDS_INT64 if ids.dtype == torch.int64 else 0, ids.data_ptr(),
-        None if padding is None else padding.data_ptr(), offsets.data_ptr(), places.data_ptr(),
-        pairs.data_ptr(), None if scratch is None else scratch.data_ptr(), tokens,
-    )
+    offsets, places, pairs = _ext.operators().sort_by_expert(ids, experts, padding)
     # (as made here the three need no check)
     order = ExpertOrder.__new__(ExpertOrder)
     order.__dict__.update(offsets=offsets, places=places, pairs=pairs)
@@ -127,7 +117,7 @@ def gather_rows(hidden: Tensor, order: ExpertOrder) -> Tensor:
     in a graph (a backward pass only where no eager graph of the same leaves is alive).
     """
     _check_rows(hidden, order.places.shape[0], order, "rows [tokens, H]")
-    return _ext.autograd().gather_rows(hidden, order.places)
+    return _ext.operators().gather_rows(hidden, order.places)
 
 
 def combine_rows(rows: Tensor, order: ExpertOrder, weights: Tensor | None = None) -> Tensor:
@@ -149,7 +139,7 @@ def combine_rows(rows: Tensor, order: ExpertOrder, weights: Tensor | None = None
         or not weights.is_contiguous()
     ):
         raise ValueError("weights must be contiguous FP32 or BF16 [tokens, K] on the rows' device")
-    return _ext.autograd().combine_rows(rows, places, weights)
+    return _ext.operators().combine_rows(rows, places, weights)
 
 
 __all__ = ["ExpertOrder", "combine_rows", "gather_rows", "sort_by_expert"]

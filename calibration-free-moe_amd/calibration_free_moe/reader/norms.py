@@ -75,7 +75,7 @@ def norm_rows(hidden: Tensor, weight: Tensor, *, epsilon: float = 1e-6) -> Tenso
     """
     _check_hidden(hidden, epsilon)
     _check_weight(weight, hidden, "weight")
-    return _ext.autograd().join_block(
+    return _ext.operators().join_block(
         hidden, None, None, None, weight, 1.0, epsilon, _flags(hidden, None, None, weight)
     )[0]
 
@@ -127,7 +127,7 @@ def join_block(
         )
     if not isinstance(residual_scale, (int, float)):
         raise ValueError("residual_scale must be a number")
-    made = _ext.autograd().join_block(
+    made = _ext.operators().join_block(
         hidden, block, post_weight, gate, next_weight, residual_scale, epsilon,
         _flags(hidden, post_weight, gate, next_weight),
     )

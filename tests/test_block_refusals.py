@@ -199,17 +199,17 @@ def test_overlaps_of_out():
     assert not _overlap(wide[:1, :16], wide[:1, 16:32])
 
 
-def test_gradients_module_is_of_this_library(monkeypatch):
-    module = _ext.autograd()
+def test_operators_module_is_of_this_library(monkeypatch):
+    module = _ext.operators()
     assert module.ABI_VERSION == _ext.ABI_VERSION
-    _ext.autograd.cache_clear()
+    _ext.operators.cache_clear()
     with monkeypatch.context() as patch:
         patch.setattr(module, "ABI_VERSION", _ext.ABI_VERSION - 1)
         with pytest.raises(RuntimeError, match="ABI mismatch"):
-            _ext.autograd()
+            _ext.operators()
     with monkeypatch.context() as patch:
-        patch.setitem(sys.modules, "calibration_free_moe.reader._autograd", None)
-        patch.delattr("calibration_free_moe.reader._autograd")
-        with pytest.raises(RuntimeError, match="_autograd.so is missing"):
-            _ext.autograd()
-    assert _ext.autograd() is module
+        patch.setitem(sys.modules, "calibration_free_moe.reader._torch", None)
+        patch.delattr("calibration_free_moe.reader._torch")
+        with pytest.raises(RuntimeError, match="_torch.so is missing"):
+            _ext.operators()
+    assert _ext.operators() is module

@@ -144,7 +144,7 @@ def test_refusals_are_errors_of_the_call():
     wide = torch.zeros(2, 8200, device=DEVICE, requires_grad=True)
     weight = torch.ones(8200, device=DEVICE)
     with pytest.raises(ValueError, match="1 to 8192"):
-        _ext.autograd().join_block(wide, None, None, None, weight, 1.0, 1e-6, _ext.FP32)
+        _ext.operators().join_block(wide, None, None, None, weight, 1.0, 1e-6, _ext.FP32)
 
 
 def test_rows_are_kept_for_the_weights_gradient_alone():
