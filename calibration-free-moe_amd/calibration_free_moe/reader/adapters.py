@@ -71,8 +71,8 @@ def apply_adapters(
     encoder BF16 [N, R, H] and decoder BF16 [N, O, R] hold N adapters of rank R (one of lower
     rank with zeros behind), contiguous; slots (int32/int64) [tokens] names each token's
     adapter, and a slot outside [0, N) none: its row comes out as it is in base, bit for bit.
-    scales FP32 [N], or None for ones. Sums are FP32, the R inner values are held to 2^-16,
-    and the output is rounded once.
+    scales FP32 [N], or None for ones. Sums are FP32, the R inner values are held in
+    FP32's 24 bits, and the output is rounded once.
 
     base, hidden and out may be column slices of wider rows (first stride a multiple of 8,
     16-byte aligned). `out` may be `base`, whose rows without an adapter are then left

@@ -14,8 +14,9 @@
 // their parts of v; of few ranks one workgroup reads all (adapter_one_kernel). Many tokens
 // are sorted by adapter first.
 //
-// As operand of the second product v is the sum of two BF16 numbers (2^-16 off; one would
-// leave out 2^-8 off v's largest terms, more than out's own rounding), and out is rounded once.
+// As operand of the second product v is the sum of three BF16 numbers, which hold all 24 bits
+// of it, and out is rounded once. (Two hold 16: 4001 tokens of rank 64 then had 51000 of 16
+// million outputs next to their exact value's rounding, where FP32 sums leave 7000.)
 
 #include "cfmoe_rows.h"
 
@@ -125,21 +126,37 @@ __device__ __forceinline__ bool find_sorted_tile(const AdapterArgs &a, int index
 
 __device__ __forceinline__ u32x4 load16(const uint16_t *p) { return *reinterpret_cast<const u32x4 *>(p); }
 
-// Pairs of BF16 numbers whose sums are v to 2^-16. The first is cut off from the number
-// below v, so that neither is zero where v is not (down to 2^-132): an infinite weight times
-// them is that infinity, and where v is infinite the second is.
-__device__ __forceinline__ void split(f32x4 v, u32x2 &high, u32x2 &low) {
-  uint32_t cut[4];
+constexpr int kParts = 3;
+
+// BF16 numbers whose sum is v. All but the last are cut off from the FP32 number below what
+// is left, so that none is zero or of the other sign where v is not: an infinite weight times
+// them is that infinity, and where v is infinite the last is. After the second cut at most 8
+// bits are left or a power of two, so that the last number is exact. (So down to |v| =
+// 2^-102; from there it is rounded up to BF16's last step, 2^-133, and below 2^-109 the
+// second may be zero.)
+__device__ __forceinline__ void split(f32x4 v, u32x2 (&part)[kParts]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t bits = __float_as_uint(v[i]), size = bits & 0x7fffffffu;
-    cut[i] = ((size - (size != 0)) | (bits & 0x80000000u)) & 0xffff0000u;
+  for (int k = 0; k + 1 < kParts; ++k) {
+    uint32_t cut[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t bits = __float_as_uint(v[i]), size = bits & 0x7fffffffu;
+      cut[i] = ((size - (size != 0)) | (bits & 0x80000000u)) & 0xffff0000u;
+      v[i] -= __uint_as_float(cut[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) part[k][i] = cut[2 * i] >> 16 | cut[2 * i + 1];
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    high[i] = cut[2 * i] >> 16 | cut[2 * i + 1];
-    low[i] = bf16_pair(v[2 * i] - __uint_as_float(cut[2 * i]), v[2 * i + 1] - __uint_as_float(cut[2 * i + 1]));
-  }
+  for (int i = 0; i < 2; ++i)
+    part[kParts - 1][i] = (__float_as_uint(v[2 * i]) + 0xffffu) >> 16 | ((__float_as_uint(v[2 * i + 1]) + 0xffffu) & 0xffff0000u);
+}
+
+// sum + w v of 16 outputs and tokens, the parts of v from the smallest on.
+__device__ __forceinline__ f32x4 parts_product(u32x4 w, const u32x4 (&v)[kParts], f32x4 sum) {
+#pragma unroll
+  for (int k = kParts - 1; k >= 0; --k) sum = mma(w, v[k], sum);
+  return sum;
 }
 
 // Values of a row of v in LDS: whole steps of 32, and a unit for the banks.
@@ -267,7 +284,7 @@ __device__ __forceinline__ u32x4 added(u32x4 base, const f32x4 *sum, int s) {
 }
 
 // out = base + D v for a tile of tokens, a wave 64 outputs of them at a time: rows of base
-// and D on their way first, then v from its parts, as two BF16 numbers in LDS. kShort is for
+// and D on their way first, then v from its splits, as three BF16 numbers in LDS. kShort is for
 // ranks up to 32, whose rows of D are read ahead with base. 4001 tokens of rank 64 to 4096
 // outputs take 21 us, 14 of which the same call takes for tokens without an adapter (66 MB of
 // base and out): the rest is a tile's chain of reads and its vector arithmetic. Rows of D
@@ -276,7 +293,7 @@ __device__ __forceinline__ u32x4 added(u32x4 base, const f32x4 *sum, int s) {
 template <bool kSorted, bool kShort>
 __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a) {
   constexpr int kTile = kSorted ? kManyTokens : kTokens, kGroups = kTile / 16;
-  extern __shared__ __attribute__((aligned(16))) uint16_t parts[];  // [2, kTile, parts_row(R)]
+  extern __shared__ __attribute__((aligned(16))) uint16_t parts[];  // [kParts, kTile, parts_row(R)]
   __shared__ int members[kTokens];
   int adapter, start = 0, count;
   if constexpr (kSorted) {
@@ -346,10 +363,10 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a)
         for (int s = 1; s < a.splits; ++s)
           v += *reinterpret_cast<const f32x4 *>(inner + static_cast<int64_t>(s) * a.tokens * a.rank);
       }
-      u32x2 high, low;
-      split(v, high, low);
-      *reinterpret_cast<u32x2 *>(parts + t * stride + r) = high;
-      *reinterpret_cast<u32x2 *>(parts + (kTile + t) * stride + r) = low;
+      u32x2 part[kParts];
+      split(v, part);
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) *reinterpret_cast<u32x2 *>(parts + (k * kTile + t) * stride + r) = part[k];
     }
     __syncthreads();
   }
@@ -361,9 +378,11 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a)
     auto multiply = [&](int r0, const u32x4 *rows) {
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        const u32x4 high = load16(v + 16 * g * stride + r0), low = load16(v + (kTile + 16 * g) * stride + r0);
+        u32x4 part[kParts];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[g][i] = mma(rows[i], low, mma(rows[i], high, sum[g][i]));
+        for (int k = 0; k < kParts; ++k) part[k] = load16(v + (k * kTile + 16 * g) * stride + r0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[g][i] = parts_product(rows[i], part, sum[g][i]);
       }
     };
     if (!bare) {
@@ -397,7 +416,7 @@ template <int kTiles>
 __global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(AdapterArgs a) {
   constexpr int kRow = 32 + kUnit, kLoads = 2 * (kTiles + 1);
   __shared__ __attribute__((aligned(16))) uint16_t stage[kOneWaves][16 * (kTiles + 1)][kStageRow];
-  __shared__ __attribute__((aligned(16))) uint16_t parts[2][kTokens][kRow];
+  __shared__ __attribute__((aligned(16))) uint16_t parts[kParts][kTokens][kRow];
   __shared__ int members[kTokens];
   static_assert(sizeof(float) * kOneWaves * kTiles * 256 <= sizeof(stage), "the sums take the stage's place");
   float(*sums)[kTiles][256] = reinterpret_cast<float(*)[kTiles][256]>(stage);
@@ -447,15 +466,17 @@ __global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(AdapterArgs
         for (int k = 0; k < kOneWaves; ++k) v += *reinterpret_cast<const f32x4 *>(&sums[k][r / 16][t * 16 + r % 16]);
         v *= scale;
       }
-      u32x2 high, low;
-      split(v, high, low);
-      *reinterpret_cast<u32x2 *>(&parts[0][t][r]) = high;
-      *reinterpret_cast<u32x2 *>(&parts[1][t][r]) = low;
+      u32x2 part[kParts];
+      split(v, part);
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) *reinterpret_cast<u32x2 *>(&parts[k][t][r]) = part[k];
     }
     __syncthreads();
-    const u32x4 high = load16(&parts[0][m][kUnit * q]), low = load16(&parts[1][m][kUnit * q]);
+    u32x4 part[kParts];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = mma(w[i], low, mma(w[i], high, sum[i]));
+    for (int k = 0; k < kParts; ++k) part[k] = load16(&parts[k][m][kUnit * q]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = parts_product(w[i], part, sum[i]);
   }
   if (m >= count) return;
 #pragma unroll
@@ -598,7 +619,7 @@ CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t
   // (4001 tokens to 4096 outputs: 40.5 us with up to 2048 workgroups, 44.2 with 4400)
   int columns = (outputs + kWaves * kColumns - 1) / (kWaves * kColumns);
   while (columns > 1 && static_cast<int64_t>(most) * columns > kMostGroups) columns = (columns + 1) / 2;
-  const unsigned lds = 2 * tile * parts_row(rank) * 2;
+  const unsigned lds = kParts * tile * parts_row(rank) * 2;
   auto finish = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(most, columns), block, lds, stream, a);
     return check_launch("adapter_out");

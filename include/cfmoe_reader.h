@@ -375,8 +375,8 @@ CFMOE_API int cfmoe_join_block_backward(
  * base[t] itself, bit for bit, where a lies outside [0, N). bf16 rows base and out [T, O]
  * and hidden [T, H] with row strides in values; contiguous bf16 encoder [N, R, H] and
  * decoder [N, O, R]; slots int32 (CFMOE_IDS_INT64: int64) [T], scales fp32 [N] or NULL
- * (1). FP32 sums; the inner values are held as two BF16 numbers (2^-16 off), and out is
- * rounded once. out may be base, with its stride, or hidden; no other overlap. H and O
+ * (1). FP32 sums; the inner values are held as three BF16 numbers (FP32's 24 bits), and out
+ * is rounded once. out may be base, with its stride, or hidden; no other overlap. H and O
  * multiples of 8 up to 65536, R of 8 up to 256, strides of 8; N at most 4096, T 2^24. All
  * 16-byte aligned but slots and scales. scratch: cfmoe_apply_adapters_scratch_bytes (NULL
  * where 0, as it is for few tokens of few ranks whose out is not hidden); calls that overlap
