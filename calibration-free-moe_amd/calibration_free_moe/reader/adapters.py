@@ -80,8 +80,8 @@ def apply_adapters(
     to 256, N up to 4096, tokens up to 2^24; zero tokens give an empty output. One or two HIP
     launches on the current stream of the tensors' device, up to four for more than 256 tokens,
     with scratch allocated per call where they need any; they can be captured in a graph. `out`
-    counts as written in place. Tensors that require gradients are refused while gradients are
-    on.
+    counts as written in place. Tensors that require gradients, `out` among them, are refused
+    while gradients are on.
     """
     if hidden.dim() != 2 or base.dim() != 2 or encoder.dim() != 3 or decoder.dim() != 3:
         raise ValueError(
@@ -147,8 +147,11 @@ def apply_adapters(
         or encoder.requires_grad
         or decoder.requires_grad
         or (scales is not None and scales.requires_grad)
+        or (out is not None and out.requires_grad)
     ):
-        raise ValueError("apply_adapters is forward only: detach its inputs or call it in no_grad")
+        raise ValueError(
+            "apply_adapters is forward only: detach its inputs and out or call it in no_grad"
+        )
     if out is not None:
         if out.shape != base.shape or not _rows(out, device) or _stride(out) < o:
             raise ValueError(
