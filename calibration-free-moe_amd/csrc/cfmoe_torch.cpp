@@ -36,6 +36,16 @@ void check(int status) {
   TORCH_CHECK(false, cfmoe_last_error());
 }
 
+bool dual(const Tensor &t) { return t.defined() && t._fw_grad(0).defined(); }
+bool dual(const Optional &t) { return t && dual(*t); }
+
+// The kernels read values alone and have no derivative forwards: a tensor's tangent would be
+// lost without a word, which stands for zero.
+template <typename... T>
+void check_tangents(const char *name, const T &...tensors) {
+  TORCH_CHECK_VALUE(!(dual(tensors) || ...), name, " has no forward-mode derivative: call it with tensors without a tangent");
+}
+
 Tensor contiguous(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
 
 // A workspace of the call's own, undefined where it needs none.
@@ -214,6 +224,7 @@ int64_t row_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.siz
 
 Tensor apply_adapters(const Tensor &base, const Tensor &hidden, const Tensor &encoder, const Tensor &decoder,
                       const Tensor &slots, const Optional &scales, const Optional &to) {
+  check_tangents("apply_adapters", base, hidden, encoder, decoder, scales, to);
   c10::DeviceGuard guard(hidden.device());
   const int32_t tokens = narrow(hidden.size(0)), size = narrow(hidden.size(1)), outputs = narrow(base.size(1));
   const int32_t adapters = narrow(encoder.size(0)), rank = narrow(encoder.size(1));
@@ -235,17 +246,20 @@ bool trained(const Optional &t) { return t && t->requires_grad(); }
 // The module's functions: a node in the graph where a gradient is asked for.
 
 Tensor gather_rows(const Tensor &hidden, const Tensor &places) {
+  check_tangents("gather_rows", hidden);
   if (at::GradMode::is_enabled() && trained(hidden)) return Gather::apply(hidden, places);
   return gathered(hidden, places);
 }
 
 Tensor combine_rows(const Tensor &rows, const Tensor &places, const Optional &weights) {
+  check_tangents("combine_rows", rows, weights);
   if (at::GradMode::is_enabled() && (trained(rows) || trained(weights))) return Combine::apply(rows, places, weights);
   return combined(rows, places, given(weights));
 }
 
 variable_list join_block(const Tensor &hidden, const Optional &block, const Optional &post, const Optional &gate,
                          const Optional &next, double scale, double epsilon, int64_t flags) {
+  check_tangents(block ? "join_block" : "norm_rows", hidden, block, post, gate, next);
   if (at::GradMode::is_enabled() &&
       (trained(hidden) || trained(block) || trained(post) || trained(gate) || trained(next)))
     return Join::apply(hidden, block, post, gate, next, scale, epsilon, flags);

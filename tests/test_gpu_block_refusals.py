@@ -3,8 +3,11 @@
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from calibration_free_moe.reader.adapters import apply_adapters
+from calibration_free_moe.reader.dispatch import combine_rows, gather_rows, sort_by_expert
+from calibration_free_moe.reader.norms import join_block, norm_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +46,44 @@ def test_adapters_refuse_a_trained_out():
         with torch.no_grad():
             assert apply_adapters(**t, out=out) is out
             assert bool((out == 512).all())
+
+
+def calls():
+    """name -> (call, its float tensors)"""
+    order = sort_by_expert(torch.zeros(4, 2, dtype=torch.int32, device=DEVICE), 2)
+
+    def ones(*shape):
+        return torch.ones(shape, device=DEVICE)
+
+    t = adapters()
+    names = ("base", "hidden", "encoder", "decoder", "scales")
+    return {
+        "gather": (lambda x: gather_rows(x, order), [ones(4, 64)]),
+        "combine": (lambda x, w: combine_rows(x, order, w), [ones(8, 64), ones(4, 2)]),
+        "norm": (norm_rows, [ones(4, 64), ones(64)]),
+        "join": (lambda x, b, p, g, w: join_block(x, b, post_weight=p, gate=g, next_weight=w),
+                 [ones(4, 64), ones(4, 64), ones(64), ones(4, 1), ones(64)]),
+        "adapters": (lambda *v: apply_adapters(**dict(zip(names, v)), slots=t["slots"]),
+                     [t[n] for n in names]),
+    }
+
+
+NAMES = ["gather", "combine", "norm", "join", "adapters"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tangents_are_refused(name):
+    """No operator has a forward-mode derivative; a dual tensor's would be taken for zero."""
+    call, tensors = calls()[name]
+    with forward_ad.dual_level():
+        for i, t in enumerate(tensors):
+            for trained in (False, True):
+                if trained and name == "adapters":
+                    continue
+                u = t.clone().requires_grad_(trained)
+                arguments = [forward_ad.make_dual(u, torch.ones_like(t)) if j == i else v
+                             for j, v in enumerate(tensors)]
+                with pytest.raises(ValueError, match="forward-mode"):
+                    call(*arguments)
+        call(*tensors)
+    call(*tensors)
