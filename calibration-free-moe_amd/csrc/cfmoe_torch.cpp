@@ -8,6 +8,7 @@
 // us, from here 15.5. Tensors are checked by the functions' callers in Python; every launch goes
 // through the C entry points, on the current stream of the tensors' device.
 
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -39,10 +40,12 @@ void check(int status) {
 bool dual(const Tensor &t) { return t.defined() && t._fw_grad(0).defined(); }
 bool dual(const Optional &t) { return t && dual(*t); }
 
-// The kernels read values alone and have no derivative forwards: a tensor's tangent would be
-// lost without a word, which stands for zero.
+// What would be answered wrongly without a word: the kernels read values alone and have no
+// derivative forwards, so that a tensor's tangent would be lost, which stands for zero; and a
+// trace holds torch's own calls, so that of an operator it would have the output's allocation.
 template <typename... T>
-void check_tangents(const char *name, const T &...tensors) {
+void check_mode(const char *name, const T &...tensors) {
+  TORCH_CHECK_VALUE(!at::tracer::impl::is_dispatch_enabled(), name, " cannot be recorded by torch.jit.trace");
   TORCH_CHECK_VALUE(!(dual(tensors) || ...), name, " has no forward-mode derivative: call it with tensors without a tangent");
 }
 
@@ -206,6 +209,7 @@ struct Join : torch::autograd::Function<Join> {
 
 // offsets, places and pairs of the batch's order.
 std::tuple<Tensor, Tensor, Tensor> sort_by_expert(const Tensor &ids, int64_t experts, const Optional &padding) {
+  check_mode("sort_by_expert");
   c10::DeviceGuard guard(ids.device());
   const int32_t tokens = narrow(ids.size(0)), top_k = narrow(ids.size(1));
   const auto options = ids.options().dtype(at::kInt);
@@ -224,7 +228,7 @@ int64_t row_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.siz
 
 Tensor apply_adapters(const Tensor &base, const Tensor &hidden, const Tensor &encoder, const Tensor &decoder,
                       const Tensor &slots, const Optional &scales, const Optional &to) {
-  check_tangents("apply_adapters", base, hidden, encoder, decoder, scales, to);
+  check_mode("apply_adapters", base, hidden, encoder, decoder, scales, to);
   c10::DeviceGuard guard(hidden.device());
   const int32_t tokens = narrow(hidden.size(0)), size = narrow(hidden.size(1)), outputs = narrow(base.size(1));
   const int32_t adapters = narrow(encoder.size(0)), rank = narrow(encoder.size(1));
@@ -246,20 +250,20 @@ bool trained(const Optional &t) { return t && t->requires_grad(); }
 // The module's functions: a node in the graph where a gradient is asked for.
 
 Tensor gather_rows(const Tensor &hidden, const Tensor &places) {
-  check_tangents("gather_rows", hidden);
+  check_mode("gather_rows", hidden);
   if (at::GradMode::is_enabled() && trained(hidden)) return Gather::apply(hidden, places);
   return gathered(hidden, places);
 }
 
 Tensor combine_rows(const Tensor &rows, const Tensor &places, const Optional &weights) {
-  check_tangents("combine_rows", rows, weights);
+  check_mode("combine_rows", rows, weights);
   if (at::GradMode::is_enabled() && (trained(rows) || trained(weights))) return Combine::apply(rows, places, weights);
   return combined(rows, places, given(weights));
 }
 
 variable_list join_block(const Tensor &hidden, const Optional &block, const Optional &post, const Optional &gate,
                          const Optional &next, double scale, double epsilon, int64_t flags) {
-  check_tangents(block ? "join_block" : "norm_rows", hidden, block, post, gate, next);
+  check_mode(block ? "join_block" : "norm_rows", hidden, block, post, gate, next);
   if (at::GradMode::is_enabled() &&
       (trained(hidden) || trained(block) || trained(post) || trained(gate) || trained(next)))
     return Join::apply(hidden, block, post, gate, next, scale, epsilon, flags);

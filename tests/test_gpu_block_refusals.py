@@ -87,3 +87,22 @@ def test_tangents_are_refused(name):
                     call(*arguments)
         call(*tensors)
     call(*tensors)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("trained", [False, True])
+def test_tracing_is_refused(name, trained):
+    """A trace would hold the outputs' allocation and none of the kernels."""
+    call, tensors = calls()[name]
+    tensors = [t.clone().requires_grad_(trained and name != "adapters") for t in tensors]
+    with pytest.raises(ValueError, match="torch.jit.trace"):
+        torch.jit.trace(call, tuple(tensors))
+    call(*tensors)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_tracing_the_order_is_refused():
+    ids = torch.zeros(4, 2, dtype=torch.int32, device=DEVICE)
+    with pytest.raises(ValueError, match="torch.jit.trace"):
+        torch.jit.trace(lambda t: sort_by_expert(t, 2).places, (ids,))
