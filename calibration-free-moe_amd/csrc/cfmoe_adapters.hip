@@ -6,7 +6,7 @@
 // a token whose slot names none keeps its row of `base`, bit for bit.
 //
 // Tokens of one adapter share its weights: they form tiles, and a tile's products are
-// matrix instructions, v = s_a C_a x over the hidden dimension and D_a v over the rank. A
+// matrix instructions, C_a x over the hidden dimension and D_a v, v = s_a C_a x, over the rank. A
 // decode step's tiles hold a token or two, which leaves most columns of an instruction
 // empty: what bounds it is the weights' reading, once for each tile, and a compute unit
 // takes about 75 GB/s from memory. So the hidden dimension and the ranks are spread over
@@ -46,7 +46,7 @@ struct AdapterArgs {
   const void *slots;
   const float *scales;
   uint16_t *out;
-  float *inner;            // [splits, T, R]: parts of v, tokens in sorted order where they are sorted
+  float *inner;            // [splits, T, R]: parts of C x, tokens in sorted order where they are sorted
   const int32_t *offsets;  // [N + 1] and
   const int32_t *pairs;    // [T]: tokens by adapter (many tokens only)
   int64_t base_stride, x_stride, out_stride;
@@ -212,8 +212,9 @@ __device__ __forceinline__ void staged_product(uint16_t (*stage)[kStageRow], con
   }
 }
 
-// inner[split, token, r] = a split's part of s sum_h C[r, h] x[token, h], of a tile of
-// tokens and kTiles tiles of 16 ranks. The waves take the split's hidden values in turns of
+// inner[split, token, r] = a split's part of sum_h C[r, h] x[token, h], of a tile of
+// tokens and kTiles tiles of 16 ranks (s multiplies the whole sum, in the second launch: parts
+// that it takes out of FP32 may cancel). The waves take the split's hidden values in turns of
 // 64 and add up in LDS. What bounds it is the chain of offsets, tokens and rows in memory,
 // four turns of them for a wave.
 template <bool kSorted, int kTiles>
@@ -251,7 +252,6 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_inner_kernel(AdapterArgs 
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) *reinterpret_cast<f32x4 *>(&sums[wave][g][i][m * 16 + 4 * q]) = d[g][i];
   __syncthreads();
-  const float scale = a.scales ? a.scales[adapter] : 1.0f;
   const int n = threadIdx.x % 16;
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_inner_kernel(AdapterArgs 
       float total = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) total += sums[w][g][i][threadIdx.x];
-      to[16 * i] = scale * total;
+      to[16 * i] = total;
     }
   }
 }
@@ -353,6 +353,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a)
   if (!bare) {
     // (zeros behind the last rank: the matrix instructions take 32 at a time)
     const int fours = (stride - kUnit) / 4;
+    const float scale = a.scales ? a.scales[adapter] : 1.0f;
     for (int i = threadIdx.x; i < count * fours; i += 64 * kWaves) {
       const int t = i / fours, r = i % fours * 4;
       const float *inner = a.inner + static_cast<int64_t>(kSorted ? start + t : members[t]) * a.rank + r;
@@ -362,6 +363,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a)
 #pragma unroll 4
         for (int s = 1; s < a.splits; ++s)
           v += *reinterpret_cast<const f32x4 *>(inner + static_cast<int64_t>(s) * a.tokens * a.rank);
+        v *= scale;
       }
       u32x2 part[kParts];
       split(v, part);

@@ -59,3 +59,28 @@ def test_infinite_weights_of_small_inner_values(shape):
     assert bool((out[:, 3] == -float("inf")).all()) and bool((out[:, 5] == float("inf")).all())
     out[:, [3, 5]] = 0
     assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_scales_apply_to_whole_inner_values(shape):
+    """Inner values of terms that cancel to 1 before a scale of 2^110, which would take the
+    terms out of FP32: 2^110, times weights of 2^-110."""
+    tokens, hidden, outputs, adapters, rank = shape
+    t = zeros(*shape)
+    t["hidden"][:, 0], t["hidden"][:, hidden - 1], t["hidden"][:, hidden // 2] = 2.0 ** 20, -2.0 ** 20, 1
+    t["encoder"][:] = 1
+    t["decoder"][:, :, 0] = 2.0 ** -110
+    t["scales"] = torch.full((adapters,), 2.0 ** 110)
+    out = apply_adapters(**{k: v.to(DEVICE) for k, v in t.items()}).cpu()
+    assert bool((out == 1).all())
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_infinite_scales(shape):
+    """Of hidden values that are zero but in one place."""
+    t = zeros(*shape)
+    t["hidden"][:, 0] = 1
+    t["encoder"][:], t["decoder"][:] = 1, 1
+    t["scales"] = torch.full((shape[3],), float("inf"))
+    out = apply_adapters(**{k: v.to(DEVICE) for k, v in t.items()}).cpu()
+    assert bool((out == float("inf")).all())
