@@ -226,6 +226,16 @@ std::tuple<Tensor, Tensor, Tensor> sort_by_expert(const Tensor &ids, int64_t exp
 // Values from one row to the next; of a single row, which has none, its length.
 int64_t row_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
+// Whether out's rows [tokens, O] and a contiguous tensor have memory in common.
+bool overlaps(const Tensor &out, const Tensor &t) {
+  if (!t.defined() || t.numel() == 0 || out.numel() == 0) return false;
+  const int64_t size = out.element_size(), step = row_stride(out) * size, row = out.size(1) * size;
+  const int64_t at = static_cast<const char *>(t.const_data_ptr()) - static_cast<const char *>(out.const_data_ptr());
+  // the first of out's rows that ends behind t's begin, if it begins before t's end
+  const int64_t first = at < row ? 0 : (at - row) / step + 1;
+  return first < out.size(0) && first * step < at + static_cast<int64_t>(t.nbytes());
+}
+
 Tensor apply_adapters(const Tensor &base, const Tensor &hidden, const Tensor &encoder, const Tensor &decoder,
                       const Tensor &slots, const Optional &scales, const Optional &to) {
   check_mode("apply_adapters", base, hidden, encoder, decoder, scales, to);
@@ -233,6 +243,9 @@ Tensor apply_adapters(const Tensor &base, const Tensor &hidden, const Tensor &en
   const int32_t tokens = narrow(hidden.size(0)), size = narrow(hidden.size(1)), outputs = narrow(base.size(1));
   const int32_t adapters = narrow(encoder.size(0)), rank = narrow(encoder.size(1));
   Tensor out = to ? *to : at::empty({tokens, outputs}, hidden.options());
+  if (to)
+    for (const Tensor &t : {encoder, decoder, slots, given(scales)})
+      TORCH_CHECK_VALUE(!overlaps(out, t), "out overlaps the adapters, their slots or their scales");
   const Tensor scratch = bytes(cfmoe_apply_adapters_scratch_bytes(size, outputs, rank, adapters, tokens,
                                                                   out.data_ptr() == hidden.data_ptr()), hidden);
   check(cfmoe_apply_adapters(size, outputs, rank, adapters, slots.scalar_type() == at::kLong ? CFMOE_IDS_INT64 : 0,

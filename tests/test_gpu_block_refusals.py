@@ -48,6 +48,30 @@ def test_adapters_refuse_a_trained_out():
             assert bool((out == 512).all())
 
 
+def test_adapters_refuse_an_out_over_their_weights():
+    """Rows of `out` in memory that other tokens' products still read."""
+    t = adapters()
+    memory = torch.ones(4096, dtype=torch.bfloat16, device=DEVICE)
+    # values 512 .. 1535, 512 .. 519 and 512 .. 515
+    cases = {"encoder": memory[512:1536].view(2, 8, 64), "decoder": memory[512:1536].view(2, 64, 8),
+             "slots": memory[512:520].view(torch.int32).zero_(),
+             "scales": memory[512:516].view(torch.float32).fill_(1.0)}
+    for name, value in cases.items():
+        for out in (memory[:1024].view(4, 256)[:, :64],      # its third row begins there
+                    memory[264:520].view(4, 64),             # its last row ends there
+                    memory[448:1472].view(4, 256)[:, 8:72]):  # its first row ends behind
+            with pytest.raises(ValueError, match="overlaps"):
+                apply_adapters(**{**t, name: value}, out=out)
+    # between the rows of out, and right before and behind them
+    rows = torch.ones(6, 256, dtype=torch.bfloat16, device=DEVICE)
+    for at in (rows[2, 64:72], rows[2, 248:], rows[0, 248:], rows[4, 64:72], rows[5, :8]):
+        slots = at.view(torch.int32).zero_()
+        out = rows[1:5, :64]
+        out.fill_(7.0)
+        apply_adapters(**{**t, "slots": slots}, out=out)
+        assert bool((out == 512).all()) and bool((slots == 0).all())
+
+
 def calls():
     """name -> (call, its float tensors)"""
     order = sort_by_expert(torch.zeros(4, 2, dtype=torch.int32, device=DEVICE), 2)
