@@ -11,7 +11,7 @@
 // empty: what bounds it is the weights' reading, once for each tile, and a compute unit
 // takes about 75 GB/s from memory. So the hidden dimension and the ranks are spread over
 // workgroups (adapter_inner_kernel), and the second launch (adapter_out_kernel) adds up
-// their parts of v; of few ranks one workgroup reads all (adapter_one_kernel). Many tokens
+// their parts; of few ranks one workgroup reads all (adapter_one_kernel). Many tokens
 // are sorted by adapter first.
 //
 // As operand of the second product v is the sum of three BF16 numbers, which hold all 24 bits
