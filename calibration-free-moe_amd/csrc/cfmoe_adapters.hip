@@ -516,13 +516,15 @@ bool one_launch(int tokens, int hidden, int outputs, int rank, int adapters) {
 // 64 (2816 to 1408 values) take 19 us either way, 512 of 8 adapters of rank 32 26 and 17.
 bool sorts(int tokens) { return tokens > kFewTokens; }
 
-// Workgroups share the hidden dimension: of few tokens 256 values each or a sixteenth, of
-// many two halves, whose parts the second launch reads again for every 256 outputs or more.
+// Workgroups share the hidden dimension in whole turns of 256 values: of few tokens 16 of them
+// at most, of many two, whose parts the second launch reads again for every 256 outputs or
+// more. Each has as many turns but the last, so that 17 turns are shared by nine.
 // 1 / 2 / 4 of them: 4001 tokens of rank 64 (2048 to 4096 values) 42 / 40 / 44 us, 1000 tokens
 // 29 / 25 / 25, 1500 of rank 128 (4096 to 4096) 44 / 38 / 42.
 int splits_of(int tokens, int hidden) {
   const int turns = (hidden + kTurn - 1) / kTurn, most = sorts(tokens) ? kManySplits : kFewSplits;
-  return turns < most ? turns : most;
+  const int each = (turns + most - 1) / most;
+  return (turns + each - 1) / each;
 }
 
 }  // namespace
