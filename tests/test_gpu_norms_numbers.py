@@ -1,10 +1,10 @@
 """Ends of the norms' and joins' ranges (needs an MI355X): rows whose squares pass FP32,
-and epsilons of their size."""
+epsilons of their size, and gradients summed over many rows."""
 
 import pytest
 import torch
 
-from calibration_free_moe.reader.norms import norm_rows
+from calibration_free_moe.reader.norms import join_block, norm_rows
 from tests import block_reference as plain
 
 pytestmark = pytest.mark.gpu
@@ -38,3 +38,27 @@ def test_epsilon_beside_rows_whose_squares_pass_fp32(size, epsilon):
     terms = inverse * (grad.double() * w.double()).abs().max(-1, keepdim=True).values
     plain.within(got[0], wanted[0], bounds["hidden"] + 4 * plain.U * terms + 2.0 ** -148)
     plain.within(got[1], wanted[1], bounds["next"] + 2 * plain.U * grad.double().abs().sum(0))
+
+
+@pytest.mark.parametrize("tokens,size", [(515, 1003), (1024, 64), (1024, 700)])
+@pytest.mark.parametrize("large", [0, 16, 400])
+def test_gradients_summed_over_rows_pass_few_roundings(tokens, size, large):
+    """A row of 1 among rows of 2^-25, each of which an FP32 sum of 1 loses. Every row has a
+    workgroup of its own here; of their sums 16 waves take every 16th, in 8 sums each, and
+    both are added in pairs: tokens / 128 roundings, 3 and 4."""
+    rows = torch.full((tokens, size), 2.0 ** -25)
+    rows[large] = 1
+    want = torch.full((size,), 1 + (tokens - 1) * 2.0 ** -25, dtype=torch.float64)
+    allowed = ((tokens + 127) // 128 + 3 + 4) * plain.U * want
+    grad, ones = rows.to(DEVICE), torch.ones(tokens, size, device=DEVICE)
+    # (rows of ones have the root 1, so that each gradient is the sum of `rows`)
+    for which in ("next", "post", "gate"):
+        w = torch.ones(size, device=DEVICE, requires_grad=True)
+        if which == "next":
+            out = norm_rows(ones, w, epsilon=1e-30)
+        elif which == "post":
+            out = join_block(0 * ones, ones, post_weight=w, epsilon=1e-30)
+        else:
+            out = join_block(0 * ones, ones, gate=w)
+        (got,) = torch.autograd.grad(out, w, grad)
+        plain.within(got, want, allowed)
