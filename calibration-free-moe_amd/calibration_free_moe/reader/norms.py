@@ -15,6 +15,7 @@ from calibration_free_moe.reader import _ext
 
 MAX_HIDDEN = 8192
 MAX_TOKENS = 2 ** 31 - 1
+LARGEST = torch.finfo(torch.float32).max
 
 
 def _gate_flag(gate: Tensor | None, hidden: Tensor) -> int:
@@ -96,7 +97,8 @@ def join_block(
     the norm of joined, before joined is rounded, with `next_weight`: what the next block
     takes. hidden and block BF16 or FP32 [tokens, H], of one type; weights [H] of that type or
     FP32; gate, if given, per channel [H] or per row [tokens, 1] of that type or FP32, or
-    per value [tokens, H] of that type. H any size from 1 to 8192.
+    per value [tokens, H] of that type. H any size from 1 to 8192. residual_scale is a finite
+    FP32 number, of the residual stream: one of the block's output is a gate [H] filled with it.
 
     Gradients go to all tensors, those of weights and of a gate that is spread over rows or
     columns summed in FP32 in an order that depends on sizes alone; they are formed from the
@@ -125,8 +127,8 @@ def join_block(
             "gate must be contiguous [H] or [tokens, 1] of the rows' type or FP32, or [tokens, H] "
             "of their type, on their device"
         )
-    if not isinstance(residual_scale, (int, float)):
-        raise ValueError("residual_scale must be a number")
+    if not isinstance(residual_scale, (int, float)) or not -LARGEST <= residual_scale <= LARGEST:
+        raise ValueError("residual_scale must be a finite FP32 number")
     made = _ext.operators().join_block(
         hidden, block, post_weight, gate, next_weight, residual_scale, epsilon,
         _flags(hidden, post_weight, gate, next_weight),

@@ -130,3 +130,13 @@ def test_tracing_the_order_is_refused():
     ids = torch.zeros(4, 2, dtype=torch.int32, device=DEVICE)
     with pytest.raises(ValueError, match="torch.jit.trace"):
         torch.jit.trace(lambda t: sort_by_expert(t, 2).places, (ids,))
+
+
+@pytest.mark.parametrize("number", [
+    1e39, -1e39, pytest.param(10 ** 400, id="long"), float("inf"), float("-inf"), float("nan")])
+def test_scales_that_are_no_fp32_numbers_are_refused(number):
+    x = torch.ones(2, 64, device=DEVICE)
+    with pytest.raises(ValueError, match="residual_scale"):
+        join_block(x, x, residual_scale=number)
+    for largest in (3.4028234663852886e38, -3.4028234663852886e38, 0, 1, True):
+        assert torch.equal(join_block(x, 0 * x, residual_scale=largest), x * float(largest))
