@@ -200,6 +200,7 @@ def library() -> ctypes.CDLL:
     lib.cfmoe_routed_experts_scratch_bytes.argtypes = [count] * 4 + [flags, count]
     lib.cfmoe_routed_experts.restype = ctypes.c_int
     lib.cfmoe_routed_experts.argtypes = [count] * 4 + [flags] + [pointer] * 10 + [count, pointer]
+    # (the package calls those below from C++; bound here for who calls the C ABI from Python)
     stride, number = ctypes.c_int64, ctypes.c_float
     lib.cfmoe_sort_by_expert_scratch_bytes.restype = ctypes.c_int64
     lib.cfmoe_sort_by_expert_scratch_bytes.argtypes = [count] * 3

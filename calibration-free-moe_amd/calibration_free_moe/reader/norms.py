@@ -18,7 +18,7 @@ MAX_TOKENS = 2 ** 31 - 1
 LARGEST = torch.finfo(torch.float32).max
 
 
-def _gate_flag(gate: Tensor | None, hidden: Tensor) -> int:
+def _gate_flag(gate: Tensor | None) -> int:
     if gate is None:
         return 0
     if gate.dim() == 1:
@@ -27,7 +27,7 @@ def _gate_flag(gate: Tensor | None, hidden: Tensor) -> int:
 
 
 def _flags(hidden: Tensor, post: Tensor | None, gate: Tensor | None, following: Tensor | None) -> int:
-    flags = _gate_flag(gate, hidden)
+    flags = _gate_flag(gate)
     if hidden.dtype == torch.float32:
         return flags | _ext.FP32
     fp32 = torch.float32
@@ -119,7 +119,7 @@ def join_block(
     if gate is not None and (
         gate.shape not in (hidden.shape[1:], (hidden.shape[0], 1), hidden.shape)
         or gate.dtype not in (hidden.dtype, torch.float32)
-        or (_gate_flag(gate, hidden) == _ext.GATE_FULL and gate.dtype != hidden.dtype)
+        or (_gate_flag(gate) == _ext.GATE_FULL and gate.dtype != hidden.dtype)
         or gate.device != hidden.device
         or not gate.is_contiguous()
     ):

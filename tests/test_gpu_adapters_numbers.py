@@ -84,3 +84,28 @@ def test_infinite_scales(shape):
     t["scales"] = torch.full((shape[3],), float("inf"))
     out = apply_adapters(**{k: v.to(DEVICE) for k, v in t.items()}).cpu()
     assert bool((out == float("inf")).all())
+
+
+@pytest.mark.parametrize("tokens", [9, 257, 700, 1024, 1100])
+def test_out_is_hidden_beside_nan_and_infinities(tokens):
+    """Rows with a NaN or an infinity stay alone where each token's rows are read and written."""
+    g = torch.Generator().manual_seed(tokens)
+    t = {"base": torch.randn(tokens, 128, generator=g).to(BF16),
+         "hidden": torch.randn(tokens, 128, generator=g).to(BF16),
+         "encoder": (torch.randn(3, 16, 128, generator=g) / 11).to(BF16),
+         "decoder": torch.randn(3, 128, 16, generator=g).to(BF16),
+         "slots": torch.arange(tokens) % 3}
+    clean = apply_adapters(**{k: v.to(DEVICE) for k, v in t.items()})
+    t["hidden"][2, 7], t["hidden"][5, 70] = float("nan"), float("inf")
+    t["base"][8, 3] = float("nan")
+    on = {k: v.to(DEVICE) for k, v in t.items()}
+    apart = apply_adapters(**on)
+    assert apply_adapters(**on, out=on["hidden"]) is on["hidden"]
+    mask = torch.zeros(tokens, 128, dtype=torch.bool, device=DEVICE)
+    mask[2], mask[8, 3] = True, True
+    for out in (apart, on["hidden"]):
+        assert torch.equal(out[:5].isnan(), mask[:5]) and torch.equal(out[6:].isnan(), mask[6:])
+        assert not bool(out[5].isfinite().any())
+        others = ~mask
+        others[5] = False
+        assert torch.equal(out[others], clean[others])
