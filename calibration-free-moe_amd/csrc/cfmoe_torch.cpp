@@ -10,6 +10,7 @@
 
 #include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -45,7 +46,11 @@ bool dual(const Optional &t) { return t && dual(*t); }
 // trace holds torch's own calls, so that of an operator it would have the output's allocation.
 template <typename... T>
 void check_mode(const char *name, const T &...tensors) {
-  TORCH_CHECK_VALUE(!at::tracer::impl::is_dispatch_enabled(), name, " cannot be recorded by torch.jit.trace");
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  const bool traced = at::tracer::impl::is_dispatch_enabled() ||
+                      (TorchDispatchModeTLS::any_modes_set() && TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY));
+  TORCH_CHECK_VALUE(!traced, name, " cannot be recorded by torch.jit.trace or torch.fx");
   TORCH_CHECK_VALUE(!(dual(tensors) || ...), name, " has no forward-mode derivative: call it with tensors without a tangent");
 }
 

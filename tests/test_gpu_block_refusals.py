@@ -4,6 +4,8 @@
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils.flop_counter import FlopCounterMode
 
 from calibration_free_moe.reader.adapters import apply_adapters
 from calibration_free_moe.reader.dispatch import combine_rows, gather_rows, sort_by_expert
@@ -80,15 +82,14 @@ def calls():
         return torch.ones(shape, device=DEVICE)
 
     t = adapters()
-    names = ("base", "hidden", "encoder", "decoder", "scales")
     return {
         "gather": (lambda x: gather_rows(x, order), [ones(4, 64)]),
         "combine": (lambda x, w: combine_rows(x, order, w), [ones(8, 64), ones(4, 2)]),
-        "norm": (norm_rows, [ones(4, 64), ones(64)]),
+        "norm": (lambda x, w: norm_rows(x, w), [ones(4, 64), ones(64)]),
         "join": (lambda x, b, p, g, w: join_block(x, b, post_weight=p, gate=g, next_weight=w),
                  [ones(4, 64), ones(4, 64), ones(64), ones(4, 1), ones(64)]),
-        "adapters": (lambda *v: apply_adapters(**dict(zip(names, v)), slots=t["slots"]),
-                     [t[n] for n in names]),
+        "adapters": (lambda base, x, c, d, s: apply_adapters(base, x, c, d, t["slots"], s),
+                     [t[n] for n in ("base", "hidden", "encoder", "decoder", "scales")]),
     }
 
 
@@ -130,6 +131,21 @@ def test_tracing_the_order_is_refused():
     ids = torch.zeros(4, 2, dtype=torch.int32, device=DEVICE)
     with pytest.raises(ValueError, match="torch.jit.trace"):
         torch.jit.trace(lambda t: sort_by_expert(t, 2).places, (ids,))
+    with pytest.raises(ValueError, match="torch.fx"):
+        make_fx(lambda t: sort_by_expert(t, 2).places)(ids)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_recording_as_torch_calls_is_refused(name):
+    """Modes that look at torch's calls without recording them are none of it."""
+    call, tensors = calls()[name]
+    with pytest.raises(ValueError, match="torch.fx"):
+        make_fx(call)(*tensors)
+    want = call(*tensors)
+    with FlopCounterMode(display=False):
+        got = call(*tensors)
+    for a, b in zip(got, want) if isinstance(want, tuple) else [(got, want)]:
+        assert torch.equal(a, b)
 
 
 @pytest.mark.parametrize("number", [
