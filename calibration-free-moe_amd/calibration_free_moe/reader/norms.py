@@ -102,7 +102,8 @@ def join_block(
 
     Gradients go to all tensors, those of weights and of a gate that is spread over rows or
     columns summed in FP32 in an order that depends on sizes alone; they are formed from the
-    inputs again, with no other rounding than their own. Numbers and launches as `norm_rows`.
+    inputs again, with no other rounding than their own. All inputs are kept for that, and are
+    not to change before it. Numbers and launches as `norm_rows`.
     """
     _check_hidden(hidden, epsilon)
     if (

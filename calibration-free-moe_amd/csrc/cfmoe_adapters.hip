@@ -286,7 +286,7 @@ __device__ __forceinline__ u32x4 added(u32x4 base, const f32x4 *sum, int s) {
 // out = base + D v for a tile of tokens, a wave 64 outputs of them at a time: rows of base
 // and D on their way first, then v from its splits, as three BF16 numbers in LDS. kShort is for
 // ranks up to 32, whose rows of D are read ahead with base. 4001 tokens of rank 64 to 4096
-// outputs take 21 us, 14 of which the same call takes for tokens without an adapter (66 MB of
+// outputs take 22 us, 14 of which the same call takes for tokens without an adapter (66 MB of
 // base and out): the rest is a tile's chain of reads and its vector arithmetic. Rows of D
 // and out through LDS, tiles of 16 or 64 tokens and D's rows read ahead at rank 64 took
 // 21 to 26.
@@ -412,8 +412,8 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_out_kernel(AdapterArgs a)
 }
 
 // Both products of few tokens and ranks in one launch: workgroup = a tile and 1024 of its
-// outputs, v formed again for each (so out cannot be x, which others still read). The waves take the hidden dimension in turns of 64; rows
-// of base and D are on their way meanwhile.
+// outputs, v formed again for each (so out cannot be x, which others still read). The waves
+// take the hidden dimension in turns of 64; rows of base and D are on their way meanwhile.
 template <int kTiles>
 __global__ __launch_bounds__(64 * kOneWaves) void adapter_one_kernel(AdapterArgs a) {
   constexpr int kRow = 32 + kUnit, kLoads = 2 * (kTiles + 1);
@@ -519,8 +519,8 @@ bool sorts(int tokens) { return tokens > kFewTokens; }
 // Workgroups share the hidden dimension in whole turns of 256 values: of few tokens 16 of them
 // at most, of many two, whose parts the second launch reads again for every 256 outputs or
 // more. Each has as many turns but the last, so that 17 turns are shared by nine.
-// 1 / 2 / 4 of them: 4001 tokens of rank 64 (2048 to 4096 values) 42 / 40 / 44 us, 1000 tokens
-// 29 / 25 / 25, 1500 of rank 128 (4096 to 4096) 44 / 38 / 42.
+// 1 / 2 / 4 of them: 4001 tokens of rank 64 (2048 to 4096 values) 38.7 / 37.4 / 39.2 us, 1000 of
+// rank 32 (2048 to 2048) 20.6 / 17.3 / 16.0, 1500 of rank 128 (4096 to 4096) 43.9 / 39.8 / 42.7.
 int splits_of(int tokens, int hidden) {
   const int turns = (hidden + kTurn - 1) / kTurn, most = sorts(tokens) ? kManySplits : kFewSplits;
   const int each = (turns + most - 1) / most;
@@ -620,7 +620,7 @@ CFMOE_API int cfmoe_apply_adapters(int32_t hidden_size, int32_t outputs, int32_t
                : held == 2 ? start(adapter_inner_kernel<true, 2>)
                            : start(adapter_inner_kernel<true, 4>))
     return rc;
-  // (4001 tokens to 4096 outputs: 40.5 us with up to 2048 workgroups, 44.2 with 4400)
+  // (4001 tokens of 5 adapters to 4096 outputs: 37.4 us with 1048 workgroups, 42.4 with 2096)
   int columns = (outputs + kWaves * kColumns - 1) / (kWaves * kColumns);
   while (columns > 1 && static_cast<int64_t>(most) * columns > kMostGroups) columns = (columns + 1) / 2;
   const unsigned lds = kParts * tile * parts_row(rank) * 2;

@@ -17,9 +17,10 @@
 // What a dropped pair's row or weight holds is never read, so it may hold a NaN.
 //
 // All but the order is one pass over rows, bound by memory. 4096 and 8191 tokens of eight
-// BF16 rows of 2048: laid out 24 and 50 to 59 us (151 and 302 MB, 5.1 to 6.3 TB/s), summed 27
-// and 58 (5.2 to 5.6), the sum's gradients 112 (570 MB, 5.1 TB/s). Rows that are read once
-// are loaded past the caches: 62 -> 59 us the sum, 121 -> 109 its gradients; stores past them
+// BF16 rows of 2048, new ones each time: laid out 24 and 59 us (151 and 302 MB, 6.2 and 5.1
+// TB/s), summed 26 and 58 (5.7 and 5.2), the sum's gradients 116 (570 MB, 4.9 TB/s). Rows
+// that are read once are loaded past the caches, which keep the others: 8192 tokens, the
+// same ones again and again, 73 -> 46 us the sum, 103 -> 87 its gradients; stores past them
 // made a sum that follows slower (104 -> 112 both).
 
 #include "cfmoe_rows.h"
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void order_count_kernel(OrderArgs 
 // LDS, the counts become first rows (a scan over the keys, then over workgroups and waves),
 // and a pair's row is its key's first row of the wave and its rank there, which the counting
 // gave; pairs that the lanes do not hold from then are ranked again. Round trips and barriers
-// bound it: 3.6 us for one token, 4.8 for 1048 pairs in one workgroup, 4.6 and 6.4 in two
+// bound it: 3.5 us for one token, 4.7 for 1048 pairs in one workgroup, 4.6 and 6.4 in two
 // launches for 32768 in 32. (Counting by LDS atomics took 9.3 us for 4001 pairs of five
 // keys, which now take 6.1.)
 __global__ __launch_bounds__(64 * kSortWaves) void order_kernel(OrderArgs a) {
@@ -203,7 +204,10 @@ __global__ __launch_bounds__(64 * kSortWaves) void order_kernel(OrderArgs a) {
   }
 }
 
-// Waves of a sorting workgroup at most: 16, fewer where the counts of many experts need the LDS.
+// Waves of a sorting workgroup at most: 16, fewer where the counts of many experts need the
+// LDS. That costs much: 65536 pairs of 512 / 1024 / 2048 / 4096 experts take 15 / 26 / 70 / 391
+// us in both launches, of 16 / 8 / 4 / 1 waves, each of which reads as many more of the 64
+// workgroups' counts.
 int most_waves(int experts) {
   int waves = kSortWaves;
   while ((waves + 2) * (experts + 1) * 4 > kCountBytes) waves /= 2;
@@ -414,9 +418,9 @@ int check_rows(const RowsArgs &a) {
 }
 
 // A wave takes a token of up to two lanes' worth, a workgroup of four a longer one. 8192
-// tokens of 8 rows, BF16, one wave against four: laying out rows of 264 / 1024 / 2048 9.1 / 23.6
-// / 58.5 us and 10.0 / 23.9 / 50.1, their sum 10.0 / 27.3 / 62.2 and 11.4 / 26.8 / 52.4, its
-// gradients 19.8 / 48.0 / 107.6 and 31.6 / 48.7 / 95.6.
+// tokens of 8 rows, BF16, the same ones again and again, one wave against four: laying out
+// rows of 264 / 1024 / 2048 9.4 / 24.1 / 55.2 us and 11.4 / 24.0 / 47.1, their sum 9.8 / 23.3 /
+// 57.6 and 11.5 / 23.9 / 45.9, its gradients 21.0 / 47.4 / 98.9 and 41.2 / 48.3 / 87.4.
 #define CFMOE_ROWS_LAUNCH(KERNEL, fp32, a, stream)                                                          \
   do {                                                                                                      \
     const Rows rows = rows_of((a).hidden, fp32);                                                            \
